@@ -440,6 +440,101 @@ int miso_attn_layer_ingest(const miso_attn_layer* layer, uint16_t* k_cache, uint
                            const float* delta, float* y, float eps, float* decode_ws,
                            float* prefill_ws, uint32_t max_tok, uint32_t chunk, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * A bounded KV cache (no reference counterpart: the reference's cache only grows)
+ *
+ * weights: f32 [2][max_ctx], the caller's, zeroed once: per KV head and cache row, the softmax
+ * weight that the head's 8 query heads have given the row, summed over the queries seen so far
+ * (1 per query head and query in all). Operators add to rows [0, len); other rows are not touched.
+ * weights and index need 4-byte alignment, workspaces 16-byte; the workspaces hold nothing between
+ * calls. Sums are in a fixed order, so equal calls give equal bits. Queries and visible cache rows
+ * are finite; what lies past the rows a query sees is not used, whatever it holds.
+ * ---------------------------------------------------------------------------------------------- */
+
+/* Bytes of the workspace of the decodes with weights, for len <= max_len and n_splits <= max_splits. */
+uint64_t miso_attn_decode_weights_workspace_bytes(uint32_t max_len, uint32_t max_splits);
+
+/* miso_attn_decode (core equal to its, bit for bit) that also adds each key's weight to
+ * weights[][0 .. len). Rejects what miso_attn_decode rejects and a workspace that is too small. */
+int miso_attn_decode_weights(const float* q, const float* qg, const uint16_t* k_cache,
+                             const uint16_t* v_cache, float* core, float* weights, float* part_m,
+                             float* part_l, float* part_o, uint32_t len, uint32_t max_ctx,
+                             uint32_t n_splits, void* workspace, uint64_t workspace_bytes,
+                             void* stream);
+
+/* The same over the e4m3-row cache (core equal to miso_attn_decode_fp8's). */
+int miso_attn_decode_weights_fp8(const float* q, const float* qg, const uint8_t* k8,
+                                 const uint8_t* v8, const float* k_scale, const float* v_scale,
+                                 float* core, float* weights, float* part_m, float* part_l,
+                                 float* part_o, uint32_t len, uint32_t max_ctx, uint32_t n_splits,
+                                 void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Bytes of the workspace of the prefill weights, for n <= max_n and pos0 + n <= max_rows. */
+uint64_t miso_attn_prefill_weights_workspace_bytes(uint32_t max_n, uint32_t max_rows, int fp8);
+
+/* The weights that n queries ([n][16][256], as the batched prep writes them) at rows pos0 .. give
+ * the rows they see: row j gets the causal softmax weights of every token t with j <= pos0 + t, at
+ * f32 precision (the queries as exact pairs of f16). Run beside miso_attn_prefill over the same
+ * cache; the last tokens of a prompt alone may vote (q of those, pos0 their first row). Rejects
+ * n == 0, pos0 + n > max_ctx, max_ctx > 2^29 and a workspace that is too small. */
+int miso_attn_prefill_weights(const float* q, const uint16_t* k_cache, float* weights,
+                              uint32_t pos0, uint32_t n, uint32_t max_ctx, void* workspace,
+                              uint64_t workspace_bytes, void* stream);
+
+/* The same over the e4m3-row cache, its K rows widened to f16 as miso_attn_prefill_fp8 does. */
+int miso_attn_prefill_weights_fp8(const float* q, const uint8_t* k8, const float* k_scale,
+                                  float* weights, uint32_t pos0, uint32_t n, uint32_t max_ctx,
+                                  void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Bytes of the workspace of miso_attn_evict_select for len <= max_len. */
+uint64_t miso_attn_evict_workspace_bytes(uint32_t max_len);
+
+/* The rows of [0, len) to keep, per KV head: the first `sinks`, the last `recent` and the
+ * keep - sinks - recent others of the largest weight; of equal weights the lower rows (-0 equals
+ * +0, a NaN ranks below every number). index: [2][keep], ascending. Rejects keep == 0 or > len,
+ * sinks + recent > keep, len > max_ctx, len >= 2^31 and a workspace that is too small. */
+int miso_attn_evict_select(const float* weights, uint32_t len, uint32_t max_ctx, uint32_t keep,
+                           uint32_t sinks, uint32_t recent, int32_t* index, void* workspace,
+                           uint64_t workspace_bytes, void* stream);
+
+/* Row index[g][j] of the source becomes row j < keep of the destination, K, V and weight; the
+ * weights of rows keep .. out_ctx - 1 become 0, their K and V rows stay as they are. An index
+ * outside [0, max_ctx) gives a row of zeros with weight 0. The destination is another cache: one
+ * that overlaps the source is rejected, as are keep == 0, keep > max_ctx and keep > out_ctx. */
+int miso_attn_evict_gather(const uint16_t* k_cache, const uint16_t* v_cache, const float* weights,
+                           uint32_t max_ctx, const int32_t* index, uint32_t keep, uint16_t* k_out,
+                           uint16_t* v_out, float* weights_out, uint32_t out_ctx, void* stream);
+
+/* The same over the e4m3-row cache (codes and row scales). */
+int miso_attn_evict_gather_fp8(const uint8_t* k8, const uint8_t* v8, const float* k_scale,
+                               const float* v_scale, const float* weights, uint32_t max_ctx,
+                               const int32_t* index, uint32_t keep, uint8_t* k8_out,
+                               uint8_t* v8_out, float* k_scale_out, float* v_scale_out,
+                               float* weights_out, uint32_t out_ctx, void* stream);
+
+/* The preps with the cache row apart from the position: the token is rotated for position pos and
+ * appended at row `row` (pos0 + t at row0 + t), which differ once a cache has been shortened. The
+ * decode and prefill that follow take rows: len = row + 1, pos0 = row0. Equal to the preps above
+ * where row == pos. Reject row >= max_ctx (row0 + n > max_ctx) and pos0 + n >= 2^32. */
+int miso_attn_prep_at(const float* qg, const float* k, const float* v, const float* q_norm,
+                      const float* k_norm, const float* inv_freq, uint16_t* k_cache,
+                      uint16_t* v_cache, float* q, uint32_t pos, uint32_t row, uint32_t max_ctx,
+                      float eps, void* stream);
+int miso_attn_prep_batch_at(const float* qg, const float* k, const float* v, const float* q_norm,
+                            const float* k_norm, const float* inv_freq, uint16_t* k_cache,
+                            uint16_t* v_cache, float* q, uint32_t pos0, uint32_t row0,
+                            uint32_t max_ctx, float eps, uint32_t n, uint32_t proj_stride,
+                            void* stream);
+int miso_attn_prep_at_fp8(const float* qg, const float* k, const float* v, const float* q_norm,
+                          const float* k_norm, const float* inv_freq, uint8_t* k8, uint8_t* v8,
+                          float* k_scale, float* v_scale, float* q, uint32_t pos, uint32_t row,
+                          uint32_t max_ctx, float eps, void* stream);
+int miso_attn_prep_batch_at_fp8(const float* qg, const float* k, const float* v,
+                                const float* q_norm, const float* k_norm, const float* inv_freq,
+                                uint8_t* k8, uint8_t* v8, float* k_scale, float* v_scale, float* q,
+                                uint32_t pos0, uint32_t row0, uint32_t max_ctx, float eps,
+                                uint32_t n, uint32_t proj_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -74,6 +74,26 @@ SIGNATURES = {
                                         P, c_uint32, P]),
     "miso_attn_layer_ingest": (c_int, [P, P, P, c_uint32, c_uint32, c_uint32, P, P, P, c_float,
                                        P, P, c_uint32, c_uint32, P]),
+    "miso_attn_decode_weights_workspace_bytes": (c_uint64, [c_uint32, c_uint32]),
+    "miso_attn_decode_weights": (c_int, [P] * 9 + [c_uint32, c_uint32, c_uint32, P, c_uint64, P]),
+    "miso_attn_decode_weights_fp8": (c_int, [P] * 11 + [c_uint32, c_uint32, c_uint32, P, c_uint64,
+                                                        P]),
+    "miso_attn_prefill_weights_workspace_bytes": (c_uint64, [c_uint32, c_uint32, c_int]),
+    "miso_attn_prefill_weights": (c_int, [P, P, P, c_uint32, c_uint32, c_uint32, P, c_uint64, P]),
+    "miso_attn_prefill_weights_fp8": (c_int, [P, P, P, P, c_uint32, c_uint32, c_uint32, P,
+                                              c_uint64, P]),
+    "miso_attn_evict_workspace_bytes": (c_uint64, [c_uint32]),
+    "miso_attn_evict_select": (c_int, [P, c_uint32, c_uint32, c_uint32, c_uint32, c_uint32, P, P,
+                                       c_uint64, P]),
+    "miso_attn_evict_gather": (c_int, [P, P, P, c_uint32, P, c_uint32, P, P, P, c_uint32, P]),
+    "miso_attn_evict_gather_fp8": (c_int, [P, P, P, P, P, c_uint32, P, c_uint32, P, P, P, P, P,
+                                           c_uint32, P]),
+    "miso_attn_prep_at": (c_int, [P] * 9 + [c_uint32, c_uint32, c_uint32, c_float, P]),
+    "miso_attn_prep_batch_at": (c_int, [P] * 9 + [c_uint32, c_uint32, c_uint32, c_float, c_uint32,
+                                                  c_uint32, P]),
+    "miso_attn_prep_at_fp8": (c_int, [P] * 11 + [c_uint32, c_uint32, c_uint32, c_float, P]),
+    "miso_attn_prep_batch_at_fp8": (c_int, [P] * 11 + [c_uint32, c_uint32, c_uint32, c_float,
+                                                       c_uint32, c_uint32, P]),
 }
 
 _lib = None

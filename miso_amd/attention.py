@@ -50,6 +50,21 @@ def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int) -> None:
         raise ValueError(f"{name} has {t.numel()} elements, needs >= {numel}")
 
 
+def _count(x: int, name: str) -> int:
+    """A count or row as the C ABI takes it (ctypes would wrap what does not fit 32 bits)."""
+    if not 0 <= x < 1 << 32:
+        raise ValueError(f"{name} must be in [0, 2^32), got {x}")
+    return x
+
+
+def _here(**tensors: torch.Tensor) -> None:
+    """The tensors lie on the current device, whose stream the launches go to."""
+    device = torch.cuda.current_device() if _device is None else _device()
+    for name, t in tensors.items():
+        if t.device.index != device:
+            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{device}")
+
+
 def _cache_dtype(t: torch.Tensor) -> torch.dtype:
     return torch.float16 if t.dtype == torch.float16 else torch.int16
 
@@ -64,8 +79,9 @@ def attn_prefill_items(n: int) -> int:
 
 
 def attn_prep(qg, k, v, q_norm, k_norm, inv_freq, k_cache, v_cache, q, pos: int, max_ctx: int,
-              eps: float, stream=None) -> None:
-    """RMSNorm + RoPE of one token's 16 query and 2 key heads; appends K/V at `pos`."""
+              eps: float, stream=None, row: Optional[int] = None) -> None:
+    """RMSNorm + RoPE of one token's 16 query and 2 key heads; appends K/V at `pos`, or at cache
+    row `row` where the cache has been shortened (miso_attn_prep_at)."""
     f32 = torch.float32
     _need(qg, "qg", f32, Q_HEADS * 2 * DIM)
     _need(k, "k", f32, KV_HEADS * DIM)
@@ -76,15 +92,21 @@ def attn_prep(qg, k, v, q_norm, k_norm, inv_freq, k_cache, v_cache, q, pos: int,
     _need(k_cache, "k_cache", _cache_dtype(k_cache), KV_HEADS * max_ctx * DIM)
     _need(v_cache, "v_cache", _cache_dtype(v_cache), KV_HEADS * max_ctx * DIM)
     _need(q, "q", f32, Q_HEADS * DIM)
-    _lib.check(_lib.load().miso_attn_prep(
-        _ptr(qg), _ptr(k), _ptr(v), _ptr(q_norm), _ptr(k_norm), _ptr(inv_freq), _ptr(k_cache),
-        _ptr(v_cache), _ptr(q), pos, max_ctx, eps, _stream(stream)))
+    tensors = (_ptr(qg), _ptr(k), _ptr(v), _ptr(q_norm), _ptr(k_norm), _ptr(inv_freq),
+               _ptr(k_cache), _ptr(v_cache), _ptr(q))
+    if row is None:
+        _lib.check(_lib.load().miso_attn_prep(*tensors, pos, max_ctx, eps, _stream(stream)))
+    else:
+        pos, row = _count(pos, "pos"), _count(row, "row")
+        _lib.check(_lib.load().miso_attn_prep_at(*tensors, pos, row, max_ctx, eps,
+                                                 _stream(stream)))
 
 
 def attn_prep_batch(qg, k, v, q_norm, k_norm, inv_freq, k_cache, v_cache, q, pos0: int,
-                    max_ctx: int, eps: float, n: int, proj_stride: int, stream=None) -> None:
+                    max_ctx: int, eps: float, n: int, proj_stride: int, stream=None,
+                    row0: Optional[int] = None) -> None:
     """attn_prep for n tokens; qg/k/v are views into a token-major projection buffer whose
-    rows are proj_stride floats apart."""
+    rows are proj_stride floats apart. Appends at pos0 .., or at cache rows row0 .. (row0 given)."""
     f32 = torch.float32
     for name, t in (("qg", qg), ("k", k), ("v", v)):
         if not t.is_cuda or t.dtype != f32:
@@ -95,9 +117,15 @@ def attn_prep_batch(qg, k, v, q_norm, k_norm, inv_freq, k_cache, v_cache, q, pos
     _need(k_cache, "k_cache", _cache_dtype(k_cache), KV_HEADS * max_ctx * DIM)
     _need(v_cache, "v_cache", _cache_dtype(v_cache), KV_HEADS * max_ctx * DIM)
     _need(q, "q", f32, n * Q_HEADS * DIM)
-    _lib.check(_lib.load().miso_attn_prep_batch(
-        _ptr(qg), _ptr(k), _ptr(v), _ptr(q_norm), _ptr(k_norm), _ptr(inv_freq), _ptr(k_cache),
-        _ptr(v_cache), _ptr(q), pos0, max_ctx, eps, n, proj_stride, _stream(stream)))
+    tensors = (_ptr(qg), _ptr(k), _ptr(v), _ptr(q_norm), _ptr(k_norm), _ptr(inv_freq),
+               _ptr(k_cache), _ptr(v_cache), _ptr(q))
+    if row0 is None:
+        _lib.check(_lib.load().miso_attn_prep_batch(*tensors, pos0, max_ctx, eps, n, proj_stride,
+                                                    _stream(stream)))
+    else:
+        pos0, row0 = _count(pos0, "pos0"), _count(row0, "row0")
+        _lib.check(_lib.load().miso_attn_prep_batch_at(*tensors, pos0, row0, max_ctx, eps, n,
+                                                       proj_stride, _stream(stream)))
 
 
 def attn_split(q, k_cache, v_cache, part_m, part_l, part_o, length: int, max_ctx: int,
@@ -338,8 +366,9 @@ def attn_kv_encode_fp8(k_cache, v_cache, cache: Fp8Cache, pos0: int, n: int,
 
 
 def attn_prep_fp8(qg, k, v, q_norm, k_norm, inv_freq, cache: Fp8Cache, q, pos: int,
-                  eps: float = 1e-6, stream=None) -> None:
-    """attn_prep appending the token's K / V to `cache` as e4m3 rows at position pos."""
+                  eps: float = 1e-6, stream=None, row: Optional[int] = None) -> None:
+    """attn_prep appending the token's K / V to `cache` as e4m3 rows at position pos (or at row
+    `row`)."""
     f32 = torch.float32
     _need(qg, "qg", f32, Q_HEADS * 2 * DIM)
     _need(k, "k", f32, KV_HEADS * DIM)
@@ -348,15 +377,23 @@ def attn_prep_fp8(qg, k, v, q_norm, k_norm, inv_freq, cache: Fp8Cache, q, pos: i
                        ("inv_freq", inv_freq, 32), ("q", q, Q_HEADS * DIM)):
         _need(t, name, f32, n)
     _need_fp8(cache)
-    _lib.check(_lib.load().miso_attn_prep_fp8(
-        _ptr(qg), _ptr(k), _ptr(v), _ptr(q_norm), _ptr(k_norm), _ptr(inv_freq),
-        *(_ptr(b) for b in cache.buffers()), _ptr(q), pos, cache.max_ctx, eps, _stream(stream)))
+    tensors = (_ptr(qg), _ptr(k), _ptr(v), _ptr(q_norm), _ptr(k_norm), _ptr(inv_freq),
+               *(_ptr(b) for b in cache.buffers()), _ptr(q))
+    if row is None:
+        _lib.check(_lib.load().miso_attn_prep_fp8(*tensors, pos, cache.max_ctx, eps,
+                                                  _stream(stream)))
+    else:
+        pos, row = _count(pos, "pos"), _count(row, "row")
+        _lib.check(_lib.load().miso_attn_prep_at_fp8(*tensors, pos, row, cache.max_ctx, eps,
+                                                     _stream(stream)))
 
 
 def attn_prep_batch_fp8(qg, k, v, q_norm, k_norm, inv_freq, cache: Fp8Cache, q, pos0: int,
-                        n: int, proj_stride: int, eps: float = 1e-6, stream=None) -> None:
-    """attn_prep_batch appending the tokens' K / V to `cache` as e4m3 rows at pos0 .. pos0 + n - 1;
-    qg / k / v are views into a token-major projection buffer, rows proj_stride floats apart."""
+                        n: int, proj_stride: int, eps: float = 1e-6, stream=None,
+                        row0: Optional[int] = None) -> None:
+    """attn_prep_batch appending the tokens' K / V to `cache` as e4m3 rows at pos0 .. pos0 + n - 1
+    (or at rows row0 ..); qg / k / v are views into a token-major projection buffer, rows
+    proj_stride floats apart."""
     f32 = torch.float32
     for name, t in (("qg", qg), ("k", k), ("v", v)):
         if not t.is_cuda or t.dtype != f32:
@@ -365,10 +402,15 @@ def attn_prep_batch_fp8(qg, k, v, q_norm, k_norm, inv_freq, cache: Fp8Cache, q, 
                        ("inv_freq", inv_freq, 32), ("q", q, n * Q_HEADS * DIM)):
         _need(t, name, f32, m)
     _need_fp8(cache)
-    _lib.check(_lib.load().miso_attn_prep_batch_fp8(
-        _ptr(qg), _ptr(k), _ptr(v), _ptr(q_norm), _ptr(k_norm), _ptr(inv_freq),
-        *(_ptr(b) for b in cache.buffers()), _ptr(q), pos0, cache.max_ctx, eps, n, proj_stride,
-        _stream(stream)))
+    tensors = (_ptr(qg), _ptr(k), _ptr(v), _ptr(q_norm), _ptr(k_norm), _ptr(inv_freq),
+               *(_ptr(b) for b in cache.buffers()), _ptr(q))
+    if row0 is None:
+        _lib.check(_lib.load().miso_attn_prep_batch_fp8(*tensors, pos0, cache.max_ctx, eps, n,
+                                                        proj_stride, _stream(stream)))
+    else:
+        pos0, row0 = _count(pos0, "pos0"), _count(row0, "row0")
+        _lib.check(_lib.load().miso_attn_prep_batch_at_fp8(
+            *tensors, pos0, row0, cache.max_ctx, eps, n, proj_stride, _stream(stream)))
 
 
 class Fp8PrefillScratch:
@@ -430,6 +472,173 @@ def attn_decode_fp8(q, qg, cache: Fp8Cache, core, scratch: DecodeScratch, length
         _ptr(scratch.part_m), _ptr(scratch.part_l), _ptr(scratch.part_o), length, cache.max_ctx,
         n_splits, _stream(stream)))
     return n_splits
+
+
+# ------------------------------------------------------------------------------------------------
+# A bounded KV cache: attention that accumulates the weight every cached key receives (weights: f32
+# [2][max_ctx], zeroed once by the caller), the rows to keep by it, and their move into another
+# cache. After a move the next token's row is behind its position: the preps take row= / row0=.
+# ------------------------------------------------------------------------------------------------
+
+class DecodeWeightsScratch(DecodeScratch):
+    """DecodeScratch with the workspace of attn_decode_weights for up to max_len keys (64 bytes a
+    key)."""
+
+    def __init__(self, max_splits: int, max_len: int, device="cuda"):
+        super().__init__(max_splits, device)
+        self.max_len = _count(max_len, "max_len")
+        nbytes = int(_lib.load().miso_attn_decode_weights_workspace_bytes(max_len, max_splits))
+        self.ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _decode_weights(name: str, q, qg, cache, core, weights, scratch, length, max_ctx, n_splits,
+                    stream) -> int:
+    length, max_ctx = _count(length, "length"), _count(max_ctx, "max_ctx")
+    if n_splits is None:
+        n_splits = attn_n_splits(length, scratch.max_splits)
+    if not 0 < n_splits <= scratch.max_splits:
+        raise ValueError("n_splits must be at least 1 and within the scratch capacity")
+    if length > scratch.max_len:
+        raise ValueError("length exceeds the scratch capacity")
+    f32 = torch.float32
+    _need(q, "q", f32, Q_HEADS * DIM)
+    _need(qg, "qg", f32, Q_HEADS * 2 * DIM)
+    _need(core, "core", f32, Q_HEADS * DIM)
+    _need(weights, "weights", f32, KV_HEADS * max_ctx)
+    _here(q=q, qg=qg, k_cache=cache[0], v_cache=cache[1], core=core, weights=weights,
+          scratch=scratch.ws)
+    _lib.check(getattr(_lib.load(), name)(
+        _ptr(q), _ptr(qg), *(_ptr(b) for b in cache), _ptr(core), _ptr(weights),
+        _ptr(scratch.part_m), _ptr(scratch.part_l), _ptr(scratch.part_o), length, max_ctx,
+        n_splits, _ptr(scratch.ws), scratch.ws.numel(), _stream(stream)))
+    return n_splits
+
+
+def attn_decode_weights(q, qg, k_cache, v_cache, core, weights, scratch: DecodeWeightsScratch,
+                        length: int, max_ctx: int, n_splits: Optional[int] = None,
+                        stream=None) -> int:
+    """attn_decode (the same core, bit for bit) that also adds to weights[g, j], j < length, the
+    softmax weights that KV head g's 8 query heads give row j. Returns n_splits used."""
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _need(t, name, _cache_dtype(t), KV_HEADS * max_ctx * DIM)
+    return _decode_weights("miso_attn_decode_weights", q, qg, (k_cache, v_cache), core, weights,
+                           scratch, length, max_ctx, n_splits, stream)
+
+
+def attn_decode_weights_fp8(q, qg, cache: Fp8Cache, core, weights, scratch: DecodeWeightsScratch,
+                            length: int, n_splits: Optional[int] = None, stream=None) -> int:
+    """attn_decode_weights over an e4m3 cache (the core of attn_decode_fp8)."""
+    _need_fp8(cache)
+    return _decode_weights("miso_attn_decode_weights_fp8", q, qg, cache.buffers(), core, weights,
+                           scratch, length, cache.max_ctx, n_splits, stream)
+
+
+class PrefillWeightsScratch:
+    """Workspace of attn_prefill_weights for up to max_n tokens over up to max_rows cache rows (with
+    fp8, of attn_prefill_weights_fp8 too, which widens K rows into it): 16 KiB per token and
+    some MB."""
+
+    def __init__(self, max_n: int, max_rows: int, fp8: bool = False, device="cuda"):
+        self.max_n, self.max_rows = _count(max_n, "max_n"), _count(max_rows, "max_rows")
+        self.fp8 = fp8
+        nbytes = int(_lib.load().miso_attn_prefill_weights_workspace_bytes(max_n, max_rows,
+                                                                           int(fp8)))
+        self.ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _prefill_weights(name: str, q, cache, weights, pos0, n, max_ctx, scratch, stream) -> None:
+    pos0, n, max_ctx = _count(pos0, "pos0"), _count(n, "n"), _count(max_ctx, "max_ctx")
+    if n > scratch.max_n or pos0 + n > scratch.max_rows:
+        raise ValueError("n or pos0 + n exceeds the scratch capacity")
+    _need(q, "q", torch.float32, n * Q_HEADS * DIM)
+    _need(weights, "weights", torch.float32, KV_HEADS * max_ctx)
+    _here(q=q, k_cache=cache[0], weights=weights, scratch=scratch.ws)
+    _lib.check(getattr(_lib.load(), name)(
+        _ptr(q), *(_ptr(b) for b in cache), _ptr(weights), pos0, n, max_ctx, _ptr(scratch.ws),
+        scratch.ws.numel(), _stream(stream)))
+
+
+def attn_prefill_weights(q, k_cache, weights, pos0: int, n: int, max_ctx: int,
+                         scratch: PrefillWeightsScratch, stream=None) -> None:
+    """Adds to weights[g, j] the causal softmax weights that the n queries q ([n][16][256], as
+    attn_prep_batch writes them) at rows pos0 .. pos0 + n - 1 give row j <= their own. The last
+    tokens of a prompt alone may vote: their queries, and pos0 their first row."""
+    _need(k_cache, "k_cache", _cache_dtype(k_cache), KV_HEADS * max_ctx * DIM)
+    _prefill_weights("miso_attn_prefill_weights", q, (k_cache,), weights, pos0, n, max_ctx,
+                     scratch, stream)
+
+
+def attn_prefill_weights_fp8(q, cache: Fp8Cache, weights, pos0: int, n: int,
+                             scratch: PrefillWeightsScratch, stream=None) -> None:
+    """attn_prefill_weights over an e4m3 cache (scratch made with fp8=True)."""
+    if not scratch.fp8:
+        raise ValueError("the scratch was made without fp8=True")
+    _need_fp8(cache)
+    _prefill_weights("miso_attn_prefill_weights_fp8", q, (cache.k8, cache.k_scale), weights, pos0,
+                     n, cache.max_ctx, scratch, stream)
+
+
+class EvictScratch:
+    """Workspace of attn_evict_select for up to max_len rows."""
+
+    def __init__(self, max_len: int, device="cuda"):
+        self.max_len = _count(max_len, "max_len")
+        nbytes = int(_lib.load().miso_attn_evict_workspace_bytes(max_len))
+        self.ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def attn_evict_select(weights, length: int, max_ctx: int, keep: int, sinks: int, recent: int,
+                      index, scratch: EvictScratch, stream=None) -> None:
+    """Per KV head, the `keep` rows of [0, length) to keep, ascending, into index (int32
+    [2][keep]): the first `sinks`, the last `recent`, and the others of the largest weight; of
+    equal weights the lower rows (-0 equals +0, a NaN ranks below every number)."""
+    for name, x in (("length", length), ("max_ctx", max_ctx), ("keep", keep), ("sinks", sinks),
+                    ("recent", recent)):
+        _count(x, name)
+    if length > scratch.max_len:
+        raise ValueError("length exceeds the scratch capacity")
+    _need(weights, "weights", torch.float32, KV_HEADS * max_ctx)
+    _need(index, "index", torch.int32, KV_HEADS * keep)
+    _here(weights=weights, index=index, scratch=scratch.ws)
+    _lib.check(_lib.load().miso_attn_evict_select(
+        _ptr(weights), length, max_ctx, keep, sinks, recent, _ptr(index), _ptr(scratch.ws),
+        scratch.ws.numel(), _stream(stream)))
+
+
+def attn_evict_gather(k_cache, v_cache, weights, max_ctx: int, index, keep: int, k_out, v_out,
+                      weights_out, out_ctx: int, stream=None) -> None:
+    """Row index[g, j] of the source becomes row j < keep of the destination cache (out_ctx rows),
+    K, V and weight; the weights of the rows behind become 0, their K and V rows stay. Rows whose
+    index is outside the source become zero. The destination must not overlap the source."""
+    max_ctx, keep, out_ctx = (_count(max_ctx, "max_ctx"), _count(keep, "keep"),
+                              _count(out_ctx, "out_ctx"))
+    dtype = _cache_dtype(k_cache)
+    for name, t, rows in (("k_cache", k_cache, max_ctx), ("v_cache", v_cache, max_ctx),
+                          ("k_out", k_out, out_ctx), ("v_out", v_out, out_ctx)):
+        _need(t, name, dtype, KV_HEADS * rows * DIM)
+    _need(weights, "weights", torch.float32, KV_HEADS * max_ctx)
+    _need(weights_out, "weights_out", torch.float32, KV_HEADS * out_ctx)
+    _need(index, "index", torch.int32, KV_HEADS * keep)
+    _here(k_cache=k_cache, v_cache=v_cache, weights=weights, index=index, k_out=k_out, v_out=v_out,
+          weights_out=weights_out)
+    _lib.check(_lib.load().miso_attn_evict_gather(
+        _ptr(k_cache), _ptr(v_cache), _ptr(weights), max_ctx, _ptr(index), keep, _ptr(k_out),
+        _ptr(v_out), _ptr(weights_out), out_ctx, _stream(stream)))
+
+
+def attn_evict_gather_fp8(cache: Fp8Cache, weights, index, keep: int, out: Fp8Cache, weights_out,
+                          stream=None) -> None:
+    """attn_evict_gather from one e4m3 cache into another."""
+    _count(keep, "keep")
+    _need_fp8(cache)
+    _need_fp8(out)
+    _need(weights, "weights", torch.float32, KV_HEADS * cache.max_ctx)
+    _need(weights_out, "weights_out", torch.float32, KV_HEADS * out.max_ctx)
+    _need(index, "index", torch.int32, KV_HEADS * keep)
+    _here(cache=cache.k8, weights=weights, index=index, out=out.k8, weights_out=weights_out)
+    _lib.check(_lib.load().miso_attn_evict_gather_fp8(
+        *(_ptr(b) for b in cache.buffers()), _ptr(weights), cache.max_ctx, _ptr(index), keep,
+        *(_ptr(b) for b in out.buffers()), _ptr(weights_out), out.max_ctx, _stream(stream)))
 
 
 # ------------------------------------------------------------------------------------------------

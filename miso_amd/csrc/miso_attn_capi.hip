@@ -13,6 +13,7 @@
 #include "../../include/miso_attn.h"
 #include "attention_decode.hpp"
 #include "attention_decode_fp8.hpp"
+#include "attention_evict.hpp"
 #include "attention_prefill.hpp"
 #include "q4k_gemv.hpp"
 #include "q6k_gemv.hpp"
@@ -112,6 +113,17 @@ float* noalloc_scratch(const char* fn) {
 const half_t* as_half(const uint16_t* p) { return reinterpret_cast<const half_t*>(p); }
 half_t* as_half(uint16_t* p) { return reinterpret_cast<half_t*>(p); }
 
+// The preps append at cache row `pos`; for another row the cache pointers move by as many rows, so
+// that row pos of the moved cache is row `row` of the caller's (in both KV heads: the head stride
+// stays max_ctx). Only addresses inside the caller's cache are formed by the kernel.
+template <class T>
+T* moved_rows(T* cache, uint32_t row, uint32_t pos, int64_t row_elements) {
+  return reinterpret_cast<T*>(reinterpret_cast<uintptr_t>(cache) +
+                              static_cast<uintptr_t>((int64_t{row} - int64_t{pos}) *
+                                                     row_elements *
+                                                     static_cast<int64_t>(sizeof(T))));
+}
+
 }  // namespace
 
 extern "C" {
@@ -158,6 +170,57 @@ int miso_attn_prep_batch(const float* qg, const float* kp, const float* v, const
                                  proj_stride};
   k::attn_prep_batch_kernel<256><<<n * 18, 256, 0, as_stream(stream)>>>(p);
   return launched("miso_attn_prep_batch");
+}
+
+int miso_attn_prep_at(const float* qg, const float* kp, const float* v, const float* q_norm,
+                      const float* k_norm, const float* inv_freq, uint16_t* k_cache,
+                      uint16_t* v_cache, float* q, uint32_t pos, uint32_t row, uint32_t max_ctx,
+                      float eps, void* stream) {
+  constexpr const char* fn = "miso_attn_prep_at";
+  if (any_bad(qg, kp, v, q_norm, k_norm, inv_freq, k_cache, v_cache, q))
+    return fail(fn, kBadPtr);
+  if (row >= max_ctx)
+    return fail(fn, "KV cache is full (row >= max_ctx)");
+  const k::AttnPrepParams p{qg,
+                            kp,
+                            v,
+                            q_norm,
+                            k_norm,
+                            inv_freq,
+                            moved_rows(as_half(k_cache), row, pos, 256),
+                            moved_rows(as_half(v_cache), row, pos, 256),
+                            q,
+                            pos,
+                            max_ctx,
+                            eps};
+  k::attn_prep_kernel<256><<<18, 256, 0, as_stream(stream)>>>(p);
+  return launched(fn);
+}
+
+int miso_attn_prep_batch_at(const float* qg, const float* kp, const float* v, const float* q_norm,
+                            const float* k_norm, const float* inv_freq, uint16_t* k_cache,
+                            uint16_t* v_cache, float* q, uint32_t pos0, uint32_t row0,
+                            uint32_t max_ctx, float eps, uint32_t n, uint32_t proj_stride,
+                            void* stream) {
+  constexpr const char* fn = "miso_attn_prep_batch_at";
+  if (n == 0)
+    return 0;
+  if (any_bad(qg, kp, v, q_norm, k_norm, inv_freq, k_cache, v_cache, q))
+    return fail(fn, kBadPtr);
+  if (static_cast<uint64_t>(row0) + n > max_ctx)
+    return fail(fn, "KV cache is full (row0 + n > max_ctx)");
+  if (static_cast<uint64_t>(pos0) + n > 0xFFFFFFFFull)
+    return fail(fn, "pos0 + n passes 2^32");
+  if (proj_stride < 8192 + 1024)
+    return fail(fn, "proj_stride must cover [q+gate 8192 | k 512 | v 512]");
+  const k::AttnPrepBatchParams p{{qg, kp, v, q_norm, k_norm, inv_freq,
+                                  moved_rows(as_half(k_cache), row0, pos0, 256),
+                                  moved_rows(as_half(v_cache), row0, pos0, 256), q, pos0, max_ctx,
+                                  eps},
+                                 n,
+                                 proj_stride};
+  k::attn_prep_batch_kernel<256><<<n * 18, 256, 0, as_stream(stream)>>>(p);
+  return launched(fn);
 }
 
 int miso_attn_split(const float* q, const uint16_t* k_cache, const uint16_t* v_cache,
@@ -607,6 +670,62 @@ int miso_attn_prep_fp8(const float* qg, const float* kp, const float* v, const f
   return launched("miso_attn_prep_fp8");
 }
 
+int miso_attn_prep_at_fp8(const float* qg, const float* kp, const float* v, const float* q_norm,
+                          const float* k_norm, const float* inv_freq, uint8_t* k8, uint8_t* v8,
+                          float* k_scale, float* v_scale, float* q, uint32_t pos, uint32_t row,
+                          uint32_t max_ctx, float eps, void* stream) {
+  constexpr const char* fn = "miso_attn_prep_at_fp8";
+  if (any_bad(qg, kp, v, q_norm, k_norm, inv_freq, k8, v8, q) || bad_scalars(k_scale) ||
+      bad_scalars(v_scale))
+    return fail(fn, kBadPtr);
+  if (row >= max_ctx)
+    return fail(fn, "KV cache is full (row >= max_ctx)");
+  const k::AttnPrepFp8Params p{qg,
+                               kp,
+                               v,
+                               q_norm,
+                               k_norm,
+                               inv_freq,
+                               moved_rows(k8, row, pos, 256),
+                               moved_rows(v8, row, pos, 256),
+                               moved_rows(k_scale, row, pos, 1),
+                               moved_rows(v_scale, row, pos, 1),
+                               q,
+                               pos,
+                               max_ctx,
+                               eps};
+  k::attn_prep_fp8_kernel<256><<<18, 256, 0, as_stream(stream)>>>(p);
+  return launched(fn);
+}
+
+int miso_attn_prep_batch_at_fp8(const float* qg, const float* kp, const float* v,
+                                const float* q_norm, const float* k_norm, const float* inv_freq,
+                                uint8_t* k8, uint8_t* v8, float* k_scale, float* v_scale, float* q,
+                                uint32_t pos0, uint32_t row0, uint32_t max_ctx, float eps,
+                                uint32_t n, uint32_t proj_stride, void* stream) {
+  constexpr const char* fn = "miso_attn_prep_batch_at_fp8";
+  if (n == 0)
+    return 0;
+  if (any_bad(qg, kp, v, q_norm, k_norm, inv_freq, k8, v8, q) || bad_scalars(k_scale) ||
+      bad_scalars(v_scale))
+    return fail(fn, kBadPtr);
+  if (static_cast<uint64_t>(row0) + n > max_ctx)
+    return fail(fn, "KV cache is full (row0 + n > max_ctx)");
+  if (static_cast<uint64_t>(pos0) + n > 0xFFFFFFFFull)
+    return fail(fn, "pos0 + n passes 2^32");
+  if (proj_stride < 8192 + 1024)
+    return fail(fn, "proj_stride must cover [q+gate 8192 | k 512 | v 512]");
+  const k::AttnPrepBatchFp8Params p{{qg, kp, v, q_norm, k_norm, inv_freq,
+                                     moved_rows(k8, row0, pos0, 256),
+                                     moved_rows(v8, row0, pos0, 256),
+                                     moved_rows(k_scale, row0, pos0, 1),
+                                     moved_rows(v_scale, row0, pos0, 1), q, pos0, max_ctx, eps},
+                                    n,
+                                    proj_stride};
+  k::attn_prep_batch_fp8_kernel<256><<<n * 18, 256, 0, as_stream(stream)>>>(p);
+  return launched(fn);
+}
+
 int miso_attn_decode_fp8(const float* q, const float* qg, const uint8_t* k8, const uint8_t* v8,
                          const float* k_scale, const float* v_scale, float* core, float* part_m,
                          float* part_l, float* part_o, uint32_t len, uint32_t max_ctx,
@@ -908,6 +1027,260 @@ int miso_attn_layer_ingest(const miso_attn_layer* layer, uint16_t* k_cache, uint
                            eps, k::layer::decode_workspace(decode_ws),
                            k::layer::prefill_workspace(prefill_ws, max_tok), max_tok, chunk,
                            as_stream(stream)));
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------------------
+// A bounded KV cache: accumulated attention weights, the rows to keep, their move
+// ------------------------------------------------------------------------------------------------
+
+namespace {
+
+// The checks that both decodes with weights share; nullptr if the arguments are good.
+const char* bad_decode_weights(const float* weights, const void* workspace, uint64_t bytes,
+                               uint32_t len, uint32_t max_ctx, uint32_t n_splits) {
+  if (bad_scalars(weights) || bad_ptr(workspace))
+    return kBadPtr;
+  if (len == 0)
+    return "len must be >= 1";
+  if (len > max_ctx)
+    return "len exceeds max_ctx";
+  if (n_splits == 0)
+    return "n_splits must be >= 1";
+  if (bytes < miso_attn_decode_weights_workspace_bytes(len, n_splits))
+    return "workspace smaller than miso_attn_decode_weights_workspace_bytes(len, n_splits)";
+  return nullptr;
+}
+
+// The merge of the split's partials and of its scores.
+int combine_weights(const char* fn, const float* part_m, const float* part_l, const float* part_o,
+                    const float* qg, float* core, float* weights, const float* ws, uint32_t len,
+                    uint32_t max_ctx, uint32_t n_splits, void* stream) {
+  const k::AttnWeightsParams p{{part_m, part_l, part_o, qg, core, n_splits}, ws, weights, len,
+                               max_ctx};
+  const unsigned blocks = (len + k::kWeightKeys - 1) / k::kWeightKeys;
+  k::attn_combine_weights_kernel<><<<k::kCombineItems + 2 * blocks, 64, 0, as_stream(stream)>>>(p);
+  return launched(fn);
+}
+
+// Row indexes are read and written one at a time.
+bool bad_index(const int32_t* p) {
+  return p == nullptr || (reinterpret_cast<uintptr_t>(p) & 3u) != 0;
+}
+
+// Whether [a, a + bytes) and [b, b + more) share a byte.
+bool overlap(const void* a, uint64_t bytes, const void* b, uint64_t more) {
+  const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + more && y < x + bytes;
+}
+
+struct Range {
+  const void* at;
+  uint64_t bytes;
+};
+
+// Whether a destination shares memory with a source or with another destination.
+template <std::size_t S, std::size_t D>
+bool any_overlap(const Range (&src)[S], const Range (&dst)[D]) {
+  for (std::size_t i = 0; i < D; ++i) {
+    for (std::size_t j = 0; j < S; ++j)
+      if (overlap(dst[i].at, dst[i].bytes, src[j].at, src[j].bytes))
+        return true;
+    for (std::size_t j = 0; j < i; ++j)
+      if (overlap(dst[i].at, dst[i].bytes, dst[j].at, dst[j].bytes))
+        return true;
+  }
+  return false;
+}
+
+constexpr const char* kOverlap = "the destination overlaps the source or itself";
+
+const char* bad_gather(uint32_t max_ctx, uint32_t keep, uint32_t out_ctx) {
+  if (keep == 0)
+    return "keep must be >= 1";
+  if (keep > max_ctx)
+    return "keep exceeds max_ctx";
+  if (keep > out_ctx)
+    return "keep exceeds out_ctx";
+  return nullptr;
+}
+
+template <bool kFp8>
+int gather(const char* fn, const k::AttnEvictGatherParams& p, void* stream) {
+  const uint64_t groups = (uint64_t{2} * p.keep + 7) / 8;
+  k::attn_evict_gather_kernel<kFp8>
+      <<<static_cast<unsigned>(std::min<uint64_t>(groups, 1u << 20)), 256, 0, as_stream(stream)>>>(
+          p);
+  return launched(fn);
+}
+
+const char* bad_key_weights(const void* workspace, uint64_t bytes, uint32_t pos0, uint32_t n,
+                            uint32_t max_ctx, bool fp8) {
+  if (bad_ptr(workspace))
+    return kBadPtr;
+  if (n == 0)
+    return "n must be >= 1";
+  if (static_cast<uint64_t>(pos0) + n > max_ctx)
+    return "pos0 + n exceeds max_ctx";
+  if (max_ctx > 0x20000000u)
+    return "max_ctx must be at most 2^29";
+  if (bytes <
+      k::attn_key_weights_layout(pos0 + n, k::attn_key_weights_cut(pos0, n), fp8).bytes)
+    return "workspace smaller than miso_attn_prefill_weights_workspace_bytes";
+  return nullptr;
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t miso_attn_decode_weights_workspace_bytes(uint32_t max_len, uint32_t max_splits) {
+  return 4 * k::attn_decode_weights_floats(max_len, max_splits);
+}
+
+int miso_attn_decode_weights(const float* q, const float* qg, const uint16_t* k_cache,
+                             const uint16_t* v_cache, float* core, float* weights, float* part_m,
+                             float* part_l, float* part_o, uint32_t len, uint32_t max_ctx,
+                             uint32_t n_splits, void* workspace, uint64_t workspace_bytes,
+                             void* stream) {
+  constexpr const char* fn = "miso_attn_decode_weights";
+  if (any_bad(q, qg, k_cache, v_cache, core, part_o) || bad_scalars(part_m) ||
+      bad_scalars(part_l))
+    return fail(fn, kBadPtr);
+  if (const char* err =
+          bad_decode_weights(weights, workspace, workspace_bytes, len, max_ctx, n_splits))
+    return fail(fn, err);
+  float* const ws = static_cast<float*>(workspace);
+  const k::AttnSplitParams p{q,      as_half(k_cache), as_half(v_cache), part_m, part_l,
+                             part_o, len,              max_ctx,          n_splits};
+  k::attn_split_scores_kernel<256><<<dim3(n_splits, 2), 256, 0, as_stream(stream)>>>(p, ws);
+  if (const int rc = launched(fn))
+    return rc;
+  return combine_weights(fn, part_m, part_l, part_o, qg, core, weights, ws, len, max_ctx, n_splits,
+                         stream);
+}
+
+int miso_attn_decode_weights_fp8(const float* q, const float* qg, const uint8_t* k8,
+                                 const uint8_t* v8, const float* k_scale, const float* v_scale,
+                                 float* core, float* weights, float* part_m, float* part_l,
+                                 float* part_o, uint32_t len, uint32_t max_ctx, uint32_t n_splits,
+                                 void* workspace, uint64_t workspace_bytes, void* stream) {
+  constexpr const char* fn = "miso_attn_decode_weights_fp8";
+  if (any_bad(q, qg, k8, v8, core, part_o) || bad_scalars(k_scale) || bad_scalars(v_scale) ||
+      bad_scalars(part_m) || bad_scalars(part_l))
+    return fail(fn, kBadPtr);
+  if (const char* err =
+          bad_decode_weights(weights, workspace, workspace_bytes, len, max_ctx, n_splits))
+    return fail(fn, err);
+  float* const ws = static_cast<float*>(workspace);
+  const k::AttnSplitFp8Params p{q,      k8,     v8,  k_scale, v_scale, part_m,
+                                part_l, part_o, len, max_ctx, n_splits};
+  k::attn_split_fp8_scores_kernel<256><<<dim3(n_splits, 2), 256, 0, as_stream(stream)>>>(p, ws);
+  if (const int rc = launched(fn))
+    return rc;
+  return combine_weights(fn, part_m, part_l, part_o, qg, core, weights, ws, len, max_ctx, n_splits,
+                         stream);
+}
+
+uint64_t miso_attn_prefill_weights_workspace_bytes(uint32_t max_n, uint32_t max_rows, int fp8) {
+  return k::attn_key_weights_bytes(max_n, max_rows, fp8 != 0);
+}
+
+int miso_attn_prefill_weights(const float* q, const uint16_t* k_cache, float* weights,
+                              uint32_t pos0, uint32_t n, uint32_t max_ctx, void* workspace,
+                              uint64_t workspace_bytes, void* stream) {
+  constexpr const char* fn = "miso_attn_prefill_weights";
+  if (any_bad(q, k_cache) || bad_scalars(weights))
+    return fail(fn, kBadPtr);
+  if (const char* err = bad_key_weights(workspace, workspace_bytes, pos0, n, max_ctx, false))
+    return fail(fn, err);
+  k::attn_key_weights_launch(q, as_half(k_cache), nullptr, nullptr, weights, pos0, n, max_ctx,
+                             workspace, as_stream(stream));
+  return launched(fn);
+}
+
+int miso_attn_prefill_weights_fp8(const float* q, const uint8_t* k8, const float* k_scale,
+                                  float* weights, uint32_t pos0, uint32_t n, uint32_t max_ctx,
+                                  void* workspace, uint64_t workspace_bytes, void* stream) {
+  constexpr const char* fn = "miso_attn_prefill_weights_fp8";
+  if (any_bad(q, k8) || bad_scalars(k_scale) || bad_scalars(weights))
+    return fail(fn, kBadPtr);
+  if (const char* err = bad_key_weights(workspace, workspace_bytes, pos0, n, max_ctx, true))
+    return fail(fn, err);
+  k::attn_key_weights_launch(q, nullptr, k8, k_scale, weights, pos0, n, max_ctx, workspace,
+                             as_stream(stream));
+  return launched(fn);
+}
+
+uint64_t miso_attn_evict_workspace_bytes(uint32_t max_len) {
+  (void)max_len;
+  return 256;
+}
+
+int miso_attn_evict_select(const float* weights, uint32_t len, uint32_t max_ctx, uint32_t keep,
+                           uint32_t sinks, uint32_t recent, int32_t* index, void* workspace,
+                           uint64_t workspace_bytes, void* stream) {
+  constexpr const char* fn = "miso_attn_evict_select";
+  if (bad_scalars(weights) || bad_index(index) || bad_ptr(workspace))
+    return fail(fn, kBadPtr);
+  if (len > max_ctx)
+    return fail(fn, "len exceeds max_ctx");
+  if (len > 0x7FFFFFFFu)
+    return fail(fn, "len must be below 2^31");
+  if (keep == 0 || keep > len)
+    return fail(fn, "keep must be in [1, len]");
+  if (static_cast<uint64_t>(sinks) + recent > keep)
+    return fail(fn, "sinks + recent exceeds keep");
+  if (workspace_bytes < miso_attn_evict_workspace_bytes(len))
+    return fail(fn, "workspace smaller than miso_attn_evict_workspace_bytes(len)");
+  const k::AttnEvictSelectParams p{weights, index, len, max_ctx, keep, sinks, recent};
+  k::attn_evict_select_kernel<><<<2, 1024, 0, as_stream(stream)>>>(p);
+  return launched(fn);
+}
+
+int miso_attn_evict_gather(const uint16_t* k_cache, const uint16_t* v_cache, const float* weights,
+                           uint32_t max_ctx, const int32_t* index, uint32_t keep, uint16_t* k_out,
+                           uint16_t* v_out, float* weights_out, uint32_t out_ctx, void* stream) {
+  constexpr const char* fn = "miso_attn_evict_gather";
+  if (any_bad(k_cache, v_cache, k_out, v_out) || bad_index(index) || bad_scalars(weights) ||
+      bad_scalars(weights_out))
+    return fail(fn, kBadPtr);
+  if (const char* err = bad_gather(max_ctx, keep, out_ctx))
+    return fail(fn, err);
+  const uint64_t in = uint64_t{max_ctx} * 2, out = uint64_t{out_ctx} * 2;  // rows
+  const Range src[] = {{k_cache, in * 512}, {v_cache, in * 512}, {weights, in * 4},
+                       {index, uint64_t{keep} * 8}};
+  const Range dst[] = {{k_out, out * 512}, {v_out, out * 512}, {weights_out, out * 4}};
+  if (any_overlap(src, dst))
+    return fail(fn, kOverlap);
+  return gather<false>(fn, {k_cache, v_cache, weights, index, k_out, v_out, weights_out, max_ctx,
+                            keep, out_ctx, nullptr, nullptr, nullptr, nullptr},
+                       stream);
+}
+
+int miso_attn_evict_gather_fp8(const uint8_t* k8, const uint8_t* v8, const float* k_scale,
+                               const float* v_scale, const float* weights, uint32_t max_ctx,
+                               const int32_t* index, uint32_t keep, uint8_t* k8_out,
+                               uint8_t* v8_out, float* k_scale_out, float* v_scale_out,
+                               float* weights_out, uint32_t out_ctx, void* stream) {
+  constexpr const char* fn = "miso_attn_evict_gather_fp8";
+  if (any_bad(k8, v8, k8_out, v8_out) || bad_index(index) || bad_scalars(k_scale) ||
+      bad_scalars(v_scale) || bad_scalars(k_scale_out) || bad_scalars(v_scale_out) ||
+      bad_scalars(weights) || bad_scalars(weights_out))
+    return fail(fn, kBadPtr);
+  if (const char* err = bad_gather(max_ctx, keep, out_ctx))
+    return fail(fn, err);
+  const uint64_t in = uint64_t{max_ctx} * 2, out = uint64_t{out_ctx} * 2;  // rows
+  const Range src[] = {{k8, in * 256},     {v8, in * 256},    {k_scale, in * 4},
+                       {v_scale, in * 4},  {weights, in * 4}, {index, uint64_t{keep} * 8}};
+  const Range dst[] = {{k8_out, out * 256},     {v8_out, out * 256}, {k_scale_out, out * 4},
+                       {v_scale_out, out * 4},  {weights_out, out * 4}};
+  if (any_overlap(src, dst))
+    return fail(fn, kOverlap);
+  return gather<true>(fn, {k8, v8, weights, index, k8_out, v8_out, weights_out, max_ctx, keep,
+                           out_ctx, k_scale, v_scale, k_scale_out, v_scale_out},
+                      stream);
 }
 
 }  // extern "C"

@@ -1247,6 +1247,39 @@ __device__ __attribute__((always_inline)) inline void tile_scores_joined(
   }
 }
 
+// What a split writes beside its partial. NoScores (every decode): nothing. SplitScores (the decode
+// that accumulates attention weights): each score in log2 units, and the split's true maxima in the
+// same units, from which a second kernel forms the weights without the natural-log rounding of
+// part_m. A tile's scores are x + m with the m they were taken relative to; lanes c < 8 hold head
+// c's keys 4 g + i and 16 + 4 g + i, so each stores two 16-byte groups. Spans begin at multiples of
+// 8 and end at one or at len, so a group is wholly the span's or starts past it; only len's own
+// group is stored beyond len, into the row's padding.
+struct NoScores {
+  static constexpr bool kOn = false;
+};
+struct SplitScores {
+  static constexpr bool kOn = true;
+  float* s;          // the KV head's [8][stride], 16-byte aligned; stride a multiple of 4, >= len
+  std::size_t stride;
+  float* m2;         // as part_m, [2][n_splits][8], log2 units
+};
+template <class Scores>
+__device__ __attribute__((always_inline)) inline void store_scores(const Scores& sc,
+                                                                  const TileSoftmax& sm, float m,
+                                                                  unsigned k0, unsigned end,
+                                                                  unsigned lane) {
+  if constexpr (Scores::kOn) {
+    const unsigned c = lane & 15u, key = k0 + 4 * (lane >> 4);
+    float* row = sc.s + c * sc.stride + key;
+    if (c < 8 && key < end)
+      *reinterpret_cast<float4*>(row) =
+          float4{sm.x[0] + m, sm.x[1] + m, sm.x[2] + m, sm.x[3] + m};
+    if (c < 8 && key + 16 < end)
+      *reinterpret_cast<float4*>(row + 16) =
+          float4{sm.x[4] + m, sm.x[5] + m, sm.x[6] + m, sm.x[7] + m};
+  }
+}
+
 // The numerators p = 2^(x - shift) (times vr, the V row scale ratios, when kV), their sum (of the
 // unscaled p) and this lane's half of each as the P^T operand.
 template <bool kV>
@@ -1343,11 +1376,11 @@ __device__ __attribute__((always_inline)) inline void tile_rescale(TileSoftmax& 
 // kCoherent: the partial is stored with agent-coherent accesses (cache policy sc1, what a relaxed
 // agent-scope atomic access compiles to on gfx950), so a workgroup on another XCD can read it
 // after a counter hand-off (attn_decode_fused_kernel); `part_floats` bounds those stores.
-template <class Tiles, bool kCoherent = false, class Query = const float*>
+template <class Tiles, bool kCoherent = false, class Query = const float*, class Scores = NoScores>
 __device__ __attribute__((always_inline)) inline void split_partial_tiles(
     const Query& q, const Tiles& tl, AttnSpan span, unsigned kvh, float* part_m,
     float* part_l, float* part_o, std::size_t base, TileShared& sh, bool more,
-    unsigned part_floats = 0) {
+    unsigned part_floats = 0, const Scores& scores = Scores{}) {
   using cdna4::half8_t;
   const unsigned t = threadIdx.x, lane = t & 63u, g = lane >> 4, c = lane & 15u;
   const unsigned wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -1473,6 +1506,8 @@ __device__ __attribute__((always_inline)) inline void split_partial_tiles(
       tile_scores_joined<true>(sm, s_cur, st.m, k0, span.end, lane, tln);
     else
       tile_scores_joined<false>(sm, s_cur, st.m, k0, span.end, lane, tln);
+    if (Scores::kOn && ti % kWaves == wave)  // the four waves hold the same scores
+      store_scores(scores, sm, st.m, k0, span.end, lane);
   };
   for (unsigned ti = 0; ti + 1 < n_tiles; ++ti) {
     const unsigned ahead = n_tiles - 2 - ti;  // copies issued after tile ti + 1's
@@ -1555,6 +1590,8 @@ __device__ __attribute__((always_inline)) inline void split_partial_tiles(
       part_m[base * kGroup + h] = m_nat;
       part_l[base * kGroup + h] = L;
     }
+    if constexpr (Scores::kOn)
+      scores.m2[base * kGroup + h] = st.mt;
   }
   if (more)
     tile_barrier();  // LDS is reused by the next item
@@ -1758,13 +1795,15 @@ __device__ __attribute__((always_inline)) inline void wave_scores(f32x4 (&s)[2],
 
 // The softmax of one tile whose scores are s; keys k0 + key >= end are masked (only an item's
 // last tile reaches past it). first: the wave's first tile of the item.
+template <class Scores = NoScores>
 __device__ __attribute__((always_inline)) inline void wave_softmax(
     TileSoftmax& sm, WaveTileState& st, const f32x4 (&s)[2], unsigned k0, unsigned end,
-    bool first, unsigned lane, const TileLane& tln) {
+    bool first, unsigned lane, const TileLane& tln, const Scores& scores = Scores{}) {
   if (k0 + kTileKeys > end)  // uniform
     tile_scores_joined<true>(sm, s, st.m, k0, end, lane, tln);
   else
     tile_scores_joined<false>(sm, s, st.m, k0, end, lane, tln);
+  store_scores(scores, sm, st.m, k0, end, lane);
   const bool moved = tile_decide(sm, st, first, tln);
   if (moved)
     tile_rescale(sm, st, first, tln);
@@ -1884,12 +1923,14 @@ __device__ __attribute__((always_inline)) inline void wave_merge_out(
       wave_merge_o(ms, o);
 }
 
-__device__ __attribute__((always_inline)) inline void wave_merge_ml_out(const WaveMergeScale& ms,
-                                                                       unsigned h, float* part_m,
-                                                                       float* part_l,
-                                                                       std::size_t base) {
+template <class Scores = NoScores>
+__device__ __attribute__((always_inline)) inline void wave_merge_ml_out(
+    const WaveMergeScale& ms, unsigned h, float* part_m, float* part_l, std::size_t base,
+    const Scores& scores = Scores{}) {
   part_m[base * kGroup + h] = ms.m * kLn2;  // -inf stays -inf for an empty item
   part_l[base * kGroup + h] = ms.l;
+  if constexpr (Scores::kOn)
+    scores.m2[base * kGroup + h] = ms.m;
 }
 
 // Partial (m, l, o) of KV head kvh over keys [span.begin, span.end) at `base`, as
@@ -1897,10 +1938,11 @@ __device__ __attribute__((always_inline)) inline void wave_merge_ml_out(const Wa
 // four results merge at the end through the K slots (wave w's result in its own slot, which no
 // other wave reads before the merge barrier). `more`: the workgroup runs another item
 // afterwards (its LDS is then reused).
-template <class Tiles, class Query = const float*>
+template <class Tiles, class Query = const float*, class Scores = NoScores>
 __device__ __attribute__((always_inline)) inline void split_partial_waves(
     const Query& q, const Tiles& tl, AttnSpan span, unsigned kvh, float* part_m,
-    float* part_l, float* part_o, std::size_t base, TileShared& sh, bool more) {
+    float* part_l, float* part_o, std::size_t base, TileShared& sh, bool more,
+    const Scores& scores = Scores{}) {
   using cdna4::half8_t;
   const unsigned t = threadIdx.x, lane = t & 63u;
   const unsigned wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -1971,7 +2013,7 @@ __device__ __attribute__((always_inline)) inline void split_partial_waves(
     read_v_all(va, v_lds, op.vl);
     __builtin_amdgcn_sched_barrier(0);  // the V reads in flight under the softmax
     TileSoftmax sm;
-    wave_softmax(sm, st, s, span.begin + ti * kTileKeys, span.end, j == 0, lane, tln);
+    wave_softmax(sm, st, s, span.begin + ti * kTileKeys, span.end, j == 0, lane, tln, scores);
     if (next) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the V operands are in registers
       issue_v(ti + 4);
@@ -2001,7 +2043,7 @@ __device__ __attribute__((always_inline)) inline void split_partial_waves(
     wave_merge_out(area, kStride, ms, d, d, h, part_o, base);
     wave_merge_out(area, kStride, ms, d + 32, d + 32, h, part_o, base);
     if (d == 0)
-      wave_merge_ml_out(ms, h, part_m, part_l, base);
+      wave_merge_ml_out(ms, h, part_m, part_l, base, scores);
   }
   if (more)
     tile_barrier();  // LDS is reused by the next item

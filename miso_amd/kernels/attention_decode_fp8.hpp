@@ -430,10 +430,11 @@ __device__ __attribute__((always_inline)) inline void read_fp8_stage(Fp8Raw& raw
 // Partial (m, l, o) of keys [span.begin, span.end) of KV head kvh over e4m3 rows (K8 / V8 / KS /
 // VS: the KV head's bases) at `base`, in the reference's partial layout (m: natural-log max of
 // the scaled scores). `more`: the workgroup runs another item afterwards.
+template <class Scores = NoScores>
 __device__ __attribute__((always_inline)) inline void split_partial_fp8_waves(
     const float* __restrict__ q, const uint8_t* K8, const uint8_t* V8, const float* KS,
     const float* VS, AttnSpan span, unsigned kvh, float* part_m, float* part_l, float* part_o,
-    std::size_t base, Fp8WaveShared& sh, bool more) {
+    std::size_t base, Fp8WaveShared& sh, bool more, const Scores& scores = Scores{}) {
   using cdna4::half8_t;
   const unsigned t = threadIdx.x, lane = t & 63u, g = lane >> 4, c = lane & 15u;
   const unsigned wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -538,6 +539,7 @@ __device__ __attribute__((always_inline)) inline void split_partial_fp8_waves(
       tile_scores_joined<true, true>(sm, s, st.m, k0, span.end, lane, tln, ksc);
     else
       tile_scores_joined<false, true>(sm, s, st.m, k0, span.end, lane, tln, ksc);
+    store_scores(scores, sm, st.m, k0, span.end, lane);
     const bool first = j == 0;
     if (tile_decide<true>(sm, st, first, tln, vr))
       tile_rescale<true>(sm, st, first, tln, vr);
@@ -564,7 +566,7 @@ __device__ __attribute__((always_inline)) inline void split_partial_fp8_waves(
     wave_merge_out(area, kStride, ms, d, d, h, part_o, base);
     wave_merge_out(area, kStride, ms, d + 32, d + 32, h, part_o, base);
     if (d == 0)
-      wave_merge_ml_out(ms, h, part_m, part_l, base);
+      wave_merge_ml_out(ms, h, part_m, part_l, base, scores);
   }
   if (more)
     tile_barrier();  // LDS is reused by the next item
