@@ -189,13 +189,15 @@ struct AttnKeyWeightsParams {
   const attn::half_t* k_cache;   // [2][k_ctx][256]
   float* weights;                // [2][max_ctx]
   attn::half_t* halves;          // [2][blocks][2][16][64][8]
-  float* scale;                  // [2][32 blocks]: log2(e) / 16 over the row's power of two
-  float* lse;                    // [2][32 blocks], log2 units; +inf in the padding columns
-  float2* stats;                 // [row_parts][2][32 blocks]: (maximum, sum)
-  float* sums;                   // [col_parts][2][pos0 + n]
+  float* meta;                   // [2][blocks][32 scales, 32 lse]: a scale is log2(e) / 16 over the
+                                 // row's power of two, an lse in log2 units, +inf in padding columns
+  float2* stats;                 // [row parts][2][32 blocks]: (maximum, sum)
+  float* sums;                   // [column parts][2][pos0 + n]
   unsigned pos0, n, max_ctx, k_ctx;
   unsigned blocks;               // column blocks: ceil(n / 4)
-  unsigned row_parts, col_parts;
+  unsigned row_blocks;           // column blocks of a row pass workgroup, <= 8
+  unsigned row_tiles;            // key tiles of a row part
+  unsigned col_blocks;           // column blocks of a column part
 };
 
 namespace weights_detail {
@@ -277,73 +279,182 @@ __device__ __attribute__((always_inline)) inline void load_keys(cdna4::half8_t (
     a[s] = *reinterpret_cast<const cdna4::half8_t*>(at + 16 * s);
 }
 
+// Row pass: a ring of K tiles, chunk c of row r at position c ^ (r % 16) of the row (the A operand
+// read of 16 lanes takes one chunk of 16 rows: 16 positions).
+constexpr unsigned kRowWaves = 8, kRowStages = 4, kRowTileBytes = kKeys * attn::kDim * 2;
+struct alignas(1024) RowShared {
+  unsigned char k[kRowStages][kRowTileBytes];
+};
+
+// Column pass: a ring of column blocks' halves, as they lie in memory, and each wave's copy of the
+// block's scales and lse.
+constexpr unsigned kColWaves = 4, kColStages = 4;
+constexpr unsigned kColKeys = 2 * kKeys * kColWaves;  // keys of a workgroup, 64 a wave
+struct alignas(1024) ColShared {
+  unsigned char b[kColStages][kBlockHalves * 2];
+  float meta[kColStages][kColWaves][2 * kCols];
+};
+
+// 256 bytes, 4 per lane, to LDS.
+__device__ __attribute__((always_inline)) inline void lds_load4(const void* gaddr, unsigned lds) {
+  unsigned saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %1, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(gaddr), "s"(lds)
+      : "memory");
+}
+
+constexpr float kNoScore = -3e38f;  // below every score, and finite: differences stay numbers
+
+// The running maximum m and sum l (relative to it) of a lane's column over its 16 keys of a tile;
+// hidden keys are -inf.
+__device__ __attribute__((always_inline)) inline void add_tile(float& m, float& l,
+                                                              const cdna4::float16_t& x,
+                                                              float scale) {
+  float mx = x[0];
+#pragma unroll
+  for (int i = 1; i < 15; i += 2)
+    mx = decode_detail::tile_max3(mx, x[i], x[i + 1]);
+  mx = decode_detail::tile_max(mx, x[15]);
+  const float top = decode_detail::tile_max(m, mx * scale);
+  float part[4] = {l * __builtin_amdgcn_exp2f(m - top), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    part[i % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], scale, -top));
+  l = (part[0] + part[1]) + (part[2] + part[3]);
+  m = top;
+}
+
 }  // namespace weights_detail
 
-// Row pass: one wave per (KV head, column block, part of the keys), its columns' halves in
-// registers, 32 keys at a time straight from memory. Items are wave-sized; grid-stride, x 256.
+// Row pass. A workgroup takes `row_blocks` column blocks of one KV head (one a wave, its halves in
+// registers; further waves only copy) and one part of the keys they see, 32 at a time through LDS.
+// Items (part, group of blocks, KV head), the head fastest: an XCD's workgroups read one head's
+// keys, and about the same ones at a time. Iteration t forms the scores of tile t while the vector
+// units take tile t - 1 into the running sums.
 template <int = 0>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
 attn_key_weights_rows_kernel(AttnKeyWeightsParams p) {
   using namespace weights_detail;
+  __shared__ RowShared sh;
   const unsigned lane = threadIdx.x & 63u;
   const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned items = 2 * p.blocks * p.row_parts;
-  for (unsigned item = 4 * blockIdx.x + wave; item < items; item += 4 * gridDim.x) {
-    const unsigned kvh = item % 2, block = item / 2 % p.blocks, part = item / 2 / p.blocks;
-    const attn::half_t* K = p.k_cache + std::size_t{kvh} * p.k_ctx * attn::kDim;
-    Halves b;
-    const float scale = cut_column(b, p, kvh, block, lane);
-    const std::size_t col = (std::size_t{kvh} * p.blocks + block) * kCols + (lane & 31u);
+  const unsigned groups = (p.blocks + p.row_blocks - 1) / p.row_blocks;
+  const unsigned kvh = blockIdx.x % 2, group = blockIdx.x / 2 % groups;
+  const unsigned part = blockIdx.x / 2 / groups;
+  const unsigned block = group * p.row_blocks + wave;
+  // Keys the group's last token sees, and the part's tiles of them.
+  unsigned t_end = kTokens * (group + 1) * p.row_blocks;
+  t_end = t_end < p.n ? t_end : p.n;
+  const unsigned keys = p.pos0 + t_end, tiles = (keys + kKeys - 1) / kKeys;
+  const unsigned first = part * p.row_tiles;
+  if (first >= tiles)
+    return;
+  const unsigned past = first + p.row_tiles < tiles ? first + p.row_tiles : tiles;
+  const attn::half_t* K = p.k_cache + std::size_t{kvh} * p.k_ctx * attn::kDim;
+  const unsigned ring = cdna4::lds_offset(sh.k[0]);
+
+  // Tile ti into its stage: this wave copies rows 4 wave .. + 3, two an instruction.
+  auto issue = [&](unsigned ti) __attribute__((always_inline)) {
+#pragma unroll
+    for (unsigned i = 0; i < 2; ++i) {
+      const unsigned r = 4 * wave + 2 * i + (lane >> 5);
+      const unsigned row = ti * kKeys + r < keys ? ti * kKeys + r : keys - 1;
+      cdna4::lds_load16(K + std::size_t{row} * attn::kDim + 8 * ((lane & 31u) ^ (r & 15u)),
+                        ring + ti % kRowStages * kRowTileBytes + 512 * (4 * wave + 2 * i));
+    }
+  };
+#pragma unroll
+  for (unsigned i = 0; i < kRowStages - 1; ++i)
+    if (first + i < past)
+      issue(first + i);
+
+  const bool active = wave < p.row_blocks && block < p.blocks;  // wave-uniform
+  Halves b;
+  float scale = 0.0f;
+  const std::size_t at = std::size_t{kvh} * p.blocks + block;
+  if (active) {
+    scale = cut_column(b, p, kvh, block, lane);
     if (part == 0) {
-      attn::half_t* out = p.halves + (std::size_t{kvh} * p.blocks + block) * kBlockHalves + 8 * lane;
+      attn::half_t* out = p.halves + at * kBlockHalves + 8 * lane;
 #pragma unroll
       for (unsigned s = 0; s < kSteps; ++s) {
         *reinterpret_cast<cdna4::half8_t*>(out + 512 * s) = b.hi[s];
         *reinterpret_cast<cdna4::half8_t*>(out + 512 * (kSteps + s)) = b.lo[s];
       }
       if (lane < kCols)
-        p.scale[col] = scale;
+        p.meta[at * 2 * kCols + lane] = scale;
     }
-    // The block's last token sees keys [0, end); the lane's own token those up to `seen`.
-    const unsigned t = kTokens * block + (lane & 31u) / decode_detail::kGroup;
-    const unsigned t_last = kTokens * block + kTokens - 1 < p.n ? kTokens * block + kTokens - 1 : p.n - 1;
-    const unsigned seen = p.pos0 + (t < p.n ? t : p.n - 1), end = p.pos0 + t_last + 1;
-    const unsigned tiles = (end + kKeys - 1) / kKeys;
-    const unsigned per = (tiles + p.row_parts - 1) / p.row_parts;
-    const unsigned first = part * per, past = first + per < tiles ? first + per : tiles;
-    float m = -__builtin_inff(), l = 0.0f;
-    for (unsigned ti = first; ti < past; ++ti) {
-      const unsigned k0 = ti * kKeys;
-      cdna4::half8_t a[kSteps];
-      load_keys(a, K, k0, end - 1, lane);
-      cdna4::float16_t acc = {};
-#pragma unroll
-      for (unsigned s = 0; s < kSteps; ++s) {
-        acc = mfma32(a[s], b.hi[s], acc);
-        acc = mfma32(a[s], b.lo[s], acc);
-      }
-      float x[16], mx = -__builtin_inff();
-#pragma unroll
-      for (unsigned i = 0; i < 16; ++i) {
-        x[i] = k0 + tile_row(lane, i) <= seen ? acc[i] * scale : -__builtin_inff();
-        mx = fmaxf(mx, x[i]);
-      }
-      const float top = fmaxf(m, mx);
-      if (top != -__builtin_inff()) {
-        l *= __builtin_amdgcn_exp2f(m - top);
-#pragma unroll
-        for (unsigned i = 0; i < 16; ++i)
-          l += __builtin_amdgcn_exp2f(x[i] - top);
-        m = top;
-      }
-    }
-    // The two halves of the wave hold the other keys of the same columns.
-    const float top = cdna4::max_xor32(m);
-    const float mine = m == -__builtin_inff() ? 0.0f : l * __builtin_amdgcn_exp2f(m - top);
-    const float sum = cdna4::sum_xor32(mine);
-    if (lane < kCols)
-      p.stats[std::size_t{part} * 2 * p.blocks * kCols + col] = float2{top, sum};
   }
+  // Operand address of k-step s: row lane % 32, chunk 2 s + lane / 32, i.e. kl ^ 32 s.
+  const unsigned kl = 512 * (lane & 31u) + 16 * ((lane >> 5) ^ (lane & 15u));
+  const unsigned t = kTokens * block + (lane & 31u) / decode_detail::kGroup;
+  const unsigned seen = p.pos0 + t;                // the lane's token sees keys up to its own
+  const unsigned open = p.pos0 + kTokens * block;  // and every token of the block these
+  auto mask = [&](cdna4::float16_t& x, unsigned k0) __attribute__((always_inline)) {
+#pragma unroll
+    for (unsigned i = 0; i < 16; ++i)
+      x[i] = k0 + tile_row(lane, i) <= seen ? x[i] : -__builtin_inff();
+  };
+
+  float m = kNoScore, l = 0.0f;
+  cdna4::float16_t prev;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    prev[i] = -__builtin_inff();
+  for (unsigned ti = first; ti < past; ++ti) {
+    // Tile ti has landed: this wave's copies by the count, every wave's by the barrier, which also
+    // says that every wave has read tile ti - 1, whose stage the next copy takes.
+    const unsigned after = past - 1 - ti;
+    if (after >= 2)
+      cdna4::wait_vmcnt<4>();
+    else if (after == 1)
+      cdna4::wait_vmcnt<2>();
+    else
+      cdna4::wait_vmcnt<0>();
+    decode_detail::tile_barrier();
+    if (ti + kRowStages - 1 < past)
+      issue(ti + kRowStages - 1);
+    if (!active)
+      continue;
+    if (ti > first && ti * kKeys - 1 > open)  // the tile before reaches past what all see
+      mask(prev, (ti - 1) * kKeys);
+    const unsigned slot = ring + ti % kRowStages * kRowTileBytes + kl;
+    cdna4::float16_t acc = {};
+#pragma unroll
+    for (unsigned s = 0; s < kSteps; ++s) {
+      const cdna4::half8_t a = decode_detail::lds_b128(slot ^ (32u * s));
+      acc = mfma32(a, b.hi[s], acc);
+      acc = mfma32(a, b.lo[s], acc);
+    }
+    add_tile(m, l, prev, scale);
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (unsigned s = 0; s < kSteps; ++s) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+    }
+    prev = acc;
+  }
+  if (!active)
+    return;
+  if (past * kKeys - 1 > open)
+    mask(prev, (past - 1) * kKeys);
+  add_tile(m, l, prev, scale);
+  // The two halves of the wave hold the other keys of the same columns.
+  const float top = cdna4::max_xor32(m);
+  const float sum = cdna4::sum_xor32(l * __builtin_amdgcn_exp2f(m - top));
+  if (lane < kCols)
+    p.stats[(std::size_t{part} * 2 * p.blocks + at) * kCols + lane] = float2{top, sum};
 }
 
 // lse of every column from the row parts, in part order. One thread per column.
@@ -354,85 +465,166 @@ __global__ void __launch_bounds__(256) attn_key_weights_lse_kernel(AttnKeyWeight
   const std::size_t col = std::size_t{blockIdx.x} * 256 + threadIdx.x;
   if (col >= cols)
     return;
-  float m = -__builtin_inff(), l = 0.0f;
-  for (unsigned part = 0; part < p.row_parts; ++part)
+  const unsigned block = static_cast<unsigned>(col / kCols % p.blocks);
+  const unsigned t = kTokens * block + static_cast<unsigned>(col % kCols) / decode_detail::kGroup;
+  unsigned t_end = kTokens * (block / p.row_blocks + 1) * p.row_blocks;  // as the row pass
+  t_end = t_end < p.n ? t_end : p.n;
+  const unsigned parts = (p.pos0 + t_end + kKeys * p.row_tiles - 1) / (kKeys * p.row_tiles);
+  float m = kNoScore, l = 0.0f;
+  for (unsigned part = 0; part < parts; ++part)
     m = fmaxf(m, p.stats[part * cols + col].x);
-  for (unsigned part = 0; part < p.row_parts; ++part) {
+  for (unsigned part = 0; part < parts; ++part) {
     const float2 s = p.stats[part * cols + col];
-    l = __builtin_fmaf(s.y, s.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(s.x - m), l);
+    l = __builtin_fmaf(s.y, __builtin_amdgcn_exp2f(s.x - m), l);
   }
-  const unsigned t = static_cast<unsigned>(col % (std::size_t{p.blocks} * kCols)) / decode_detail::kGroup;
-  p.lse[col] = t < p.n ? m + __builtin_amdgcn_logf(l) : __builtin_inff();
+  p.meta[col / kCols * 2 * kCols + kCols + col % kCols] =
+      t < p.n ? m + __builtin_amdgcn_logf(l) : __builtin_inff();
 }
 
-// Column pass: one wave per (KV head, 32 keys, part of the column blocks), its keys in registers,
-// the columns' halves straight from memory. Grid-stride, x 256.
+// Column pass. A workgroup takes 256 keys of one KV head, 64 a wave, in registers, and one part of
+// the column blocks, whose halves come through LDS in the order of the operands. Iteration t forms
+// the scores of block t while the vector units turn block t - 1 into weights and sum them.
 template <int = 0>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
 attn_key_weights_cols_kernel(AttnKeyWeightsParams p) {
   using namespace weights_detail;
+  __shared__ ColShared sh;
   const unsigned lane = threadIdx.x & 63u;
   const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned rows = p.pos0 + p.n, tiles = (rows + kKeys - 1) / kKeys;
-  const unsigned items = 2 * tiles * p.col_parts;
-  for (unsigned item = 4 * blockIdx.x + wave; item < items; item += 4 * gridDim.x) {
-    const unsigned kvh = item % 2, tile = item / 2 % tiles, part = item / 2 / tiles;
-    const attn::half_t* K = p.k_cache + std::size_t{kvh} * p.k_ctx * attn::kDim;
-    const unsigned k0 = tile * kKeys;
-    cdna4::half8_t a[kSteps];
-    load_keys(a, K, k0, rows - 1, lane);
-    // Tokens before k0 - pos0 see none of these keys.
-    const unsigned b_min = k0 > p.pos0 ? (k0 - p.pos0) / kTokens : 0;
-    const unsigned per = (p.blocks - b_min + p.col_parts - 1) / p.col_parts;
-    const unsigned b0 = b_min + part * per;
-    const unsigned b1 = b0 + per < p.blocks ? b0 + per : p.blocks;
-    float sum[16] = {};
-    for (unsigned block = b0; block < b1; ++block) {
-      const std::size_t at = std::size_t{kvh} * p.blocks + block;
-      const attn::half_t* in = p.halves + at * kBlockHalves + 8 * lane;
-      cdna4::float16_t acc = {};
+  const unsigned rows = p.pos0 + p.n, key_blocks = (rows + kColKeys - 1) / kColKeys;
+  const unsigned kvh = blockIdx.x % 2, kb = blockIdx.x / 2 % key_blocks;
+  const unsigned part = blockIdx.x / 2 / key_blocks;
+  // Tokens before kb's first key see none of its keys.
+  const unsigned k_wg = kb * kColKeys;
+  const unsigned b_min = k_wg > p.pos0 ? (k_wg - p.pos0) / kTokens : 0;
+  const unsigned b1 = (part + 1) * p.col_blocks < p.blocks ? (part + 1) * p.col_blocks : p.blocks;
+  const unsigned b0 = part * p.col_blocks > b_min ? part * p.col_blocks : b_min;
+  if (b0 >= b1)
+    return;
+  const attn::half_t* halves = p.halves + std::size_t{kvh} * p.blocks * kBlockHalves;
+  const float* meta = p.meta + std::size_t{kvh} * p.blocks * 2 * kCols;
+  auto issue = [&](unsigned block) __attribute__((always_inline)) {
+    const unsigned stage = block % kColStages;
+    const attn::half_t* in = halves + block * kBlockHalves + 4096 * wave + 8 * lane;
+    const unsigned lds = cdna4::lds_offset(sh.b[stage]) + 8192 * wave;
 #pragma unroll
-      for (unsigned s = 0; s < kSteps; ++s) {
-        acc = mfma32(a[s], *reinterpret_cast<const cdna4::half8_t*>(in + 512 * s), acc);
-        acc = mfma32(a[s], *reinterpret_cast<const cdna4::half8_t*>(in + 512 * (kSteps + s)), acc);
-      }
-      const float scale = p.scale[at * kCols + (lane & 31u)];
-      const float lse = p.lse[at * kCols + (lane & 31u)];
-      const unsigned seen = p.pos0 + kTokens * block + (lane & 31u) / decode_detail::kGroup;
+    for (unsigned i = 0; i < 8; ++i)
+      cdna4::lds_load16(in + 512 * i, lds + 1024 * i);
+    lds_load4(meta + std::size_t{block} * 2 * kCols + lane,
+              cdna4::lds_offset(sh.meta[stage][wave]));
+  };
 #pragma unroll
-      for (unsigned i = 0; i < 16; ++i) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i], scale, -lse));
-        sum[i] += k0 + tile_row(lane, i) <= seen ? x : 0.0f;
-      }
+  for (unsigned i = 0; i < kColStages - 1; ++i)
+    if (b0 + i < b1)
+      issue(b0 + i);
+
+  const unsigned k0 = k_wg + 2 * kKeys * wave;  // the wave's first key
+  const attn::half_t* K = p.k_cache + std::size_t{kvh} * p.k_ctx * attn::kDim;
+  cdna4::half8_t a[2][kSteps];
+  load_keys(a[0], K, k0, rows - 1, lane);
+  load_keys(a[1], K, k0 + kKeys, rows - 1, lane);
+
+  float sum[2][16] = {};
+  cdna4::float16_t prev[2];
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    prev[0][i] = prev[1][i] = -__builtin_inff();
+  float scale = 1.0f, lse = 0.0f;  // of the block before
+  auto mask = [&](unsigned block) __attribute__((always_inline)) {
+    const unsigned seen = p.pos0 + kTokens * block + (lane & 31u) / decode_detail::kGroup;
+#pragma unroll
+    for (unsigned j = 0; j < 2; ++j)
+#pragma unroll
+      for (unsigned i = 0; i < 16; ++i)
+        prev[j][i] = k0 + kKeys * j + tile_row(lane, i) <= seen ? prev[j][i] : -__builtin_inff();
+  };
+  auto add = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (unsigned j = 0; j < 2; ++j)
+#pragma unroll
+      for (unsigned i = 0; i < 16; ++i)
+        sum[j][i] += __builtin_amdgcn_exp2f(__builtin_fmaf(prev[j][i], scale, -lse));
+  };
+  // Block b reaches keys that some of its tokens do not see.
+  auto cut = [&](unsigned b) { return k0 + 2 * kKeys - 1 > p.pos0 + kTokens * b; };
+  for (unsigned block = b0; block < b1; ++block) {
+    const unsigned after = b1 - 1 - block;  // as the row pass: 9 copies a block
+    if (after >= 2)
+      cdna4::wait_vmcnt<18>();
+    else if (after == 1)
+      cdna4::wait_vmcnt<9>();
+    else
+      cdna4::wait_vmcnt<0>();
+    decode_detail::tile_barrier();
+    if (block + kColStages - 1 < b1)
+      issue(block + kColStages - 1);
+    if (block > b0 && cut(block - 1))
+      mask(block - 1);
+    const unsigned stage = block % kColStages;
+    const unsigned slot = cdna4::lds_offset(sh.b[stage]) + 16 * lane;
+    cdna4::float16_t acc[2] = {};
+#pragma unroll
+    for (unsigned s = 0; s < kSteps; ++s) {
+      const cdna4::half8_t hi = decode_detail::lds_b128(slot + 1024 * s);
+      const cdna4::half8_t lo = decode_detail::lds_b128(slot + 1024 * (kSteps + s));
+      acc[0] = mfma32(a[0][s], hi, acc[0]);
+      acc[1] = mfma32(a[1][s], hi, acc[1]);
+      acc[0] = mfma32(a[0][s], lo, acc[0]);
+      acc[1] = mfma32(a[1][s], lo, acc[1]);
     }
-    // A key's sum over the 32 columns of its lanes.
+    add();
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+    for (unsigned s = 0; s < 2 * kSteps; ++s) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+    }
+    prev[0] = acc[0];
+    prev[1] = acc[1];
+    scale = sh.meta[stage][wave][lane & 31u];
+    lse = sh.meta[stage][wave][kCols + (lane & 31u)];
+  }
+  if (cut(b1 - 1))
+    mask(b1 - 1);
+  add();
+  // A key's sum over the 32 columns of its lanes.
+#pragma unroll
+  for (unsigned j = 0; j < 2; ++j)
 #pragma unroll
     for (unsigned i = 0; i < 16; ++i) {
-      float v = sum[i];
+      float v = sum[j][i];
       v += cdna4::dpp_mov<cdna4::kQuadXor1>(v);
       v += cdna4::dpp_mov<cdna4::kQuadXor2>(v);
       v += cdna4::dpp_mov<cdna4::kRowHalfMirror>(v);
       v += cdna4::dpp_mov<cdna4::kRowMirror>(v);
       v = cdna4::sum_xor16(v);
-      const unsigned key = k0 + tile_row(lane, i);
+      const unsigned key = k0 + kKeys * j + tile_row(lane, i);
       if ((lane & 31u) == 0 && key < rows) {
-        if (p.col_parts == 1)
+        if (p.col_blocks >= p.blocks)  // one part
           p.weights[std::size_t{kvh} * p.max_ctx + key] += v;
         else
           p.sums[(std::size_t{part} * 2 + kvh) * rows + key] = v;
       }
     }
-  }
 }
 
-// weights += the column parts' sums, in part order. One thread per key.
+// weights += the column parts' sums, in part order (the parts before a key's block was seen wrote
+// none). One thread per key.
 template <int = 0>
 __global__ void __launch_bounds__(256) attn_key_weights_join_kernel(AttnKeyWeightsParams p) {
+  using namespace weights_detail;
   const std::size_t rows = p.pos0 + p.n, i = std::size_t{blockIdx.x} * 256 + threadIdx.x;
   if (i >= 2 * rows)
     return;
+  const unsigned k_wg = static_cast<unsigned>(i % rows) / kColKeys * kColKeys;
+  const unsigned b_min = k_wg > p.pos0 ? (k_wg - p.pos0) / kTokens : 0;
+  const unsigned parts = (p.blocks + p.col_blocks - 1) / p.col_blocks;
   float v = 0.0f;
-  for (unsigned part = 0; part < p.col_parts; ++part)
+  for (unsigned part = b_min / p.col_blocks; part < parts; ++part)
     v += p.sums[part * 2 * rows + i];
   p.weights[(i / rows) * p.max_ctx + i % rows] += v;
 }
@@ -463,25 +655,38 @@ __global__ void __launch_bounds__(256) attn_k_fp8_widen_kernel(const uint8_t* k8
   }
 }
 
-// How a launch is cut: parts of the keys in the row pass, of the column blocks in the column pass,
-// so that there are some 2048 waves' items where the launch has the work for them.
+// How a launch is cut. A row workgroup takes up to 8 column blocks, evenly, and row_tiles key tiles
+// of 32; a column workgroup 256 keys and col_blocks column blocks. Both units of work, one tile for
+// 8 column blocks and one block for 256 keys, take 2048 matrix cycles of a CU.
 struct AttnKeyWeightsCut {
-  unsigned blocks, row_parts, col_parts;
+  unsigned blocks, row_blocks, row_tiles, row_parts, col_blocks, col_parts;
 };
+__host__ __device__ constexpr unsigned attn_key_weights_span(std::size_t units, unsigned most) {
+  const std::size_t span = (units + 1023) / 1024;  // about 4 workgroups per CU
+  return span < 4 ? 4u : span < most ? static_cast<unsigned>(span) : most;
+}
 __host__ __device__ constexpr AttnKeyWeightsCut attn_key_weights_cut(unsigned pos0, unsigned n) {
-  constexpr unsigned kItems = 2048, kMost = 128;
-  const unsigned blocks = (n + weights_detail::kTokens - 1) / weights_detail::kTokens;
-  const unsigned tiles = (pos0 + n + weights_detail::kKeys - 1) / weights_detail::kKeys;
-  unsigned row = (kItems + 2 * blocks - 1) / (2 * blocks);
-  row = row < tiles ? row : tiles;
-  unsigned col = (kItems + 2 * tiles - 1) / (2 * tiles);
-  col = col < blocks ? col : blocks;
-  return {blocks, row < kMost ? row : kMost, col < kMost ? col : kMost};
+  using namespace weights_detail;
+  const unsigned rows = pos0 + n, tiles = (rows + kKeys - 1) / kKeys;
+  AttnKeyWeightsCut c{};
+  c.blocks = (n + kTokens - 1) / kTokens;
+  const unsigned groups = (c.blocks + kRowWaves - 1) / kRowWaves;
+  c.row_blocks = (c.blocks + groups - 1) / groups;
+  // Of the n x n square of new keys half is seen.
+  const std::size_t row_units = std::size_t{groups} * (2 * std::size_t{pos0} + n) / kKeys;
+  const std::size_t col_units = std::size_t{c.blocks} * (2 * std::size_t{pos0} + n) / kColKeys;
+  c.row_tiles = attn_key_weights_span(row_units, 128);
+  c.col_blocks = attn_key_weights_span(col_units, 64);
+  c.row_tiles = c.row_tiles < tiles ? c.row_tiles : tiles;
+  c.col_blocks = c.col_blocks < c.blocks ? c.col_blocks : c.blocks;
+  c.row_parts = (tiles + c.row_tiles - 1) / c.row_tiles;
+  c.col_parts = (c.blocks + c.col_blocks - 1) / c.col_blocks;
+  return c;
 }
 
 // The workspace's parts, in bytes from its start, each 256-byte aligned.
 struct AttnKeyWeightsLayout {
-  std::size_t halves, scale, lse, stats, sums, k_wide, bytes;
+  std::size_t halves, meta, stats, sums, k_wide, bytes;
 };
 __host__ __device__ constexpr AttnKeyWeightsLayout attn_key_weights_layout(
     unsigned rows, const AttnKeyWeightsCut& cut, bool fp8) {
@@ -494,8 +699,7 @@ __host__ __device__ constexpr AttnKeyWeightsLayout attn_key_weights_layout(
     return was;
   };
   l.halves = take(2 * cut.blocks * weights_detail::kBlockHalves * sizeof(attn::half_t));
-  l.scale = take(cols * 4);
-  l.lse = take(cols * 4);
+  l.meta = take(cols * 8);
   l.stats = take(cols * 8 * cut.row_parts);
   l.sums = take(cut.col_parts > 1 ? std::size_t{2} * rows * 4 * cut.col_parts : 0);
   l.k_wide = take(fp8 ? std::size_t{2} * rows * attn::kDim * sizeof(attn::half_t) : 0);
@@ -503,18 +707,20 @@ __host__ __device__ constexpr AttnKeyWeightsLayout attn_key_weights_layout(
   return l;
 }
 
-// Bytes that serve every launch of up to max_n tokens (of them at least one) over up to max_rows
-// rows: each part at its own largest. Its parts: row_parts <= 128 and blocks * row_parts <= blocks
-// + 1024; col_parts <= 128 and tiles * col_parts <= tiles + 1024, 32 rows a tile.
+// Bytes that serve every launch of up to max_n tokens over up to max_rows rows, each part at its
+// largest. Blocks times row parts: where row_tiles is 128, at most blocks (tiles / 128 + 1); below,
+// row_tiles >= units / 1024 and units >= groups tiles less roundings, or row_tiles = 4 with at most
+// 4096 units, either way at most 16400 and 3 a block. Rows times column parts likewise: rows (blocks
+// / 64 + 1), or 256 keys a unit, 300000 and 2 a row.
 __host__ __device__ constexpr std::size_t attn_key_weights_bytes(unsigned max_n, unsigned max_rows,
                                                                  bool fp8) {
-  const std::size_t blocks = (std::size_t{max_n} + 3) / 4;
-  const std::size_t tiles = (std::size_t{max_rows} + 31) / 32;
-  const std::size_t cols = 2 * blocks * weights_detail::kCols;
-  const std::size_t row_items = blocks + 1024, col_items = tiles + 1024;
-  return 2 * blocks * weights_detail::kBlockHalves * sizeof(attn::half_t) + 2 * cols * 4 +
-         2 * row_items * weights_detail::kCols * 8 + 2 * col_items * 32 * 4 +
-         (fp8 ? std::size_t{2} * max_rows * attn::kDim * sizeof(attn::half_t) : 0) + 6 * 256;
+  using namespace weights_detail;
+  const std::size_t rows = max_rows, blocks = (std::size_t{max_n} + kTokens - 1) / kTokens;
+  const std::size_t row_items = blocks * (rows / (kKeys * 128) + 4) + 16400;
+  const std::size_t col_items = rows * (blocks / 64 + 3) + 300000;
+  return 2 * blocks * kBlockHalves * sizeof(attn::half_t) + 2 * blocks * kCols * 8 +
+         2 * row_items * kCols * 8 + 2 * col_items * 4 +
+         (fp8 ? 2 * rows * attn::kDim * sizeof(attn::half_t) : 0) + 5 * 256;
 }
 
 // The launches of a chunk whose arguments are good (workspace of at least the layout's bytes). k8 /
@@ -530,8 +736,7 @@ inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
                          k_cache,
                          weights,
                          reinterpret_cast<attn::half_t*>(ws + l.halves),
-                         reinterpret_cast<float*>(ws + l.scale),
-                         reinterpret_cast<float*>(ws + l.lse),
+                         reinterpret_cast<float*>(ws + l.meta),
                          reinterpret_cast<float2*>(ws + l.stats),
                          reinterpret_cast<float*>(ws + l.sums),
                          pos0,
@@ -539,9 +744,10 @@ inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
                          max_ctx,
                          max_ctx,
                          cut.blocks,
-                         cut.row_parts,
-                         cut.col_parts};
-  const unsigned rows = pos0 + n, tiles = (rows + 31) / 32;
+                         cut.row_blocks,
+                         cut.row_tiles,
+                         cut.col_blocks};
+  const unsigned rows = pos0 + n;
   if (k8 != nullptr) {
     attn::half_t* const wide = reinterpret_cast<attn::half_t*>(ws + l.k_wide);
     const unsigned grid = (2 * rows + 3) / 4;
@@ -550,9 +756,11 @@ inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
     p.k_cache = wide;
     p.k_ctx = rows;
   }
-  attn_key_weights_rows_kernel<><<<(2 * cut.blocks * cut.row_parts + 3) / 4, 256, 0, stream>>>(p);
+  const unsigned groups = (cut.blocks + cut.row_blocks - 1) / cut.row_blocks;
+  const unsigned key_blocks = (rows + weights_detail::kColKeys - 1) / weights_detail::kColKeys;
+  attn_key_weights_rows_kernel<><<<2 * groups * cut.row_parts, 512, 0, stream>>>(p);
   attn_key_weights_lse_kernel<><<<(64 * cut.blocks + 255) / 256, 256, 0, stream>>>(p);
-  attn_key_weights_cols_kernel<><<<(2 * tiles * cut.col_parts + 3) / 4, 256, 0, stream>>>(p);
+  attn_key_weights_cols_kernel<><<<2 * key_blocks * cut.col_parts, 256, 0, stream>>>(p);
   if (cut.col_parts > 1)
     attn_key_weights_join_kernel<><<<(2 * rows + 255) / 256, 256, 0, stream>>>(p);
 }
