@@ -1125,8 +1125,7 @@ const char* bad_key_weights(const void* workspace, uint64_t bytes, uint32_t pos0
     return "pos0 + n exceeds max_ctx";
   if (max_ctx > 0x20000000u)
     return "max_ctx must be at most 2^29";
-  if (bytes <
-      k::attn_key_weights_layout(pos0 + n, k::attn_key_weights_cut(pos0, n), fp8).bytes)
+  if (bytes < k::attn_key_weights_layout(pos0, n, fp8).bytes)
     return "workspace smaller than miso_attn_prefill_weights_workspace_bytes";
   return nullptr;
 }

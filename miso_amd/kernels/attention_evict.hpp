@@ -169,35 +169,42 @@ __global__ void __launch_bounds__(64) attn_combine_weights_kernel(AttnWeightsPar
 //
 // Queries q[t][h], t < n, at rows pos0 + t: weights[g][j] += sum over t and the heads h of g of
 // p[t][h][j], p the causal softmax over j <= pos0 + t. A weight needs its row's maximum and sum
-// before it can join its column's sum, so the products q k are formed twice: the row pass gives
-// each query's lse = M + log2 L, the column pass sums 2^(s - lse) over the queries. (Keeping the
-// scores instead would move 64 bytes per token and key through memory twice, against 1024 flop.)
+// before it can join its column's sum, so the products q k are formed twice: the first pass gives
+// each query's maximum and sum, the second sums 2^(s - lse) over the queries. (Keeping the scores
+// instead would move 64 bytes per token and key through memory twice, against 1024 flop.)
+//
 // A query is 32 bits wide and the matrix cores take 16: each row is scaled by the power of two that
 // puts its largest element in [2^13, 2^14), and cut into f16 halves x = hi + lo, exact to 2^-22 of
 // x, or 2^-38 of the row's largest element where lo is subnormal. hi k + lo k are exact products
-// summed in f32, the row's scale comes off in the exponent's fma. So a score costs 1024 flop of
+// summed in f32; the row's scale comes off in the exponent's fma. So a score costs 1024 flop of
 // f16 matrix work per pass, and the passes are bound by it once there are some hundred queries.
 //
-// A KV head's queries are columns c = 8 t + h % 8, in blocks of 32 (4 tokens): the B operand of
-// v_mfma_f32_32x32x16_f16, whose A operand is 32 K rows. The row pass writes the halves as the
-// column pass reads them: per KV head and block [hi, lo][k-step][lane][8], one lane's 16 bytes
-// after the other's.
+// A KV head's queries are columns c = 8 t + h % 8 in blocks of 32 (4 tokens). A wave holds one
+// block's halves in registers (128 VGPRs) and a workgroup of W waves, W blocks (a group), streams K
+// tiles of 32 rows through an LDS ring: one read of a K operand serves the hi and the lo product,
+// and the ring takes 64 of the 128 bytes a clock that LDS gives. Both passes have this form; in the
+// first a tile's result has the keys in registers and the columns in lanes (the running maximum and
+// sum stay in a lane), in the second the columns in registers and the keys in lanes (a key's sum
+// over the block is 16 adds).
+//
+// The work of a pass is the tiles of (KV head, group), laid end to end and cut into equal spans, one
+// per workgroup: causal groups differ in length, and a span takes up where the one before it ends.
 // ------------------------------------------------------------------------------------------------
 
 struct AttnKeyWeightsParams {
-  const float* q;                // [n][16][256]
-  const attn::half_t* k_cache;   // [2][k_ctx][256]
-  float* weights;                // [2][max_ctx]
-  attn::half_t* halves;          // [2][blocks][2][16][64][8]
-  float* meta;                   // [2][blocks][32 scales, 32 lse]: a scale is log2(e) / 16 over the
-                                 // row's power of two, an lse in log2 units, +inf in padding columns
-  float2* stats;                 // [row parts][2][32 blocks]: (maximum, sum)
-  float* sums;                   // [column parts][2][pos0 + n]
+  const float* q;               // [n][16][256]
+  const attn::half_t* k_cache;  // [2][k_ctx][256]
+  float* weights;               // [2][max_ctx]
+  attn::half_t* halves;         // [2][blocks][hi, lo][16][64][8], in the order of the operands
+  float* scale;                 // [2][blocks][32]: log2(e) / 16 over the row's power of two
+  float2* stats;                // [span + group][32 W]: a span's (maximum, sum) of a group's columns
+  float* sums;                  // [2][groups][row_tiles][32]: a group's sums of its keys
   unsigned pos0, n, max_ctx, k_ctx;
-  unsigned blocks;               // column blocks: ceil(n / 4)
-  unsigned row_blocks;           // column blocks of a row pass workgroup, <= 8
-  unsigned row_tiles;            // key tiles of a row part
-  unsigned col_blocks;           // column blocks of a column part
+  unsigned blocks;              // column blocks: ceil(n / 4)
+  unsigned groups;              // ceil(blocks / W)
+  unsigned row_tiles;           // tiles of 32 rows: ceil((pos0 + n) / 32)
+  unsigned spans;               // workgroups of a pass
+  unsigned long long span;      // tiles of one
 };
 
 namespace weights_detail {
@@ -206,107 +213,32 @@ constexpr unsigned kCols = 32, kKeys = 32, kSteps = 16;  // of a tile; k-steps o
 constexpr unsigned kTokens = kCols / decode_detail::kGroup;
 constexpr std::size_t kBlockHalves = 2 * kSteps * 64 * 8;  // one column block's halves
 
+__host__ __device__ constexpr unsigned div_up(unsigned a, unsigned b) {
+  return a / b + (a % b != 0);
+}
+
+// Tiles of group g, for W = 8 (32 tokens) and W = 4 (16): those up to the last row that a token of
+// its 32-token run sees. It may name one tile past the rows for the last groups, whose keys nobody
+// sees.
+__host__ __device__ constexpr unsigned group_tiles(unsigned W, unsigned pos0, unsigned g) {
+  return div_up(pos0, kKeys) + 1 + (W == 8 ? g : g / 2);
+}
+// Their sum over the groups before g.
+__host__ __device__ constexpr unsigned long long tiles_before(unsigned W, unsigned pos0,
+                                                              unsigned g) {
+  const unsigned long long x = g, h = g / 2;
+  return x * (div_up(pos0, kKeys) + 1) +
+         (W == 8 ? x * (x - (x != 0)) / 2 : h * (h - (h != 0)) + (g % 2 ? h : 0));
+}
+
 __device__ __attribute__((always_inline)) inline cdna4::float16_t mfma32(
     const cdna4::half8_t& a, const cdna4::half8_t& b, const cdna4::float16_t& c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// Row of a tile that a lane's result i belongs to.
+// Row of a tile's result that a lane's value i belongs to.
 __device__ __attribute__((always_inline)) inline unsigned tile_row(unsigned lane, unsigned i) {
   return 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
-}
-
-// This lane's halves of column lane % 32 of a block: dimensions 16 s + 8 (lane / 32) .. + 7.
-struct Halves {
-  cdna4::half8_t hi[kSteps], lo[kSteps];
-};
-
-// Reads and cuts the lane's column (zeros in the padding columns); returns the column's scale.
-__device__ __attribute__((always_inline)) inline float cut_column(Halves& b,
-                                                                 const AttnKeyWeightsParams& p,
-                                                                 unsigned kvh, unsigned block,
-                                                                 unsigned lane) {
-  const unsigned col = kCols * block + (lane & 31u);
-  const unsigned t = col / decode_detail::kGroup, h = col % decode_detail::kGroup;
-  const bool in = t < p.n;
-  const float* row = p.q + (std::size_t{in ? t : 0} * attn::kQHeads + kvh * decode_detail::kGroup +
-                            h) * attn::kDim + 8 * (lane >> 5);
-  float4 x[kSteps][2];
-#pragma unroll
-  for (unsigned s = 0; s < kSteps; ++s) {
-    x[s][0] = *reinterpret_cast<const float4*>(row + 16 * s);
-    x[s][1] = *reinterpret_cast<const float4*>(row + 16 * s + 4);
-  }
-  float top = 0.0f;
-#pragma unroll
-  for (unsigned s = 0; s < kSteps; ++s)
-#pragma unroll
-    for (unsigned j = 0; j < 2; ++j) {
-      if (!in)
-        x[s][j] = float4{0.0f, 0.0f, 0.0f, 0.0f};
-      top = fmaxf(top, fmaxf(fmaxf(__builtin_fabsf(x[s][j].x), __builtin_fabsf(x[s][j].y)),
-                             fmaxf(__builtin_fabsf(x[s][j].z), __builtin_fabsf(x[s][j].w))));
-    }
-  top = cdna4::max_xor32(top);
-  // 2^(13 - e), e the exponent of top; rows of zeros or beyond 2^-87 keep a finite factor, and one
-  // that holds an infinity stays as it is (its scores are infinite or NaN either way).
-  int e = 13 - (static_cast<int>(cdna4::as_uint(top) >> 23) - 127);
-  e = top == 0.0f || top == __builtin_inff() ? 0 : (e < 100 ? e : 100);
-  const float up = __builtin_ldexpf(1.0f, e);
-#pragma unroll
-  for (unsigned s = 0; s < kSteps; ++s) {
-    const float v[8] = {x[s][0].x, x[s][0].y, x[s][0].z, x[s][0].w,
-                        x[s][1].x, x[s][1].y, x[s][1].z, x[s][1].w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float y = v[j] * up;  // a power of two: exact
-      const _Float16 hi = static_cast<_Float16>(y);
-      b.hi[s][j] = hi;
-      b.lo[s][j] = static_cast<_Float16>(y - static_cast<float>(hi));
-    }
-  }
-  return __builtin_ldexpf(decode_detail::kLog2e / 16.0f, -e);
-}
-
-// K rows k0 + lane % 32 (clamped to `last`), as the A operand.
-__device__ __attribute__((always_inline)) inline void load_keys(cdna4::half8_t (&a)[kSteps],
-                                                               const attn::half_t* K, unsigned k0,
-                                                               unsigned last, unsigned lane) {
-  const unsigned row = k0 + (lane & 31u) < last ? k0 + (lane & 31u) : last;
-  const attn::half_t* at = K + std::size_t{row} * attn::kDim + 8 * (lane >> 5);
-#pragma unroll
-  for (unsigned s = 0; s < kSteps; ++s)
-    a[s] = *reinterpret_cast<const cdna4::half8_t*>(at + 16 * s);
-}
-
-// Row pass: a ring of K tiles, chunk c of row r at position c ^ (r % 16) of the row (the A operand
-// read of 16 lanes takes one chunk of 16 rows: 16 positions).
-constexpr unsigned kRowWaves = 8, kRowStages = 4, kRowTileBytes = kKeys * attn::kDim * 2;
-struct alignas(1024) RowShared {
-  unsigned char k[kRowStages][kRowTileBytes];
-};
-
-// Column pass: a ring of column blocks' halves, as they lie in memory, and each wave's copy of the
-// block's scales and lse.
-constexpr unsigned kColWaves = 4, kColStages = 4;
-constexpr unsigned kColKeys = 2 * kKeys * kColWaves;  // keys of a workgroup, 64 a wave
-struct alignas(1024) ColShared {
-  unsigned char b[kColStages][kBlockHalves * 2];
-  float meta[kColStages][kColWaves][2 * kCols];
-};
-
-// 256 bytes, 4 per lane, to LDS.
-__device__ __attribute__((always_inline)) inline void lds_load4(const void* gaddr, unsigned lds) {
-  unsigned saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %2\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dword %1, off\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "v"(gaddr), "s"(lds)
-      : "memory");
 }
 
 constexpr float kNoScore = -3e38f;  // below every score, and finite: differences stay numbers
@@ -330,303 +262,342 @@ __device__ __attribute__((always_inline)) inline void add_tile(float& m, float& 
   m = top;
 }
 
+// A ring of K tiles, chunk c of row r at position c ^ (r % 16) of the row (the operand read of 16
+// lanes takes one chunk of 16 rows: 16 positions); in the second pass, the waves' sums of a tile
+// and the columns' scales and lse.
+constexpr unsigned kStages = 4, kTileBytes = kKeys * attn::kDim * 2;
+template <unsigned W>
+struct alignas(1024) PassShared {
+  unsigned char k[kStages][kTileBytes];
+  float red[2][W][kKeys];
+  float scale[W][kCols], lse[W][kCols];
+};
+
+// This lane's halves of its block: column lane % 32, dimensions 16 s + 8 (lane / 32) .. + 7.
+struct Halves {
+  cdna4::half8_t hi[kSteps], lo[kSteps];
+};
+
 }  // namespace weights_detail
 
-// Row pass. A workgroup takes `row_blocks` column blocks of one KV head (one a wave, its halves in
-// registers; further waves only copy) and one part of the keys they see, 32 at a time through LDS.
-// Items (part, group of blocks, KV head), the head fastest: an XCD's workgroups read one head's
-// keys, and about the same ones at a time. Iteration t forms the scores of tile t while the vector
-// units take tile t - 1 into the running sums.
+// The queries' halves and scales. One wave per (KV head, column block), 4 per workgroup: lane l of
+// load (s, i) takes dimensions 16 s + 4 (l % 4) .. of column 16 i + l / 4, 64 bytes a row, and
+// stores the two halves of its four elements, 256 bytes together. Padding columns are zero.
 template <int = 0>
-__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
-attn_key_weights_rows_kernel(AttnKeyWeightsParams p) {
+__global__ void __launch_bounds__(256) attn_key_weights_cut_kernel(AttnKeyWeightsParams p) {
   using namespace weights_detail;
-  __shared__ RowShared sh;
+  const unsigned lane = threadIdx.x & 63u;
+  const unsigned item = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (item >= 2 * p.blocks)
+    return;
+  const unsigned kvh = item / p.blocks, block = item % p.blocks;
+  float4 x[2][kSteps];
+#pragma unroll
+  for (unsigned i = 0; i < 2; ++i) {
+    const unsigned c = 16 * i + lane / 4, t = kTokens * block + c / decode_detail::kGroup;
+    const float* row = p.q + (std::size_t{t < p.n ? t : 0} * attn::kQHeads +
+                              kvh * decode_detail::kGroup + c % decode_detail::kGroup) * attn::kDim;
+#pragma unroll
+    for (unsigned s = 0; s < kSteps; ++s)
+      x[i][s] = *reinterpret_cast<const float4*>(row + 16 * s + 4 * (lane % 4));
+  }
+  attn::half_t* out = p.halves + item * kBlockHalves;
+#pragma unroll
+  for (unsigned i = 0; i < 2; ++i) {
+    const unsigned c = 16 * i + lane / 4, t = kTokens * block + c / decode_detail::kGroup;
+    float top = 0.0f;
+#pragma unroll
+    for (unsigned s = 0; s < kSteps; ++s) {
+      if (t >= p.n)
+        x[i][s] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+      top = fmaxf(top, fmaxf(fmaxf(__builtin_fabsf(x[i][s].x), __builtin_fabsf(x[i][s].y)),
+                             fmaxf(__builtin_fabsf(x[i][s].z), __builtin_fabsf(x[i][s].w))));
+    }
+    top = fmaxf(top, cdna4::dpp_mov<cdna4::kQuadXor1>(top));
+    top = fmaxf(top, cdna4::dpp_mov<cdna4::kQuadXor2>(top));
+    // 2^(13 - e), e the exponent of top; rows of zeros or below 2^-87 keep a finite factor, and
+    // one that holds an infinity stays as it is (its scores are infinite or NaN either way).
+    int e = 13 - (static_cast<int>(cdna4::as_uint(top) >> 23) - 127);
+    e = top == 0.0f || top == __builtin_inff() ? 0 : (e < 100 ? e : 100);
+    const float up = __builtin_ldexpf(1.0f, e);
+    attn::half_t* at = out + 8 * (c + 32 * (lane / 2 % 2)) + 4 * (lane % 2);
+#pragma unroll
+    for (unsigned s = 0; s < kSteps; ++s) {
+      const float v[4] = {x[i][s].x, x[i][s].y, x[i][s].z, x[i][s].w};
+      cdna4::half4_t hi, lo;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float y = v[j] * up;  // a power of two: exact
+        hi[j] = static_cast<_Float16>(y);
+        lo[j] = static_cast<_Float16>(y - static_cast<float>(hi[j]));
+      }
+      *reinterpret_cast<cdna4::half4_t*>(at + 512 * s) = hi;
+      *reinterpret_cast<cdna4::half4_t*>(at + 512 * (kSteps + s)) = lo;
+    }
+    if (lane % 4 == 0)
+      p.scale[std::size_t{item} * kCols + c] = __builtin_ldexpf(decode_detail::kLog2e / 16.0f, -e);
+  }
+}
+
+// One span of a pass (kSum: the second), x 64 W, one workgroup of 8 waves or two of 4 per CU.
+// Iteration t of a segment (the span's tiles of one group) forms the scores of tile t while the
+// vector units work on those of tile t - 1.
+template <unsigned W, bool kSum>
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2)))
+attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
+  using namespace weights_detail;
+  using cdna4::float16_t;
+  __shared__ PassShared<W> sh;
   const unsigned lane = threadIdx.x & 63u;
   const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned groups = (p.blocks + p.row_blocks - 1) / p.row_blocks;
-  const unsigned kvh = blockIdx.x % 2, group = blockIdx.x / 2 % groups;
-  const unsigned part = blockIdx.x / 2 / groups;
-  const unsigned block = group * p.row_blocks + wave;
-  // Keys the group's last token sees, and the part's tiles of them.
-  unsigned t_end = kTokens * (group + 1) * p.row_blocks;
-  t_end = t_end < p.n ? t_end : p.n;
-  const unsigned keys = p.pos0 + t_end, tiles = (keys + kKeys - 1) / kKeys;
-  const unsigned first = part * p.row_tiles;
-  if (first >= tiles)
+  // Neighbouring spans on one XCD (blocks go round robin), so that its L2 serves one KV head.
+  const unsigned w = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+  if (w >= p.spans)
     return;
-  const unsigned past = first + p.row_tiles < tiles ? first + p.row_tiles : tiles;
-  const attn::half_t* K = p.k_cache + std::size_t{kvh} * p.k_ctx * attn::kDim;
-  const unsigned ring = cdna4::lds_offset(sh.k[0]);
-
-  // Tile ti into its stage: this wave copies rows 4 wave .. + 3, two an instruction.
-  auto issue = [&](unsigned ti) __attribute__((always_inline)) {
-#pragma unroll
-    for (unsigned i = 0; i < 2; ++i) {
-      const unsigned r = 4 * wave + 2 * i + (lane >> 5);
-      const unsigned row = ti * kKeys + r < keys ? ti * kKeys + r : keys - 1;
-      cdna4::lds_load16(K + std::size_t{row} * attn::kDim + 8 * ((lane & 31u) ^ (r & 15u)),
-                        ring + ti % kRowStages * kRowTileBytes + 512 * (4 * wave + 2 * i));
+  const unsigned long long per_head = tiles_before(W, p.pos0, p.groups);
+  unsigned long long x = w * p.span;
+  const unsigned long long x_end = x + p.span < 2 * per_head ? x + p.span : 2 * per_head;
+  unsigned kvh = x >= per_head;
+  unsigned group = 0, tile;
+  {  // the group that holds tile x - kvh per_head
+    const unsigned long long at = x - kvh * per_head;
+    unsigned past = p.groups;
+    while (past - group > 1) {
+      const unsigned mid = (group + past) / 2;
+      if (tiles_before(W, p.pos0, mid) <= at)
+        group = mid;
+      else
+        past = mid;
     }
-  };
-#pragma unroll
-  for (unsigned i = 0; i < kRowStages - 1; ++i)
-    if (first + i < past)
-      issue(first + i);
+    tile = static_cast<unsigned>(at - tiles_before(W, p.pos0, group));
+  }
+  const unsigned ring = cdna4::lds_offset(sh.k[0]);
+  const unsigned rows = p.pos0 + p.n;
+  const unsigned kl = 512 * (lane & 31u) + 16 * ((lane >> 5) ^ (lane & 15u));
 
-  const bool active = wave < p.row_blocks && block < p.blocks;  // wave-uniform
-  Halves b;
-  float scale = 0.0f;
-  const std::size_t at = std::size_t{kvh} * p.blocks + block;
-  if (active) {
-    scale = cut_column(b, p, kvh, block, lane);
-    if (part == 0) {
-      attn::half_t* out = p.halves + at * kBlockHalves + 8 * lane;
+  for (bool again = false; x < x_end; again = true) {
+    const unsigned tiles = group_tiles(W, p.pos0, group);
+    const unsigned first = tile;
+    const unsigned past = tiles - first < x_end - x ? tiles : first + static_cast<unsigned>(x_end - x);
+    const attn::half_t* K = p.k_cache + std::size_t{kvh} * p.k_ctx * attn::kDim;
+    // Tile ti into its stage: this wave copies rows 32 / W wave .. , two an instruction.
+    constexpr unsigned kCopies = kKeys / W / 2;
+    auto issue = [&](unsigned ti) __attribute__((always_inline)) {
+#pragma unroll
+      for (unsigned i = 0; i < kCopies; ++i) {
+        const unsigned r0 = kKeys / W * wave + 2 * i, r = r0 + (lane >> 5);
+        const unsigned row = ti * kKeys + r < rows ? ti * kKeys + r : rows - 1;
+        cdna4::lds_load16(K + std::size_t{row} * attn::kDim + 8 * ((lane & 31u) ^ (r & 15u)),
+                          ring + ti % kStages * kTileBytes + 512 * r0);
+      }
+    };
+    if (again)
+      decode_detail::tile_barrier();  // every wave is done with the segment before
+#pragma unroll
+    for (unsigned i = 0; i < kStages - 1; ++i)
+      if (first + i < past)
+        issue(first + i);
+
+    const unsigned block = group * W + wave;
+    const bool active = block < p.blocks;  // wave-uniform
+    const unsigned lin = kvh * p.groups + group;
+    Halves b;
+    float scale[kSum ? 16 : 1], lse[kSum ? 16 : 1];
+    if (active) {
+      const std::size_t at = std::size_t{kvh} * p.blocks + block;
+      const attn::half_t* in = p.halves + at * kBlockHalves + 8 * lane;
 #pragma unroll
       for (unsigned s = 0; s < kSteps; ++s) {
-        *reinterpret_cast<cdna4::half8_t*>(out + 512 * s) = b.hi[s];
-        *reinterpret_cast<cdna4::half8_t*>(out + 512 * (kSteps + s)) = b.lo[s];
+        b.hi[s] = *reinterpret_cast<const cdna4::half8_t*>(in + 512 * s);
+        b.lo[s] = *reinterpret_cast<const cdna4::half8_t*>(in + 512 * (kSteps + s));
       }
-      if (lane < kCols)
-        p.meta[at * 2 * kCols + lane] = scale;
-    }
-  }
-  // Operand address of k-step s: row lane % 32, chunk 2 s + lane / 32, i.e. kl ^ 32 s.
-  const unsigned kl = 512 * (lane & 31u) + 16 * ((lane >> 5) ^ (lane & 15u));
-  const unsigned t = kTokens * block + (lane & 31u) / decode_detail::kGroup;
-  const unsigned seen = p.pos0 + t;                // the lane's token sees keys up to its own
-  const unsigned open = p.pos0 + kTokens * block;  // and every token of the block these
-  auto mask = [&](cdna4::float16_t& x, unsigned k0) __attribute__((always_inline)) {
+      const float mine = p.scale[at * kCols + (lane & 31u)];
+      if constexpr (!kSum) {
+        scale[0] = mine;
+      } else {
+        // The column's lse from the spans that hold tiles of the group: each half of the wave takes
+        // every other one, 16 loads in flight (a short chunk over a long cache has a hundred).
+        const unsigned long long g0 = kvh * per_head + tiles_before(W, p.pos0, group);
+        const unsigned w0 = static_cast<unsigned>(g0 / p.span);
+        const unsigned w1 = static_cast<unsigned>((g0 + tiles - 1) / p.span);
+        const float2* st = p.stats + std::size_t{lin} * (W * kCols) + wave * kCols + (lane & 31u);
+        float m = kNoScore, l = 0.0f;
+        for (unsigned v0 = w0; v0 <= w1; v0 += 32) {  // wave-uniform
+          float2 one[16];
 #pragma unroll
-    for (unsigned i = 0; i < 16; ++i)
-      x[i] = k0 + tile_row(lane, i) <= seen ? x[i] : -__builtin_inff();
-  };
-
-  float m = kNoScore, l = 0.0f;
-  cdna4::float16_t prev;
+          for (unsigned i = 0; i < 16; ++i) {
+            const unsigned v = v0 + 2 * i + (lane >> 5);
+            one[i] = st[std::size_t{v <= w1 ? v : w0} * (W * kCols)];
+            if (v > w1)
+              one[i] = float2{kNoScore, 0.0f};
+          }
+          float top = m;
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    prev[i] = -__builtin_inff();
-  for (unsigned ti = first; ti < past; ++ti) {
-    // Tile ti has landed: this wave's copies by the count, every wave's by the barrier, which also
-    // says that every wave has read tile ti - 1, whose stage the next copy takes.
-    const unsigned after = past - 1 - ti;
-    if (after >= 2)
-      cdna4::wait_vmcnt<4>();
-    else if (after == 1)
-      cdna4::wait_vmcnt<2>();
-    else
-      cdna4::wait_vmcnt<0>();
-    decode_detail::tile_barrier();
-    if (ti + kRowStages - 1 < past)
-      issue(ti + kRowStages - 1);
-    if (!active)
-      continue;
-    if (ti > first && ti * kKeys - 1 > open)  // the tile before reaches past what all see
-      mask(prev, (ti - 1) * kKeys);
-    const unsigned slot = ring + ti % kRowStages * kRowTileBytes + kl;
-    cdna4::float16_t acc = {};
+          for (unsigned i = 0; i < 16; ++i)
+            top = fmaxf(top, one[i].x);
+          l *= __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
-    for (unsigned s = 0; s < kSteps; ++s) {
-      const cdna4::half8_t a = decode_detail::lds_b128(slot ^ (32u * s));
-      acc = mfma32(a, b.hi[s], acc);
-      acc = mfma32(a, b.lo[s], acc);
-    }
-    add_tile(m, l, prev, scale);
-    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+          for (unsigned i = 0; i < 16; ++i)
+            l = __builtin_fmaf(one[i].y, __builtin_amdgcn_exp2f(one[i].x - top), l);
+          m = top;
+        }
+        const float top = cdna4::max_xor32(m);
+        const float all = cdna4::sum_xor32(l * __builtin_amdgcn_exp2f(m - top));
+        const unsigned t = kTokens * block + (lane & 31u) / decode_detail::kGroup;
+        // Both halves of the wave write the same values.
+        sh.scale[wave][lane & 31u] = mine;
+        sh.lse[wave][lane & 31u] = t < p.n ? top + __builtin_amdgcn_logf(all) : __builtin_inff();
 #pragma unroll
-    for (unsigned s = 0; s < kSteps; ++s) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
-    }
-    prev = acc;
-  }
-  if (!active)
-    return;
-  if (past * kKeys - 1 > open)
-    mask(prev, (past - 1) * kKeys);
-  add_tile(m, l, prev, scale);
-  // The two halves of the wave hold the other keys of the same columns.
-  const float top = cdna4::max_xor32(m);
-  const float sum = cdna4::sum_xor32(l * __builtin_amdgcn_exp2f(m - top));
-  if (lane < kCols)
-    p.stats[(std::size_t{part} * 2 * p.blocks + at) * kCols + lane] = float2{top, sum};
-}
-
-// lse of every column from the row parts, in part order. One thread per column.
-template <int = 0>
-__global__ void __launch_bounds__(256) attn_key_weights_lse_kernel(AttnKeyWeightsParams p) {
-  using namespace weights_detail;
-  const std::size_t cols = std::size_t{2} * p.blocks * kCols;
-  const std::size_t col = std::size_t{blockIdx.x} * 256 + threadIdx.x;
-  if (col >= cols)
-    return;
-  const unsigned block = static_cast<unsigned>(col / kCols % p.blocks);
-  const unsigned t = kTokens * block + static_cast<unsigned>(col % kCols) / decode_detail::kGroup;
-  unsigned t_end = kTokens * (block / p.row_blocks + 1) * p.row_blocks;  // as the row pass
-  t_end = t_end < p.n ? t_end : p.n;
-  const unsigned parts = (p.pos0 + t_end + kKeys * p.row_tiles - 1) / (kKeys * p.row_tiles);
-  float m = kNoScore, l = 0.0f;
-  for (unsigned part = 0; part < parts; ++part)
-    m = fmaxf(m, p.stats[part * cols + col].x);
-  for (unsigned part = 0; part < parts; ++part) {
-    const float2 s = p.stats[part * cols + col];
-    l = __builtin_fmaf(s.y, __builtin_amdgcn_exp2f(s.x - m), l);
-  }
-  p.meta[col / kCols * 2 * kCols + kCols + col % kCols] =
-      t < p.n ? m + __builtin_amdgcn_logf(l) : __builtin_inff();
-}
-
-// Column pass. A workgroup takes 256 keys of one KV head, 64 a wave, in registers, and one part of
-// the column blocks, whose halves come through LDS in the order of the operands. Iteration t forms
-// the scores of block t while the vector units turn block t - 1 into weights and sum them.
-template <int = 0>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
-attn_key_weights_cols_kernel(AttnKeyWeightsParams p) {
-  using namespace weights_detail;
-  __shared__ ColShared sh;
-  const unsigned lane = threadIdx.x & 63u;
-  const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned rows = p.pos0 + p.n, key_blocks = (rows + kColKeys - 1) / kColKeys;
-  const unsigned kvh = blockIdx.x % 2, kb = blockIdx.x / 2 % key_blocks;
-  const unsigned part = blockIdx.x / 2 / key_blocks;
-  // Tokens before kb's first key see none of its keys.
-  const unsigned k_wg = kb * kColKeys;
-  const unsigned b_min = k_wg > p.pos0 ? (k_wg - p.pos0) / kTokens : 0;
-  const unsigned b1 = (part + 1) * p.col_blocks < p.blocks ? (part + 1) * p.col_blocks : p.blocks;
-  const unsigned b0 = part * p.col_blocks > b_min ? part * p.col_blocks : b_min;
-  if (b0 >= b1)
-    return;
-  const attn::half_t* halves = p.halves + std::size_t{kvh} * p.blocks * kBlockHalves;
-  const float* meta = p.meta + std::size_t{kvh} * p.blocks * 2 * kCols;
-  auto issue = [&](unsigned block) __attribute__((always_inline)) {
-    const unsigned stage = block % kColStages;
-    const attn::half_t* in = halves + block * kBlockHalves + 4096 * wave + 8 * lane;
-    const unsigned lds = cdna4::lds_offset(sh.b[stage]) + 8192 * wave;
-#pragma unroll
-    for (unsigned i = 0; i < 8; ++i)
-      cdna4::lds_load16(in + 512 * i, lds + 1024 * i);
-    lds_load4(meta + std::size_t{block} * 2 * kCols + lane,
-              cdna4::lds_offset(sh.meta[stage][wave]));
-  };
-#pragma unroll
-  for (unsigned i = 0; i < kColStages - 1; ++i)
-    if (b0 + i < b1)
-      issue(b0 + i);
-
-  const unsigned k0 = k_wg + 2 * kKeys * wave;  // the wave's first key
-  const attn::half_t* K = p.k_cache + std::size_t{kvh} * p.k_ctx * attn::kDim;
-  cdna4::half8_t a[2][kSteps];
-  load_keys(a[0], K, k0, rows - 1, lane);
-  load_keys(a[1], K, k0 + kKeys, rows - 1, lane);
-
-  float sum[2][16] = {};
-  cdna4::float16_t prev[2];
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    prev[0][i] = prev[1][i] = -__builtin_inff();
-  float scale = 1.0f, lse = 0.0f;  // of the block before
-  auto mask = [&](unsigned block) __attribute__((always_inline)) {
-    const unsigned seen = p.pos0 + kTokens * block + (lane & 31u) / decode_detail::kGroup;
-#pragma unroll
-    for (unsigned j = 0; j < 2; ++j)
-#pragma unroll
-      for (unsigned i = 0; i < 16; ++i)
-        prev[j][i] = k0 + kKeys * j + tile_row(lane, i) <= seen ? prev[j][i] : -__builtin_inff();
-  };
-  auto add = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (unsigned j = 0; j < 2; ++j)
-#pragma unroll
-      for (unsigned i = 0; i < 16; ++i)
-        sum[j][i] += __builtin_amdgcn_exp2f(__builtin_fmaf(prev[j][i], scale, -lse));
-  };
-  // Block b reaches keys that some of its tokens do not see.
-  auto cut = [&](unsigned b) { return k0 + 2 * kKeys - 1 > p.pos0 + kTokens * b; };
-  for (unsigned block = b0; block < b1; ++block) {
-    const unsigned after = b1 - 1 - block;  // as the row pass: 9 copies a block
-    if (after >= 2)
-      cdna4::wait_vmcnt<18>();
-    else if (after == 1)
-      cdna4::wait_vmcnt<9>();
-    else
-      cdna4::wait_vmcnt<0>();
-    decode_detail::tile_barrier();
-    if (block + kColStages - 1 < b1)
-      issue(block + kColStages - 1);
-    if (block > b0 && cut(block - 1))
-      mask(block - 1);
-    const unsigned stage = block % kColStages;
-    const unsigned slot = cdna4::lds_offset(sh.b[stage]) + 16 * lane;
-    cdna4::float16_t acc[2] = {};
-#pragma unroll
-    for (unsigned s = 0; s < kSteps; ++s) {
-      const cdna4::half8_t hi = decode_detail::lds_b128(slot + 1024 * s);
-      const cdna4::half8_t lo = decode_detail::lds_b128(slot + 1024 * (kSteps + s));
-      acc[0] = mfma32(a[0][s], hi, acc[0]);
-      acc[1] = mfma32(a[1][s], hi, acc[1]);
-      acc[0] = mfma32(a[0][s], lo, acc[0]);
-      acc[1] = mfma32(a[1][s], lo, acc[1]);
-    }
-    add();
-    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
-#pragma unroll
-    for (unsigned s = 0; s < 2 * kSteps; ++s) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
-    }
-    prev[0] = acc[0];
-    prev[1] = acc[1];
-    scale = sh.meta[stage][wave][lane & 31u];
-    lse = sh.meta[stage][wave][kCols + (lane & 31u)];
-  }
-  if (cut(b1 - 1))
-    mask(b1 - 1);
-  add();
-  // A key's sum over the 32 columns of its lanes.
-#pragma unroll
-  for (unsigned j = 0; j < 2; ++j)
-#pragma unroll
-    for (unsigned i = 0; i < 16; ++i) {
-      float v = sum[j][i];
-      v += cdna4::dpp_mov<cdna4::kQuadXor1>(v);
-      v += cdna4::dpp_mov<cdna4::kQuadXor2>(v);
-      v += cdna4::dpp_mov<cdna4::kRowHalfMirror>(v);
-      v += cdna4::dpp_mov<cdna4::kRowMirror>(v);
-      v = cdna4::sum_xor16(v);
-      const unsigned key = k0 + kKeys * j + tile_row(lane, i);
-      if ((lane & 31u) == 0 && key < rows) {
-        if (p.col_blocks >= p.blocks)  // one part
-          p.weights[std::size_t{kvh} * p.max_ctx + key] += v;
-        else
-          p.sums[(std::size_t{part} * 2 + kvh) * rows + key] = v;
+        for (unsigned i = 0; i < 16; ++i) {
+          scale[i] = sh.scale[wave][tile_row(lane, i)];
+          lse[i] = sh.lse[wave][tile_row(lane, i)];
+        }
       }
     }
+    const unsigned open = p.pos0 + kTokens * block;  // every token of the block sees keys up to it
+    float m = kNoScore, l = 0.0f;
+    float16_t prev;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      prev[i] = -__builtin_inff();
+
+    // The scores of tile ti, in prev, with the keys that a column does not see as -inf.
+    auto mask = [&](unsigned ti) __attribute__((always_inline)) {
+      if (ti * kKeys + kKeys - 1 <= open)  // wave-uniform
+        return;
+#pragma unroll
+      for (unsigned i = 0; i < 16; ++i) {
+        const unsigned key = ti * kKeys + (kSum ? lane & 31u : tile_row(lane, i));
+        const unsigned seen = open + (kSum ? i / 4 : (lane & 31u) / decode_detail::kGroup);
+        prev[i] = key <= seen ? prev[i] : -__builtin_inff();
+      }
+    };
+    float part[4];
+    auto work = [&]() __attribute__((always_inline)) {
+      if constexpr (!kSum) {
+        add_tile(m, l, prev, scale[0]);
+      } else {
+        part[0] = part[1] = part[2] = part[3] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          part[i % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(prev[i], scale[i], -lse[i]));
+      }
+    };
+    // A tile's sums: the wave's into LDS (`put`), and one wave's addition of all of them (`take`).
+    auto put = [&](unsigned ti) __attribute__((always_inline)) {
+      const float v = cdna4::sum_xor32((part[0] + part[1]) + (part[2] + part[3]));
+      if (lane < kKeys)
+        sh.red[ti % 2][wave][lane] = v;
+    };
+    auto take = [&](unsigned ti) __attribute__((always_inline)) {
+      if (ti % W != wave || ti >= p.row_tiles || lane >= kKeys)
+        return;
+      const unsigned count = p.blocks - group * W < W ? p.blocks - group * W : W;
+      float v = 0.0f;
+#pragma unroll
+      for (unsigned k = 0; k < W; ++k)
+        v += k < count ? sh.red[ti % 2][k][lane] : 0.0f;
+      p.sums[(std::size_t{lin} * p.row_tiles + ti) * kKeys + lane] = v;
+    };
+
+    for (unsigned ti = first; ti < past; ++ti) {
+      // Tile ti has landed: this wave's copies by the count, every wave's by the barrier, which
+      // also says that every wave has read tile ti - 1, whose stage the next copy takes.
+      const unsigned after = past - 1 - ti;
+      if (after >= 2)
+        cdna4::wait_vmcnt<2 * kCopies>();
+      else if (after == 1)
+        cdna4::wait_vmcnt<kCopies>();
+      else
+        cdna4::wait_vmcnt<0>();
+      decode_detail::tile_barrier();
+      if (ti + kStages - 1 < past)
+        issue(ti + kStages - 1);
+      if constexpr (kSum)
+        if (ti > first + 1)
+          take(ti - 2);
+      if (!active)
+        continue;
+      if (ti > first)
+        mask(ti - 1);
+      const unsigned slot = ring + ti % kStages * kTileBytes + kl;
+      float16_t acc = {};
+#pragma unroll
+      for (unsigned s = 0; s < kSteps; ++s) {
+        const cdna4::half8_t a = decode_detail::lds_b128(slot ^ (32u * s));
+        acc = kSum ? mfma32(b.hi[s], a, acc) : mfma32(a, b.hi[s], acc);
+        acc = kSum ? mfma32(b.lo[s], a, acc) : mfma32(a, b.lo[s], acc);
+      }
+      work();
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (unsigned s = 0; s < kSteps; ++s) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+      }
+      if constexpr (kSum)
+        if (ti > first)
+          put(ti - 1);
+      prev = acc;
+    }
+    if (active) {
+      mask(past - 1);
+      work();
+      if constexpr (kSum) {
+        put(past - 1);
+      } else {  // the two halves of the wave hold the other keys of the same columns
+        const float top = cdna4::max_xor32(m);
+        const float sum = cdna4::sum_xor32(l * __builtin_amdgcn_exp2f(m - top));
+        if (lane < kCols)
+          p.stats[(std::size_t{w} + lin) * (W * kCols) + wave * kCols + lane] = float2{top, sum};
+      }
+    }
+    if constexpr (kSum) {
+      decode_detail::tile_barrier();
+      if (past - first > 1)
+        take(past - 2);
+      take(past - 1);
+    }
+    x += past - first;
+    tile = past;
+    if (tile == tiles) {
+      tile = 0;
+      if (++group == p.groups) {
+        group = 0;
+        ++kvh;
+      }
+    }
+  }
 }
 
-// weights += the column parts' sums, in part order (the parts before a key's block was seen wrote
-// none). One thread per key.
-template <int = 0>
+// weights += the groups' sums, in a fixed order: one workgroup per (KV head, tile of rows), 8
+// slices of the groups that hold the tile, joined in slice order.
+template <unsigned W>
 __global__ void __launch_bounds__(256) attn_key_weights_join_kernel(AttnKeyWeightsParams p) {
   using namespace weights_detail;
-  const std::size_t rows = p.pos0 + p.n, i = std::size_t{blockIdx.x} * 256 + threadIdx.x;
-  if (i >= 2 * rows)
-    return;
-  const unsigned k_wg = static_cast<unsigned>(i % rows) / kColKeys * kColKeys;
-  const unsigned b_min = k_wg > p.pos0 ? (k_wg - p.pos0) / kTokens : 0;
-  const unsigned parts = (p.blocks + p.col_blocks - 1) / p.col_blocks;
+  __shared__ float part[8][kKeys];
+  const unsigned kvh = blockIdx.x / p.row_tiles, tile = blockIdx.x % p.row_tiles;
+  const unsigned lane = threadIdx.x % kKeys, slice = threadIdx.x / kKeys;
+  const unsigned base = div_up(p.pos0, kKeys);  // group_tiles(g) > tile from here on
+  const unsigned g0 = tile > base ? (tile - base) * (W == 8 ? 1 : 2) : 0;
+  const float* s = p.sums + (std::size_t{kvh} * p.groups * p.row_tiles + tile) * kKeys + lane;
   float v = 0.0f;
-  for (unsigned part = b_min / p.col_blocks; part < parts; ++part)
-    v += p.sums[part * 2 * rows + i];
-  p.weights[(i / rows) * p.max_ctx + i % rows] += v;
+#pragma unroll 4
+  for (unsigned g = g0 + slice; g < p.groups; g += 8)
+    v += s[std::size_t{g} * p.row_tiles * kKeys];
+  part[slice][lane] = v;
+  __syncthreads();
+  const unsigned key = tile * kKeys + lane;
+  if (slice != 0 || key >= p.pos0 + p.n)
+    return;
+#pragma unroll
+  for (unsigned i = 1; i < 8; ++i)
+    v += part[i][lane];
+  p.weights[std::size_t{kvh} * p.max_ctx + key] += v;
 }
 
 // K codes [2][max_ctx][256] widened to f16 [2][n][256] (attn_kv_fp8_widen_kernel's values, K alone).
@@ -655,42 +626,46 @@ __global__ void __launch_bounds__(256) attn_k_fp8_widen_kernel(const uint8_t* k8
   }
 }
 
-// How a launch is cut. A row workgroup takes up to 8 column blocks, evenly, and row_tiles key tiles
-// of 32; a column workgroup 256 keys and col_blocks column blocks. Both units of work, one tile for
-// 8 column blocks and one block for 256 keys, take 2048 matrix cycles of a CU.
+// How a chunk is cut: column blocks, the waves W of a workgroup (8: one workgroup per CU; 4: two, for
+// chunks whose last group of 8 would be mostly empty), the groups, and the spans of a pass.
 struct AttnKeyWeightsCut {
-  unsigned blocks, row_blocks, row_tiles, row_parts, col_blocks, col_parts;
+  unsigned blocks, waves, groups, row_tiles, spans;
+  unsigned long long span;
 };
-__host__ __device__ constexpr unsigned attn_key_weights_span(std::size_t units, unsigned most) {
-  const std::size_t span = (units + 1023) / 1024;  // about 4 workgroups per CU
-  return span < 4 ? 4u : span < most ? static_cast<unsigned>(span) : most;
-}
+constexpr unsigned kWeightsCus = 256;
 __host__ __device__ constexpr AttnKeyWeightsCut attn_key_weights_cut(unsigned pos0, unsigned n) {
   using namespace weights_detail;
-  const unsigned rows = pos0 + n, tiles = (rows + kKeys - 1) / kKeys;
   AttnKeyWeightsCut c{};
-  c.blocks = (n + kTokens - 1) / kTokens;
-  const unsigned groups = (c.blocks + kRowWaves - 1) / kRowWaves;
-  c.row_blocks = (c.blocks + groups - 1) / groups;
-  // Of the n x n square of new keys half is seen.
-  const std::size_t row_units = std::size_t{groups} * (2 * std::size_t{pos0} + n) / kKeys;
-  const std::size_t col_units = std::size_t{c.blocks} * (2 * std::size_t{pos0} + n) / kColKeys;
-  c.row_tiles = attn_key_weights_span(row_units, 128);
-  c.col_blocks = attn_key_weights_span(col_units, 64);
-  c.row_tiles = c.row_tiles < tiles ? c.row_tiles : tiles;
-  c.col_blocks = c.col_blocks < c.blocks ? c.col_blocks : c.blocks;
-  c.row_parts = (tiles + c.row_tiles - 1) / c.row_tiles;
-  c.col_parts = (c.blocks + c.col_blocks - 1) / c.col_blocks;
+  c.blocks = div_up(n, kTokens);
+  c.waves = c.blocks < 32 && (c.blocks - 1) % 8 < 4 ? 4 : 8;
+  c.groups = div_up(c.blocks, c.waves);
+  c.row_tiles = div_up(pos0 + n, kKeys);
+  const unsigned long long tiles = 2 * tiles_before(c.waves, pos0, c.groups);
+  const unsigned most = kWeightsCus * (8 / c.waves);
+  c.span = (tiles + most - 1) / most;
+  c.spans = static_cast<unsigned>((tiles + c.span - 1) / c.span);
   return c;
+}
+
+// A chunk runs in pieces of at most this many tokens, so that the groups' sums (8 bytes per group
+// and row) stay within 64 MiB over long caches.
+__host__ __device__ constexpr unsigned attn_key_weights_tokens(unsigned rows) {
+  const unsigned groups = (1u << 23) / (rows < 64 ? 64 : rows);
+  return 32 * (groups < 8 ? 8 : groups);
+}
+
+// The groups that a piece of up to `blocks` column blocks has at most.
+__host__ __device__ constexpr std::size_t attn_key_weights_groups(std::size_t blocks) {
+  return blocks < 32 ? blocks / 4 + 1 : blocks / 8 + 4;
 }
 
 // The workspace's parts, in bytes from its start, each 256-byte aligned.
 struct AttnKeyWeightsLayout {
-  std::size_t halves, meta, stats, sums, k_wide, bytes;
+  std::size_t halves, scale, stats, sums, k_wide, bytes;
 };
-__host__ __device__ constexpr AttnKeyWeightsLayout attn_key_weights_layout(
-    unsigned rows, const AttnKeyWeightsCut& cut, bool fp8) {
-  const std::size_t cols = std::size_t{2} * cut.blocks * weights_detail::kCols;
+__host__ __device__ constexpr AttnKeyWeightsLayout attn_key_weights_parts(
+    std::size_t blocks, std::size_t sums_floats, std::size_t wide_rows) {
+  using namespace weights_detail;
   AttnKeyWeightsLayout l{};
   std::size_t at = 0;
   auto take = [&](std::size_t bytes) {
@@ -698,71 +673,95 @@ __host__ __device__ constexpr AttnKeyWeightsLayout attn_key_weights_layout(
     at += (bytes + 255) / 256 * 256;
     return was;
   };
-  l.halves = take(2 * cut.blocks * weights_detail::kBlockHalves * sizeof(attn::half_t));
-  l.meta = take(cols * 8);
-  l.stats = take(cols * 8 * cut.row_parts);
-  l.sums = take(cut.col_parts > 1 ? std::size_t{2} * rows * 4 * cut.col_parts : 0);
-  l.k_wide = take(fp8 ? std::size_t{2} * rows * attn::kDim * sizeof(attn::half_t) : 0);
+  l.halves = take(2 * blocks * kBlockHalves * sizeof(attn::half_t));
+  l.scale = take(2 * blocks * kCols * 4);
+  // (spans + 2 groups) x 32 W columns, spans x W <= 8 x 256
+  l.stats = take((kWeightsCus + 2 * attn_key_weights_groups(blocks)) * 8 * kCols * sizeof(float2));
+  l.sums = take(sums_floats * 4);
+  l.k_wide = take(2 * wide_rows * attn::kDim * sizeof(attn::half_t));
   l.bytes = at;
   return l;
 }
 
-// Bytes that serve every launch of up to max_n tokens over up to max_rows rows, each part at its
-// largest. Blocks times row parts: where row_tiles is 128, at most blocks (tiles / 128 + 1); below,
-// row_tiles >= units / 1024 and units >= groups tiles less roundings, or row_tiles = 4 with at most
-// 4096 units, either way at most 16400 and 3 a block. Rows times column parts likewise: rows (blocks
-// / 64 + 1), or 256 keys a unit, 300000 and 2 a row.
+// Of one chunk.
+__host__ __device__ constexpr AttnKeyWeightsLayout attn_key_weights_layout(unsigned pos0, unsigned n,
+                                                                           bool fp8) {
+  using namespace weights_detail;
+  const unsigned rows = pos0 + n, most = attn_key_weights_tokens(rows);
+  const unsigned blocks = div_up(n < most ? n : most, kTokens);
+  return attn_key_weights_parts(
+      blocks,
+      2 * attn_key_weights_groups(blocks) * (std::size_t{div_up(rows, kKeys)} * kKeys),
+      fp8 ? rows : 0);
+}
+
+// Bytes that serve every chunk of up to max_n tokens over up to max_rows rows. A piece has at most
+// 16384 tokens (its tokens times its rows, at least as many, are at most 2^28); its groups are those
+// of max_n at most, or 12 more than what 2^23 group rows allow.
 __host__ __device__ constexpr std::size_t attn_key_weights_bytes(unsigned max_n, unsigned max_rows,
                                                                  bool fp8) {
   using namespace weights_detail;
-  const std::size_t rows = max_rows, blocks = (std::size_t{max_n} + kTokens - 1) / kTokens;
-  const std::size_t row_items = blocks * (rows / (kKeys * 128) + 4) + 16400;
-  const std::size_t col_items = rows * (blocks / 64 + 3) + 300000;
-  return 2 * blocks * kBlockHalves * sizeof(attn::half_t) + 2 * blocks * kCols * 8 +
-         2 * row_items * kCols * 8 + 2 * col_items * 4 +
-         (fp8 ? 2 * rows * attn::kDim * sizeof(attn::half_t) : 0) + 5 * 256;
+  const std::size_t blocks = div_up(max_n < 16384 ? max_n : 16384, kTokens);
+  const std::size_t rows = std::size_t{div_up(max_rows, kKeys)} * kKeys;
+  const std::size_t by_n = attn_key_weights_groups(blocks) * rows;
+  const std::size_t by_rows = (std::size_t{1} << 23) + 12 * (rows + 64);
+  return attn_key_weights_parts(blocks, 2 * (by_n < by_rows ? by_n : by_rows), fp8 ? max_rows : 0)
+      .bytes;
 }
 
-// The launches of a chunk whose arguments are good (workspace of at least the layout's bytes). k8 /
-// k_scale: the codes of an e4m3 cache of max_ctx rows (k_cache then unused), widened first.
+template <unsigned W>
+void attn_key_weights_passes(const AttnKeyWeightsParams& p, hipStream_t stream) {
+  const unsigned grid = (p.spans + 7) / 8 * 8;
+  attn_key_weights_cut_kernel<><<<(2 * p.blocks + 3) / 4, 256, 0, stream>>>(p);
+  attn_key_weights_pass_kernel<W, false><<<grid, 64 * W, 0, stream>>>(p);
+  attn_key_weights_pass_kernel<W, true><<<grid, 64 * W, 0, stream>>>(p);
+  attn_key_weights_join_kernel<W><<<2 * p.row_tiles, 256, 0, stream>>>(p);
+}
+
+// The launches of a chunk whose arguments are good, with a workspace of the bytes of its own layout
+// at least. k8 / k_scale: the codes of an e4m3 cache of max_ctx rows (k_cache then unused), widened
+// first.
 inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
                                     const uint8_t* k8, const float* k_scale, float* weights,
                                     unsigned pos0, unsigned n, unsigned max_ctx, void* workspace,
                                     hipStream_t stream) {
-  const AttnKeyWeightsCut cut = attn_key_weights_cut(pos0, n);
-  const AttnKeyWeightsLayout l = attn_key_weights_layout(pos0 + n, cut, k8 != nullptr);
-  char* const ws = static_cast<char*>(workspace);
-  AttnKeyWeightsParams p{q,
-                         k_cache,
-                         weights,
-                         reinterpret_cast<attn::half_t*>(ws + l.halves),
-                         reinterpret_cast<float*>(ws + l.meta),
-                         reinterpret_cast<float2*>(ws + l.stats),
-                         reinterpret_cast<float*>(ws + l.sums),
-                         pos0,
-                         n,
-                         max_ctx,
-                         max_ctx,
-                         cut.blocks,
-                         cut.row_blocks,
-                         cut.row_tiles,
-                         cut.col_blocks};
   const unsigned rows = pos0 + n;
+  const AttnKeyWeightsLayout l = attn_key_weights_layout(pos0, n, k8 != nullptr);
+  char* const ws = static_cast<char*>(workspace);
+  unsigned k_ctx = max_ctx;
   if (k8 != nullptr) {
     attn::half_t* const wide = reinterpret_cast<attn::half_t*>(ws + l.k_wide);
     const unsigned grid = (2 * rows + 3) / 4;
     attn_k_fp8_widen_kernel<><<<grid < 4096 ? grid : 4096, 256, 0, stream>>>(k8, k_scale, wide,
                                                                              rows, max_ctx);
-    p.k_cache = wide;
-    p.k_ctx = rows;
+    k_cache = wide;
+    k_ctx = rows;
   }
-  const unsigned groups = (cut.blocks + cut.row_blocks - 1) / cut.row_blocks;
-  const unsigned key_blocks = (rows + weights_detail::kColKeys - 1) / weights_detail::kColKeys;
-  attn_key_weights_rows_kernel<><<<2 * groups * cut.row_parts, 512, 0, stream>>>(p);
-  attn_key_weights_lse_kernel<><<<(64 * cut.blocks + 255) / 256, 256, 0, stream>>>(p);
-  attn_key_weights_cols_kernel<><<<2 * key_blocks * cut.col_parts, 256, 0, stream>>>(p);
-  if (cut.col_parts > 1)
-    attn_key_weights_join_kernel<><<<(2 * rows + 255) / 256, 256, 0, stream>>>(p);
+  const unsigned most = attn_key_weights_tokens(rows);
+  for (unsigned t = 0; t < n; t += most) {
+    const unsigned m = n - t < most ? n - t : most;
+    const AttnKeyWeightsCut cut = attn_key_weights_cut(pos0 + t, m);
+    const AttnKeyWeightsParams p{q + std::size_t{t} * attn::kQHeads * attn::kDim,
+                                 k_cache,
+                                 weights,
+                                 reinterpret_cast<attn::half_t*>(ws + l.halves),
+                                 reinterpret_cast<float*>(ws + l.scale),
+                                 reinterpret_cast<float2*>(ws + l.stats),
+                                 reinterpret_cast<float*>(ws + l.sums),
+                                 pos0 + t,
+                                 m,
+                                 max_ctx,
+                                 k_ctx,
+                                 cut.blocks,
+                                 cut.groups,
+                                 cut.row_tiles,
+                                 cut.spans,
+                                 cut.span};
+    if (cut.waves == 8)
+      attn_key_weights_passes<8>(p, stream);
+    else
+      attn_key_weights_passes<4>(p, stream);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
