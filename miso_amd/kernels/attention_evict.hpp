@@ -173,11 +173,13 @@ __global__ void __launch_bounds__(64) attn_combine_weights_kernel(AttnWeightsPar
 // each query's maximum and sum, the second sums 2^(s - lse) over the queries. (Keeping the scores
 // instead would move 64 bytes per token and key through memory twice, against 1024 flop.)
 //
-// A query is 32 bits wide and the matrix cores take 16: each row is scaled by the power of two that
-// puts its largest element in [2^13, 2^14), and cut into f16 halves x = hi + lo, exact to 2^-22 of
-// x, or 2^-38 of the row's largest element where lo is subnormal. hi k + lo k are exact products
-// summed in f32; the row's scale comes off in the exponent's fma. So a score costs 1024 flop of
-// f16 matrix work per pass, and the passes are bound by it once there are some hundred queries.
+// A query is 32 bits wide and the matrix cores take 16: each block of 32 columns is scaled by the
+// power of two that puts its largest element in [2^13, 2^14), and cut into f16 halves x = hi + lo,
+// exact to 2^-22 of x, or 2^-38 of the block's largest element where lo is subnormal (what counts
+// is a score's absolute error: beside a query element of 1000, that is 4e-9 per unit of K). hi k +
+// lo k are exact products summed in f32; the scale comes off in the exponent's fma. So a score
+// costs 1024 flop of f16 matrix work per pass, and the passes are bound by it once there are some
+// hundred queries.
 //
 // A KV head's queries are columns c = 8 t + h % 8 in blocks of 32 (4 tokens). A wave holds one
 // block's halves in registers (128 VGPRs) and a workgroup of W waves, W blocks (a group), streams K
@@ -196,7 +198,7 @@ struct AttnKeyWeightsParams {
   const attn::half_t* k_cache;  // [2][k_ctx][256]
   float* weights;               // [2][max_ctx]
   attn::half_t* halves;         // [2][blocks][hi, lo][16][64][8], in the order of the operands
-  float* scale;                 // [2][blocks][32]: log2(e) / 16 over the row's power of two
+  float* scale;                 // [2][blocks]: log2(e) / 16 over the block's power of two
   float2* stats;                // [span + group][32 W]: a span's (maximum, sum) of a group's columns
   float* sums;                  // [2][groups][row_tiles][32]: a group's sums of its keys
   unsigned pos0, n, max_ctx, k_ctx;
@@ -243,25 +245,6 @@ __device__ __attribute__((always_inline)) inline unsigned tile_row(unsigned lane
 
 constexpr float kNoScore = -3e38f;  // below every score, and finite: differences stay numbers
 
-// The running maximum m and sum l (relative to it) of a lane's column over its 16 keys of a tile;
-// hidden keys are -inf.
-__device__ __attribute__((always_inline)) inline void add_tile(float& m, float& l,
-                                                              const cdna4::float16_t& x,
-                                                              float scale) {
-  float mx = x[0];
-#pragma unroll
-  for (int i = 1; i < 15; i += 2)
-    mx = decode_detail::tile_max3(mx, x[i], x[i + 1]);
-  mx = decode_detail::tile_max(mx, x[15]);
-  const float top = decode_detail::tile_max(m, mx * scale);
-  float part[4] = {l * __builtin_amdgcn_exp2f(m - top), 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    part[i % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], scale, -top));
-  l = (part[0] + part[1]) + (part[2] + part[3]);
-  m = top;
-}
-
 // A ring of K tiles, chunk c of row r at position c ^ (r % 16) of the row (the operand read of 16
 // lanes takes one chunk of 16 rows: 16 positions); in the second pass, the waves' sums of a tile
 // and the columns' scales and lse.
@@ -269,8 +252,8 @@ constexpr unsigned kStages = 4, kTileBytes = kKeys * attn::kDim * 2;
 template <unsigned W>
 struct alignas(1024) PassShared {
   unsigned char k[kStages][kTileBytes];
-  float red[2][W][kKeys];
-  float scale[W][kCols], lse[W][kCols];
+  float red[2][W][64];
+  float lse[W][kCols];
 };
 
 // This lane's halves of its block: column lane % 32, dimensions 16 s + 8 (lane / 32) .. + 7.
@@ -301,26 +284,26 @@ __global__ void __launch_bounds__(256) attn_key_weights_cut_kernel(AttnKeyWeight
     for (unsigned s = 0; s < kSteps; ++s)
       x[i][s] = *reinterpret_cast<const float4*>(row + 16 * s + 4 * (lane % 4));
   }
-  attn::half_t* out = p.halves + item * kBlockHalves;
+  float top = 0.0f;
 #pragma unroll
-  for (unsigned i = 0; i < 2; ++i) {
-    const unsigned c = 16 * i + lane / 4, t = kTokens * block + c / decode_detail::kGroup;
-    float top = 0.0f;
+  for (unsigned i = 0; i < 2; ++i)
 #pragma unroll
     for (unsigned s = 0; s < kSteps; ++s) {
-      if (t >= p.n)
+      if (kTokens * block + (16 * i + lane / 4) / decode_detail::kGroup >= p.n)
         x[i][s] = float4{0.0f, 0.0f, 0.0f, 0.0f};
       top = fmaxf(top, fmaxf(fmaxf(__builtin_fabsf(x[i][s].x), __builtin_fabsf(x[i][s].y)),
                              fmaxf(__builtin_fabsf(x[i][s].z), __builtin_fabsf(x[i][s].w))));
     }
-    top = fmaxf(top, cdna4::dpp_mov<cdna4::kQuadXor1>(top));
-    top = fmaxf(top, cdna4::dpp_mov<cdna4::kQuadXor2>(top));
-    // 2^(13 - e), e the exponent of top; rows of zeros or below 2^-87 keep a finite factor, and
-    // one that holds an infinity stays as it is (its scores are infinite or NaN either way).
-    int e = 13 - (static_cast<int>(cdna4::as_uint(top) >> 23) - 127);
-    e = top == 0.0f || top == __builtin_inff() ? 0 : (e < 100 ? e : 100);
-    const float up = __builtin_ldexpf(1.0f, e);
-    attn::half_t* at = out + 8 * (c + 32 * (lane / 2 % 2)) + 4 * (lane % 2);
+  top = cdna4::wave_allmax(top);
+  // 2^(13 - e), e the exponent of top; blocks of zeros or below 2^-87 keep a finite factor, and one
+  // that holds an infinity stays as it is (its scores are infinite or NaN either way).
+  int e = 13 - (static_cast<int>(cdna4::as_uint(top) >> 23) - 127);
+  e = top == 0.0f || top == __builtin_inff() ? 0 : (e < 100 ? e : 100);
+  const float up = __builtin_ldexpf(1.0f, e);
+#pragma unroll
+  for (unsigned i = 0; i < 2; ++i) {
+    attn::half_t* at = p.halves + item * kBlockHalves +
+                       8 * (16 * i + lane / 4 + 32 * (lane / 2 % 2)) + 4 * (lane % 2);
 #pragma unroll
     for (unsigned s = 0; s < kSteps; ++s) {
       const float v[4] = {x[i][s].x, x[i][s].y, x[i][s].z, x[i][s].w};
@@ -334,9 +317,9 @@ __global__ void __launch_bounds__(256) attn_key_weights_cut_kernel(AttnKeyWeight
       *reinterpret_cast<cdna4::half4_t*>(at + 512 * s) = hi;
       *reinterpret_cast<cdna4::half4_t*>(at + 512 * (kSteps + s)) = lo;
     }
-    if (lane % 4 == 0)
-      p.scale[std::size_t{item} * kCols + c] = __builtin_ldexpf(decode_detail::kLog2e / 16.0f, -e);
   }
+  if (lane == 0)
+    p.scale[item] = __builtin_ldexpf(decode_detail::kLog2e / 16.0f, -e);
 }
 
 // One span of a pass (kSum: the second), x 64 W, one workgroup of 8 waves or two of 4 per CU.
@@ -402,7 +385,7 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
     const bool active = block < p.blocks;  // wave-uniform
     const unsigned lin = kvh * p.groups + group;
     Halves b;
-    float scale[kSum ? 16 : 1], lse[kSum ? 16 : 1];
+    float scale = 0.0f, lse[kSum ? 16 : 1];
     if (active) {
       const std::size_t at = std::size_t{kvh} * p.blocks + block;
       const attn::half_t* in = p.halves + at * kBlockHalves + 8 * lane;
@@ -411,10 +394,8 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
         b.hi[s] = *reinterpret_cast<const cdna4::half8_t*>(in + 512 * s);
         b.lo[s] = *reinterpret_cast<const cdna4::half8_t*>(in + 512 * (kSteps + s));
       }
-      const float mine = p.scale[at * kCols + (lane & 31u)];
-      if constexpr (!kSum) {
-        scale[0] = mine;
-      } else {
+      scale = p.scale[at];
+      if constexpr (kSum) {
         // The column's lse from the spans that hold tiles of the group: each half of the wave takes
         // every other one, 16 loads in flight (a short chunk over a long cache has a hundred).
         const unsigned long long g0 = kvh * per_head + tiles_before(W, p.pos0, group);
@@ -445,50 +426,62 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
         const float all = cdna4::sum_xor32(l * __builtin_amdgcn_exp2f(m - top));
         const unsigned t = kTokens * block + (lane & 31u) / decode_detail::kGroup;
         // Both halves of the wave write the same values.
-        sh.scale[wave][lane & 31u] = mine;
         sh.lse[wave][lane & 31u] = t < p.n ? top + __builtin_amdgcn_logf(all) : __builtin_inff();
 #pragma unroll
-        for (unsigned i = 0; i < 16; ++i) {
-          scale[i] = sh.scale[wave][tile_row(lane, i)];
+        for (unsigned i = 0; i < 16; ++i)
           lse[i] = sh.lse[wave][tile_row(lane, i)];
-        }
       }
     }
     const unsigned open = p.pos0 + kTokens * block;  // every token of the block sees keys up to it
+    // First pass: the column's sum l relative to the reference m, which follows the largest score
+    // only when that leads by more than 2^kLead (sums stay far inside f32's range, and the
+    // exponentials need not wait for a tile's maximum).
+    constexpr float kLead = 40.0f;
     float m = kNoScore, l = 0.0f;
-    float16_t prev;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      prev[i] = -__builtin_inff();
+    float part[4];
+    float16_t acc[2];
+    cdna4::half8_t a[4];  // the operands of the next four k-steps
 
-    // The scores of tile ti, in prev, with the keys that a column does not see as -inf.
-    auto mask = [&](unsigned ti) __attribute__((always_inline)) {
+    // The scores of tile ti with the keys that a column does not see as -inf.
+    auto mask = [&](float16_t& y, unsigned ti) __attribute__((always_inline)) {
       if (ti * kKeys + kKeys - 1 <= open)  // wave-uniform
         return;
 #pragma unroll
       for (unsigned i = 0; i < 16; ++i) {
         const unsigned key = ti * kKeys + (kSum ? lane & 31u : tile_row(lane, i));
         const unsigned seen = open + (kSum ? i / 4 : (lane & 31u) / decode_detail::kGroup);
-        prev[i] = key <= seen ? prev[i] : -__builtin_inff();
+        y[i] = key <= seen ? y[i] : -__builtin_inff();
       }
     };
-    float part[4];
-    auto work = [&]() __attribute__((always_inline)) {
-      if constexpr (!kSum) {
-        add_tile(m, l, prev, scale[0]);
-      } else {
-        part[0] = part[1] = part[2] = part[3] = 0.0f;
+    auto weight = [&](const float16_t& y, unsigned i) __attribute__((always_inline)) {
+      return __builtin_amdgcn_exp2f(__builtin_fmaf(y[i], scale, kSum ? -lse[kSum ? i : 0] : -m));
+    };
+    auto largest = [&](const float16_t& y) __attribute__((always_inline)) {
+      float mx = y[0];
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          part[i % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(prev[i], scale[i], -lse[i]));
+      for (int i = 1; i < 15; i += 2)
+        mx = decode_detail::tile_max3(mx, y[i], y[i + 1]);
+      return decode_detail::tile_max(mx, y[15]) * scale;
+    };
+    // After a tile's weights: its sums to LDS (second pass), or into l.
+    auto finish = [&](const float16_t& y, unsigned ti) __attribute__((always_inline)) {
+      if constexpr (kSum) {
+        sh.red[ti % 2][wave][lane] = (part[0] + part[1]) + (part[2] + part[3]);
+      } else {
+        const float mx = largest(y);
+        if (__builtin_amdgcn_ballot_w64(mx > m + kLead)) {  // rare, and every column's first tile
+          const float top = fmaxf(m, mx);
+          l *= __builtin_amdgcn_exp2f(m - top);
+          m = top;
+          part[0] = part[1] = part[2] = part[3] = 0.0f;
+#pragma unroll
+          for (unsigned i = 0; i < 16; ++i)
+            part[i % 4] += weight(y, i);
+        }
+        l += (part[0] + part[1]) + (part[2] + part[3]);
       }
     };
-    // A tile's sums: the wave's into LDS (`put`), and one wave's addition of all of them (`take`).
-    auto put = [&](unsigned ti) __attribute__((always_inline)) {
-      const float v = cdna4::sum_xor32((part[0] + part[1]) + (part[2] + part[3]));
-      if (lane < kKeys)
-        sh.red[ti % 2][wave][lane] = v;
-    };
+    // One wave's addition of every wave's sums of a tile.
     auto take = [&](unsigned ti) __attribute__((always_inline)) {
       if (ti % W != wave || ti >= p.row_tiles || lane >= kKeys)
         return;
@@ -496,17 +489,37 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
       float v = 0.0f;
 #pragma unroll
       for (unsigned k = 0; k < W; ++k)
-        v += k < count ? sh.red[ti % 2][k][lane] : 0.0f;
+        v += k < count ? sh.red[ti % 2][k][lane] + sh.red[ti % 2][k][lane + 32] : 0.0f;
       p.sums[(std::size_t{lin} * p.row_tiles + ti) * kKeys + lane] = v;
     };
-
-    for (unsigned ti = first; ti < past; ++ti) {
-      // Tile ti has landed: this wave's copies by the count, every wave's by the barrier, which
-      // also says that every wave has read tile ti - 1, whose stage the next copy takes.
-      const unsigned after = past - 1 - ti;
-      if (after >= 2)
-        cdna4::wait_vmcnt<2 * kCopies>();
-      else if (after == 1)
+    // K-step s of tile ti: the address is kl ^ 32 s of its stage; kl has no bit of 256.
+    auto read = [&](unsigned ti, unsigned s) __attribute__((always_inline)) {
+      return decode_detail::lds_b128((((ring + ti % kStages * kTileBytes) | kl) ^ (32u * (s % 8))) +
+                                     32u * (s & 8u));
+    };
+    // The scores of tile ti into cur and the weights of tile ti - 1, whose scores prev holds: a
+    // weight (fma, exponential, sum) to every two matrix instructions, in this order.
+    auto step = [&](float16_t& cur, float16_t& prev, unsigned ti) __attribute__((always_inline)) {
+      mask(prev, ti - 1);
+      part[0] = part[1] = part[2] = part[3] = 0.0f;
+#pragma unroll
+      for (unsigned s = 0; s < kSteps; ++s) {
+        __builtin_amdgcn_sched_barrier(0);
+        const cdna4::half8_t next = s + 4 < kSteps ? read(ti, s + 4) : read(ti + 1, s + 4 - kSteps);
+        const float16_t from = s == 0 ? float16_t{} : cur;
+        cur = kSum ? mfma32(b.hi[s], a[s % 4], from) : mfma32(a[s % 4], b.hi[s], from);
+        const float e = weight(prev, s);
+        cur = kSum ? mfma32(b.lo[s], a[s % 4], cur) : mfma32(a[s % 4], b.lo[s], cur);
+        a[s % 4] = next;
+        part[s % 4] += e;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // Tile ti + 1 has landed: this wave's copies by the count, every wave's by the barrier, which
+    // also says that every wave has read tile ti - 1, whose stage the next copy takes. So a wave
+    // reads the first operands of tile ti + 1 at the end of its tile ti.
+    auto turn = [&](unsigned ti) __attribute__((always_inline)) {
+      if (ti + 2 < past)
         cdna4::wait_vmcnt<kCopies>();
       else
         cdna4::wait_vmcnt<0>();
@@ -516,40 +529,46 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
       if constexpr (kSum)
         if (ti > first + 1)
           take(ti - 2);
-      if (!active)
-        continue;
-      if (ti > first)
-        mask(ti - 1);
-      const unsigned slot = ring + ti % kStages * kTileBytes + kl;
-      float16_t acc = {};
+    };
+
+    if (!active) {
+      for (unsigned ti = first; ti < past; ++ti)
+        turn(ti);
+    } else {
+      turn(first);
+#pragma unroll
+      for (unsigned s = 0; s < 4; ++s)
+        a[s] = read(first, s);
 #pragma unroll
       for (unsigned s = 0; s < kSteps; ++s) {
-        const cdna4::half8_t a = decode_detail::lds_b128(slot ^ (32u * s));
-        acc = kSum ? mfma32(b.hi[s], a, acc) : mfma32(a, b.hi[s], acc);
-        acc = kSum ? mfma32(b.lo[s], a, acc) : mfma32(a, b.lo[s], acc);
+        const cdna4::half8_t next = s + 4 < kSteps ? read(first, s + 4) : read(first + 1, s + 4 - kSteps);
+        const float16_t from = s == 0 ? float16_t{} : acc[0];
+        acc[0] = kSum ? mfma32(b.hi[s], a[s % 4], from) : mfma32(a[s % 4], b.hi[s], from);
+        acc[0] = kSum ? mfma32(b.lo[s], a[s % 4], acc[0]) : mfma32(a[s % 4], b.lo[s], acc[0]);
+        a[s % 4] = next;
       }
-      work();
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+      unsigned ti = first + 1;
+      for (; ti + 1 < past; ti += 2) {
+        turn(ti);
+        step(acc[1], acc[0], ti);
+        finish(acc[0], ti - 1);
+        turn(ti + 1);
+        step(acc[0], acc[1], ti + 1);
+        finish(acc[1], ti);
+      }
+      if (ti < past) {
+        turn(ti);
+        step(acc[1], acc[0], ti);
+        finish(acc[0], ti - 1);
+        acc[0] = acc[1];
+      }
+      mask(acc[0], past - 1);
+      part[0] = part[1] = part[2] = part[3] = 0.0f;
 #pragma unroll
-      for (unsigned s = 0; s < kSteps; ++s) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
-      }
-      if constexpr (kSum)
-        if (ti > first)
-          put(ti - 1);
-      prev = acc;
-    }
-    if (active) {
-      mask(past - 1);
-      work();
-      if constexpr (kSum) {
-        put(past - 1);
-      } else {  // the two halves of the wave hold the other keys of the same columns
+      for (unsigned i = 0; i < 16; ++i)
+        part[i % 4] += weight(acc[0], i);
+      finish(acc[0], past - 1);
+      if constexpr (!kSum) {  // the two halves of the wave hold the other keys of the same columns
         const float top = cdna4::max_xor32(m);
         const float sum = cdna4::sum_xor32(l * __builtin_amdgcn_exp2f(m - top));
         if (lane < kCols)
@@ -674,7 +693,7 @@ __host__ __device__ constexpr AttnKeyWeightsLayout attn_key_weights_parts(
     return was;
   };
   l.halves = take(2 * blocks * kBlockHalves * sizeof(attn::half_t));
-  l.scale = take(2 * blocks * kCols * 4);
+  l.scale = take(2 * blocks * 4);
   // (spans + 2 groups) x 32 W columns, spans x W <= 8 x 256
   l.stats = take((kWeightsCus + 2 * attn_key_weights_groups(blocks)) * 8 * kCols * sizeof(float2));
   l.sums = take(sums_floats * 4);
