@@ -246,15 +246,41 @@ __device__ __attribute__((always_inline)) inline unsigned tile_row(unsigned lane
 constexpr float kNoScore = -3e38f;  // below every score, and finite: differences stay numbers
 
 // A ring of K tiles, chunk c of row r at position c ^ (r % 16) of the row (the operand read of 16
-// lanes takes one chunk of 16 rows: 16 positions); in the second pass, the waves' sums of a tile
-// and the columns' scales and lse.
+// lanes takes one chunk of 16 rows: 16 positions); in the second pass, the waves' sums of W tiles,
+// twice, and the columns' lse.
 constexpr unsigned kStages = 4, kTileBytes = kKeys * attn::kDim * 2;
 template <unsigned W>
 struct alignas(1024) PassShared {
   unsigned char k[kStages][kTileBytes];
-  float red[2][W][64];
+  float red[2][W][W][64];  // [run of W tiles][tile][wave][lane]
   float lse[W][kCols];
 };
+
+// The statistics of N spans a wave half, v0 .. w1 at most, of a lane's column of group lin, joined
+// into (m, l): all loads in flight together.
+template <unsigned W, unsigned N>
+__device__ __attribute__((always_inline)) inline void add_stats(float& m, float& l,
+                                                               const float2* stats, unsigned lin,
+                                                               unsigned v0, unsigned w1,
+                                                               unsigned wave, unsigned lane) {
+  float2 one[N];
+#pragma unroll
+  for (unsigned i = 0; i < N; ++i) {
+    const unsigned v = v0 + 2 * i + (lane >> 5);  // 32-bit offsets: at most 512 + 2 groups slots
+    const unsigned at = ((v < w1 ? v : w1) + lin) * (W * kCols) + wave * kCols + (lane & 31u);
+    one[i] = stats[at];
+    one[i] = v <= w1 ? one[i] : float2{kNoScore, 0.0f};
+  }
+  float top = m;
+#pragma unroll
+  for (unsigned i = 0; i < N; ++i)
+    top = fmaxf(top, one[i].x);
+  l *= __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+  for (unsigned i = 0; i < N; ++i)
+    l = __builtin_fmaf(one[i].y, __builtin_amdgcn_exp2f(one[i].x - top), l);
+  m = top;
+}
 
 // This lane's halves of its block: column lane % 32, dimensions 16 s + 8 (lane / 32) .. + 7.
 struct Halves {
@@ -397,31 +423,17 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
       scale = p.scale[at];
       if constexpr (kSum) {
         // The column's lse from the spans that hold tiles of the group: each half of the wave takes
-        // every other one, 16 loads in flight (a short chunk over a long cache has a hundred).
+        // every other one, in its order; a long chunk has a few of them, a short one over a long
+        // cache a hundred.
         const unsigned long long g0 = kvh * per_head + tiles_before(W, p.pos0, group);
         const unsigned w0 = static_cast<unsigned>(g0 / p.span);
         const unsigned w1 = static_cast<unsigned>((g0 + tiles - 1) / p.span);
-        const float2* st = p.stats + std::size_t{lin} * (W * kCols) + wave * kCols + (lane & 31u);
         float m = kNoScore, l = 0.0f;
-        for (unsigned v0 = w0; v0 <= w1; v0 += 32) {  // wave-uniform
-          float2 one[16];
-#pragma unroll
-          for (unsigned i = 0; i < 16; ++i) {
-            const unsigned v = v0 + 2 * i + (lane >> 5);
-            one[i] = st[std::size_t{v <= w1 ? v : w0} * (W * kCols)];
-            if (v > w1)
-              one[i] = float2{kNoScore, 0.0f};
-          }
-          float top = m;
-#pragma unroll
-          for (unsigned i = 0; i < 16; ++i)
-            top = fmaxf(top, one[i].x);
-          l *= __builtin_amdgcn_exp2f(m - top);
-#pragma unroll
-          for (unsigned i = 0; i < 16; ++i)
-            l = __builtin_fmaf(one[i].y, __builtin_amdgcn_exp2f(one[i].x - top), l);
-          m = top;
-        }
+        if (w1 - w0 < 4)
+          add_stats<W, 2>(m, l, p.stats, lin, w0, w1, wave, lane);
+        else
+          for (unsigned v = w0; v <= w1; v += 32)
+            add_stats<W, 16>(m, l, p.stats, lin, v, w1, wave, lane);
         const float top = cdna4::max_xor32(m);
         const float all = cdna4::sum_xor32(l * __builtin_amdgcn_exp2f(m - top));
         const unsigned t = kTokens * block + (lane & 31u) / decode_detail::kGroup;
@@ -453,8 +465,11 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
         y[i] = key <= seen ? y[i] : -__builtin_inff();
       }
     };
+    auto exponent = [&](const float16_t& y, unsigned i) __attribute__((always_inline)) {
+      return __builtin_fmaf(y[i], scale, kSum ? -lse[kSum ? i : 0] : -m);
+    };
     auto weight = [&](const float16_t& y, unsigned i) __attribute__((always_inline)) {
-      return __builtin_amdgcn_exp2f(__builtin_fmaf(y[i], scale, kSum ? -lse[kSum ? i : 0] : -m));
+      return __builtin_amdgcn_exp2f(exponent(y, i));
     };
     auto largest = [&](const float16_t& y) __attribute__((always_inline)) {
       float mx = y[0];
@@ -466,7 +481,7 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
     // After a tile's weights: its sums to LDS (second pass), or into l.
     auto finish = [&](const float16_t& y, unsigned ti) __attribute__((always_inline)) {
       if constexpr (kSum) {
-        sh.red[ti % 2][wave][lane] = (part[0] + part[1]) + (part[2] + part[3]);
+        sh.red[ti / W % 2][ti % W][wave][lane] = (part[0] + part[1]) + (part[2] + part[3]);
       } else {
         const float mx = largest(y);
         if (__builtin_amdgcn_ballot_w64(mx > m + kLead)) {  // rare, and every column's first tile
@@ -481,39 +496,58 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
         l += (part[0] + part[1]) + (part[2] + part[3]);
       }
     };
-    // One wave's addition of every wave's sums of a tile.
-    auto take = [&](unsigned ti) __attribute__((always_inline)) {
-      if (ti % W != wave || ti >= p.row_tiles || lane >= kKeys)
+    // The waves' sums of a run of W tiles, one tile a wave, added in wave order.
+    auto take = [&](unsigned run) __attribute__((always_inline)) {
+      const unsigned ti = run * W + wave;
+      if (ti < first || ti >= past || ti >= p.row_tiles)
         return;
-      const unsigned count = p.blocks - group * W < W ? p.blocks - group * W : W;
-      float v = 0.0f;
+      float v[W];
 #pragma unroll
       for (unsigned k = 0; k < W; ++k)
-        v += k < count ? sh.red[ti % 2][k][lane] + sh.red[ti % 2][k][lane + 32] : 0.0f;
-      p.sums[(std::size_t{lin} * p.row_tiles + ti) * kKeys + lane] = v;
+        v[k] = sh.red[run % 2][wave][k][lane];
+#pragma unroll
+      for (unsigned k = 1; k < W; ++k)
+        v[0] += v[k];
+      const float all = cdna4::sum_xor32(v[0]);
+      if (lane < kKeys)
+        p.sums[(std::size_t{lin} * p.row_tiles + ti) * kKeys + lane] = all;
     };
     // K-step s of tile ti: the address is kl ^ 32 s of its stage; kl has no bit of 256.
     auto read = [&](unsigned ti, unsigned s) __attribute__((always_inline)) {
       return decode_detail::lds_b128((((ring + ti % kStages * kTileBytes) | kl) ^ (32u * (s % 8))) +
                                      32u * (s & 8u));
     };
-    // The scores of tile ti into cur and the weights of tile ti - 1, whose scores prev holds: a
-    // weight (fma, exponential, sum) to every two matrix instructions, in this order.
+    // The scores of tile ti into cur and the weights of tile ti - 1, whose scores prev holds. Between
+    // two matrix instructions stand one fma, one exponential and one sum, of three neighbouring
+    // weights, so that none waits for another; the next copies and the sums of a run of tiles go
+    // behind the first matrix instructions.
     auto step = [&](float16_t& cur, float16_t& prev, unsigned ti) __attribute__((always_inline)) {
       mask(prev, ti - 1);
       part[0] = part[1] = part[2] = part[3] = 0.0f;
+      float x1 = 0.0f, e1 = 0.0f;
 #pragma unroll
       for (unsigned s = 0; s < kSteps; ++s) {
         __builtin_amdgcn_sched_barrier(0);
         const cdna4::half8_t next = s + 4 < kSteps ? read(ti, s + 4) : read(ti + 1, s + 4 - kSteps);
         const float16_t from = s == 0 ? float16_t{} : cur;
         cur = kSum ? mfma32(b.hi[s], a[s % 4], from) : mfma32(a[s % 4], b.hi[s], from);
-        const float e = weight(prev, s);
+        const float x = exponent(prev, s);
+        if (s > 1)
+          part[(s - 2) % 4] += e1;
+        const float e = __builtin_amdgcn_exp2f(x1);
         cur = kSum ? mfma32(b.lo[s], a[s % 4], cur) : mfma32(a[s % 4], b.lo[s], cur);
         a[s % 4] = next;
-        part[s % 4] += e;
+        e1 = e;
+        x1 = x;
+        if (s == 1 && ti + kStages - 1 < past)
+          issue(ti + kStages - 1);
+        if constexpr (kSum)
+          if (s == 3 && (ti - 2) % W == W - 1 && ti > first + 1)
+            take((ti - 2) / W);
       }
       __builtin_amdgcn_sched_barrier(0);
+      part[2] += e1;
+      part[3] += __builtin_amdgcn_exp2f(x1);
     };
     // Tile ti + 1 has landed: this wave's copies by the count, every wave's by the barrier, which
     // also says that every wave has read tile ti - 1, whose stage the next copy takes. So a wave
@@ -524,16 +558,22 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
       else
         cdna4::wait_vmcnt<0>();
       decode_detail::tile_barrier();
-      if (ti + kStages - 1 < past)
-        issue(ti + kStages - 1);
-      if constexpr (kSum)
-        if (ti > first + 1)
-          take(ti - 2);
     };
 
-    if (!active) {
-      for (unsigned ti = first; ti < past; ++ti)
+    if (!active) {  // copies, and sums nothing
+      if constexpr (kSum) {
+#pragma unroll
+        for (unsigned i = 0; i < 2 * W; ++i)
+          sh.red[i / W][i % W][wave][lane] = 0.0f;
+      }
+      for (unsigned ti = first; ti < past; ++ti) {
         turn(ti);
+        if (ti + kStages - 1 < past)
+          issue(ti + kStages - 1);
+        if constexpr (kSum)
+          if ((ti - 2) % W == W - 1 && ti > first + 1)
+            take((ti - 2) / W);
+      }
     } else {
       turn(first);
 #pragma unroll
@@ -547,6 +587,8 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
         acc[0] = kSum ? mfma32(b.lo[s], a[s % 4], acc[0]) : mfma32(a[s % 4], b.lo[s], acc[0]);
         a[s % 4] = next;
       }
+      if (first + kStages - 1 < past)
+        issue(first + kStages - 1);
       unsigned ti = first + 1;
       for (; ti + 1 < past; ti += 2) {
         turn(ti);
@@ -577,9 +619,11 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
     }
     if constexpr (kSum) {
       decode_detail::tile_barrier();
-      if (past - first > 1)
-        take(past - 2);
-      take(past - 1);
+      // The last run, and the one before it where that ended with tile past - 2 (its turn to be taken
+      // would have come with a tile `past`).
+      if (past % W == 1 && past - first > 1)
+        take((past - 2) / W);
+      take((past - 1) / W);
     }
     x += past - first;
     tile = past;
@@ -645,20 +689,26 @@ __global__ void __launch_bounds__(256) attn_k_fp8_widen_kernel(const uint8_t* k8
   }
 }
 
-// How a chunk is cut: column blocks, the waves W of a workgroup (8: one workgroup per CU; 4: two, for
-// chunks whose last group of 8 would be mostly empty), the groups, and the spans of a pass.
+// How a chunk is cut: column blocks, the waves W of a workgroup, the groups, and the spans of a pass.
+// W = 8 is one workgroup per CU, W = 4 two, which hide each other's starts and barriers but stream K
+// twice. Two are faster while K stays in an XCD's L2 (2048 tokens: 110 us against 120; 1000 after
+// 1000: 74.7 against 75.0), slower beyond (2048 after 12001: 855 against 794), except for few
+// blocks that fill groups of 4 better by more than that (33 tokens after 40000, 9 blocks: 86 against
+// 94; 17 after 40000, 5 blocks: 70 against 60).
 struct AttnKeyWeightsCut {
   unsigned blocks, waves, groups, row_tiles, spans;
   unsigned long long span;
 };
-constexpr unsigned kWeightsCus = 256;
+constexpr unsigned kWeightsCus = 256, kWeightsNearRows = 4096;
 __host__ __device__ constexpr AttnKeyWeightsCut attn_key_weights_cut(unsigned pos0, unsigned n) {
   using namespace weights_detail;
   AttnKeyWeightsCut c{};
   c.blocks = div_up(n, kTokens);
-  c.waves = c.blocks < 32 && (c.blocks - 1) % 8 < 4 ? 4 : 8;
+  const unsigned rows = pos0 + n;
+  const bool fills = c.blocks < 64 && 27 * div_up(c.blocks, 4) < 50 * div_up(c.blocks, 8);
+  c.waves = rows <= kWeightsNearRows || fills ? 4 : 8;
   c.groups = div_up(c.blocks, c.waves);
-  c.row_tiles = div_up(pos0 + n, kKeys);
+  c.row_tiles = div_up(rows, kKeys);
   const unsigned long long tiles = 2 * tiles_before(c.waves, pos0, c.groups);
   const unsigned most = kWeightsCus * (8 / c.waves);
   c.span = (tiles + most - 1) / most;
@@ -673,9 +723,19 @@ __host__ __device__ constexpr unsigned attn_key_weights_tokens(unsigned rows) {
   return 32 * (groups < 8 ? 8 : groups);
 }
 
-// The groups that a piece of up to `blocks` column blocks has at most.
+// The groups that a piece of up to `blocks` column blocks over up to `rows` rows has at most, where
+// its groups of 4 are not among the near rows' (those are counted by themselves).
 __host__ __device__ constexpr std::size_t attn_key_weights_groups(std::size_t blocks) {
-  return blocks < 32 ? blocks / 4 + 1 : blocks / 8 + 4;
+  return (blocks < 64 ? blocks / 4 : blocks < 120 ? 15 : blocks / 8) + 1;
+}
+// Floats of the groups' sums.
+__host__ __device__ constexpr std::size_t attn_key_weights_sums(std::size_t blocks,
+                                                                std::size_t rows) {
+  const std::size_t far = attn_key_weights_groups(blocks) * rows;
+  const std::size_t near_blocks = blocks < kWeightsNearRows / 4 ? blocks : kWeightsNearRows / 4;
+  const std::size_t near =
+      (near_blocks / 4 + 1) * (rows < kWeightsNearRows ? rows : std::size_t{kWeightsNearRows});
+  return 2 * (far > near ? far : near);
 }
 
 // The workspace's parts, in bytes from its start, each 256-byte aligned.
@@ -694,8 +754,8 @@ __host__ __device__ constexpr AttnKeyWeightsLayout attn_key_weights_parts(
   };
   l.halves = take(2 * blocks * kBlockHalves * sizeof(attn::half_t));
   l.scale = take(2 * blocks * 4);
-  // (spans + 2 groups) x 32 W columns, spans x W <= 8 x 256
-  l.stats = take((kWeightsCus + 2 * attn_key_weights_groups(blocks)) * 8 * kCols * sizeof(float2));
+  // (spans + 2 groups) x 32 W columns, spans x W <= 8 x 256, groups x W <= 8 (blocks / 8 + 1)
+  l.stats = take((kWeightsCus + 2 * (blocks / 8 + 1)) * 8 * kCols * sizeof(float2));
   l.sums = take(sums_floats * 4);
   l.k_wide = take(2 * wide_rows * attn::kDim * sizeof(attn::half_t));
   l.bytes = at;
@@ -710,22 +770,21 @@ __host__ __device__ constexpr AttnKeyWeightsLayout attn_key_weights_layout(unsig
   const unsigned blocks = div_up(n < most ? n : most, kTokens);
   return attn_key_weights_parts(
       blocks,
-      2 * attn_key_weights_groups(blocks) * (std::size_t{div_up(rows, kKeys)} * kKeys),
+      attn_key_weights_sums(blocks, std::size_t{div_up(rows, kKeys)} * kKeys),
       fp8 ? rows : 0);
 }
 
 // Bytes that serve every chunk of up to max_n tokens over up to max_rows rows. A piece has at most
-// 16384 tokens (its tokens times its rows, at least as many, are at most 2^28); its groups are those
-// of max_n at most, or 12 more than what 2^23 group rows allow.
+// 16384 tokens (its tokens times its rows, at least as many, are at most 2^28); its sums are those
+// of max_n at most, or of 2^23 group rows and 16 groups more.
 __host__ __device__ constexpr std::size_t attn_key_weights_bytes(unsigned max_n, unsigned max_rows,
                                                                  bool fp8) {
   using namespace weights_detail;
   const std::size_t blocks = div_up(max_n < 16384 ? max_n : 16384, kTokens);
   const std::size_t rows = std::size_t{div_up(max_rows, kKeys)} * kKeys;
-  const std::size_t by_n = attn_key_weights_groups(blocks) * rows;
-  const std::size_t by_rows = (std::size_t{1} << 23) + 12 * (rows + 64);
-  return attn_key_weights_parts(blocks, 2 * (by_n < by_rows ? by_n : by_rows), fp8 ? max_rows : 0)
-      .bytes;
+  const std::size_t by_n = attn_key_weights_sums(blocks, rows);
+  const std::size_t by_rows = 2 * ((std::size_t{1} << 23) + 16 * (rows + 64));
+  return attn_key_weights_parts(blocks, by_n < by_rows ? by_n : by_rows, fp8 ? max_rows : 0).bytes;
 }
 
 template <unsigned W>
