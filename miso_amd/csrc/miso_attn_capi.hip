@@ -1213,8 +1213,7 @@ int miso_attn_prefill_weights_fp8(const float* q, const uint8_t* k8, const float
 }
 
 uint64_t miso_attn_evict_workspace_bytes(uint32_t max_len) {
-  (void)max_len;
-  return 256;
+  return k::attn_evict_bytes(max_len);
 }
 
 int miso_attn_evict_select(const float* weights, uint32_t len, uint32_t max_ctx, uint32_t keep,
@@ -1233,8 +1232,8 @@ int miso_attn_evict_select(const float* weights, uint32_t len, uint32_t max_ctx,
     return fail(fn, "sinks + recent exceeds keep");
   if (workspace_bytes < miso_attn_evict_workspace_bytes(len))
     return fail(fn, "workspace smaller than miso_attn_evict_workspace_bytes(len)");
-  const k::AttnEvictSelectParams p{weights, index, len, max_ctx, keep, sinks, recent};
-  k::attn_evict_select_kernel<><<<2, 1024, 0, as_stream(stream)>>>(p);
+  k::attn_evict_select_launch({weights, index, len, max_ctx, keep, sinks, recent, 1, 0, nullptr},
+                              workspace, as_stream(stream));
   return launched(fn);
 }
 

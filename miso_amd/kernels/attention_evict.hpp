@@ -848,98 +848,389 @@ inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
 // Per KV head: rows [0, sinks), rows [len - recent, len) and, of the rows between, the
 // keep - sinks - recent of the largest weight; of equal weights the lower row. A NaN ranks below
 // every number, -0 equals +0. index [2][keep], ascending.
+//
+// A row's rank is an unsigned that orders as its weight does, all ones for the rows that are kept in
+// any case and 0 for what lies behind the last row. The last kept row's rank is found digit by digit,
+// 11, 11 and 10 bits: a histogram of the rows that agree so far, and the bin in which the count from
+// the top reaches what is still to be kept. Then the rows above that rank are kept, and of those
+// equal to it the first ones. Counts are whole numbers, so their order does not matter.
 // ------------------------------------------------------------------------------------------------
 
 struct AttnEvictSelectParams {
   const float* weights;  // [2][max_ctx]
   int* index;            // [2][keep]
   unsigned len, max_ctx, keep, sinks, recent;
+  // Caches of several workgroups a head: a workgroup's rows, and the workspace [2] of per-workgroup
+  // histograms [3][groups][2048], then the rows of each above what is found [groups], then the
+  // (prefix, rows still to be kept) that the second and third launch found.
+  unsigned groups, rows;
+  unsigned* ws;
 };
 
 namespace evict_detail {
 
-// An unsigned that orders as the weight does: NaN lowest, then the numbers.
-__device__ __attribute__((always_inline)) inline unsigned rank_of(float x) {
-  if (x != x)
-    return 0;
-  const unsigned u = cdna4::as_uint(x == 0.0f ? 0.0f : x);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+constexpr unsigned kBins = 2048;  // of a digit; the last one uses 1024
+constexpr unsigned kSelectWaves = 16;
+constexpr unsigned kShift[3] = {21, 10, 0};
+
+// The rank of row `row`, whose weight is x: NaN 1, then the numbers, -0 as +0.
+__device__ __attribute__((always_inline)) inline unsigned rank_of(const AttnEvictSelectParams& p,
+                                                                 unsigned row, float x) {
+  const unsigned u = cdna4::as_uint(x + 0.0f);  // -0 becomes +0
+  unsigned rank = u & 0x80000000u ? ~u : u | 0x80000000u;
+  rank = x != x ? 1u : rank;
+  rank = row < p.sinks || row >= p.len - p.recent ? ~0u : rank;
+  return row < p.len ? rank : 0u;
+}
+
+// The digit of a rank, and whether the rank agrees with the prefix above it.
+template <unsigned kDigit>
+__device__ __attribute__((always_inline)) inline unsigned digit_of(unsigned rank) {
+  return rank >> kShift[kDigit] & (kDigit == 2 ? 1023u : 2047u);
+}
+template <unsigned kDigit>
+__device__ __attribute__((always_inline)) inline bool agrees(unsigned rank, unsigned prefix) {
+  return kDigit == 0 || rank >> kShift[kDigit == 0 ? 0 : kDigit - 1] ==
+                            prefix >> kShift[kDigit == 0 ? 0 : kDigit - 1];
+}
+
+// The inclusive sum over the lanes up to this one.
+__device__ __attribute__((always_inline)) inline unsigned wave_scan(unsigned x, unsigned lane) {
+#pragma unroll
+  for (unsigned d = 1; d < 64; d *= 2) {
+    const unsigned y = __shfl_up(x, d);
+    x += lane >= d ? y : 0;
+  }
+  return x;
+}
+
+// Lanes below this one that are set in a wave's mask.
+__device__ __attribute__((always_inline)) inline unsigned lanes_below(unsigned long long mask) {
+  return __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
+                                   __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0));
+}
+
+// Words of a head's part of the workspace (an even number: histograms move 8 bytes a lane).
+__host__ __device__ constexpr std::size_t part_words(std::size_t groups) {
+  return groups * 3 * kBins + (groups + 1) / 2 * 2 + 4;
+}
+
+struct SelectShared {
+  unsigned hist[kBins + 64];  // one more bin a lane, for rows that do not count
+  unsigned waves[2][kSelectWaves];
+  unsigned digit, above;
+};
+
+// One row a lane into the histogram. 64 rows of one digit (untouched rows, the newest ones) are added
+// in one go, since the additions of one bin follow one another.
+template <unsigned kDigit>
+__device__ __attribute__((always_inline)) inline void count_digit(SelectShared& sh, unsigned rank,
+                                                                 unsigned prefix, unsigned lane) {
+  const unsigned bin = agrees<kDigit>(rank, prefix) ? digit_of<kDigit>(rank) : kBins + lane;
+  const unsigned one = __builtin_amdgcn_readfirstlane(bin);
+  if (__builtin_amdgcn_ballot_w64(bin != one) == 0) {  // wave-uniform
+    if (lane == 0)
+      atomicAdd(&sh.hist[one], 64u);
+  } else {
+    atomicAdd(&sh.hist[bin], 1u);
+  }
+}
+
+__device__ __attribute__((always_inline)) inline void clear_digits(SelectShared& sh) {
+  sh.hist[threadIdx.x] = 0;
+  sh.hist[threadIdx.x + 1024] = 0;
+  __syncthreads();
+}
+
+// The bin in which the count from the top reaches `want` (sh.digit) and the count of the bins above
+// it (sh.above); thread t holds bins 2047 - 2 t and 2046 - 2 t, `high` and `low` of them. 1 <= want
+// <= the histogram's total. Ends with a barrier.
+__device__ __attribute__((always_inline)) inline void find_digit(SelectShared& sh, unsigned high,
+                                                                unsigned low, unsigned want) {
+  const unsigned t = threadIdx.x, lane = t & 63u, wave = t >> 6;
+  const unsigned incl = wave_scan(high + low, lane);
+  if (lane == 63)
+    sh.waves[0][wave] = incl;
+  __syncthreads();
+  unsigned above = incl - (high + low);
+#pragma unroll
+  for (unsigned k = 0; k < kSelectWaves; ++k)
+    above += k < wave ? sh.waves[0][k] : 0;
+  if (above < want && want <= above + high + low) {  // one thread
+    const bool first = want <= above + high;
+    sh.digit = kBins - 1 - 2 * t - (first ? 0 : 1);
+    sh.above = above + (first ? 0 : high);
+  }
+  __syncthreads();
+}
+
+// Where this wave's kept rows go. `sure` and `equals`: its rows above the found rank and equal to
+// it (wave-uniform); `before` and `same`: kept rows and equal rows before the workgroup; `want`: how
+// many equal rows are kept. Returns the place of the wave's first kept row and moves `same` on to
+// the equal rows before the wave.
+__device__ __attribute__((always_inline)) inline unsigned place_wave(SelectShared& sh,
+                                                                    unsigned sure, unsigned equals,
+                                                                    unsigned before,
+                                                                    unsigned& same, unsigned want) {
+  const unsigned wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63u) == 0) {
+    sh.waves[0][wave] = sure;
+    sh.waves[1][wave] = equals;
+  }
+  __syncthreads();
+  const unsigned kept = same < want ? same : want;  // equal rows kept before the workgroup
+#pragma unroll
+  for (unsigned k = 0; k < kSelectWaves; ++k) {
+    before += k < wave ? sh.waves[0][k] : 0;
+    same += k < wave ? sh.waves[1][k] : 0;
+  }
+  return before + (same < want ? same : want) - kept;
+}
+
+// Writes the kept rows of 64, row `row` of rank `rank` this lane's, from out[at] on.
+__device__ __attribute__((always_inline)) inline void write_kept(int* out, unsigned& at,
+                                                                unsigned& same, unsigned want,
+                                                                unsigned rank, unsigned last,
+                                                                unsigned row) {
+  const unsigned long long equal = __builtin_amdgcn_ballot_w64(rank == last);
+  const bool keep = rank > last || (rank == last && same + lanes_below(equal) < want);
+  const unsigned long long kept = __builtin_amdgcn_ballot_w64(keep);
+  if (keep)
+    out[at + lanes_below(kept)] = static_cast<int>(row);
+  at += __popcll(kept);
+  same += __popcll(equal);
 }
 
 }  // namespace evict_detail
 
-// One workgroup of 1024 per KV head. Four passes over the rows narrow the rank of the last kept
-// row 8 bits at a time (histograms in LDS); a last one writes the kept rows in order.
-template <int = 0>
+// One workgroup of 1024 per KV head for up to 1024 R rows, their ranks in registers: wave w's
+// register i holds row 64 (R w + i) + lane, so that the registers in turn are the rows' order.
+template <unsigned R>
 __global__ void __launch_bounds__(1024) attn_evict_select_kernel(AttnEvictSelectParams p) {
-  __shared__ unsigned hist[256], found[2], waves[16], equals[16];
-  const unsigned kvh = blockIdx.x, t = threadIdx.x, lane = t & 63u, wave = t >> 6;
+  using namespace evict_detail;
+  __shared__ SelectShared sh;
+  const unsigned kvh = blockIdx.x, t = threadIdx.x, lane = t & 63u;
+  const unsigned wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const float* w = p.weights + std::size_t{kvh} * p.max_ctx;
-  const unsigned lo = p.sinks, hi = p.len - p.recent;
-  unsigned want = p.keep - p.sinks - p.recent;  // rows of the middle still to be found
-  unsigned prefix = 0;
-  if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (t < 256)
-        hist[t] = 0;
-      __syncthreads();
-      for (unsigned i = lo + t; i < hi; i += 1024) {
-        const unsigned r = evict_detail::rank_of(w[i]);
-        if (shift == 24 || r >> (shift + 8) == prefix >> (shift + 8))
-          atomicAdd(&hist[r >> shift & 255u], 1u);
+  const unsigned row0 = 64 * R * wave + lane;
+  float x[R];
+  unsigned rank[R];
+#pragma unroll
+  for (unsigned i = 0; i < R; ++i)
+    x[i] = row0 + 64 * i < p.len ? w[row0 + 64 * i] : 0.0f;
+#pragma unroll
+  for (unsigned i = 0; i < R; ++i)
+    rank[i] = rank_of(p, row0 + 64 * i, x[i]);
+  unsigned want = p.keep, last = 0;
+  auto digit = [&](auto which) __attribute__((always_inline)) {
+    constexpr unsigned kDigit = decltype(which)::value;
+    clear_digits(sh);
+#pragma unroll
+    for (unsigned i = 0; i < R; ++i)
+      count_digit<kDigit>(sh, rank[i], last, lane);
+    __syncthreads();
+    find_digit(sh, sh.hist[kBins - 1 - 2 * t], sh.hist[kBins - 2 - 2 * t], want);
+    last |= sh.digit << kShift[kDigit];
+    want -= sh.above;
+  };
+  digit(std::integral_constant<unsigned, 0>{});
+  digit(std::integral_constant<unsigned, 1>{});
+  digit(std::integral_constant<unsigned, 2>{});
+  unsigned sure = 0, equals = 0, same = 0;
+#pragma unroll
+  for (unsigned i = 0; i < R; ++i) {
+    sure += __popcll(__builtin_amdgcn_ballot_w64(rank[i] > last));
+    equals += __popcll(__builtin_amdgcn_ballot_w64(rank[i] == last));
+  }
+  unsigned at = place_wave(sh, sure, equals, 0, same, want);
+  int* out = p.index + std::size_t{kvh} * p.keep;
+#pragma unroll
+  for (unsigned i = 0; i < R; ++i)
+    write_kept(out, at, same, want, rank[i], last, row0 + 64 * i);
+}
+
+// Longer caches: `groups` workgroups per head, p.rows rows each, in four launches, a digit each and
+// the writing. Launch d >= 1 first joins the histograms of digit d - 1 (every workgroup for
+// itself), then counts its own rows' digit d. Grid dim3(groups, 2) x 1024.
+template <unsigned kLaunch>
+__global__ void __launch_bounds__(1024) attn_evict_select_part_kernel(AttnEvictSelectParams p) {
+  using namespace evict_detail;
+  __shared__ SelectShared sh;
+  const unsigned kvh = blockIdx.y, g = blockIdx.x, t = threadIdx.x, lane = t & 63u;
+  const unsigned wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const float* w = p.weights + std::size_t{kvh} * p.max_ctx;
+  const unsigned r0 = g * p.rows < p.len ? g * p.rows : p.len;  // the last groups may have none
+  const unsigned r1 = p.len - r0 < p.rows ? p.len : r0 + p.rows;
+  const std::size_t hists = std::size_t{3} * p.groups * kBins;
+  unsigned* const ws = p.ws + kvh * part_words(p.groups);
+  unsigned* const above = ws + hists;
+  unsigned* const state = above + (p.groups + 1) / 2 * 2;  // (prefix, want) after digits 0 and 1
+  // Each wave takes a stretch of the rows, 64 at a time; the first 512 are loaded before all else.
+  const unsigned per = p.rows / kSelectWaves;
+  const unsigned s0 = r0 + wave * per < r1 ? r0 + wave * per : r1;
+  const unsigned s1 = s0 + per < r1 ? s0 + per : r1;
+  constexpr unsigned kChunk = 512;
+  float x[kChunk / 64];
+  auto load = [&](unsigned from) __attribute__((always_inline)) {
+#pragma unroll
+    for (unsigned i = 0; i < kChunk / 64; ++i) {
+      const unsigned row = from + 64 * i + lane;
+      x[i] = row < s1 ? w[row] : 0.0f;
+    }
+  };
+  auto rank_at = [&](unsigned from, unsigned i) __attribute__((always_inline)) {
+    const unsigned row = from + 64 * i + lane;
+    return row < s1 ? rank_of(p, row, x[i]) : 0u;
+  };
+  load(s0);
+  unsigned want = p.keep, last = 0;
+  if constexpr (kLaunch > 1) {
+    last = state[2 * (kLaunch - 2)];
+    want = state[2 * (kLaunch - 2) + 1];
+  }
+  if constexpr (kLaunch > 0) {
+    const unsigned bin = kBins - 2 - 2 * t;
+    const unsigned* h = ws + (kLaunch - 1) * std::size_t{p.groups} * kBins + bin;
+    const uint2 own = *reinterpret_cast<const uint2*>(h + std::size_t{g} * kBins);
+    unsigned high = 0, low = 0;
+    for (unsigned k0 = 0; k0 < p.groups; k0 += 16) {  // 16 loads in flight
+      uint2 one[16];
+#pragma unroll
+      for (unsigned i = 0; i < 16; ++i)
+        one[i] = *reinterpret_cast<const uint2*>(
+            h + std::size_t{k0 + i < p.groups ? k0 + i : k0} * kBins);
+#pragma unroll
+      for (unsigned i = 0; i < 16; ++i) {
+        low += k0 + i < p.groups ? one[i].x : 0;
+        high += k0 + i < p.groups ? one[i].y : 0;
       }
+    }
+    find_digit(sh, high, low, want);
+    const unsigned digit = sh.digit;
+    last |= digit << kShift[kLaunch - 1];
+    want -= sh.above;
+    if constexpr (kLaunch < 3) {
+      // This workgroup's rows above the digit join those above the digits before.
+      const unsigned sum =
+          wave_scan((bin > digit ? own.x : 0) + (bin + 1 > digit ? own.y : 0), lane);
+      if (lane == 63)
+        sh.waves[1][wave] = sum;
       __syncthreads();
       if (t == 0) {
-        unsigned above = 0;
-        int d = 255;
-        while (d > 0 && above + hist[d] < want)
-          above += hist[d--];
-        found[0] = static_cast<unsigned>(d);
-        found[1] = above;
+        unsigned all = kLaunch == 1 ? 0 : above[g];
+        for (unsigned k = 0; k < kSelectWaves; ++k)
+          all += sh.waves[1][k];
+        above[g] = all;
+        if (g == 0) {
+          state[2 * (kLaunch - 1)] = last;
+          state[2 * (kLaunch - 1) + 1] = want;
+        }
       }
-      __syncthreads();
-      prefix |= found[0] << shift;
-      want -= found[1];
-      __syncthreads();
     }
   }
-  // Kept: the ends, ranks above the prefix, and the first `want` of those equal to it.
-  unsigned at = 0, same = 0;
-  for (unsigned i0 = 0; i0 < p.len; i0 += 1024) {
-    const unsigned i = i0 + t;
-    bool end = false, above = false, equal = false;
-    if (i < p.len) {
-      end = i < lo || i >= hi;
-      if (!end && p.keep > p.sinks + p.recent) {
-        const unsigned r = evict_detail::rank_of(w[i]);
-        above = r > prefix;
-        equal = r == prefix;
+  if constexpr (kLaunch < 3) {
+    clear_digits(sh);
+    for (unsigned from = s0; from < s1; from += kChunk) {  // wave-uniform
+      if (from != s0)
+        load(from);
+#pragma unroll
+      for (unsigned i = 0; i < kChunk / 64; ++i)
+        count_digit<kLaunch>(sh, rank_at(from, i), last, lane);
+    }
+    __syncthreads();
+    unsigned* out = ws + (kLaunch * std::size_t{p.groups} + g) * kBins;
+    *reinterpret_cast<uint2*>(out + 2 * t) = *reinterpret_cast<const uint2*>(&sh.hist[2 * t]);
+  } else {
+    // Rows above the found rank, and rows equal to it, in the workgroups before this one.
+    unsigned a = 0, e = 0;
+    const unsigned digit = last & 1023u;
+    for (unsigned k = wave; k < g; k += kSelectWaves) {  // wave-uniform
+      const unsigned* h = ws + (2 * std::size_t{p.groups} + k) * kBins;
+      unsigned c[16];
+#pragma unroll
+      for (unsigned i = 0; i < 16; ++i)
+        c[i] = h[64 * i + lane];
+      a += lane == 0 ? above[k] : 0;
+#pragma unroll
+      for (unsigned i = 0; i < 16; ++i) {
+        a += 64 * i + lane > digit ? c[i] : 0;
+        e += 64 * i + lane == digit ? c[i] : 0;
       }
     }
-    const unsigned long long eq = __ballot(equal);
-    const unsigned long long below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
-    if (lane == 0)
-      equals[wave] = __popcll(eq);
-    __syncthreads();
-    unsigned eq0 = same, eq_all = 0;
-    for (unsigned k = 0; k < 16; ++k) {
-      eq0 += k < wave ? equals[k] : 0;
-      eq_all += equals[k];
+    a = wave_scan(a, lane);
+    e = wave_scan(e, lane);
+    if (lane == 63) {  // (sh.waves was last read before find_digit's second barrier)
+      sh.waves[0][wave] = a;
+      sh.waves[1][wave] = e;
     }
-    const bool kept = end || above || (equal && eq0 + __popcll(eq & below) < want);
-    const unsigned long long kb = __ballot(kept);
-    if (lane == 0)
-      waves[wave] = __popcll(kb);
     __syncthreads();
-    unsigned k0 = at, k_all = 0;
-    for (unsigned k = 0; k < 16; ++k) {
-      k0 += k < wave ? waves[k] : 0;
-      k_all += waves[k];
+    unsigned before = 0, same = 0;
+#pragma unroll
+    for (unsigned k = 0; k < kSelectWaves; ++k) {
+      before += sh.waves[0][k];
+      same += sh.waves[1][k];
     }
-    if (kept)
-      p.index[std::size_t{kvh} * p.keep + k0 + __popcll(kb & below)] = static_cast<int>(i);
-    at += k_all;
-    same += eq_all;
+    before += same < want ? same : want;
+    __syncthreads();
+    // Each wave counts its stretch, and writes behind the waves before it.
+    unsigned sure = 0, equals = 0;
+    for (unsigned from = s0; from < s1; from += kChunk) {
+      if (from != s0)
+        load(from);
+#pragma unroll
+      for (unsigned i = 0; i < kChunk / 64; ++i) {
+        const unsigned rank = rank_at(from, i);
+        sure += __popcll(__builtin_amdgcn_ballot_w64(rank > last));
+        equals += __popcll(__builtin_amdgcn_ballot_w64(rank == last));
+      }
+    }
+    unsigned at = place_wave(sh, sure, equals, before, same, want);
+    int* out = p.index + std::size_t{kvh} * p.keep;
+    for (unsigned from = s0; from < s1; from += kChunk) {
+      if (per > kChunk)
+        load(from);
+#pragma unroll
+      for (unsigned i = 0; i < kChunk / 64; ++i)
+        write_kept(out, at, same, want, rank_at(from, i), last, from + 64 * i + lane);
+    }
+  }
+}
+
+// Up to this many rows one workgroup a head holds them all; beyond, at most 64 of 8192 rows or more.
+constexpr unsigned kSelectOneGroup = 32768, kSelectMostGroups = 64;
+__host__ __device__ constexpr unsigned attn_evict_groups(unsigned len) {
+  if (len <= kSelectOneGroup)
+    return 1;
+  const unsigned groups = (len + 8191) / 8192;
+  return groups < kSelectMostGroups ? groups : kSelectMostGroups;
+}
+
+// Bytes of the selection's workspace for len rows (more rows never need less).
+__host__ __device__ constexpr std::size_t attn_evict_bytes(unsigned len) {
+  const std::size_t groups = attn_evict_groups(len);
+  return groups == 1 ? 256 : 2 * evict_detail::part_words(groups) * sizeof(unsigned);
+}
+
+// The launches of a selection whose arguments are good; ws of attn_evict_bytes(p.len).
+inline void attn_evict_select_launch(AttnEvictSelectParams p, void* ws, hipStream_t stream) {
+  p.ws = static_cast<unsigned*>(ws);
+  p.groups = attn_evict_groups(p.len);
+  if (p.len <= 2048) {
+    attn_evict_select_kernel<2><<<2, 1024, 0, stream>>>(p);
+  } else if (p.len <= 8192) {
+    attn_evict_select_kernel<8><<<2, 1024, 0, stream>>>(p);
+  } else if (p.len <= 16384) {
+    attn_evict_select_kernel<16><<<2, 1024, 0, stream>>>(p);
+  } else if (p.len <= kSelectOneGroup) {
+    attn_evict_select_kernel<32><<<2, 1024, 0, stream>>>(p);
+  } else {
+    // Whole runs of 1024 rows; with them the last groups may have none left.
+    p.rows = ((p.len + p.groups - 1) / p.groups + 1023) / 1024 * 1024;
+    const dim3 grid(p.groups, 2);
+    attn_evict_select_part_kernel<0><<<grid, 1024, 0, stream>>>(p);
+    attn_evict_select_part_kernel<1><<<grid, 1024, 0, stream>>>(p);
+    attn_evict_select_part_kernel<2><<<grid, 1024, 0, stream>>>(p);
+    attn_evict_select_part_kernel<3><<<grid, 1024, 0, stream>>>(p);
   }
 }
 
