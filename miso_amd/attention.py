@@ -57,12 +57,12 @@ def _count(x: int, name: str) -> int:
     return x
 
 
-def _here(**tensors: torch.Tensor) -> None:
+def _here(*tensors: torch.Tensor) -> None:
     """The tensors lie on the current device, whose stream the launches go to."""
     device = torch.cuda.current_device() if _device is None else _device()
-    for name, t in tensors.items():
-        if t.device.index != device:
-            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{device}")
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{device}")
 
 
 def _cache_dtype(t: torch.Tensor) -> torch.dtype:
@@ -487,11 +487,11 @@ class DecodeWeightsScratch(DecodeScratch):
     def __init__(self, max_splits: int, max_len: int, device="cuda"):
         super().__init__(max_splits, device)
         self.max_len = _count(max_len, "max_len")
-        nbytes = int(_lib.load().miso_attn_decode_weights_workspace_bytes(max_len, max_splits))
-        self.ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self.nbytes = int(_lib.load().miso_attn_decode_weights_workspace_bytes(max_len, max_splits))
+        self.ws = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
 
 
-def _decode_weights(name: str, q, qg, cache, core, weights, scratch, length, max_ctx, n_splits,
+def _decode_weights(fn, q, qg, cache, core, weights, scratch, length, max_ctx, n_splits,
                     stream) -> int:
     length, max_ctx = _count(length, "length"), _count(max_ctx, "max_ctx")
     if n_splits is None:
@@ -505,12 +505,12 @@ def _decode_weights(name: str, q, qg, cache, core, weights, scratch, length, max
     _need(qg, "qg", f32, Q_HEADS * 2 * DIM)
     _need(core, "core", f32, Q_HEADS * DIM)
     _need(weights, "weights", f32, KV_HEADS * max_ctx)
-    _here(q=q, qg=qg, k_cache=cache[0], v_cache=cache[1], core=core, weights=weights,
-          scratch=scratch.ws)
-    _lib.check(getattr(_lib.load(), name)(
-        _ptr(q), _ptr(qg), *(_ptr(b) for b in cache), _ptr(core), _ptr(weights),
-        _ptr(scratch.part_m), _ptr(scratch.part_l), _ptr(scratch.part_o), length, max_ctx,
-        n_splits, _ptr(scratch.ws), scratch.ws.numel(), _stream(stream)))
+    _here(q, qg, *cache, core, weights, scratch.ws)
+    _lib.check(fn(
+        q.data_ptr(), qg.data_ptr(), *[b.data_ptr() for b in cache], core.data_ptr(),
+        weights.data_ptr(), scratch.part_m.data_ptr(), scratch.part_l.data_ptr(),
+        scratch.part_o.data_ptr(), length, max_ctx, n_splits, scratch.ws.data_ptr(),
+        scratch.nbytes, _stream(stream)))
     return n_splits
 
 
@@ -521,7 +521,7 @@ def attn_decode_weights(q, qg, k_cache, v_cache, core, weights, scratch: DecodeW
     softmax weights that KV head g's 8 query heads give row j. Returns n_splits used."""
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         _need(t, name, _cache_dtype(t), KV_HEADS * max_ctx * DIM)
-    return _decode_weights("miso_attn_decode_weights", q, qg, (k_cache, v_cache), core, weights,
+    return _decode_weights(_lib.load().miso_attn_decode_weights, q, qg, (k_cache, v_cache), core, weights,
                            scratch, length, max_ctx, n_splits, stream)
 
 
@@ -529,8 +529,8 @@ def attn_decode_weights_fp8(q, qg, cache: Fp8Cache, core, weights, scratch: Deco
                             length: int, n_splits: Optional[int] = None, stream=None) -> int:
     """attn_decode_weights over an e4m3 cache (the core of attn_decode_fp8)."""
     _need_fp8(cache)
-    return _decode_weights("miso_attn_decode_weights_fp8", q, qg, cache.buffers(), core, weights,
-                           scratch, length, cache.max_ctx, n_splits, stream)
+    return _decode_weights(_lib.load().miso_attn_decode_weights_fp8, q, qg, cache.buffers(), core,
+                           weights, scratch, length, cache.max_ctx, n_splits, stream)
 
 
 class PrefillWeightsScratch:
@@ -546,16 +546,15 @@ class PrefillWeightsScratch:
         self.ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
-def _prefill_weights(name: str, q, cache, weights, pos0, n, max_ctx, scratch, stream) -> None:
+def _prefill_weights(fn, q, cache, weights, pos0, n, max_ctx, scratch, stream) -> None:
     pos0, n, max_ctx = _count(pos0, "pos0"), _count(n, "n"), _count(max_ctx, "max_ctx")
     if n > scratch.max_n or pos0 + n > scratch.max_rows:
         raise ValueError("n or pos0 + n exceeds the scratch capacity")
     _need(q, "q", torch.float32, n * Q_HEADS * DIM)
     _need(weights, "weights", torch.float32, KV_HEADS * max_ctx)
-    _here(q=q, k_cache=cache[0], weights=weights, scratch=scratch.ws)
-    _lib.check(getattr(_lib.load(), name)(
-        _ptr(q), *(_ptr(b) for b in cache), _ptr(weights), pos0, n, max_ctx, _ptr(scratch.ws),
-        scratch.ws.numel(), _stream(stream)))
+    _here(q, *cache, weights, scratch.ws)
+    _lib.check(fn(_ptr(q), *[_ptr(b) for b in cache], _ptr(weights), pos0, n, max_ctx,
+                  _ptr(scratch.ws), scratch.ws.numel(), _stream(stream)))
 
 
 def attn_prefill_weights(q, k_cache, weights, pos0: int, n: int, max_ctx: int,
@@ -564,8 +563,8 @@ def attn_prefill_weights(q, k_cache, weights, pos0: int, n: int, max_ctx: int,
     attn_prep_batch writes them) at rows pos0 .. pos0 + n - 1 give row j <= their own. The last
     tokens of a prompt alone may vote: their queries, and pos0 their first row."""
     _need(k_cache, "k_cache", _cache_dtype(k_cache), KV_HEADS * max_ctx * DIM)
-    _prefill_weights("miso_attn_prefill_weights", q, (k_cache,), weights, pos0, n, max_ctx,
-                     scratch, stream)
+    _prefill_weights(_lib.load().miso_attn_prefill_weights, q, (k_cache,), weights, pos0, n,
+                     max_ctx, scratch, stream)
 
 
 def attn_prefill_weights_fp8(q, cache: Fp8Cache, weights, pos0: int, n: int,
@@ -574,8 +573,8 @@ def attn_prefill_weights_fp8(q, cache: Fp8Cache, weights, pos0: int, n: int,
     if not scratch.fp8:
         raise ValueError("the scratch was made without fp8=True")
     _need_fp8(cache)
-    _prefill_weights("miso_attn_prefill_weights_fp8", q, (cache.k8, cache.k_scale), weights, pos0,
-                     n, cache.max_ctx, scratch, stream)
+    _prefill_weights(_lib.load().miso_attn_prefill_weights_fp8, q, (cache.k8, cache.k_scale),
+                     weights, pos0, n, cache.max_ctx, scratch, stream)
 
 
 class EvictScratch:
@@ -599,7 +598,7 @@ def attn_evict_select(weights, length: int, max_ctx: int, keep: int, sinks: int,
         raise ValueError("length exceeds the scratch capacity")
     _need(weights, "weights", torch.float32, KV_HEADS * max_ctx)
     _need(index, "index", torch.int32, KV_HEADS * keep)
-    _here(weights=weights, index=index, scratch=scratch.ws)
+    _here(weights, index, scratch.ws)
     _lib.check(_lib.load().miso_attn_evict_select(
         _ptr(weights), length, max_ctx, keep, sinks, recent, _ptr(index), _ptr(scratch.ws),
         scratch.ws.numel(), _stream(stream)))
@@ -619,8 +618,7 @@ def attn_evict_gather(k_cache, v_cache, weights, max_ctx: int, index, keep: int,
     _need(weights, "weights", torch.float32, KV_HEADS * max_ctx)
     _need(weights_out, "weights_out", torch.float32, KV_HEADS * out_ctx)
     _need(index, "index", torch.int32, KV_HEADS * keep)
-    _here(k_cache=k_cache, v_cache=v_cache, weights=weights, index=index, k_out=k_out, v_out=v_out,
-          weights_out=weights_out)
+    _here(k_cache, v_cache, weights, index, k_out, v_out, weights_out)
     _lib.check(_lib.load().miso_attn_evict_gather(
         _ptr(k_cache), _ptr(v_cache), _ptr(weights), max_ctx, _ptr(index), keep, _ptr(k_out),
         _ptr(v_out), _ptr(weights_out), out_ctx, _stream(stream)))
@@ -635,7 +633,7 @@ def attn_evict_gather_fp8(cache: Fp8Cache, weights, index, keep: int, out: Fp8Ca
     _need(weights, "weights", torch.float32, KV_HEADS * cache.max_ctx)
     _need(weights_out, "weights_out", torch.float32, KV_HEADS * out.max_ctx)
     _need(index, "index", torch.int32, KV_HEADS * keep)
-    _here(cache=cache.k8, weights=weights, index=index, out=out.k8, weights_out=weights_out)
+    _here(*cache.buffers(), weights, index, *out.buffers(), weights_out)
     _lib.check(_lib.load().miso_attn_evict_gather_fp8(
         *(_ptr(b) for b in cache.buffers()), _ptr(weights), cache.max_ctx, _ptr(index), keep,
         *(_ptr(b) for b in out.buffers()), _ptr(weights_out), out.max_ctx, _stream(stream)))

@@ -1196,13 +1196,16 @@ __global__ void __launch_bounds__(1024) attn_evict_select_part_kernel(AttnEvictS
   }
 }
 
-// Up to this many rows one workgroup a head holds them all; beyond, at most 64 of 8192 rows or more.
+// Up to this many rows one workgroup a head holds them all (24 us at 32768 rows). Beyond, 16
+// workgroups or one per 8192 rows, at most 64: every launch joins all their histograms, 8 KiB each,
+// which more groups lengthen (100000 rows: 30 us with 16, 35 with 25; 262144: 38 with 32, 49 with
+// 64) and fewer shorten less than their own rows take (262144 with 16: 43).
 constexpr unsigned kSelectOneGroup = 32768, kSelectMostGroups = 64;
 __host__ __device__ constexpr unsigned attn_evict_groups(unsigned len) {
   if (len <= kSelectOneGroup)
     return 1;
-  const unsigned groups = (len + 8191) / 8192;
-  return groups < kSelectMostGroups ? groups : kSelectMostGroups;
+  const unsigned groups = len / 8192 + (len % 8192 != 0);
+  return groups < 16 ? 16 : groups < kSelectMostGroups ? groups : kSelectMostGroups;
 }
 
 // Bytes of the selection's workspace for len rows (more rows never need less).
@@ -1225,7 +1228,7 @@ inline void attn_evict_select_launch(AttnEvictSelectParams p, void* ws, hipStrea
     attn_evict_select_kernel<32><<<2, 1024, 0, stream>>>(p);
   } else {
     // Whole runs of 1024 rows; with them the last groups may have none left.
-    p.rows = ((p.len + p.groups - 1) / p.groups + 1023) / 1024 * 1024;
+    p.rows = ((p.len - 1) / p.groups / 1024 + 1) * 1024;
     const dim3 grid(p.groups, 2);
     attn_evict_select_part_kernel<0><<<grid, 1024, 0, stream>>>(p);
     attn_evict_select_part_kernel<1><<<grid, 1024, 0, stream>>>(p);
