@@ -289,63 +289,68 @@ struct Halves {
 
 }  // namespace weights_detail
 
-// The queries' halves and scales. One wave per (KV head, column block), 4 per workgroup: lane l of
-// load (s, i) takes dimensions 16 s + 4 (l % 4) .. of column 16 i + l / 4, 64 bytes a row, and
-// stores the two halves of its four elements, 256 bytes together. Padding columns are zero.
+// The queries' halves and scales. One workgroup of 4 waves per (KV head, column block): wave w reads
+// columns 8 w .. 8 w + 7, one row of 1 KiB an instruction, and the halves go out through LDS in the
+// order of the operands, 16 bytes a lane. In LDS the 512 bytes of a k-step's half (s, dimension /
+// 8 % 2) are 528 apart, so that the 32 of them that one row touches lie in different banks.
+// Padding columns are zero.
 template <int = 0>
 __global__ void __launch_bounds__(256) attn_key_weights_cut_kernel(AttnKeyWeightsParams p) {
   using namespace weights_detail;
-  const unsigned lane = threadIdx.x & 63u;
-  const unsigned item = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (item >= 2 * p.blocks)
-    return;
-  const unsigned kvh = item / p.blocks, block = item % p.blocks;
-  float4 x[2][kSteps];
-#pragma unroll
-  for (unsigned i = 0; i < 2; ++i) {
-    const unsigned c = 16 * i + lane / 4, t = kTokens * block + c / decode_detail::kGroup;
-    const float* row = p.q + (std::size_t{t < p.n ? t : 0} * attn::kQHeads +
-                              kvh * decode_detail::kGroup + c % decode_detail::kGroup) * attn::kDim;
-#pragma unroll
-    for (unsigned s = 0; s < kSteps; ++s)
-      x[i][s] = *reinterpret_cast<const float4*>(row + 16 * s + 4 * (lane % 4));
-  }
+  constexpr unsigned kPer = kCols / 4, kStep = 528, kHalf = 2 * kSteps * kStep;
+  __shared__ __attribute__((aligned(16))) unsigned char sh[2 * kHalf];
+  __shared__ float most[4];
+  const unsigned t = threadIdx.x, lane = t & 63u, wave = t >> 6;
+  const unsigned kvh = blockIdx.x / p.blocks, block = blockIdx.x % p.blocks;
+  float4 x[kPer];
   float top = 0.0f;
 #pragma unroll
-  for (unsigned i = 0; i < 2; ++i)
+  for (unsigned i = 0; i < kPer; ++i) {
+    const unsigned c = kPer * wave + i, tok = kTokens * block + c / decode_detail::kGroup;
+    x[i] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (tok < p.n)  // wave-uniform
+      x[i] = *reinterpret_cast<const float4*>(
+          p.q + (std::size_t{tok} * attn::kQHeads + kvh * decode_detail::kGroup +
+                 c % decode_detail::kGroup) * attn::kDim + 4 * lane);
+  }
 #pragma unroll
-    for (unsigned s = 0; s < kSteps; ++s) {
-      if (kTokens * block + (16 * i + lane / 4) / decode_detail::kGroup >= p.n)
-        x[i][s] = float4{0.0f, 0.0f, 0.0f, 0.0f};
-      top = fmaxf(top, fmaxf(fmaxf(__builtin_fabsf(x[i][s].x), __builtin_fabsf(x[i][s].y)),
-                             fmaxf(__builtin_fabsf(x[i][s].z), __builtin_fabsf(x[i][s].w))));
-    }
+  for (unsigned i = 0; i < kPer; ++i)
+    top = fmaxf(top, fmaxf(fmaxf(__builtin_fabsf(x[i].x), __builtin_fabsf(x[i].y)),
+                           fmaxf(__builtin_fabsf(x[i].z), __builtin_fabsf(x[i].w))));
   top = cdna4::wave_allmax(top);
+  if (lane == 0)
+    most[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
   // 2^(13 - e), e the exponent of top; blocks of zeros or below 2^-87 keep a finite factor, and one
   // that holds an infinity stays as it is (its scores are infinite or NaN either way).
   int e = 13 - (static_cast<int>(cdna4::as_uint(top) >> 23) - 127);
   e = top == 0.0f || top == __builtin_inff() ? 0 : (e < 100 ? e : 100);
   const float up = __builtin_ldexpf(1.0f, e);
 #pragma unroll
-  for (unsigned i = 0; i < 2; ++i) {
-    attn::half_t* at = p.halves + item * kBlockHalves +
-                       8 * (16 * i + lane / 4 + 32 * (lane / 2 % 2)) + 4 * (lane % 2);
+  for (unsigned i = 0; i < kPer; ++i) {
+    const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    cdna4::half4_t hi, lo;
 #pragma unroll
-    for (unsigned s = 0; s < kSteps; ++s) {
-      const float v[4] = {x[i][s].x, x[i][s].y, x[i][s].z, x[i][s].w};
-      cdna4::half4_t hi, lo;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float y = v[j] * up;  // a power of two: exact
-        hi[j] = static_cast<_Float16>(y);
-        lo[j] = static_cast<_Float16>(y - static_cast<float>(hi[j]));
-      }
-      *reinterpret_cast<cdna4::half4_t*>(at + 512 * s) = hi;
-      *reinterpret_cast<cdna4::half4_t*>(at + 512 * (kSteps + s)) = lo;
+    for (int j = 0; j < 4; ++j) {
+      const float y = v[j] * up;  // a power of two: exact
+      hi[j] = static_cast<_Float16>(y);
+      lo[j] = static_cast<_Float16>(y - static_cast<float>(hi[j]));
     }
+    unsigned char* at = sh + lane / 2 * kStep + 16 * (kPer * wave + i) + 8 * (lane % 2);
+    *reinterpret_cast<cdna4::half4_t*>(at) = hi;
+    *reinterpret_cast<cdna4::half4_t*>(at + kHalf) = lo;
   }
-  if (lane == 0)
-    p.scale[item] = __builtin_ldexpf(decode_detail::kLog2e / 16.0f, -e);
+  __syncthreads();
+  uint4* out = reinterpret_cast<uint4*>(p.halves + std::size_t{blockIdx.x} * kBlockHalves);
+#pragma unroll
+  for (unsigned i = 0; i < 8; ++i) {
+    const unsigned at = 256 * i + t;  // 32 lanes of 16 bytes per half of a k-step
+    out[at] = *reinterpret_cast<const uint4*>(sh + at / 1024 * kHalf + at % 1024 / 32 * kStep +
+                                              at % 32 * 16);
+  }
+  if (t == 0)
+    p.scale[blockIdx.x] = __builtin_ldexpf(decode_detail::kLog2e / 16.0f, -e);
 }
 
 // One span of a pass (kSum: the second), x 64 W, one workgroup of 8 waves or two of 4 per CU.
@@ -509,8 +514,13 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
       for (unsigned k = 1; k < W; ++k)
         v[0] += v[k];
       const float all = cdna4::sum_xor32(v[0]);
-      if (lane < kKeys)
+      if (p.groups == 1) {  // nothing to join
+        const unsigned key = ti * kKeys + lane;
+        if (lane < kKeys && key < rows)
+          p.weights[std::size_t{kvh} * p.max_ctx + key] += all;
+      } else if (lane < kKeys) {
         p.sums[(std::size_t{lin} * p.row_tiles + ti) * kKeys + lane] = all;
+      }
     };
     // K-step s of tile ti: the address is kl ^ 32 s of its stage; kl has no bit of 256.
     auto read = [&](unsigned ti, unsigned s) __attribute__((always_inline)) {
@@ -790,10 +800,11 @@ __host__ __device__ constexpr std::size_t attn_key_weights_bytes(unsigned max_n,
 template <unsigned W>
 void attn_key_weights_passes(const AttnKeyWeightsParams& p, hipStream_t stream) {
   const unsigned grid = (p.spans + 7) / 8 * 8;
-  attn_key_weights_cut_kernel<><<<(2 * p.blocks + 3) / 4, 256, 0, stream>>>(p);
+  attn_key_weights_cut_kernel<><<<2 * p.blocks, 256, 0, stream>>>(p);
   attn_key_weights_pass_kernel<W, false><<<grid, 64 * W, 0, stream>>>(p);
   attn_key_weights_pass_kernel<W, true><<<grid, 64 * W, 0, stream>>>(p);
-  attn_key_weights_join_kernel<W><<<2 * p.row_tiles, 256, 0, stream>>>(p);
+  if (p.groups > 1)
+    attn_key_weights_join_kernel<W><<<2 * p.row_tiles, 256, 0, stream>>>(p);
 }
 
 // The launches of a chunk whose arguments are good, with a workspace of the bytes of its own layout
@@ -1260,32 +1271,50 @@ struct AttnEvictGatherParams {
   float* v_scale_out;
 };
 
-// One row per 32 lanes (f16: 16 bytes of K and of V each; e4m3: 8). Rows [0, 2 keep) are moved, the
-// 2 (out_ctx - keep) weights behind them cleared. Grid-stride, x 256.
+// A row of K or V is 32 (f16) or 16 (e4m3) lanes of 16 bytes; a thread moves its chunk of both, of two
+// rows over e4m3 rows (65535 rows: 30.3 us against 33.6; over f16 rows one is faster, 51.5 against
+// 53.8). Rows [0, 2 keep) are moved, the 2 (out_ctx - keep) weights behind them cleared. Grid-stride,
+// x 256.
 template <bool kFp8>
 __global__ void __launch_bounds__(256) attn_evict_gather_kernel(AttnEvictGatherParams p) {
-  using Chunk = std::conditional_t<kFp8, uint2, uint4>;
-  const unsigned lane = threadIdx.x & 31u;
+  constexpr unsigned kLanes = kFp8 ? 16 : 32, kRows = 256 / kLanes, kTwo = kFp8 ? 2 : 1;
+  const unsigned lane = threadIdx.x % kLanes;
   const std::size_t moved = 2 * std::size_t{p.keep};
-  for (std::size_t r = 8 * std::size_t{blockIdx.x} + threadIdx.x / 32; r < moved;
-       r += 8 * std::size_t{gridDim.x}) {
-    const unsigned kvh = r >= p.keep, j = static_cast<unsigned>(r - (kvh ? p.keep : 0));
-    const int from = p.index[r];
-    const bool in = static_cast<unsigned>(from) < p.max_ctx;
-    const std::size_t src = std::size_t{kvh} * p.max_ctx + (in ? from : 0);
-    const std::size_t dst = std::size_t{kvh} * p.out_ctx + j;
-    Chunk a = static_cast<const Chunk*>(p.k)[src * 32 + lane];
-    Chunk b = static_cast<const Chunk*>(p.v)[src * 32 + lane];
-    if (!in)
-      a = b = Chunk{};
-    static_cast<Chunk*>(p.k_out)[dst * 32 + lane] = a;
-    static_cast<Chunk*>(p.v_out)[dst * 32 + lane] = b;
-    if (lane == 0)
-      p.weights_out[dst] = in ? p.weights[src] : 0.0f;
-    if (kFp8 && lane == 1)
-      p.k_scale_out[dst] = in ? p.k_scale[src] : 0.0f;
-    if (kFp8 && lane == 2)
-      p.v_scale_out[dst] = in ? p.v_scale[src] : 0.0f;
+  for (std::size_t r0 = std::size_t{blockIdx.x} * kRows * kTwo; r0 < moved;
+       r0 += std::size_t{gridDim.x} * kRows * kTwo) {
+    uint4 a[kTwo], b[kTwo];
+    std::size_t src[kTwo], dst[kTwo];
+    bool here[kTwo], in[kTwo];
+#pragma unroll
+    for (unsigned i = 0; i < kTwo; ++i) {
+      const std::size_t r = r0 + kRows * i + threadIdx.x / kLanes;
+      here[i] = r < moved;
+      const unsigned kvh = r >= p.keep, j = static_cast<unsigned>(r - (kvh ? p.keep : 0));
+      const unsigned from = here[i] ? static_cast<unsigned>(p.index[r]) : ~0u;
+      in[i] = from < p.max_ctx;
+      src[i] = std::size_t{kvh} * p.max_ctx + from;
+      dst[i] = std::size_t{kvh} * p.out_ctx + j;
+    }
+#pragma unroll
+    for (unsigned i = 0; i < kTwo; ++i) {
+      a[i] = b[i] = uint4{};
+      if (in[i]) {
+        a[i] = static_cast<const uint4*>(p.k)[src[i] * kLanes + lane];
+        b[i] = static_cast<const uint4*>(p.v)[src[i] * kLanes + lane];
+      }
+    }
+#pragma unroll
+    for (unsigned i = 0; i < kTwo; ++i)
+      if (here[i]) {
+        static_cast<uint4*>(p.k_out)[dst[i] * kLanes + lane] = a[i];
+        static_cast<uint4*>(p.v_out)[dst[i] * kLanes + lane] = b[i];
+        if (lane == 0)
+          p.weights_out[dst[i]] = in[i] ? p.weights[src[i]] : 0.0f;
+        if (kFp8 && lane == 1)
+          p.k_scale_out[dst[i]] = in[i] ? p.k_scale[src[i]] : 0.0f;
+        if (kFp8 && lane == 2)
+          p.v_scale_out[dst[i]] = in[i] ? p.v_scale[src[i]] : 0.0f;
+      }
   }
   const std::size_t rest = p.out_ctx - p.keep;
   for (std::size_t i = std::size_t{blockIdx.x} * 256 + threadIdx.x; i < 2 * rest;
