@@ -535,6 +535,27 @@ int miso_attn_prep_batch_at_fp8(const float* qg, const float* k, const float* v,
                                 uint32_t pos0, uint32_t row0, uint32_t max_ctx, float eps,
                                 uint32_t n, uint32_t proj_stride, void* stream);
 
+/* miso_attn_layer_decode over a bounded cache: the token of position pos is appended at row `row`,
+ * attends to rows [0, row] and adds the weights it gives them. y, h and the cache as
+ * miso_attn_layer_decode's where row == pos. workspace: miso_attn_decode_weights_workspace_bytes(
+ * row + 1, 128). Rejects row >= max_ctx and what the calls above reject. */
+int miso_attn_layer_decode_weights(const miso_attn_layer* layer, uint16_t* k_cache,
+                                   uint16_t* v_cache, uint32_t row, uint32_t pos,
+                                   uint32_t max_ctx, float* h, const float* delta, float* y,
+                                   float eps, float* ws, float* weights, void* workspace,
+                                   uint64_t workspace_bytes, void* stream);
+
+/* miso_attn_layer_prefill over a bounded cache: tokens of positions pos0 .. at rows row0 .. (pos0 >=
+ * row0), the last `voters` of which (all, where n is less) add the weights they give the rows they
+ * see; 0: none, weights and workspace are not looked at. workspace:
+ * miso_attn_prefill_weights_workspace_bytes(voters, row0 + n, 0). n == 0 is a no-op. */
+int miso_attn_layer_prefill_weights(const miso_attn_layer* layer, uint16_t* k_cache,
+                                    uint16_t* v_cache, uint32_t row0, uint32_t pos0, uint32_t n,
+                                    uint32_t max_ctx, float* h, const float* delta, float* y,
+                                    float eps, float* ws, uint32_t max_tok, uint32_t voters,
+                                    float* weights, void* workspace, uint64_t workspace_bytes,
+                                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

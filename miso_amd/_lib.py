@@ -88,6 +88,11 @@ SIGNATURES = {
     "miso_attn_evict_gather": (c_int, [P, P, P, c_uint32, P, c_uint32, P, P, P, c_uint32, P]),
     "miso_attn_evict_gather_fp8": (c_int, [P, P, P, P, P, c_uint32, P, c_uint32, P, P, P, P, P,
                                            c_uint32, P]),
+    "miso_attn_layer_decode_weights": (c_int, [P, P, P, c_uint32, c_uint32, c_uint32, P, P, P,
+                                               c_float, P, P, P, c_uint64, P]),
+    "miso_attn_layer_prefill_weights": (c_int, [P, P, P, c_uint32, c_uint32, c_uint32, c_uint32, P,
+                                                P, P, c_float, P, c_uint32, c_uint32, P, P,
+                                                c_uint64, P]),
     "miso_attn_prep_at": (c_int, [P] * 9 + [c_uint32, c_uint32, c_uint32, c_float, P]),
     "miso_attn_prep_batch_at": (c_int, [P] * 9 + [c_uint32, c_uint32, c_uint32, c_float, c_uint32,
                                                   c_uint32, P]),

@@ -850,3 +850,42 @@ def layer_ingest(layer: Layer, k_cache, v_cache, max_ctx: int, pos0: int, n: int
     _lib.check(_lib.load().miso_attn_layer_ingest(
         ctypes.addressof(layer.c), kc, vc, pos0, n, max_ctx, _ptr(h), _ptr(delta), _ptr(y), eps,
         _ptr(ws.decode), _ptr(ws.prefill), ws.max_tok, chunk, _stream(stream)))
+
+
+def layer_decode_weights(layer: Layer, k_cache, v_cache, max_ctx: int, row: int, pos: int, h, delta,
+                         y, eps: float, ws: LayerWorkspace, weights,
+                         scratch: DecodeWeightsScratch, stream=None) -> None:
+    """layer_decode over a bounded cache: the token of position pos goes to row `row`, attends to
+    rows [0, row] and adds the weights it gives them to weights (scratch: of LAYER_MAX_SPLITS
+    splits)."""
+    _count(row, "row"), _count(pos, "pos"), _count(max_ctx, "max_ctx")
+    if row >= scratch.max_len or scratch.max_splits < attn_n_splits(row + 1, LAYER_MAX_SPLITS):
+        raise ValueError("row + 1 exceeds the scratch capacity")
+    _rows(1, h=h, delta=delta, y=y)
+    _need(weights, "weights", torch.float32, KV_HEADS * max_ctx)
+    kc, vc = _layer_cache(k_cache, v_cache, max_ctx)
+    _here(h, y, k_cache, v_cache, weights, scratch.ws, ws.decode)
+    _lib.check(_lib.load().miso_attn_layer_decode_weights(
+        ctypes.addressof(layer.c), kc, vc, row, pos, max_ctx, _ptr(h), _ptr(delta), _ptr(y), eps,
+        _ptr(ws.decode), _ptr(weights), _ptr(scratch.ws), scratch.nbytes, _stream(stream)))
+
+
+def layer_prefill_weights(layer: Layer, k_cache, v_cache, max_ctx: int, row0: int, pos0: int,
+                          n: int, h, delta, y, eps: float, ws: LayerWorkspace, weights,
+                          scratch: PrefillWeightsScratch, voters: Optional[int] = None,
+                          stream=None) -> None:
+    """layer_prefill over a bounded cache: tokens of positions pos0 .. at rows row0 ..; the last
+    `voters` of them (None: all) add the weights they give the rows they see to weights."""
+    for name, x in (("row0", row0), ("pos0", pos0), ("n", n), ("max_ctx", max_ctx)):
+        _count(x, name)
+    voters = n if voters is None else min(_count(voters, "voters"), n)
+    if voters > scratch.max_n or row0 + n > scratch.max_rows:
+        raise ValueError("voters or row0 + n exceeds the scratch capacity")
+    _rows(n, h=h, delta=delta, y=y)
+    _need(weights, "weights", torch.float32, KV_HEADS * max_ctx)
+    kc, vc = _layer_cache(k_cache, v_cache, max_ctx)
+    _here(h, y, k_cache, v_cache, weights, scratch.ws, ws.prefill)
+    _lib.check(_lib.load().miso_attn_layer_prefill_weights(
+        ctypes.addressof(layer.c), kc, vc, row0, pos0, n, max_ctx, _ptr(h), _ptr(delta), _ptr(y),
+        eps, _ptr(ws.prefill), ws.max_tok, voters, _ptr(weights), _ptr(scratch.ws),
+        scratch.ws.numel(), _stream(stream)))

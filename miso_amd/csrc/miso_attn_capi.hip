@@ -1057,10 +1057,15 @@ const char* bad_decode_weights(const float* weights, const void* workspace, uint
 int combine_weights(const char* fn, const float* part_m, const float* part_l, const float* part_o,
                     const float* qg, float* core, float* weights, const float* ws, uint32_t len,
                     uint32_t max_ctx, uint32_t n_splits, void* stream) {
-  const k::AttnWeightsParams p{{part_m, part_l, part_o, qg, core, n_splits}, ws, weights, len,
-                               max_ctx};
-  const unsigned blocks = (len + k::kWeightKeys - 1) / k::kWeightKeys;
-  k::attn_combine_weights_kernel<><<<k::kCombineItems + 2 * blocks, 64, 0, as_stream(stream)>>>(p);
+  const k::AttnWeightsParams p{{part_m, part_l, part_o, qg, core, n_splits},
+                               ws,
+                               weights,
+                               len,
+                               max_ctx,
+                               nullptr,
+                               nullptr};
+  k::attn_combine_weights_kernel<>
+      <<<k::attn_combine_weights_grid(len, false), 64, 0, as_stream(stream)>>>(p);
   return launched(fn);
 }
 
@@ -1280,6 +1285,62 @@ int miso_attn_evict_gather_fp8(const uint8_t* k8, const uint8_t* v8, const float
   return gather<true>(fn, {k8, v8, weights, index, k8_out, v8_out, weights_out, max_ctx, keep,
                            out_ctx, k_scale, v_scale, k_scale_out, v_scale_out},
                       stream);
+}
+
+int miso_attn_layer_decode_weights(const miso_attn_layer* layer, uint16_t* k_cache,
+                                   uint16_t* v_cache, uint32_t row, uint32_t pos,
+                                   uint32_t max_ctx, float* h, const float* delta, float* y,
+                                   float eps, float* ws, float* weights, void* workspace,
+                                   uint64_t workspace_bytes, void* stream) {
+  constexpr const char* fn = "miso_attn_layer_decode_weights";
+  k::layer::Weights w;
+  if (const char* err = layer_view(layer, w))
+    return fail(fn, err);
+  if (any_bad(k_cache, v_cache, h, y, ws) || (delta != nullptr && bad_ptr(delta)))
+    return fail(fn, kBadPtr);
+  if (row >= max_ctx)
+    return fail(fn, "KV cache is full (row >= max_ctx)");
+  if (const char* err = bad_decode_weights(weights, workspace, workspace_bytes, row + 1, max_ctx,
+                                           k::attn_n_splits(row + 1, k::layer::kMaxSplits)))
+    return fail(fn, err);
+  return layer_result(fn, k::layer::decode_step_weights(
+                              w, as_half(k_cache), as_half(v_cache), row, pos, max_ctx, h, delta,
+                              y, eps, k::layer::decode_workspace(ws), weights,
+                              static_cast<float*>(workspace), as_stream(stream)));
+}
+
+int miso_attn_layer_prefill_weights(const miso_attn_layer* layer, uint16_t* k_cache,
+                                    uint16_t* v_cache, uint32_t row0, uint32_t pos0, uint32_t n,
+                                    uint32_t max_ctx, float* h, const float* delta, float* y,
+                                    float eps, float* ws, uint32_t max_tok, uint32_t voters,
+                                    float* weights, void* workspace, uint64_t workspace_bytes,
+                                    void* stream) {
+  constexpr const char* fn = "miso_attn_layer_prefill_weights";
+  if (n == 0)
+    return 0;
+  k::layer::Weights w;
+  if (const char* err = layer_view(layer, w))
+    return fail(fn, err);
+  if (any_bad(k_cache, v_cache, h, y, ws) || (delta != nullptr && bad_ptr(delta)))
+    return fail(fn, kBadPtr);
+  if (static_cast<uint64_t>(row0) + n > max_ctx)
+    return fail(fn, "KV cache is full (row0 + n > max_ctx)");
+  if (static_cast<uint64_t>(pos0) + n > 0xFFFFFFFFull || pos0 < row0)
+    return fail(fn, "pos0 must be at least row0, and pos0 + n below 2^32");
+  if (n > max_tok)
+    return fail(fn, "chunk does not fit the prefill workspace");
+  const uint32_t m = std::min(voters, n);
+  if (m != 0) {
+    if (bad_scalars(weights))
+      return fail(fn, kBadPtr);
+    if (const char* err =
+            bad_key_weights(workspace, workspace_bytes, row0 + n - m, m, max_ctx, false))
+      return fail(fn, err);
+  }
+  return layer_result(fn, k::layer::prefill_step_weights(
+                              w, as_half(k_cache), as_half(v_cache), row0, pos0, n, max_ctx, h,
+                              delta, y, eps, k::layer::prefill_workspace(ws, max_tok), max_tok, m,
+                              weights, workspace, as_stream(stream)));
 }
 
 }  // extern "C"

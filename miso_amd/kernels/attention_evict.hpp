@@ -67,6 +67,32 @@ attn_split_scores_kernel(AttnSplitParams p, float* ws) {
                                             base, sh, false, 0u, sc);
 }
 
+// attn_prep_split_kernel (a layer step's split, the token prepared in it), the scores stored. The
+// token's row is s.len - 1, its rotation p.rope's. Grid dim3(n_splits, 2) x 256.
+template <int kBlock>
+__global__ void __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(1, 1)))
+attn_prep_split_scores_kernel(AttnPrepSplitParams p, float* ws) {
+  static_assert(kBlock == 256, "four waves per split workgroup");
+  using namespace decode_detail;
+  __shared__ TileShared sh;
+  __shared__ __attribute__((aligned(16))) PrepShared ps;
+  const unsigned split = blockIdx.x, kvh = blockIdx.y;
+  const std::size_t head = std::size_t{kvh} * p.s.max_ctx * attn::kDim;
+  const std::size_t row = head + std::size_t{p.s.len - 1} * attn::kDim;
+  const AttnSpan span = attn_split_span(p.s.len, p.s.n_splits, split);
+  const LinearTiles tl{p.s.k_cache + head, p.s.v_cache + head};
+  const std::size_t base = std::size_t{kvh} * p.s.n_splits + split;
+  const PrepQuery q{p.proj, p.q_norm, p.k_norm, p.rope,
+                    split == 0 ? p.q + std::size_t{kvh} * kGroup * attn::kDim : nullptr,
+                    p.k_cache + row, p.v_cache + row, &ps, p.eps, p.s.len - 1};
+  const SplitScores sc = scores_of(ws, p.s.len, p.s.n_splits, kvh);
+  if (span.end - span.begin > kSplitWavesMinKeys)  // as attn_prep_split_kernel
+    split_partial_waves(q, tl, span, kvh, p.s.part_m, p.s.part_l, p.s.part_o, base, sh, false, sc);
+  else
+    split_partial_tiles<LinearTiles, false>(q, tl, span, kvh, p.s.part_m, p.s.part_l, p.s.part_o,
+                                            base, sh, false, 0u, sc);
+}
+
 // attn_split_fp8_kernel, the scores stored. Grid dim3(n_splits, 2) x 256.
 template <int kBlock>
 __global__ void __launch_bounds__(kBlock) attn_split_fp8_scores_kernel(AttnSplitFp8Params p,
@@ -88,14 +114,19 @@ struct AttnWeightsParams {
   const float* ws;   // the split's workspace (attn_decode_weights_floats)
   float* weights;    // [2][max_ctx]
   unsigned len, max_ctx;
+  float* h;            // a layer step's residual row [2048]: h += delta; nullptr: none
+  const float* delta;
 };
 
 constexpr unsigned kCombineItems = attn::kQHeads * (attn::kDim / 64);  // 64-thread workgroups
 constexpr unsigned kWeightKeys = 256;  // keys per workgroup of the weights' part
 
-// Workgroups [0, 64): attn_combine_kernel's; the others one 256-key block of one KV head each:
-// every lane forms the head statistics from the splits' and adds 4 keys' weights, 64 apart. Grid
-// 64 + 2 ceil(len / 256), x 64.
+// Workgroups [0, 64): attn_combine_kernel's; with h, 8 more for the residual row; the others one
+// 256-key block of one KV head each: every lane forms the head statistics from the splits' and adds
+// 4 keys' weights, 64 apart. Grid attn_combine_weights_grid, x 64.
+__host__ __device__ constexpr unsigned attn_combine_weights_grid(unsigned len, bool add) {
+  return kCombineItems + (add ? 8 : 0) + 2 * (len / kWeightKeys + (len % kWeightKeys != 0));
+}
 template <int = 0>
 __global__ void __launch_bounds__(64) attn_combine_weights_kernel(AttnWeightsParams p) {
   using decode_detail::kGroup;
@@ -103,8 +134,16 @@ __global__ void __launch_bounds__(64) attn_combine_weights_kernel(AttnWeightsPar
     attn_combine_op<64, true, 4>(p.c, 0, kCombineItems);
     return;
   }
-  const unsigned item = blockIdx.x - kCombineItems, lane = threadIdx.x;
-  const unsigned blocks = (p.len + kWeightKeys - 1) / kWeightKeys;
+  const unsigned lane = threadIdx.x, adds = p.h != nullptr ? 8 : 0;
+  if (blockIdx.x < kCombineItems + adds) {
+    const unsigned e = 256 * (blockIdx.x - kCombineItems) + 4 * lane;
+    const float4 a = *reinterpret_cast<const float4*>(p.h + e);
+    const float4 d = *reinterpret_cast<const float4*>(p.delta + e);
+    *reinterpret_cast<float4*>(p.h + e) = float4{a.x + d.x, a.y + d.y, a.z + d.z, a.w + d.w};
+    return;
+  }
+  const unsigned item = blockIdx.x - kCombineItems - adds;
+  const unsigned blocks = p.len / kWeightKeys + (p.len % kWeightKeys != 0);
   const unsigned kvh = item / blocks, k0 = (item % blocks) * kWeightKeys + lane;
   const unsigned n = p.c.n_splits;
   const std::size_t stride = attn_scores_stride(p.len);
@@ -998,15 +1037,16 @@ __device__ __attribute__((always_inline)) inline unsigned place_wave(SelectShare
   return before + (same < want ? same : want) - kept;
 }
 
-// Writes the kept rows of 64, row `row` of rank `rank` this lane's, from out[at] on.
-__device__ __attribute__((always_inline)) inline void write_kept(int* out, unsigned& at,
-                                                                unsigned& same, unsigned want,
-                                                                unsigned rank, unsigned last,
-                                                                unsigned row) {
+// Writes the kept rows of 64, row `row` of rank `rank` this lane's, from out[at] on; never past
+// `keep` of them, which only weights that change under the selection could ask for.
+__device__ __attribute__((always_inline)) inline void write_kept(int* out, unsigned keep,
+                                                                unsigned& at, unsigned& same,
+                                                                unsigned want, unsigned rank,
+                                                                unsigned last, unsigned row) {
   const unsigned long long equal = __builtin_amdgcn_ballot_w64(rank == last);
-  const bool keep = rank > last || (rank == last && same + lanes_below(equal) < want);
-  const unsigned long long kept = __builtin_amdgcn_ballot_w64(keep);
-  if (keep)
+  const bool mine = rank > last || (rank == last && same + lanes_below(equal) < want);
+  const unsigned long long kept = __builtin_amdgcn_ballot_w64(mine);
+  if (mine && at + lanes_below(kept) < keep)
     out[at + lanes_below(kept)] = static_cast<int>(row);
   at += __popcll(kept);
   same += __popcll(equal);
@@ -1057,7 +1097,7 @@ __global__ void __launch_bounds__(1024) attn_evict_select_kernel(AttnEvictSelect
   int* out = p.index + std::size_t{kvh} * p.keep;
 #pragma unroll
   for (unsigned i = 0; i < R; ++i)
-    write_kept(out, at, same, want, rank[i], last, row0 + 64 * i);
+    write_kept(out, p.keep, at, same, want, rank[i], last, row0 + 64 * i);
 }
 
 // Longer caches: `groups` workgroups per head, p.rows rows each, in four launches, a digit each and
@@ -1202,7 +1242,7 @@ __global__ void __launch_bounds__(1024) attn_evict_select_part_kernel(AttnEvictS
         load(from);
 #pragma unroll
       for (unsigned i = 0; i < kChunk / 64; ++i)
-        write_kept(out, at, same, want, rank_at(from, i), last, from + 64 * i + lane);
+        write_kept(out, p.keep, at, same, want, rank_at(from, i), last, from + 64 * i + lane);
     }
   }
 }

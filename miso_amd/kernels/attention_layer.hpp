@@ -34,6 +34,7 @@
 #include <cstdint>
 
 #include "attention_decode.hpp"
+#include "attention_evict.hpp"
 #include "attention_prefill.hpp"
 #include "cdna4_wave.hpp"
 #include "mixed_gemv.hpp"
@@ -466,13 +467,65 @@ inline const char* decode_step(const Weights& w, attn::half_t* k_cache, attn::ha
   return gemv(w.o, ws.core, y, stream);
 }
 
+// Whole rows of an f16 cache away: row pos of the moved cache is row `row` of the given one, in both KV
+// heads (the head stride stays), so that a prep for position pos appends at `row`.
+inline attn::half_t* moved_cache(attn::half_t* cache, unsigned row, unsigned pos) {
+  return reinterpret_cast<attn::half_t*>(
+      reinterpret_cast<std::uintptr_t>(cache) +
+      static_cast<std::uintptr_t>((std::int64_t{row} - std::int64_t{pos}) *
+                                  std::int64_t{attn::kDim * sizeof(attn::half_t)}));
+}
+
+// The decode step over a bounded cache: the token of position pos is appended at row `row`, attends to
+// rows [0, row], and adds the weights it gives them to weights [2][max_ctx]; wws:
+// attn_decode_weights_floats(row + 1, kMaxSplits) floats. decode_step's launches, with the scores
+// stored by the split and turned into weights beside the merge.
+inline const char* decode_step_weights(const Weights& w, attn::half_t* k_cache,
+                                       attn::half_t* v_cache, unsigned row, unsigned pos,
+                                       unsigned max_ctx, float* h, const float* delta, float* y,
+                                       float eps, const DecodeWorkspace& ws, float* weights,
+                                       float* wws, hipStream_t stream) {
+  if (row >= max_ctx)
+    return "KV cache is full";
+  const unsigned keys = row + 1, n_splits = attn_n_splits(keys, kMaxSplits);
+  const AttnSplitParams split{ws.q,      k_cache,   v_cache, ws.part_m, ws.part_l,
+                              ws.part_o, keys,      max_ctx, n_splits};
+  AttnWeightsParams comb{{ws.part_m, ws.part_l, ws.part_o, ws.proj, ws.core, n_splits},
+                         wws, weights, keys, max_ctx, nullptr, nullptr};
+  if (qkv_mix(w) && row >= 1) {  // as decode_step
+    qkv_norm_launch(w, h, delta, eps, pos, ws.xn, ws.core, ws.proj, stream);
+    attn_prep_split_scores_kernel<256><<<dim3(n_splits, 2), 256, 0, stream>>>(
+        AttnPrepSplitParams{split, ws.proj, w.q_norm, w.k_norm, ws.core, ws.q, k_cache, v_cache,
+                            eps},
+        wws);
+    if (delta != nullptr) {
+      comb.h = h;
+      comb.delta = delta;
+    }
+  } else {
+    add_rmsnorm_kernel<false><<<1, 256, 0, stream>>>(
+        AddRmsNormParams{h, delta, w.attn_norm, ws.xn, nullptr, nullptr, eps});
+    if (const char* err = project_qkv(w, ws.xn, ws.proj, stream))
+      return err;
+    attn_prep_kernel<256><<<18, 256, 0, stream>>>(
+        AttnPrepParams{ws.proj, ws.proj + 8192, ws.proj + 8704, w.q_norm, w.k_norm, w.inv_freq,
+                       moved_cache(k_cache, row, pos), moved_cache(v_cache, row, pos), ws.q, pos,
+                       max_ctx, eps});
+    attn_split_scores_kernel<256><<<dim3(n_splits, 2), 256, 0, stream>>>(split, wws);
+  }
+  attn_combine_weights_kernel<>
+      <<<attn_combine_weights_grid(keys, comb.h != nullptr), 64, 0, stream>>>(comb);
+  return gemv(w.o, ws.core, y, stream);
+}
+
 // n consecutive tokens at pos0 ([n][2048] h / delta / y): the prefill GEMMs, batched prep and
-// causal flash attention over the cache up to each token (attn_prefill_launch).
+// causal flash attention over the cache up to each token (attn_prefill_launch). Over a shortened
+// cache the tokens' positions are `ahead` of their rows.
 inline const char* prefill_step(const Weights& w, attn::half_t* k_cache, attn::half_t* v_cache,
                                 unsigned pos0, unsigned n, unsigned max_ctx, float* h,
                                 const float* delta, float* y, float eps,
                                 const PrefillWorkspace& ws, unsigned max_tok,
-                                hipStream_t stream) {
+                                hipStream_t stream, unsigned ahead = 0) {
   if (n == 0)
     return nullptr;
   if (n > max_tok)
@@ -484,8 +537,10 @@ inline const char* prefill_step(const Weights& w, attn::half_t* k_cache, attn::h
   if (const char* err = gemm(ws.xh, ws.xs, n, kProj, stream, GemmOut{w.q, ws.proj},
                              GemmOut{w.k, ws.proj + 8192}, GemmOut{w.v, ws.proj + 8704}))
     return err;
+  const unsigned at = pos0 + ahead;
   const AttnPrepBatchParams prep{{ws.proj, ws.proj + 8192, ws.proj + 8704, w.q_norm, w.k_norm,
-                                  w.inv_freq, k_cache, v_cache, ws.q, pos0, max_ctx, eps},
+                                  w.inv_freq, moved_cache(k_cache, pos0, at),
+                                  moved_cache(v_cache, pos0, at), ws.q, at, max_ctx, eps},
                                  n,
                                  kProj};
   prep_tokens_kernel<><<<n, 256, 0, stream>>>(prep);
@@ -493,6 +548,26 @@ inline const char* prefill_step(const Weights& w, attn::half_t* k_cache, attn::h
   attn_prefill_launch(ap, ws.balance, prefill_balance_floats(max_tok) * sizeof(float), stream);
   gemm_input(ws.core, kCore, n, ws.xh, ws.xs, stream);
   return gemm(ws.xh, ws.xs, n, kHidden, stream, GemmOut{w.o, y});
+}
+
+// prefill_step over a bounded cache: tokens of positions pos0 .. at rows row0 .., the last `voters` of
+// which (all, where there are fewer) add the weights they give the rows they see; kws:
+// attn_key_weights_layout(row0 + n - voters, voters, false).bytes.
+inline const char* prefill_step_weights(const Weights& w, attn::half_t* k_cache,
+                                        attn::half_t* v_cache, unsigned row0, unsigned pos0,
+                                        unsigned n, unsigned max_ctx, float* h,
+                                        const float* delta, float* y, float eps,
+                                        const PrefillWorkspace& ws, unsigned max_tok,
+                                        unsigned voters, float* weights, void* kws,
+                                        hipStream_t stream) {
+  if (const char* err = prefill_step(w, k_cache, v_cache, row0, n, max_ctx, h, delta, y, eps, ws,
+                                     max_tok, stream, pos0 - row0))
+    return err;
+  const unsigned m = voters < n ? voters : n;
+  if (m != 0)
+    attn_key_weights_launch(ws.q + std::size_t{n - m} * kCore, k_cache, nullptr, nullptr, weights,
+                            row0 + n - m, m, max_ctx, kws, stream);
+  return nullptr;
 }
 
 // n tokens at pos0 through the layer, the engine's policy (src/engine/model.hip:130-175 for this
