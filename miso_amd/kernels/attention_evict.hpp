@@ -561,9 +561,10 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
         p.sums[(std::size_t{lin} * p.row_tiles + ti) * kKeys + lane] = all;
       }
     };
-    // K-step s of tile ti: the address is kl ^ 32 s of its stage; kl has no bit of 256.
+    // K-step s of tile ti, at kl ^ 32 s of its stage (the ring is 1 KiB aligned, so the bits that
+    // change are kl's own; kl has no bit of 256).
     auto read = [&](unsigned ti, unsigned s) __attribute__((always_inline)) {
-      return decode_detail::lds_b128((((ring + ti % kStages * kTileBytes) | kl) ^ (32u * (s % 8))) +
+      return decode_detail::lds_b128(((ring + ti % kStages * kTileBytes + kl) ^ (32u * (s % 8))) +
                                      32u * (s & 8u));
     };
     // The scores of tile ti into cur and the weights of tile ti - 1, whose scores prev holds. Between

@@ -155,7 +155,8 @@ def test_decode_weights_peaked(attn):
 
 
 CHUNKS = [(0, 1), (0, 2), (5, 1), (0, 4), (0, 5), (0, 33), (31, 2), (32, 1), (61, 7), (1000, 3),
-          (100, 301), (12001, 33), (0, 1024), (77, 1500), (3000, 2049)]
+          (100, 301), (12001, 33), (0, 1024), (77, 1500), (3000, 2049), (4100, 17), (5003, 300),
+          (40000, 3)]
 
 
 @pytest.mark.parametrize("pos0,n", CHUNKS)
@@ -195,6 +196,19 @@ def test_prefill_weights_with_a_larger_scratch(attn):
         attn.attn_prefill_weights(q, kc, w, pos0, n, 2000, sc)
         added, rel = weights64(q, kc[:, :rows].double(), pos0)
         check(w[:, :rows], torch.zeros_like(w[:, :rows]), added, rel, (pos0, n))
+
+
+def test_prefill_weights_in_pieces(attn):
+    """A chunk over a cache so long that it runs in two pieces."""
+    g = gen(10)
+    pos0, n = 66000, 4000
+    rows = pos0 + n
+    kc, _ = f16_cache(g, rows, rows)
+    q = 2.0 * randn(g, n, H, D)
+    w = torch.zeros(KV, rows, device="cuda")
+    attn.attn_prefill_weights(q, kc, w, pos0, n, rows, attn.PrefillWeightsScratch(n, rows))
+    added, rel = weights64(q, kc.double(), pos0)
+    check(w, torch.zeros_like(w), added, rel)
 
 
 def test_prefill_weights_query_magnitudes(attn):
@@ -515,6 +529,71 @@ def test_captured_and_replayed(attn):
         torch.cuda.synchronize()
         for a, b in zip(got, (core, w, index, ko, vo, wo)):
             assert torch.equal(a, b)
+
+
+def test_two_graphs_of_one_scratch(attn):
+    """Two graphs captured over the same scratches, replayed in turn with eager calls between."""
+    g = gen(32)
+    n = 9000
+    k, v = f16_cache(g, n, n)
+    q, qg = 2.0 * randn(g, 70, H, D), randn(g, H, 2, D)
+    sc, psc, esc = (attn.DecodeWeightsScratch(128, n), attn.PrefillWeightsScratch(70, n),
+                    attn.EvictScratch(40000))
+
+    def make(length, voters, keep):
+        w, core = torch.zeros(KV, n, device="cuda"), torch.empty(H, D, device="cuda")
+        index = torch.zeros(KV, keep, dtype=torch.int32, device="cuda")
+
+        def step():
+            attn.attn_prefill_weights(q, k, w, length - voters, voters, n, psc)
+            attn.attn_decode_weights(q, qg, k, v, core, w, sc, length, n)
+            attn.attn_evict_select(w, length, n, keep, 1, 8, index, esc)
+        return step, (w, core, index)
+
+    both = [make(n, 70, 4000), make(701, 3, 64)]
+    graphs = []
+    for step, _ in both:
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        graphs.append(graph)
+    for _ in range(3):
+        for (step, out), graph in zip(both, graphs):
+            out[0].zero_()
+            graph.replay()
+            got = [t.clone() for t in out]
+            out[0].zero_()
+            step()
+            torch.cuda.synchronize()
+            for a, b in zip(got, out):
+                assert torch.equal(a, b)
+
+
+def test_weights_and_indexes_need_no_alignment(attn):
+    """Weights and indexes one element past an aligned address: the results of aligned ones."""
+    g = gen(33)
+    n, keep = 5001, 1203
+    k, v = f16_cache(g, n, n)
+    q, qg = 2.0 * randn(g, 20, H, D), randn(g, H, 2, D)
+    core = torch.empty(H, D, device="cuda")
+    sc, psc, esc = (attn.DecodeWeightsScratch(128, n), attn.PrefillWeightsScratch(20, n),
+                    attn.EvictScratch(n))
+    ko, vo = (torch.zeros(KV, keep, D, dtype=torch.float16, device="cuda") for _ in range(2))
+
+    def run(off):
+        w = torch.zeros(KV * n + 8, device="cuda")[off:off + KV * n]
+        wo = torch.zeros(KV * keep + 8, device="cuda")[off:off + KV * keep]
+        index = torch.zeros(KV * keep + 8, dtype=torch.int32, device="cuda")[off:off + KV * keep]
+        attn.attn_prefill_weights(q, k, w, n - 20, 20, n, psc)
+        attn.attn_decode_weights(q, qg, k, v, core, w, sc, n, n)
+        attn.attn_evict_select(w, n, n, keep, 4, 100, index, esc)
+        attn.attn_evict_gather(k, v, w, n, index, keep, ko, vo, wo, keep)
+        return [t.clone() for t in (w, wo, index, ko, vo)]
+
+    for a, b in zip(run(0), run(1)):
+        assert torch.equal(a, b)
 
 
 def test_two_streams_with_scratches_of_their_own(attn):
