@@ -521,8 +521,8 @@ def attn_decode_weights(q, qg, k_cache, v_cache, core, weights, scratch: DecodeW
     softmax weights that KV head g's 8 query heads give row j. Returns n_splits used."""
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         _need(t, name, _cache_dtype(t), KV_HEADS * max_ctx * DIM)
-    return _decode_weights(_lib.load().miso_attn_decode_weights, q, qg, (k_cache, v_cache), core, weights,
-                           scratch, length, max_ctx, n_splits, stream)
+    return _decode_weights(_lib.load().miso_attn_decode_weights, q, qg, (k_cache, v_cache), core,
+                           weights, scratch, length, max_ctx, n_splits, stream)
 
 
 def attn_decode_weights_fp8(q, qg, cache: Fp8Cache, core, weights, scratch: DecodeWeightsScratch,
@@ -864,7 +864,8 @@ def layer_decode_weights(layer: Layer, k_cache, v_cache, max_ctx: int, row: int,
     _rows(1, h=h, delta=delta, y=y)
     _need(weights, "weights", torch.float32, KV_HEADS * max_ctx)
     kc, vc = _layer_cache(k_cache, v_cache, max_ctx)
-    _here(h, y, k_cache, v_cache, weights, scratch.ws, ws.decode)
+    _here(h, y, k_cache, v_cache, weights, scratch.ws, ws.decode,
+          *(() if delta is None else (delta,)))
     _lib.check(_lib.load().miso_attn_layer_decode_weights(
         ctypes.addressof(layer.c), kc, vc, row, pos, max_ctx, _ptr(h), _ptr(delta), _ptr(y), eps,
         _ptr(ws.decode), _ptr(weights), _ptr(scratch.ws), scratch.nbytes, _stream(stream)))
@@ -884,7 +885,8 @@ def layer_prefill_weights(layer: Layer, k_cache, v_cache, max_ctx: int, row0: in
     _rows(n, h=h, delta=delta, y=y)
     _need(weights, "weights", torch.float32, KV_HEADS * max_ctx)
     kc, vc = _layer_cache(k_cache, v_cache, max_ctx)
-    _here(h, y, k_cache, v_cache, weights, scratch.ws, ws.prefill)
+    _here(h, y, k_cache, v_cache, weights, scratch.ws, ws.prefill,
+          *(() if delta is None else (delta,)))
     _lib.check(_lib.load().miso_attn_layer_prefill_weights(
         ctypes.addressof(layer.c), kc, vc, row0, pos0, n, max_ctx, _ptr(h), _ptr(delta), _ptr(y),
         eps, _ptr(ws.prefill), ws.max_tok, voters, _ptr(weights), _ptr(scratch.ws),

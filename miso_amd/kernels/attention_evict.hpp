@@ -25,6 +25,11 @@ namespace miso::kernels {
 // M and L are known only once every split is done, so the split stores its scores (64 bytes per
 // key, both KV heads, beside the 2048 it reads) and the launch that merges the partials also turns
 // them into weights. The result of the attention is attn_decode's, bit for bit.
+//
+// Bound by the K and V stream, as attn_decode: 32768 keys take 18.8 us against 18.7 without
+// weights, 262144 103.8 against 88.5 (5.2 TB/s of what must move), of which 9 are the score stores
+// among the loads and 5.5 the merge's; 301 keys 10.8, two launches and the host's call. 100003 e4m3
+// keys 30.2.
 // ------------------------------------------------------------------------------------------------
 
 // The scores' row length for len keys: the padding lets a span store whole groups of 4.
@@ -123,7 +128,9 @@ constexpr unsigned kWeightKeys = 256;  // keys per workgroup of the weights' par
 
 // Workgroups [0, 64): attn_combine_kernel's; with h, 8 more for the residual row; the others one
 // 256-key block of one KV head each: every lane forms the head statistics from the splits' and adds
-// 4 keys' weights, 64 apart. Grid attn_combine_weights_grid, x 64.
+// 4 keys' weights, 64 apart (blocks of 64 threads, so that few keys still fill many CUs and the
+// scores are asked for before the statistics are joined). 3.6 us at 301 keys, 4.2 at 32768, 9.9 at
+// 262144: the stream of the scores. Grid attn_combine_weights_grid, x 64.
 __host__ __device__ constexpr unsigned attn_combine_weights_grid(unsigned len, bool add) {
   return kCombineItems + (add ? 8 : 0) + 2 * (len / kWeightKeys + (len % kWeightKeys != 0));
 }
@@ -228,8 +235,15 @@ __global__ void __launch_bounds__(64) attn_combine_weights_kernel(AttnWeightsPar
 // sum stay in a lane), in the second the columns in registers and the keys in lanes (a key's sum
 // over the block is 16 adds).
 //
-// The work of a pass is the tiles of (KV head, group), laid end to end and cut into equal spans, one
-// per workgroup: causal groups differ in length, and a span takes up where the one before it ends.
+// The work of a pass is the tiles of (KV head, group), laid end to end and cut into equal spans,
+// one per workgroup: causal groups differ in length, and a span takes up where the one before it
+// ends.
+//
+// Measured: 8192 tokens after 8192 in 2.55-2.65 ms, 1240-1300 TFLOP/s of f16 products (1.3 ms a
+// pass, the matrix units busy in 73 and 77% of the cycles; zeros for data take 1.88 ms, so the
+// card's power is what bounds it); 2048 tokens 99 us (passes of 43, half of each the start of its
+// spans); 1001 after 5003 e4m3 rows 164; 33 after 12001 38.8 us (four launches; passes of 17 and
+// 20, a quarter of them in tiles).
 // ------------------------------------------------------------------------------------------------
 
 struct AttnKeyWeightsParams {
@@ -328,11 +342,12 @@ struct Halves {
 
 }  // namespace weights_detail
 
-// The queries' halves and scales. One workgroup of 4 waves per (KV head, column block): wave w reads
-// columns 8 w .. 8 w + 7, one row of 1 KiB an instruction, and the halves go out through LDS in the
-// order of the operands, 16 bytes a lane. In LDS the 512 bytes of a k-step's half (s, dimension /
-// 8 % 2) are 528 apart, so that the 32 of them that one row touches lie in different banks.
-// Padding columns are zero.
+// The queries' halves and scales. One workgroup of 4 waves per (KV head, column block): wave w
+// reads columns 8 w .. 8 w + 7, one row of 1 KiB an instruction, and the halves go out through LDS
+// in the order of the operands, 16 bytes a lane. In LDS the 512 bytes of a k-step's half (s,
+// dimension / 8 % 2) are 528 apart, so that the 32 of them that one row touches lie in different
+// banks. Padding columns are zero. Bound by memory, 8 bytes per query element: 42 us for 8192
+// tokens (268 MB), 11 for 2048.
 template <int = 0>
 __global__ void __launch_bounds__(256) attn_key_weights_cut_kernel(AttnKeyWeightsParams p) {
   using namespace weights_detail;
@@ -431,7 +446,8 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
   for (bool again = false; x < x_end; again = true) {
     const unsigned tiles = group_tiles(W, p.pos0, group);
     const unsigned first = tile;
-    const unsigned past = tiles - first < x_end - x ? tiles : first + static_cast<unsigned>(x_end - x);
+    const unsigned past =
+        tiles - first < x_end - x ? tiles : first + static_cast<unsigned>(x_end - x);
     const attn::half_t* K = p.k_cache + std::size_t{kvh} * p.k_ctx * attn::kDim;
     // Tile ti into its stage: this wave copies rows 32 / W wave .. , two an instruction.
     constexpr unsigned kCopies = kKeys / W / 2;
@@ -567,10 +583,10 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
       return decode_detail::lds_b128(((ring + ti % kStages * kTileBytes + kl) ^ (32u * (s % 8))) +
                                      32u * (s & 8u));
     };
-    // The scores of tile ti into cur and the weights of tile ti - 1, whose scores prev holds. Between
-    // two matrix instructions stand one fma, one exponential and one sum, of three neighbouring
-    // weights, so that none waits for another; the next copies and the sums of a run of tiles go
-    // behind the first matrix instructions.
+    // The scores of tile ti into cur and the weights of tile ti - 1, whose scores prev holds.
+    // Between two matrix instructions stand one fma, one exponential and one sum, of three
+    // neighbouring weights, so that none waits for another; the next copies and the sums of a run
+    // of tiles go behind the first matrix instructions.
     auto step = [&](float16_t& cur, float16_t& prev, unsigned ti) __attribute__((always_inline)) {
       mask(prev, ti - 1);
       part[0] = part[1] = part[2] = part[3] = 0.0f;
@@ -631,7 +647,8 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
         a[s] = read(first, s);
 #pragma unroll
       for (unsigned s = 0; s < kSteps; ++s) {
-        const cdna4::half8_t next = s + 4 < kSteps ? read(first, s + 4) : read(first + 1, s + 4 - kSteps);
+        const cdna4::half8_t next =
+            s + 4 < kSteps ? read(first, s + 4) : read(first + 1, s + 4 - kSteps);
         const float16_t from = s == 0 ? float16_t{} : acc[0];
         acc[0] = kSum ? mfma32(b.hi[s], a[s % 4], from) : mfma32(a[s % 4], b.hi[s], from);
         acc[0] = kSum ? mfma32(b.lo[s], a[s % 4], acc[0]) : mfma32(a[s % 4], b.lo[s], acc[0]);
@@ -669,8 +686,8 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
     }
     if constexpr (kSum) {
       decode_detail::tile_barrier();
-      // The last run, and the one before it where that ended with tile past - 2 (its turn to be taken
-      // would have come with a tile `past`).
+      // The last run, and the one before it where that ended with tile past - 2 (its turn to be
+      // taken would have come with a tile `past`).
       if (past % W == 1 && past - first > 1)
         take((past - 2) / W);
       take((past - 1) / W);
@@ -688,7 +705,8 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
 }
 
 // weights += the groups' sums, in a fixed order: one workgroup per (KV head, tile of rows), 8
-// slices of the groups that hold the tile, joined in slice order.
+// slices of the groups that hold the tile, joined in slice order. Bound by memory: 256 groups over
+// 16384 rows (8192 tokens after 8192, 25 MB of sums) 6.9 us.
 template <unsigned W>
 __global__ void __launch_bounds__(256) attn_key_weights_join_kernel(AttnKeyWeightsParams p) {
   using namespace weights_detail;
@@ -713,8 +731,8 @@ __global__ void __launch_bounds__(256) attn_key_weights_join_kernel(AttnKeyWeigh
   p.weights[std::size_t{kvh} * p.max_ctx + key] += v;
 }
 
-// K codes [2][max_ctx][256] widened to f16 [2][n][256] (attn_kv_fp8_widen_kernel's values, K alone).
-// One wave per row, 4 per workgroup, grid-stride.
+// K codes [2][max_ctx][256] widened to f16 [2][n][256] (attn_kv_fp8_widen_kernel's values, K
+// alone). One wave per row, 4 per workgroup, grid-stride.
 template <int = 0>
 __global__ void __launch_bounds__(256) attn_k_fp8_widen_kernel(const uint8_t* k8,
                                                                const float* k_scale,
@@ -739,12 +757,12 @@ __global__ void __launch_bounds__(256) attn_k_fp8_widen_kernel(const uint8_t* k8
   }
 }
 
-// How a chunk is cut: column blocks, the waves W of a workgroup, the groups, and the spans of a pass.
-// W = 8 is one workgroup per CU, W = 4 two, which hide each other's starts and barriers but stream K
-// twice. Two are faster while K stays in an XCD's L2 (2048 tokens: 110 us against 120; 1000 after
-// 1000: 74.7 against 75.0), slower beyond (2048 after 12001: 855 against 794), except for few
-// blocks that fill groups of 4 better by more than that (33 tokens after 40000, 9 blocks: 86 against
-// 94; 17 after 40000, 5 blocks: 70 against 60).
+// How a chunk is cut: column blocks, the waves W of a workgroup, the groups, and the spans of a
+// pass. W = 8 is one workgroup per CU, W = 4 two, which hide each other's starts and barriers but
+// stream K twice. Two are faster while K stays in an XCD's L2 (2048 tokens: 110 us against 120;
+// 1000 after 1000: 74.7 against 75.0), slower beyond (2048 after 12001: 855 against 794), except
+// for few blocks that fill groups of 4 better by more than that (33 tokens after 40000, 9 blocks:
+// 86 against 94; 17 after 40000, 5 blocks: 70 against 60).
 struct AttnKeyWeightsCut {
   unsigned blocks, waves, groups, row_tiles, spans;
   unsigned long long span;
@@ -900,11 +918,14 @@ inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
 // keep - sinks - recent of the largest weight; of equal weights the lower row. A NaN ranks below
 // every number, -0 equals +0. index [2][keep], ascending.
 //
-// A row's rank is an unsigned that orders as its weight does, all ones for the rows that are kept in
-// any case and 0 for what lies behind the last row. The last kept row's rank is found digit by digit,
-// 11, 11 and 10 bits: a histogram of the rows that agree so far, and the bin in which the count from
-// the top reaches what is still to be kept. Then the rows above that rank are kept, and of those
-// equal to it the first ones. Counts are whole numbers, so their order does not matter.
+// A row's rank is an unsigned that orders as its weight does, all ones for the rows that are kept
+// in any case and 0 for what lies behind the last row. The last kept row's rank is found digit by
+// digit, 11, 11 and 10 bits: a histogram of the rows that agree so far, and the bin in which the
+// count from the top reaches what is still to be kept. Then the rows above that rank are kept, and
+// of those equal to it the first ones. Counts are whole numbers, so their order does not matter.
+//
+// Bound by latencies, not bytes: 6.3 us for 2048 rows (one launch), 35.6 for 262144 (2 MB, four
+// launches of 4.4, 9.9, 10 and 13.8: each joins 32 histograms before its own rows).
 // ------------------------------------------------------------------------------------------------
 
 struct AttnEvictSelectParams {
@@ -972,8 +993,8 @@ struct SelectShared {
   unsigned digit, above;
 };
 
-// One row a lane into the histogram. 64 rows of one digit (untouched rows, the newest ones) are added
-// in one go, since the additions of one bin follow one another.
+// One row a lane into the histogram. 64 rows of one digit (untouched rows, the newest ones) are
+// added in one go, since the additions of one bin follow one another.
 template <unsigned kDigit>
 __device__ __attribute__((always_inline)) inline void count_digit(SelectShared& sh, unsigned rank,
                                                                  unsigned prefix, unsigned lane) {
@@ -1016,9 +1037,9 @@ __device__ __attribute__((always_inline)) inline void find_digit(SelectShared& s
 }
 
 // Where this wave's kept rows go. `sure` and `equals`: its rows above the found rank and equal to
-// it (wave-uniform); `before` and `same`: kept rows and equal rows before the workgroup; `want`: how
-// many equal rows are kept. Returns the place of the wave's first kept row and moves `same` on to
-// the equal rows before the wave.
+// it (wave-uniform); `before` and `same`: kept rows and equal rows before the workgroup; `want`:
+// how many equal rows are kept. Returns the place of the wave's first kept row and moves `same` on
+// to the equal rows before the wave.
 __device__ __attribute__((always_inline)) inline unsigned place_wave(SelectShared& sh,
                                                                     unsigned sure, unsigned equals,
                                                                     unsigned before,
@@ -1312,10 +1333,11 @@ struct AttnEvictGatherParams {
   float* v_scale_out;
 };
 
-// A row of K or V is 32 (f16) or 16 (e4m3) lanes of 16 bytes; a thread moves its chunk of both, of two
-// rows over e4m3 rows (65535 rows: 30.3 us against 33.6; over f16 rows one is faster, 51.5 against
-// 53.8). Rows [0, 2 keep) are moved, the 2 (out_ctx - keep) weights behind them cleared. Grid-stride,
-// x 256.
+// A row of K or V is 32 (f16) or 16 (e4m3) lanes of 16 bytes; a thread moves its chunk of both, of
+// two rows over e4m3 rows (65535 rows: 30.3 us against 33.6; over f16 rows one is faster, 51.5
+// against 53.8). Rows [0, 2 keep) are moved, the 2 (out_ctx - keep) weights behind them cleared.
+// Grid-stride, x 256. Bound by memory: 8192 f16 rows of 32768 in 8.2 us (33.6 MB, 4.1 TB/s), 65535
+// e4m3 rows of 131072 in 30.2 (134 MB, 4.4 TB/s).
 template <bool kFp8>
 __global__ void __launch_bounds__(256) attn_evict_gather_kernel(AttnEvictGatherParams p) {
   constexpr unsigned kLanes = kFp8 ? 16 : 32, kRows = 256 / kLanes, kTwo = kFp8 ? 2 : 1;

@@ -19,11 +19,11 @@
 // Decode step (one token at position len): residual add + RMSNorm of h, the q / k / v projections,
 // the per-head norms, RoPE and the K/V append, split-K attention over len + 1 keys with the LSE
 // merge and the gate, and the output projection: four launches for the model's formats (Q4_K q and
-// k, Q6_K v), one per operator for any other mix. Prefill step (n tokens at pos0): the norm straight
-// into the GEMM input, the prefill GEMMs (qgemm_wide, q / k / v in one launch), the batched prep
-// and the causal attention (attn_prefill_launch). ingest() applies the engine's policy to a run of
-// n tokens: below the threshold one decode step per token, otherwise prefill chunks of at most the
-// chunk size.
+// k, Q6_K v), one per operator for any other mix. Prefill step (n tokens at pos0): the norm
+// straight into the GEMM input, the prefill GEMMs (qgemm_wide, q / k / v in one launch), the
+// batched prep and the causal attention (attn_prefill_launch). ingest() applies the engine's policy
+// to a run of n tokens: below the threshold one decode step per token, otherwise prefill chunks of
+// at most the chunk size.
 //
 // Every routine returns nullptr on success or a message naming the rejected argument; the C ABI
 // returns it as an error code, an engine front end can throw it.
@@ -467,8 +467,8 @@ inline const char* decode_step(const Weights& w, attn::half_t* k_cache, attn::ha
   return gemv(w.o, ws.core, y, stream);
 }
 
-// Whole rows of an f16 cache away: row pos of the moved cache is row `row` of the given one, in both KV
-// heads (the head stride stays), so that a prep for position pos appends at `row`.
+// Whole rows of an f16 cache away: row pos of the moved cache is row `row` of the given one, in
+// both KV heads (the head stride stays), so that a prep for position pos appends at `row`.
 inline attn::half_t* moved_cache(attn::half_t* cache, unsigned row, unsigned pos) {
   return reinterpret_cast<attn::half_t*>(
       reinterpret_cast<std::uintptr_t>(cache) +
@@ -476,8 +476,8 @@ inline attn::half_t* moved_cache(attn::half_t* cache, unsigned row, unsigned pos
                                   std::int64_t{attn::kDim * sizeof(attn::half_t)}));
 }
 
-// The decode step over a bounded cache: the token of position pos is appended at row `row`, attends to
-// rows [0, row], and adds the weights it gives them to weights [2][max_ctx]; wws:
+// The decode step over a bounded cache: the token of position pos is appended at row `row`, attends
+// to rows [0, row], and adds the weights it gives them to weights [2][max_ctx]; wws:
 // attn_decode_weights_floats(row + 1, kMaxSplits) floats. decode_step's launches, with the scores
 // stored by the split and turned into weights beside the merge.
 inline const char* decode_step_weights(const Weights& w, attn::half_t* k_cache,
@@ -550,8 +550,8 @@ inline const char* prefill_step(const Weights& w, attn::half_t* k_cache, attn::h
   return gemm(ws.xh, ws.xs, n, kHidden, stream, GemmOut{w.o, y});
 }
 
-// prefill_step over a bounded cache: tokens of positions pos0 .. at rows row0 .., the last `voters` of
-// which (all, where there are fewer) add the weights they give the rows they see; kws:
+// prefill_step over a bounded cache: tokens of positions pos0 .. at rows row0 .., the last `voters`
+// of which (all, where there are fewer) add the weights they give the rows they see; kws:
 // attn_key_weights_layout(row0 + n - voters, voters, false).bytes.
 inline const char* prefill_step_weights(const Weights& w, attn::half_t* k_cache,
                                         attn::half_t* v_cache, unsigned row0, unsigned pos0,
