@@ -924,26 +924,24 @@ inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
 // count from the top reaches what is still to be kept. Then the rows above that rank are kept, and
 // of those equal to it the first ones. Counts are whole numbers, so their order does not matter.
 //
-// Bound by latencies, not bytes: 6.3 us for 2048 rows (one launch), 35.6 for 262144 (2 MB, four
-// launches of 4.4, 9.9, 10 and 13.8: each joins 32 histograms before its own rows).
+// Bound by latencies, not bytes: 6.3 us for 2048 rows (one launch), 23.8 for 262144 (2 MB, four
+// launches). Joining all groups' histograms in every launch instead of adding them up in memory took
+// 35.6: 512 KiB to read per workgroup.
 // ------------------------------------------------------------------------------------------------
 
 struct AttnEvictSelectParams {
   const float* weights;  // [2][max_ctx]
   int* index;            // [2][keep]
   unsigned len, max_ctx, keep, sinks, recent;
-  // Caches of several workgroups a head: a workgroup's rows, and the workspace [2] of per-workgroup
-  // histograms [3][groups][2048], then the rows of each above what is found [groups], then the
-  // (prefix, rows still to be kept) that the second and third launch found.
+  // Caches of several workgroups a head: their number, a workgroup's rows, and the workspace
+  // [2][evict_detail::part_words(groups)].
   unsigned groups, rows;
   unsigned* ws;
 };
 
 namespace evict_detail {
 
-constexpr unsigned kBins = 2048;  // of a digit; the last one uses 1024
 constexpr unsigned kSelectWaves = 16;
-constexpr unsigned kShift[3] = {21, 10, 0};
 
 // The rank of row `row`, whose weight is x: NaN 1, then the numbers, -0 as +0.
 __device__ __attribute__((always_inline)) inline unsigned rank_of(const AttnEvictSelectParams& p,
@@ -955,15 +953,14 @@ __device__ __attribute__((always_inline)) inline unsigned rank_of(const AttnEvic
   return row < p.len ? rank : 0u;
 }
 
-// The digit of a rank, and whether the rank agrees with the prefix above it.
-template <unsigned kDigit>
+// Bits [kLow, kHigh) of a rank, and whether the rank agrees with the prefix found above them.
+template <unsigned kLow, unsigned kHigh>
 __device__ __attribute__((always_inline)) inline unsigned digit_of(unsigned rank) {
-  return rank >> kShift[kDigit] & (kDigit == 2 ? 1023u : 2047u);
+  return rank >> kLow & ((1u << (kHigh - kLow)) - 1);
 }
-template <unsigned kDigit>
+template <unsigned kHigh>
 __device__ __attribute__((always_inline)) inline bool agrees(unsigned rank, unsigned prefix) {
-  return kDigit == 0 || rank >> kShift[kDigit == 0 ? 0 : kDigit - 1] ==
-                            prefix >> kShift[kDigit == 0 ? 0 : kDigit - 1];
+  return kHigh == 32 || rank >> (kHigh % 32) == prefix >> (kHigh % 32);
 }
 
 // The inclusive sum over the lanes up to this one.
@@ -982,56 +979,72 @@ __device__ __attribute__((always_inline)) inline unsigned lanes_below(unsigned l
                                    __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0));
 }
 
-// Words of a head's part of the workspace (an even number: histograms move 8 bytes a lane).
-__host__ __device__ constexpr std::size_t part_words(std::size_t groups) {
-  return groups * 3 * kBins + (groups + 1) / 2 * 2 + 4;
-}
-
+template <unsigned kBins>
 struct SelectShared {
-  unsigned hist[kBins + 64];  // one more bin a lane, for rows that do not count
+  unsigned hist[kBins];
   unsigned waves[2][kSelectWaves];
   unsigned digit, above;
 };
 
-// One row a lane into the histogram. 64 rows of one digit (untouched rows, the newest ones) are
-// added in one go, since the additions of one bin follow one another.
-template <unsigned kDigit>
-__device__ __attribute__((always_inline)) inline void count_digit(SelectShared& sh, unsigned rank,
-                                                                 unsigned prefix, unsigned lane) {
-  const unsigned bin = agrees<kDigit>(rank, prefix) ? digit_of<kDigit>(rank) : kBins + lane;
-  const unsigned one = __builtin_amdgcn_readfirstlane(bin);
-  if (__builtin_amdgcn_ballot_w64(bin != one) == 0) {  // wave-uniform
+// One row a lane into the histogram of bits [kLow, kHigh), each bin kCopies times (lanes of one bin
+// follow one another). Where all of the wave's rows that agree with the prefix have one digit
+// (untouched rows, the newest ones), they are added in one go.
+template <unsigned kLow, unsigned kHigh, unsigned kCopies, unsigned kBins>
+__device__ __attribute__((always_inline)) inline void count_digit(SelectShared<kBins>& sh,
+                                                                 unsigned rank, unsigned prefix,
+                                                                 unsigned lane) {
+  const bool counts = agrees<kHigh>(rank, prefix);
+  const unsigned long long which = __builtin_amdgcn_ballot_w64(counts);
+  if (which == 0)  // wave-uniform
+    return;
+  const unsigned bin = digit_of<kLow, kHigh>(rank) * kCopies;
+  const unsigned one = __builtin_amdgcn_readlane(bin, __builtin_ctzll(which));
+  if (__builtin_amdgcn_ballot_w64(counts && bin != one) == 0) {  // wave-uniform
     if (lane == 0)
-      atomicAdd(&sh.hist[one], 64u);
-  } else {
-    atomicAdd(&sh.hist[bin], 1u);
+      atomicAdd(&sh.hist[one], static_cast<unsigned>(__popcll(which)));
+  } else if (counts) {
+    atomicAdd(&sh.hist[bin + lane % kCopies], 1u);
   }
 }
 
-__device__ __attribute__((always_inline)) inline void clear_digits(SelectShared& sh) {
-  sh.hist[threadIdx.x] = 0;
-  sh.hist[threadIdx.x + 1024] = 0;
+template <unsigned kBins>
+__device__ __attribute__((always_inline)) inline void clear_digits(SelectShared<kBins>& sh) {
+#pragma unroll
+  for (unsigned i = 0; i < kBins; i += 1024)
+    sh.hist[i + threadIdx.x] = 0;
   __syncthreads();
 }
 
 // The bin in which the count from the top reaches `want` (sh.digit) and the count of the bins above
-// it (sh.above); thread t holds bins 2047 - 2 t and 2046 - 2 t, `high` and `low` of them. 1 <= want
-// <= the histogram's total. Ends with a barrier.
-__device__ __attribute__((always_inline)) inline void find_digit(SelectShared& sh, unsigned high,
-                                                                unsigned low, unsigned want) {
+// it (sh.above); thread t holds c[i] of bin top - kPer t - i. 1 <= want <= the histogram's total.
+// Ends with a barrier.
+template <unsigned kPer, unsigned kBins>
+__device__ __attribute__((always_inline)) inline void find_digit(SelectShared<kBins>& sh,
+                                                                const unsigned (&c)[kPer],
+                                                                unsigned top, unsigned want) {
   const unsigned t = threadIdx.x, lane = t & 63u, wave = t >> 6;
-  const unsigned incl = wave_scan(high + low, lane);
+  unsigned mine = 0;
+#pragma unroll
+  for (unsigned i = 0; i < kPer; ++i)
+    mine += c[i];
+  const unsigned incl = wave_scan(mine, lane);
   if (lane == 63)
     sh.waves[0][wave] = incl;
   __syncthreads();
-  unsigned above = incl - (high + low);
+  unsigned above = incl - mine;
 #pragma unroll
   for (unsigned k = 0; k < kSelectWaves; ++k)
     above += k < wave ? sh.waves[0][k] : 0;
-  if (above < want && want <= above + high + low) {  // one thread
-    const bool first = want <= above + high;
-    sh.digit = kBins - 1 - 2 * t - (first ? 0 : 1);
-    sh.above = above + (first ? 0 : high);
+  if (above < want && want <= above + mine) {  // one thread
+    unsigned i = 0;
+#pragma unroll
+    for (unsigned k = 0; k + 1 < kPer; ++k)
+      if (i == k && want > above + c[k]) {
+        above += c[k];
+        ++i;
+      }
+    sh.digit = top - kPer * t - i;
+    sh.above = above;
   }
   __syncthreads();
 }
@@ -1040,7 +1053,8 @@ __device__ __attribute__((always_inline)) inline void find_digit(SelectShared& s
 // it (wave-uniform); `before` and `same`: kept rows and equal rows before the workgroup; `want`:
 // how many equal rows are kept. Returns the place of the wave's first kept row and moves `same` on
 // to the equal rows before the wave.
-__device__ __attribute__((always_inline)) inline unsigned place_wave(SelectShared& sh,
+template <unsigned kBins>
+__device__ __attribute__((always_inline)) inline unsigned place_wave(SelectShared<kBins>& sh,
                                                                     unsigned sure, unsigned equals,
                                                                     unsigned before,
                                                                     unsigned& same, unsigned want) {
@@ -1081,7 +1095,8 @@ __device__ __attribute__((always_inline)) inline void write_kept(int* out, unsig
 template <unsigned R>
 __global__ void __launch_bounds__(1024) attn_evict_select_kernel(AttnEvictSelectParams p) {
   using namespace evict_detail;
-  __shared__ SelectShared sh;
+  constexpr unsigned kBins = 2048;
+  __shared__ SelectShared<kBins> sh;
   const unsigned kvh = blockIdx.x, t = threadIdx.x, lane = t & 63u;
   const unsigned wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const float* w = p.weights + std::size_t{kvh} * p.max_ctx;
@@ -1095,20 +1110,21 @@ __global__ void __launch_bounds__(1024) attn_evict_select_kernel(AttnEvictSelect
   for (unsigned i = 0; i < R; ++i)
     rank[i] = rank_of(p, row0 + 64 * i, x[i]);
   unsigned want = p.keep, last = 0;
-  auto digit = [&](auto which) __attribute__((always_inline)) {
-    constexpr unsigned kDigit = decltype(which)::value;
+  auto digit = [&](auto low, auto high) __attribute__((always_inline)) {
     clear_digits(sh);
 #pragma unroll
     for (unsigned i = 0; i < R; ++i)
-      count_digit<kDigit>(sh, rank[i], last, lane);
+      count_digit<decltype(low)::value, decltype(high)::value, 1>(sh, rank[i], last, lane);
     __syncthreads();
-    find_digit(sh, sh.hist[kBins - 1 - 2 * t], sh.hist[kBins - 2 - 2 * t], want);
-    last |= sh.digit << kShift[kDigit];
+    const unsigned c[2] = {sh.hist[kBins - 1 - 2 * t], sh.hist[kBins - 2 - 2 * t]};
+    find_digit(sh, c, kBins - 1, want);
+    last |= sh.digit << decltype(low)::value;
     want -= sh.above;
   };
-  digit(std::integral_constant<unsigned, 0>{});
-  digit(std::integral_constant<unsigned, 1>{});
-  digit(std::integral_constant<unsigned, 2>{});
+  using std::integral_constant;
+  digit(integral_constant<unsigned, 21>{}, integral_constant<unsigned, 32>{});
+  digit(integral_constant<unsigned, 10>{}, integral_constant<unsigned, 21>{});
+  digit(integral_constant<unsigned, 0>{}, integral_constant<unsigned, 10>{});
   unsigned sure = 0, equals = 0, same = 0;
 #pragma unroll
   for (unsigned i = 0; i < R; ++i) {
@@ -1122,22 +1138,36 @@ __global__ void __launch_bounds__(1024) attn_evict_select_kernel(AttnEvictSelect
     write_kept(out, p.keep, at, same, want, rank[i], last, row0 + 64 * i);
 }
 
-// Longer caches: `groups` workgroups per head, p.rows rows each, in four launches, a digit each and
-// the writing. Launch d >= 1 first joins the histograms of digit d - 1 (every workgroup for
-// itself), then counts its own rows' digit d. Grid dim3(groups, 2) x 1024.
+// Longer caches: `groups` workgroups per head (64 at most), p.rows rows each, in four launches, a
+// digit of 8, 12 and 12 bits each and the writing. A head's part of the workspace:
+//   first [groups][256]: the groups' histograms of the first digit, which every workgroup of the
+//     second launch joins for itself;
+//   hist [2][4096]: those of the other two over all groups, cleared by the first launch, added to by
+//     every workgroup (counts: the order of the additions does not matter) and read by the next;
+//   upto [groups][4100]: after the third launch, a group's rows that agree with the first two digits
+//     and whose third is at least b, and its rows above them, at [b], b <= 4096: from it the last
+//     launch has the kept rows before a workgroup's with two loads a group;
+//   state [4]: (prefix, rows still to be kept) after the first and the second digit.
+// Grid dim3(groups, 2) x 1024.
+namespace evict_detail {
+constexpr unsigned kFirstBins = 256, kPartBins = 4096, kUpto = kPartBins + 4;
+__host__ __device__ constexpr std::size_t part_words(std::size_t groups) {
+  return groups * (kFirstBins + kUpto) + 2 * kPartBins + 4;
+}
+}  // namespace evict_detail
 template <unsigned kLaunch>
 __global__ void __launch_bounds__(1024) attn_evict_select_part_kernel(AttnEvictSelectParams p) {
   using namespace evict_detail;
-  __shared__ SelectShared sh;
+  __shared__ SelectShared<kPartBins> sh;
   const unsigned kvh = blockIdx.y, g = blockIdx.x, t = threadIdx.x, lane = t & 63u;
   const unsigned wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const float* w = p.weights + std::size_t{kvh} * p.max_ctx;
-  const unsigned r0 = g * p.rows < p.len ? g * p.rows : p.len;  // the last groups may have none
+  const unsigned r0 = g * p.rows;
   const unsigned r1 = p.len - r0 < p.rows ? p.len : r0 + p.rows;
-  const std::size_t hists = std::size_t{3} * p.groups * kBins;
-  unsigned* const ws = p.ws + kvh * part_words(p.groups);
-  unsigned* const above = ws + hists;
-  unsigned* const state = above + (p.groups + 1) / 2 * 2;  // (prefix, want) after digits 0 and 1
+  unsigned* const hist = p.ws + kvh * part_words(p.groups);
+  unsigned* const first = hist + 2 * kPartBins;
+  unsigned* const upto = first + p.groups * kFirstBins;
+  unsigned* const state = upto + std::size_t{p.groups} * kUpto;
   // Each wave takes a stretch of the rows, 64 at a time; the first 512 are loaded before all else.
   const unsigned per = p.rows / kSelectWaves;
   const unsigned s0 = r0 + wave * per < r1 ? r0 + wave * per : r1;
@@ -1157,94 +1187,112 @@ __global__ void __launch_bounds__(1024) attn_evict_select_part_kernel(AttnEvictS
   };
   load(s0);
   unsigned want = p.keep, last = 0;
-  if constexpr (kLaunch > 1) {
+  if constexpr (kLaunch == 0) {
+    for (unsigned i = g * 1024 + t; i < 2 * kPartBins; i += p.groups * 1024)
+      hist[i] = 0;
+  } else if constexpr (kLaunch == 1) {
+    // A quarter of the threads per quarter of the groups, 16 at most: all loads in flight.
+    const unsigned bin = kFirstBins - 1 - t % kFirstBins;
+    unsigned one[16], c[1] = {0};
+#pragma unroll
+    for (unsigned i = 0; i < 16; ++i) {
+      const unsigned k = t / kFirstBins + 4 * i;
+      one[i] = first[(k < p.groups ? k : 0) * kFirstBins + bin];
+      c[0] += k < p.groups ? one[i] : 0;
+    }
+    sh.hist[t] = c[0];
+    __syncthreads();
+    c[0] = 0;
+    if (t < kFirstBins)
+      c[0] = sh.hist[t] + sh.hist[t + 256] + sh.hist[t + 512] + sh.hist[t + 768];
+    find_digit(sh, c, kFirstBins - 1, want);
+    last = sh.digit << 24;
+  } else {
     last = state[2 * (kLaunch - 2)];
     want = state[2 * (kLaunch - 2) + 1];
+    const uint4 four = *reinterpret_cast<const uint4*>(hist + (kLaunch - 2) * kPartBins +
+                                                       kPartBins - 4 - 4 * t);
+    const unsigned c[4] = {four.w, four.z, four.y, four.x};
+    find_digit(sh, c, kPartBins - 1, want);
+    last |= sh.digit << (kLaunch == 2 ? 12 : 0);
   }
-  if constexpr (kLaunch > 0) {
-    const unsigned bin = kBins - 2 - 2 * t;
-    const unsigned* h = ws + (kLaunch - 1) * std::size_t{p.groups} * kBins + bin;
-    const uint2 own = *reinterpret_cast<const uint2*>(h + std::size_t{g} * kBins);
-    unsigned high = 0, low = 0;
-    for (unsigned k0 = 0; k0 < p.groups; k0 += 16) {  // 16 loads in flight
-      uint2 one[16];
-#pragma unroll
-      for (unsigned i = 0; i < 16; ++i)
-        one[i] = *reinterpret_cast<const uint2*>(
-            h + std::size_t{k0 + i < p.groups ? k0 + i : k0} * kBins);
-#pragma unroll
-      for (unsigned i = 0; i < 16; ++i) {
-        low += k0 + i < p.groups ? one[i].x : 0;
-        high += k0 + i < p.groups ? one[i].y : 0;
-      }
-    }
-    find_digit(sh, high, low, want);
-    const unsigned digit = sh.digit;
-    last |= digit << kShift[kLaunch - 1];
+  if constexpr (kLaunch > 0)
     want -= sh.above;
-    if constexpr (kLaunch < 3) {
-      // This workgroup's rows above the digit join those above the digits before.
-      const unsigned sum =
-          wave_scan((bin > digit ? own.x : 0) + (bin + 1 > digit ? own.y : 0), lane);
-      if (lane == 63)
-        sh.waves[1][wave] = sum;
-      __syncthreads();
-      if (t == 0) {
-        unsigned all = kLaunch == 1 ? 0 : above[g];
-        for (unsigned k = 0; k < kSelectWaves; ++k)
-          all += sh.waves[1][k];
-        above[g] = all;
-        if (g == 0) {
-          state[2 * (kLaunch - 1)] = last;
-          state[2 * (kLaunch - 1) + 1] = want;
-        }
-      }
+  if constexpr (kLaunch == 1 || kLaunch == 2) {
+    if (g == 0 && t == 0) {
+      state[2 * (kLaunch - 1)] = last;
+      state[2 * (kLaunch - 1) + 1] = want;
     }
   }
   if constexpr (kLaunch < 3) {
+    constexpr unsigned kLow = kLaunch == 0 ? 24 : kLaunch == 1 ? 12 : 0;
+    constexpr unsigned kHigh = kLaunch == 0 ? 32 : kLow + 12, kCopies = kLaunch == 0 ? 16 : 1;
+    unsigned sure = 0;  // rows above the prefix
     clear_digits(sh);
     for (unsigned from = s0; from < s1; from += kChunk) {  // wave-uniform
       if (from != s0)
         load(from);
 #pragma unroll
-      for (unsigned i = 0; i < kChunk / 64; ++i)
-        count_digit<kLaunch>(sh, rank_at(from, i), last, lane);
-    }
-    __syncthreads();
-    unsigned* out = ws + (kLaunch * std::size_t{p.groups} + g) * kBins;
-    *reinterpret_cast<uint2*>(out + 2 * t) = *reinterpret_cast<const uint2*>(&sh.hist[2 * t]);
-  } else {
-    // Rows above the found rank, and rows equal to it, in the workgroups before this one.
-    unsigned a = 0, e = 0;
-    const unsigned digit = last & 1023u;
-    for (unsigned k = wave; k < g; k += kSelectWaves) {  // wave-uniform
-      const unsigned* h = ws + (2 * std::size_t{p.groups} + k) * kBins;
-      unsigned c[16];
-#pragma unroll
-      for (unsigned i = 0; i < 16; ++i)
-        c[i] = h[64 * i + lane];
-      a += lane == 0 ? above[k] : 0;
-#pragma unroll
-      for (unsigned i = 0; i < 16; ++i) {
-        a += 64 * i + lane > digit ? c[i] : 0;
-        e += 64 * i + lane == digit ? c[i] : 0;
+      for (unsigned i = 0; i < kChunk / 64; ++i) {
+        const unsigned rank = rank_at(from, i);
+        count_digit<kLow, kHigh, kCopies>(sh, rank, last, lane);
+        if (kLaunch == 2)
+          sure += __popcll(__builtin_amdgcn_ballot_w64(rank >> 12 > last >> 12));
       }
     }
-    a = wave_scan(a, lane);
-    e = wave_scan(e, lane);
-    if (lane == 63) {  // (sh.waves was last read before find_digit's second barrier)
-      sh.waves[0][wave] = a;
-      sh.waves[1][wave] = e;
-    }
+    if (kLaunch == 2 && lane == 0)
+      sh.waves[1][wave] = sure;
     __syncthreads();
-    unsigned before = 0, same = 0;
+    if constexpr (kLaunch == 0) {
+      if (t < kFirstBins) {
+        unsigned all = 0;
 #pragma unroll
-    for (unsigned k = 0; k < kSelectWaves; ++k) {
-      before += sh.waves[0][k];
-      same += sh.waves[1][k];
+        for (unsigned i = 0; i < kCopies; ++i)
+          all += sh.hist[kCopies * t + (i + t) % kCopies];
+        first[g * kFirstBins + t] = all;
+      }
+    } else {
+      unsigned* const out = hist + (kLaunch - 1) * kPartBins;
+#pragma unroll
+      for (unsigned i = 0; i < kPartBins; i += 1024)  // neighbouring bins to neighbouring lanes
+        if (const unsigned n = sh.hist[i + t])
+          atomicAdd(&out[i + t], n);
+      if constexpr (kLaunch == 2) {
+        const unsigned bin = kPartBins - 4 - 4 * t;
+        const uint4 c = *reinterpret_cast<const uint4*>(&sh.hist[bin]);
+        const unsigned mine = c.x + c.y + c.z + c.w;
+        const unsigned incl = wave_scan(mine, lane);
+        if (lane == 63)
+          sh.waves[0][wave] = incl;
+        __syncthreads();
+        unsigned before = 0, at = incl - mine;
+#pragma unroll
+        for (unsigned k = 0; k < kSelectWaves; ++k) {
+          before += sh.waves[1][k];
+          at += k < wave ? sh.waves[0][k] : 0;
+        }
+        at += before;
+        uint4 up;
+        up.w = at + c.w;
+        up.z = up.w + c.z;
+        up.y = up.z + c.y;
+        up.x = up.y + c.x;
+        unsigned* const u = upto + std::size_t{g} * kUpto;
+        *reinterpret_cast<uint4*>(u + bin) = up;
+        if (t == 0)
+          u[kPartBins] = before;
+      }
     }
+  } else {
+    // Rows above the found rank, and rows equal to it, in the workgroups before this one: a group
+    // a lane, every wave for itself.
+    const unsigned* u = upto + std::size_t{lane < g ? lane : 0} * kUpto + (last & 4095u);
+    const unsigned from_last = u[0], past_last = u[1];
+    unsigned before = wave_scan(lane < g ? past_last : 0, lane);
+    unsigned same = wave_scan(lane < g ? from_last - past_last : 0, lane);
+    before = __builtin_amdgcn_readlane(before, 63);
+    same = __builtin_amdgcn_readlane(same, 63);
     before += same < want ? same : want;
-    __syncthreads();
     // Each wave counts its stretch, and writes behind the waves before it.
     unsigned sure = 0, equals = 0;
     for (unsigned from = s0; from < s1; from += kChunk) {
@@ -1269,39 +1317,35 @@ __global__ void __launch_bounds__(1024) attn_evict_select_part_kernel(AttnEvictS
   }
 }
 
-// Up to this many rows one workgroup a head holds them all (24 us at 32768 rows). Beyond, 16
-// workgroups or one per 8192 rows, at most 64: every launch joins all their histograms, 8 KiB each,
-// which more groups lengthen (100000 rows: 30 us with 16, 35 with 25; 262144: 38 with 32, 49 with
-// 64) and fewer shorten less than their own rows take (262144 with 16: 43).
-constexpr unsigned kSelectOneGroup = 32768, kSelectMostGroups = 64;
-__host__ __device__ constexpr unsigned attn_evict_groups(unsigned len) {
-  if (len <= kSelectOneGroup)
-    return 1;
-  const unsigned groups = len / 8192 + (len % 8192 != 0);
-  return groups < 16 ? 16 : groups < kSelectMostGroups ? groups : kSelectMostGroups;
+// Up to this many rows one workgroup a head holds them all (12.8 us at 16384 rows; the four launches
+// take 20, and one workgroup for 20000 rows 21.8). Beyond, workgroups of whole runs of 1024 rows, at
+// most 64 (262144 rows: 23.8 us, 24.7 with 32).
+constexpr unsigned kSelectOneGroup = 16384, kSelectMostGroups = 64;
+__host__ __device__ constexpr unsigned attn_evict_group_rows(unsigned len) {
+  return ((len - 1) / kSelectMostGroups / 1024 + 1) * 1024;
 }
 
 // Bytes of the selection's workspace for len rows (more rows never need less).
 __host__ __device__ constexpr std::size_t attn_evict_bytes(unsigned len) {
-  const std::size_t groups = attn_evict_groups(len);
-  return groups == 1 ? 256 : 2 * evict_detail::part_words(groups) * sizeof(unsigned);
+  if (len <= kSelectOneGroup)
+    return 256;
+  const std::size_t runs = len / 1024 + (len % 1024 != 0);
+  return 2 * evict_detail::part_words(runs < kSelectMostGroups ? runs : kSelectMostGroups) *
+         sizeof(unsigned);
 }
 
 // The launches of a selection whose arguments are good; ws of attn_evict_bytes(p.len).
 inline void attn_evict_select_launch(AttnEvictSelectParams p, void* ws, hipStream_t stream) {
   p.ws = static_cast<unsigned*>(ws);
-  p.groups = attn_evict_groups(p.len);
   if (p.len <= 2048) {
     attn_evict_select_kernel<2><<<2, 1024, 0, stream>>>(p);
   } else if (p.len <= 8192) {
     attn_evict_select_kernel<8><<<2, 1024, 0, stream>>>(p);
-  } else if (p.len <= 16384) {
-    attn_evict_select_kernel<16><<<2, 1024, 0, stream>>>(p);
   } else if (p.len <= kSelectOneGroup) {
-    attn_evict_select_kernel<32><<<2, 1024, 0, stream>>>(p);
+    attn_evict_select_kernel<16><<<2, 1024, 0, stream>>>(p);
   } else {
-    // Whole runs of 1024 rows; with them the last groups may have none left.
-    p.rows = ((p.len - 1) / p.groups / 1024 + 1) * 1024;
+    p.rows = attn_evict_group_rows(p.len);
+    p.groups = (p.len - 1) / p.rows + 1;
     const dim3 grid(p.groups, 2);
     attn_evict_select_part_kernel<0><<<grid, 1024, 0, stream>>>(p);
     attn_evict_select_part_kernel<1><<<grid, 1024, 0, stream>>>(p);

@@ -90,6 +90,12 @@ def test_select_refusals(lib):
     rejected(fn(P, 100, 100, 10, 1, 1, P, P, ws - 1, N), lib, "workspace smaller")
 
 
+def test_select_workspace_covers_smaller_calls(lib):
+    sizes = [lib.miso_attn_evict_workspace_bytes(n) for n in
+             (0, 1, 2048, 16384, 16385, 17408, 17409, 65536, 65537, 66561, 262144, 1 << 30)]
+    assert sizes == sorted(sizes)
+
+
 def test_gather_refusals(lib):
     fn, fn8 = lib.miso_attn_evict_gather, lib.miso_attn_evict_gather_fp8
     k, v, w, i, ko, vo, wo = FAR[:7]

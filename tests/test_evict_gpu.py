@@ -265,8 +265,9 @@ def run_select(attn, w, n, keep, sinks, recent, max_len=None):
     return index[:KV * keep].view(KV, keep).cpu().numpy()
 
 
-@pytest.mark.parametrize("n", [1, 2, 3, 63, 64, 65, 1000, 1023, 1024, 1025, 5000, 8192, 16411, 32768,
-                               40001, 65536, 65537, 131071, 262144])
+@pytest.mark.parametrize("n", [1, 2, 3, 63, 64, 65, 1000, 1023, 1024, 1025, 2048, 2049, 5000, 8192,
+                               8193, 16384, 16385, 16411, 17409, 32768, 40001, 65536, 65537, 131071,
+                               262144])
 def test_select(attn, n):
     rng = np.random.default_rng(n)
     ctx = n + 3
