@@ -296,6 +296,8 @@ __device__ __attribute__((always_inline)) inline unsigned tile_row(unsigned lane
   return 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
 }
 
+constexpr int kVmcnt0 = 0x0F70;  // s_waitcnt vmcnt(0), the other counters as they are
+
 constexpr float kNoScore = -3e38f;  // below every score, and finite: differences stay numbers
 
 // A ring of K tiles, chunk c of row r at position c ^ (r % 16) of the row (the operand read of 16
@@ -460,6 +462,9 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
                           ring + ti % kStages * kTileBytes + 512 * r0);
       }
     };
+    // Says to the compiler that no load is under way: it does not know of the waits below, and would
+    // wait for the copies before it loads into registers that the segment before loaded.
+    __builtin_amdgcn_s_waitcnt(kVmcnt0);
     if (again)
       decode_detail::tile_barrier();  // every wave is done with the segment before
 #pragma unroll
@@ -471,7 +476,7 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
     const bool active = block < p.blocks;  // wave-uniform
     const unsigned lin = kvh * p.groups + group;
     Halves b;
-    float scale = 0.0f, lse[kSum ? 16 : 1];
+    float scale, lse[kSum ? 16 : 1];
     if (active) {
       const std::size_t at = std::size_t{kvh} * p.blocks + block;
       const attn::half_t* in = p.halves + at * kBlockHalves + 8 * lane;
