@@ -511,9 +511,9 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
     }
     const unsigned open = p.pos0 + kTokens * block;  // every token of the block sees keys up to it
     // First pass: the column's sum l relative to the reference m, which follows the largest score
-    // only when that leads by more than 2^kLead (sums stay far inside f32's range, and the
-    // exponentials need not wait for a tile's maximum).
-    constexpr float kLead = 40.0f;
+    // only when a tile's weights sum to more than kLead (sums stay far inside f32's range, the
+    // exponentials need not wait for a tile's maximum, and most tiles need none).
+    constexpr float kLead = 0x1p40f;
     float m = kNoScore, l = 0.0f;
     float part[4];
     float16_t acc[2];
@@ -548,17 +548,18 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
       if constexpr (kSum) {
         sh.red[ti / W % 2][ti % W][wave][lane] = (part[0] + part[1]) + (part[2] + part[3]);
       } else {
-        const float mx = largest(y);
-        if (__builtin_amdgcn_ballot_w64(mx > m + kLead)) {  // rare, and every column's first tile
-          const float top = fmaxf(m, mx);
+        float sum = (part[0] + part[1]) + (part[2] + part[3]);
+        if (__builtin_amdgcn_ballot_w64(sum > kLead)) {  // rare, and every column's first tile
+          const float top = fmaxf(m, largest(y));
           l *= __builtin_amdgcn_exp2f(m - top);
           m = top;
           part[0] = part[1] = part[2] = part[3] = 0.0f;
 #pragma unroll
           for (unsigned i = 0; i < 16; ++i)
             part[i % 4] += weight(y, i);
+          sum = (part[0] + part[1]) + (part[2] + part[3]);
         }
-        l += (part[0] + part[1]) + (part[2] + part[3]);
+        l += sum;
       }
     };
     // The waves' sums of a run of W tiles, one tile a wave, added in wave order.

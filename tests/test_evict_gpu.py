@@ -211,6 +211,24 @@ def test_prefill_weights_in_pieces(attn):
     check(w, torch.zeros_like(w), added, rel)
 
 
+@pytest.mark.parametrize("pos0,n", [(2500, 70), (5000, 300), (0, 200)])
+def test_prefill_weights_peaked(attn, pos0, n):
+    """Few keys take nearly everything; rising scores lead the first tile's by far more and by less
+    than 2^40, falling ones leave the later tiles next to nothing."""
+    g = gen(pos0 + 13)
+    rows = pos0 + n
+    kc, _ = f16_cache(g, rows, rows)
+    q = randn(g, n, H, D)
+    q[::2] *= 6.0
+    ramp = torch.linspace(0.1, 1.0, rows, device="cuda")
+    for order in (ramp, ramp.flip(0)):
+        kk = (kc.float() * order[None, :, None]).half()
+        w = torch.zeros(KV, rows, device="cuda")
+        attn.attn_prefill_weights(q, kk, w, pos0, n, rows, attn.PrefillWeightsScratch(n, rows))
+        added, rel = weights64(q, kk.double(), pos0)
+        check(w, torch.zeros_like(w), added, rel)
+
+
 def test_prefill_weights_query_magnitudes(attn):
     """Rows of zeros (every key alike), rows far apart in magnitude, and elements far below their
     row's largest."""
