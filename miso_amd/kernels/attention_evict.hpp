@@ -241,9 +241,9 @@ __global__ void __launch_bounds__(64) attn_combine_weights_kernel(AttnWeightsPar
 //
 // Measured: 8192 tokens after 8192 in 2.55-2.65 ms, 1240-1300 TFLOP/s of f16 products (1.3 ms a
 // pass, the matrix units busy in 73 and 77% of the cycles; zeros for data take 1.88 ms, so the
-// card's power is what bounds it); 2048 tokens 99 us (passes of 43, half of each the start of its
-// spans); 1001 after 5003 e4m3 rows 164; 33 after 12001 38.8 us (four launches; passes of 17 and
-// 20, a quarter of them in tiles).
+// card's power is what bounds it); 2048 tokens 96 us (passes of 42, the first 6 of them the start
+// of its spans, then tiles at the rate of the long chunk); 1001 after 5003 e4m3 rows 164; 33 after
+// 12001 37.4 us (four launches; passes of 17 and 20, 5 of them in tiles).
 // ------------------------------------------------------------------------------------------------
 
 struct AttnKeyWeightsParams {
@@ -462,8 +462,8 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
                           ring + ti % kStages * kTileBytes + 512 * r0);
       }
     };
-    // Says to the compiler that no load is under way: it does not know of the waits below, and would
-    // wait for the copies before it loads into registers that the segment before loaded.
+    // Says to the compiler that no load is under way: it does not know of the waits below, and
+    // would wait for the copies before it loads into registers that the segment before loaded.
     __builtin_amdgcn_s_waitcnt(kVmcnt0);
     if (again)
       decode_detail::tile_barrier();  // every wave is done with the segment before
@@ -930,9 +930,10 @@ inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
 // count from the top reaches what is still to be kept. Then the rows above that rank are kept, and
 // of those equal to it the first ones. Counts are whole numbers, so their order does not matter.
 //
-// Bound by latencies, not bytes: 6.3 us for 2048 rows (one launch), 23.8 for 262144 (2 MB, four
-// launches). Joining all groups' histograms in every launch instead of adding them up in memory took
-// 35.6: 512 KiB to read per workgroup.
+// Bound by latencies, not bytes: 5.4 us for 2048 rows (one launch, the
+// host's call), 22.6 for 262144 (2 MB, four
+// launches). Joining all groups' histograms in every launch instead of adding them up in memory
+// took 35.6: 512 KiB to read per workgroup.
 // ------------------------------------------------------------------------------------------------
 
 struct AttnEvictSelectParams {
@@ -969,14 +970,20 @@ __device__ __attribute__((always_inline)) inline bool agrees(unsigned rank, unsi
   return kHigh == 32 || rank >> (kHigh % 32) == prefix >> (kHigh % 32);
 }
 
-// The inclusive sum over the lanes up to this one.
-__device__ __attribute__((always_inline)) inline unsigned wave_scan(unsigned x, unsigned lane) {
-#pragma unroll
-  for (unsigned d = 1; d < 64; d *= 2) {
-    const unsigned y = __shfl_up(x, d);
-    x += lane >= d ? y : 0;
-  }
-  return x;
+// The inclusive sum over the lanes up to this one: within rows of 16 lanes by row shifts, then the
+// last lane of a row into the next one and of the lower half into the upper (DPP moves; the same
+// sum by shuffles through LDS took a quarter of a microsecond).
+template <int kCtrl, int kRows>
+__device__ __attribute__((always_inline)) inline unsigned add_lanes(unsigned x) {
+  return x + __builtin_amdgcn_update_dpp(0u, x, kCtrl, kRows, 0xF, false);
+}
+__device__ __attribute__((always_inline)) inline unsigned wave_scan(unsigned x) {
+  x = add_lanes<0x111, 0xF>(x);  // row_shr:1, 2, 4, 8
+  x = add_lanes<0x112, 0xF>(x);
+  x = add_lanes<0x114, 0xF>(x);
+  x = add_lanes<0x118, 0xF>(x);
+  x = add_lanes<0x142, 0xA>(x);   // row_bcast:15 into rows 1 and 3
+  return add_lanes<0x143, 0xC>(x);  // row_bcast:31 into rows 2 and 3
 }
 
 // Lanes below this one that are set in a wave's mask.
@@ -989,16 +996,15 @@ template <unsigned kBins>
 struct SelectShared {
   unsigned hist[kBins];
   unsigned waves[2][kSelectWaves];
-  unsigned digit, above;
+  unsigned digit, above, count;
 };
 
 // One row a lane into the histogram of bits [kLow, kHigh), each bin kCopies times (lanes of one bin
 // follow one another). Where all of the wave's rows that agree with the prefix have one digit
 // (untouched rows, the newest ones), they are added in one go.
-template <unsigned kLow, unsigned kHigh, unsigned kCopies, unsigned kBins>
-__device__ __attribute__((always_inline)) inline void count_digit(SelectShared<kBins>& sh,
-                                                                 unsigned rank, unsigned prefix,
-                                                                 unsigned lane) {
+template <unsigned kLow, unsigned kHigh, unsigned kCopies>
+__device__ __attribute__((always_inline)) inline void count_digit(unsigned* hist, unsigned rank,
+                                                                 unsigned prefix, unsigned lane) {
   const bool counts = agrees<kHigh>(rank, prefix);
   const unsigned long long which = __builtin_amdgcn_ballot_w64(counts);
   if (which == 0)  // wave-uniform
@@ -1007,9 +1013,9 @@ __device__ __attribute__((always_inline)) inline void count_digit(SelectShared<k
   const unsigned one = __builtin_amdgcn_readlane(bin, __builtin_ctzll(which));
   if (__builtin_amdgcn_ballot_w64(counts && bin != one) == 0) {  // wave-uniform
     if (lane == 0)
-      atomicAdd(&sh.hist[one], static_cast<unsigned>(__popcll(which)));
+      atomicAdd(&hist[one], static_cast<unsigned>(__popcll(which)));
   } else if (counts) {
-    atomicAdd(&sh.hist[bin + lane % kCopies], 1u);
+    atomicAdd(&hist[bin + lane % kCopies], 1u);
   }
 }
 
@@ -1021,9 +1027,9 @@ __device__ __attribute__((always_inline)) inline void clear_digits(SelectShared<
   __syncthreads();
 }
 
-// The bin in which the count from the top reaches `want` (sh.digit) and the count of the bins above
-// it (sh.above); thread t holds c[i] of bin top - kPer t - i. 1 <= want <= the histogram's total.
-// Ends with a barrier.
+// The bin in which the count from the top reaches `want` (sh.digit), its count (sh.count) and that
+// of the bins above it (sh.above); thread t holds c[i] of bin top - kPer t - i. 1 <= want <= the
+// histogram's total. Ends with a barrier.
 template <unsigned kPer, unsigned kBins>
 __device__ __attribute__((always_inline)) inline void find_digit(SelectShared<kBins>& sh,
                                                                 const unsigned (&c)[kPer],
@@ -1033,7 +1039,7 @@ __device__ __attribute__((always_inline)) inline void find_digit(SelectShared<kB
 #pragma unroll
   for (unsigned i = 0; i < kPer; ++i)
     mine += c[i];
-  const unsigned incl = wave_scan(mine, lane);
+  const unsigned incl = wave_scan(mine);
   if (lane == 63)
     sh.waves[0][wave] = incl;
   __syncthreads();
@@ -1042,15 +1048,17 @@ __device__ __attribute__((always_inline)) inline void find_digit(SelectShared<kB
   for (unsigned k = 0; k < kSelectWaves; ++k)
     above += k < wave ? sh.waves[0][k] : 0;
   if (above < want && want <= above + mine) {  // one thread
-    unsigned i = 0;
+    unsigned i = 0, count = c[0];
 #pragma unroll
     for (unsigned k = 0; k + 1 < kPer; ++k)
-      if (i == k && want > above + c[k]) {
-        above += c[k];
+      if (i == k && want > above + count) {
+        above += count;
+        count = c[k + 1];
         ++i;
       }
     sh.digit = top - kPer * t - i;
     sh.above = above;
+    sh.count = count;
   }
   __syncthreads();
 }
@@ -1102,7 +1110,7 @@ template <unsigned R>
 __global__ void __launch_bounds__(1024) attn_evict_select_kernel(AttnEvictSelectParams p) {
   using namespace evict_detail;
   constexpr unsigned kBins = 2048;
-  __shared__ SelectShared<kBins> sh;
+  __shared__ SelectShared<3 * kBins> sh;
   const unsigned kvh = blockIdx.x, t = threadIdx.x, lane = t & 63u;
   const unsigned wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const float* w = p.weights + std::size_t{kvh} * p.max_ctx;
@@ -1116,21 +1124,33 @@ __global__ void __launch_bounds__(1024) attn_evict_select_kernel(AttnEvictSelect
   for (unsigned i = 0; i < R; ++i)
     rank[i] = rank_of(p, row0 + 64 * i, x[i]);
   unsigned want = p.keep, last = 0;
-  auto digit = [&](auto low, auto high) __attribute__((always_inline)) {
-    clear_digits(sh);
+  clear_digits(sh);
+  auto digit = [&](auto which, auto low, auto high) __attribute__((always_inline)) {
+    unsigned* const hist = sh.hist + decltype(which)::value * kBins;
 #pragma unroll
     for (unsigned i = 0; i < R; ++i)
-      count_digit<decltype(low)::value, decltype(high)::value, 1>(sh, rank[i], last, lane);
+      count_digit<decltype(low)::value, decltype(high)::value, 1>(hist, rank[i], last, lane);
     __syncthreads();
-    const unsigned c[2] = {sh.hist[kBins - 1 - 2 * t], sh.hist[kBins - 2 - 2 * t]};
+    const unsigned c[2] = {hist[kBins - 1 - 2 * t], hist[kBins - 2 - 2 * t]};
     find_digit(sh, c, kBins - 1, want);
     last |= sh.digit << decltype(low)::value;
     want -= sh.above;
   };
   using std::integral_constant;
-  digit(integral_constant<unsigned, 21>{}, integral_constant<unsigned, 32>{});
-  digit(integral_constant<unsigned, 10>{}, integral_constant<unsigned, 21>{});
-  digit(integral_constant<unsigned, 0>{}, integral_constant<unsigned, 10>{});
+  using Zero = integral_constant<unsigned, 0>;
+  digit(Zero{}, integral_constant<unsigned, 21>{}, integral_constant<unsigned, 32>{});
+  digit(integral_constant<unsigned, 1>{}, integral_constant<unsigned, 10>{},
+        integral_constant<unsigned, 21>{});
+  // Two digits are enough where every row that agrees with them is kept (most often a single one):
+  // the rows above the rank before theirs, and none equal to it. 8192 rows: 6.9 us against 7.6;
+  // with 16 rows a lane that is rarer and the branch itself costs more (16384 rows: 13.8 against
+  // 11.8).
+  if (R <= 8 && sh.count == want && last != 0) {
+    --last;
+    want = 0;
+  } else {
+    digit(integral_constant<unsigned, 2>{}, Zero{}, integral_constant<unsigned, 10>{});
+  }
   unsigned sure = 0, equals = 0, same = 0;
 #pragma unroll
   for (unsigned i = 0; i < R; ++i) {
@@ -1241,7 +1261,7 @@ __global__ void __launch_bounds__(1024) attn_evict_select_part_kernel(AttnEvictS
 #pragma unroll
       for (unsigned i = 0; i < kChunk / 64; ++i) {
         const unsigned rank = rank_at(from, i);
-        count_digit<kLow, kHigh, kCopies>(sh, rank, last, lane);
+        count_digit<kLow, kHigh, kCopies>(sh.hist, rank, last, lane);
         if (kLaunch == 2)
           sure += __popcll(__builtin_amdgcn_ballot_w64(rank >> 12 > last >> 12));
       }
@@ -1267,7 +1287,7 @@ __global__ void __launch_bounds__(1024) attn_evict_select_part_kernel(AttnEvictS
         const unsigned bin = kPartBins - 4 - 4 * t;
         const uint4 c = *reinterpret_cast<const uint4*>(&sh.hist[bin]);
         const unsigned mine = c.x + c.y + c.z + c.w;
-        const unsigned incl = wave_scan(mine, lane);
+        const unsigned incl = wave_scan(mine);
         if (lane == 63)
           sh.waves[0][wave] = incl;
         __syncthreads();
@@ -1294,8 +1314,8 @@ __global__ void __launch_bounds__(1024) attn_evict_select_part_kernel(AttnEvictS
     // a lane, every wave for itself.
     const unsigned* u = upto + std::size_t{lane < g ? lane : 0} * kUpto + (last & 4095u);
     const unsigned from_last = u[0], past_last = u[1];
-    unsigned before = wave_scan(lane < g ? past_last : 0, lane);
-    unsigned same = wave_scan(lane < g ? from_last - past_last : 0, lane);
+    unsigned before = wave_scan(lane < g ? past_last : 0);
+    unsigned same = wave_scan(lane < g ? from_last - past_last : 0);
     before = __builtin_amdgcn_readlane(before, 63);
     same = __builtin_amdgcn_readlane(same, 63);
     before += same < want ? same : want;
@@ -1323,9 +1343,9 @@ __global__ void __launch_bounds__(1024) attn_evict_select_part_kernel(AttnEvictS
   }
 }
 
-// Up to this many rows one workgroup a head holds them all (12.8 us at 16384 rows; the four launches
-// take 20, and one workgroup for 20000 rows 21.8). Beyond, workgroups of whole runs of 1024 rows, at
-// most 64 (262144 rows: 23.8 us, 24.7 with 32).
+// Up to this many rows one workgroup a head holds them all (11.8 us at 16384 rows; the four
+// launches take 19, and one workgroup for 20000 rows 21.8). Beyond, workgroups of whole runs of
+// 1024 rows, at most 64 (262144 rows: half a microsecond faster than 32).
 constexpr unsigned kSelectOneGroup = 16384, kSelectMostGroups = 64;
 __host__ __device__ constexpr unsigned attn_evict_group_rows(unsigned len) {
   return ((len - 1) / kSelectMostGroups / 1024 + 1) * 1024;
