@@ -930,10 +930,9 @@ inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
 // count from the top reaches what is still to be kept. Then the rows above that rank are kept, and
 // of those equal to it the first ones. Counts are whole numbers, so their order does not matter.
 //
-// Bound by latencies, not bytes: 5.4 us for 2048 rows (one launch, the
-// host's call), 22.6 for 262144 (2 MB, four
-// launches). Joining all groups' histograms in every launch instead of adding them up in memory
-// took 35.6: 512 KiB to read per workgroup.
+// Bound by latencies, not bytes: 5.4 us for 2048 rows (one launch, the host's call), 22.6 for 262144
+// (2 MB, four launches). Joining all groups' histograms in every launch instead of adding them up in
+// memory took 35.6: 512 KiB to read per workgroup.
 // ------------------------------------------------------------------------------------------------
 
 struct AttnEvictSelectParams {

@@ -317,6 +317,19 @@ def test_select_ties_and_specials(attn, n):
                 assert np.array_equal(got[h], select_np(w[h], keep, sinks, recent)), (n, keep, h)
 
 
+def test_select_of_long_stretches(attn):
+    """Workgroups of more rows than a wave loads at a time."""
+    n = 1500001
+    rng = np.random.default_rng(4)
+    spread = np.exp(2 * rng.standard_normal((KV, n))).astype(np.float32)
+    close = (1.0 + 1e-5 * rng.random((KV, n))).astype(np.float32)  # many equal, one digit apart
+    for w, keep, sinks, recent in ((spread, 700001, 4, 100), (close, 1000, 0, 0),
+                                   (close, n - 5, 1, 2)):
+        got = run_select(attn, torch.from_numpy(w).cuda(), n, keep, sinks, recent)
+        for h in range(KV):
+            assert np.array_equal(got[h], select_np(w[h], keep, sinks, recent)), (keep, h)
+
+
 GATHERS = [(1, 1, 1), (5, 3, 3), (64, 64, 70), (1000, 257, 300), (4099, 1023, 5000),
            (33000, 16001, 16384)]
 
