@@ -26,10 +26,10 @@ namespace miso::kernels {
 // key, both KV heads, beside the 2048 it reads) and the launch that merges the partials also turns
 // them into weights. The result of the attention is attn_decode's, bit for bit.
 //
-// Bound by the K and V stream, as attn_decode: 32768 keys take 18.8 us against 18.7 without
-// weights, 262144 103.8 against 88.5 (5.2 TB/s of what must move), of which 9 are the score stores
-// among the loads and 5.5 the merge's; 301 keys 10.8, two launches and the host's call. 100003 e4m3
-// keys 30.2.
+// Bound by the K and V stream, as attn_decode: 32768 keys take 19.9 us against 18.8 without
+// weights, 262144 103.9 against 89 (5.2 TB/s of what must move), of which 9 are the score stores
+// among the loads and 5.5 the merge's; 301 keys 11.3 against 9.9, two launches and the host's call.
+// 100003 e4m3 keys 30.2.
 // ------------------------------------------------------------------------------------------------
 
 // The scores' row length for len keys: the padding lets a span store whole groups of 4.
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(64) attn_combine_weights_kernel(AttnWeightsPar
 // pass, the matrix units busy in 73 and 77% of the cycles; zeros for data take 1.88 ms, so the
 // card's power is what bounds it); 2048 tokens 96 us (passes of 42, the first 6 of them the start
 // of its spans, then tiles at the rate of the long chunk); 1001 after 5003 e4m3 rows 164; 33 after
-// 12001 37.4 us (four launches; passes of 17 and 20, 5 of them in tiles).
+// 12001 37.4 us (four launches; passes of 15.5 and 19, 5 of them in tiles).
 // ------------------------------------------------------------------------------------------------
 
 struct AttnKeyWeightsParams {
