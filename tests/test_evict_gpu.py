@@ -522,10 +522,11 @@ def test_bounded_generation(attn, fp8):
             assert float(err) <= 1e-5
 
 
-def test_captured_and_replayed(attn):
+@pytest.mark.parametrize("n", [2500, 20001])  # a selection of one launch, of four
+def test_captured_and_replayed(attn, n):
     """The operators in a graph on a stream of their own, replayed with other inputs between."""
     g = gen(31)
-    n, m, keep = 2500, 40, 700
+    m, keep = 40, 700
     q, qg = 2.0 * randn(g, m, H, D), randn(g, H, 2, D)
     k, v = f16_cache(g, n, n)
     w, core = torch.zeros(KV, n, device="cuda"), torch.empty(H, D, device="cuda")
