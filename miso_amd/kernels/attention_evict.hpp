@@ -344,15 +344,67 @@ struct Halves {
 
 }  // namespace weights_detail
 
+struct AttnKWidenParams {
+  const uint8_t* k8;     // [2][max_ctx][256]
+  const float* k_scale;  // [2][max_ctx]
+  attn::half_t* out;     // [2][n][256]
+  unsigned n, max_ctx;
+};
+
+namespace weights_detail {
+// K codes widened to f16 (attn_kv_fp8_widen_kernel's values, K alone): workgroup `first` of
+// `groups` of 4 waves, 8 codes a lane, 8 rows of a wave in flight.
+constexpr unsigned kWidenRows = 32;  // a workgroup's at a time
+__device__ __attribute__((always_inline)) inline void widen_rows(const AttnKWidenParams& p,
+                                                                unsigned first, unsigned groups) {
+  const unsigned lane = threadIdx.x & 31u, half = threadIdx.x >> 5;
+  const std::size_t rows = 2 * std::size_t{p.n};
+  for (std::size_t r0 = std::size_t{kWidenRows} * first + half; r0 < rows;
+       r0 += std::size_t{kWidenRows} * groups) {
+    uint2 w[4];
+    float sc[4];
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) {
+      const std::size_t r = r0 + 8 * i < rows ? r0 + 8 * i : r0;
+      const std::size_t src = r < p.n ? r : r - p.n + p.max_ctx;
+      w[i] = *reinterpret_cast<const uint2*>(p.k8 + src * attn::kDim + 8 * lane);
+      sc[i] = p.k_scale[src];
+    }
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) {
+      const cdna4::half2_t e[4] = {
+          cdna4::as_half2(fp8kv::pair_lo(w[i].x)), cdna4::as_half2(fp8kv::pair_hi(w[i].x)),
+          cdna4::as_half2(fp8kv::pair_lo(w[i].y)), cdna4::as_half2(fp8kv::pair_hi(w[i].y))};
+      cdna4::half8_t h;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        h[k] = static_cast<_Float16>(
+            fminf(fmaxf(static_cast<float>(e[k / 2][k % 2]) * sc[i], -65504.0f), 65504.0f));
+      if (r0 + 8 * i < rows)
+        *reinterpret_cast<cdna4::half8_t*>(p.out + (r0 + 8 * i) * attn::kDim + 8 * lane) = h;
+    }
+  }
+}
+}  // namespace weights_detail
+
 // The queries' halves and scales. One workgroup of 4 waves per (KV head, column block): wave w
 // reads columns 8 w .. 8 w + 7, one row of 1 KiB an instruction, and the halves go out through LDS
 // in the order of the operands, 16 bytes a lane. In LDS the 512 bytes of a k-step's half (s,
 // dimension / 8 % 2) are 528 apart, so that the 32 of them that one row touches lie in different
 // banks. Padding columns are zero. Bound by memory, 8 bytes per query element: 42 us for 8192
 // tokens (268 MB), 11 for 2048.
-template <int = 0>
-__global__ void __launch_bounds__(256) attn_key_weights_cut_kernel(AttnKeyWeightsParams p) {
+//
+// kFp8: the workgroups from 2 p.blocks on widen the rows of an e4m3 cache, which the cut does not
+// need (33 tokens after 12001 rows: 41.8 us, with a launch of its own 44.6).
+template <bool kFp8>
+__global__ void __launch_bounds__(256) attn_key_weights_cut_kernel(AttnKeyWeightsParams p,
+                                                                  AttnKWidenParams widen) {
   using namespace weights_detail;
+  if constexpr (kFp8)
+    if (blockIdx.x >= 2 * p.blocks) {
+      widen_rows(widen, blockIdx.x - 2 * p.blocks, gridDim.x - 2 * p.blocks);
+      return;
+    }
   constexpr unsigned kPer = kCols / 4, kStep = 528, kHalf = 2 * kSteps * kStep;
   __shared__ __attribute__((aligned(16))) unsigned char sh[2 * kHalf];
   __shared__ float most[4];
@@ -737,32 +789,6 @@ __global__ void __launch_bounds__(256) attn_key_weights_join_kernel(AttnKeyWeigh
   p.weights[std::size_t{kvh} * p.max_ctx + key] += v;
 }
 
-// K codes [2][max_ctx][256] widened to f16 [2][n][256] (attn_kv_fp8_widen_kernel's values, K
-// alone). One wave per row, 4 per workgroup, grid-stride.
-template <int = 0>
-__global__ void __launch_bounds__(256) attn_k_fp8_widen_kernel(const uint8_t* k8,
-                                                               const float* k_scale,
-                                                               attn::half_t* out, unsigned n,
-                                                               unsigned max_ctx) {
-  const unsigned lane = threadIdx.x & 63u;
-  const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  for (std::size_t r = 4 * std::size_t{blockIdx.x} + wave; r < 2 * std::size_t{n};
-       r += 4 * std::size_t{gridDim.x}) {
-    const std::size_t src = r < n ? r : r - n + max_ctx;
-    const unsigned w = *reinterpret_cast<const unsigned*>(k8 + src * attn::kDim + 4 * lane);
-    const float sc = k_scale[src];
-    const cdna4::half2_t a = cdna4::as_half2(fp8kv::pair_lo(w));
-    const cdna4::half2_t b = cdna4::as_half2(fp8kv::pair_hi(w));
-    const float e[4] = {static_cast<float>(a[0]), static_cast<float>(a[1]),
-                        static_cast<float>(b[0]), static_cast<float>(b[1])};
-    _Float16 h[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      h[i] = static_cast<_Float16>(fminf(fmaxf(e[i] * sc, -65504.0f), 65504.0f));
-    *reinterpret_cast<uint2*>(out + r * attn::kDim + 4 * lane) = __builtin_bit_cast(uint2, h);
-  }
-}
-
 // How a chunk is cut: column blocks, the waves W of a workgroup, the groups, and the spans of a
 // pass. W = 8 is one workgroup per CU, W = 4 two, which hide each other's starts and barriers but
 // stream K twice. Two are faster while K stays in an XCD's L2 (2048 tokens: 110 us against 120;
@@ -864,7 +890,6 @@ __host__ __device__ constexpr std::size_t attn_key_weights_bytes(unsigned max_n,
 template <unsigned W>
 void attn_key_weights_passes(const AttnKeyWeightsParams& p, hipStream_t stream) {
   const unsigned grid = (p.spans + 7) / 8 * 8;
-  attn_key_weights_cut_kernel<><<<2 * p.blocks, 256, 0, stream>>>(p);
   attn_key_weights_pass_kernel<W, false><<<grid, 64 * W, 0, stream>>>(p);
   attn_key_weights_pass_kernel<W, true><<<grid, 64 * W, 0, stream>>>(p);
   if (p.groups > 1)
@@ -873,7 +898,7 @@ void attn_key_weights_passes(const AttnKeyWeightsParams& p, hipStream_t stream) 
 
 // The launches of a chunk whose arguments are good, with a workspace of the bytes of its own layout
 // at least. k8 / k_scale: the codes of an e4m3 cache of max_ctx rows (k_cache then unused), widened
-// first.
+// beside the first piece's cut.
 inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
                                     const uint8_t* k8, const float* k_scale, float* weights,
                                     unsigned pos0, unsigned n, unsigned max_ctx, void* workspace,
@@ -882,11 +907,10 @@ inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
   const AttnKeyWeightsLayout l = attn_key_weights_layout(pos0, n, k8 != nullptr);
   char* const ws = static_cast<char*>(workspace);
   unsigned k_ctx = max_ctx;
+  AttnKWidenParams widen{};
   if (k8 != nullptr) {
     attn::half_t* const wide = reinterpret_cast<attn::half_t*>(ws + l.k_wide);
-    const unsigned grid = (2 * rows + 3) / 4;
-    attn_k_fp8_widen_kernel<><<<grid < 4096 ? grid : 4096, 256, 0, stream>>>(k8, k_scale, wide,
-                                                                             rows, max_ctx);
+    widen = {k8, k_scale, wide, rows, max_ctx};
     k_cache = wide;
     k_ctx = rows;
   }
@@ -910,6 +934,13 @@ inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
                                  cut.row_tiles,
                                  cut.spans,
                                  cut.span};
+    if (k8 != nullptr && t == 0) {
+      const unsigned grid = 2 * rows / weights_detail::kWidenRows + 1;
+      attn_key_weights_cut_kernel<true>
+          <<<2 * cut.blocks + (grid < 4096 ? grid : 4096), 256, 0, stream>>>(p, widen);
+    } else {
+      attn_key_weights_cut_kernel<false><<<2 * cut.blocks, 256, 0, stream>>>(p, widen);
+    }
     if (cut.waves == 8)
       attn_key_weights_passes<8>(p, stream);
     else
@@ -930,9 +961,9 @@ inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
 // count from the top reaches what is still to be kept. Then the rows above that rank are kept, and
 // of those equal to it the first ones. Counts are whole numbers, so their order does not matter.
 //
-// Bound by latencies, not bytes: 5.4 us for 2048 rows (one launch, the host's call), 22.6 for 262144
-// (2 MB, four launches). Joining all groups' histograms in every launch instead of adding them up in
-// memory took 35.6: 512 KiB to read per workgroup.
+// Bound by latencies, not bytes: 5.4 us for 2048 rows (one launch, the host's call), 22.6 for
+// 262144 (2 MB, four launches). Joining all groups' histograms in every launch instead of adding
+// them up in memory took 35.6: 512 KiB to read per workgroup.
 // ------------------------------------------------------------------------------------------------
 
 struct AttnEvictSelectParams {

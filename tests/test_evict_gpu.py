@@ -198,16 +198,23 @@ def test_prefill_weights_with_a_larger_scratch(attn):
         check(w[:, :rows], torch.zeros_like(w[:, :rows]), added, rel, (pos0, n))
 
 
-def test_prefill_weights_in_pieces(attn):
+@pytest.mark.parametrize("fp8", [False, True])
+def test_prefill_weights_in_pieces(attn, fp8):
     """A chunk over a cache so long that it runs in two pieces."""
     g = gen(10)
     pos0, n = 66000, 4000
     rows = pos0 + n
-    kc, _ = f16_cache(g, rows, rows)
     q = 2.0 * randn(g, n, H, D)
     w = torch.zeros(KV, rows, device="cuda")
-    attn.attn_prefill_weights(q, kc, w, pos0, n, rows, attn.PrefillWeightsScratch(n, rows))
-    added, rel = weights64(q, kc.double(), pos0)
+    sc = attn.PrefillWeightsScratch(n, rows, fp8=fp8)
+    sc.ws.fill_(0xFF)  # a workspace of NaN
+    if fp8:
+        cache, k, _ = fp8_cache(attn, g, rows, rows)
+        attn.attn_prefill_weights_fp8(q, cache, w, pos0, n, sc)
+    else:
+        k, _ = f16_cache(g, rows, rows)
+        attn.attn_prefill_weights(q, k, w, pos0, n, rows, sc)
+    added, rel = weights64(q, k.double(), pos0)
     check(w, torch.zeros_like(w), added, rel)
 
 
