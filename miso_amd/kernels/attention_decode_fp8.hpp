@@ -10,7 +10,8 @@
 // the power of two 2^(E - 7), E = floor(log2 max_d |x[d]|) (E = -100 for rows whose max is below
 // 2^-100, zero rows included), so x / scale is exact and lies in (-256, 256): encoding is a
 // round-to-nearest-even to 3 mantissa bits (subnormal step 2^-9) and never saturates. Inputs
-// must be finite.
+// must be finite. Readers also take a scale of 0, a row of zeros (what a bounded cache's move leaves
+// for an index outside its source).
 //
 // Kernels:
 //   attn_kv_fp8_encode_kernel<256>  f16 cache rows [pos0, pos0 + n) of both KV heads -> e4m3 rows
@@ -482,7 +483,9 @@ __device__ __attribute__((always_inline)) inline void split_partial_fp8_waves(
     const unsigned key = k < 4 ? 4 * g + k : 16 + 4 * g + (k - 4);
     vl = 8192 + 256 * key + 8 * h + 16 * fp8_swz(key);
   }
-  float vref = 0.0f;  // R: the largest V row scale of the item's tiles so far (O is relative to it)
+  // R: the largest V row scale of the item's tiles so far (O is relative to it), or the least normal
+  // number: rows of scale 0 (zeros) then weigh their V with 0, also where a tile has no others.
+  float vref = 0x1p-126f;
 
   // Tile j: in flight after its copies, those of tile j + 1 (17, if it exists). Every operand of
   // the tile is read into registers first; then tile j + 2 goes into its stage.
@@ -520,7 +523,7 @@ __device__ __attribute__((always_inline)) inline void split_partial_fp8_waves(
     for (unsigned b = 0; b < 16; ++b)
       va[b] = widen8(static_cast<unsigned>(raw.v[b].x), static_cast<unsigned>(raw.v[b].y));
     // The tile's largest V row scale (rows past the span read the last row's): R moves up to it,
-    // O by the exact power-of-two ratio (0 on the first tile, whose O is 0).
+    // O by the exact power-of-two ratio (a tiny one on the first tile, whose O is 0).
     const float vmax = cdna4::wave_allmax(
         fmaxf(fmaxf(fmaxf(vsc[0], vsc[1]), fmaxf(vsc[2], vsc[3])),
               fmaxf(fmaxf(vsc[4], vsc[5]), fmaxf(vsc[6], vsc[7]))));

@@ -391,6 +391,37 @@ def test_gather_fp8(attn, n, keep, out_ctx):
         assert (b[:, keep:] == (0 if a.data_ptr() == w.data_ptr() else 3)).all()
 
 
+@pytest.mark.parametrize("keep,hidden", [(33, range(33)), (70, range(40)), (200, range(64, 170)),
+                                         (700, [*range(96), *range(300, 500), 699])])
+def test_decode_over_gathered_rows_of_zeros(attn, keep, hidden):
+    """Rows that an index outside the source left as zeros (e4m3: scale 0) are keys like others: score
+    0, value 0. Whole tiles of them, also the first ones of a wave."""
+    g = gen(keep)
+    n = 900
+    src, dst = fp8_cache(attn, g, n, n)[0], attn.Fp8Cache(keep)
+    index = torch.stack([torch.randperm(n, generator=g, device="cuda")[:keep] for _ in range(KV)])
+    index = index.to(torch.int32).contiguous()
+    index[:, list(hidden)] = n
+    attn.attn_evict_gather_fp8(src, torch.rand(KV, n, generator=g, device="cuda"), index, keep, dst,
+                               torch.empty(KV, keep, device="cuda"))
+    k, v = ((x.view(torch.float8_e4m3fn).float().double().view(KV, keep, D) *
+             s.double().view(KV, keep, 1))
+            for x, s in ((dst.k8, dst.k_scale), (dst.v8, dst.v_scale)))
+    for t in (k, v):
+        assert (t[:, list(hidden)] == 0).all()
+    q, qg = 2.0 * randn(g, 1, H, D), randn(g, 1, H, 2, D)
+    sc, zero = attn.DecodeWeightsScratch(8, keep), torch.zeros(KV, keep, device="cuda")
+    added, rel = weights64(q, k, keep - 1)
+    want = attend64(q, qg, k, v, keep - 1)[0]
+    for n_splits in (1, 2, None):
+        core, w = torch.empty(H, D, device="cuda"), zero.clone()
+        attn.attn_decode_weights_fp8(q, qg, dst, core, w, sc, keep, n_splits=n_splits)
+        check(w, zero, added, rel, n_splits)
+        for h in range(H):  # the reference's gate for a decode
+            err, size = (core[h].double() - want[h]).norm(), want[h].norm()
+            assert float(err) <= 1e-5 * float(size), (n_splits, h)
+
+
 def prep_inputs(g, n):
     proj = randn(g, n, 9216)
     norms = [1 + 0.1 * randn(g, D), 1 + 0.1 * randn(g, D)]
