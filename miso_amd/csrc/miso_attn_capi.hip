@@ -1113,10 +1113,8 @@ const char* bad_gather(uint32_t max_ctx, uint32_t keep, uint32_t out_ctx) {
 
 template <bool kFp8>
 int gather(const char* fn, const k::AttnEvictGatherParams& p, void* stream) {
-  const uint64_t rows = kFp8 ? 32 : 8;  // of a workgroup's step
-  const uint64_t groups = (uint64_t{2} * p.keep + rows - 1) / rows;
   k::attn_evict_gather_kernel<kFp8>
-      <<<static_cast<unsigned>(std::min<uint64_t>(groups, 1u << 20)), 256, 0, as_stream(stream)>>>(
+      <<<k::attn_evict_gather_grid<kFp8>(p.keep, p.out_ctx), 256, 0, as_stream(stream)>>>(
           p);
   return launched(fn);
 }

@@ -391,6 +391,55 @@ def test_gather_fp8(attn, n, keep, out_ctx):
         assert (b[:, keep:] == (0 if a.data_ptr() == w.data_ptr() else 3)).all()
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("keep,out_ctx", [(3, 20000), (1, 1025), (16, 262144), (500, 300001)])
+def test_small_move_into_a_large_cache(attn, keep, out_ctx, fp8):
+    """The weights behind the kept rows become 0, all of them and nothing else, and their clearing
+    does not set the pace (it is 2 MB for 262144 rows): a move into a cache of that size takes at most
+    4 times what the same move takes into one of its own size, by the least of several timings."""
+    g = gen(keep + out_ctx)
+    n = 600
+    w = torch.rand(KV, n, generator=g, device="cuda")
+    index = torch.stack([torch.randperm(n, generator=g, device="cuda")[:keep] for _ in range(KV)])
+    index = index.to(torch.int32).contiguous()
+    src = fp8_cache(attn, g, n, n)[0] if fp8 else f16_cache(g, n, n)
+
+    def into(rows):
+        guarded = torch.full((KV * rows + 64,), 9.0, device="cuda")
+        wo = guarded[32:32 + KV * rows]
+        if fp8:
+            out = attn.Fp8Cache(rows)
+            bufs = [t.fill_(3) for t in out.buffers()]
+            return lambda: attn.attn_evict_gather_fp8(src, w, index, keep, out, wo), guarded, bufs
+        bufs = [torch.full((KV, rows, D), 3.0, dtype=torch.float16, device="cuda") for _ in range(2)]
+        return (lambda: attn.attn_evict_gather(*src, w, n, index, keep, *bufs, wo, rows)), guarded, bufs
+
+    call, guarded, bufs = into(out_ctx)
+    call()
+    assert (guarded[:32] == 9).all() and (guarded[-32:] == 9).all()
+    got = guarded[32:-32].view(KV, out_ctx)
+    assert torch.equal(got[:, :keep], w[torch.arange(KV, device="cuda")[:, None], index.long()])
+    assert (got[:, keep:] == 0).all()
+    for t in bufs:
+        assert (t.view(KV, out_ctx, -1)[:, keep:] == 3).all()
+
+    def least(f):
+        best = math.inf
+        for _ in range(6):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(20):
+                f()
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    small = into(keep)[0]
+    least(small), least(call)  # both warm
+    assert least(call) <= 4 * least(small)
+
+
 @pytest.mark.parametrize("keep,hidden", [(33, range(33)), (70, range(40)), (200, range(64, 170)),
                                          (700, [*range(96), *range(300, 500), 699])])
 def test_decode_over_gathered_rows_of_zeros(attn, keep, hidden):
