@@ -534,9 +534,10 @@ def attn_decode_weights_fp8(q, qg, cache: Fp8Cache, core, weights, scratch: Deco
 
 
 class PrefillWeightsScratch:
-    """Workspace of attn_prefill_weights for up to max_n tokens over up to max_rows cache rows (with
-    fp8, of attn_prefill_weights_fp8 too, which widens K rows into it): 16 KiB per token and
-    some MB."""
+    """Workspace of attn_prefill_weights for up to max_n tokens over up to max_rows cache rows: 16 KiB
+    per token (of 16384 at most), some MB, and sums of 8 bytes per row and 16 to 32 tokens, 64 MiB or
+    64 bytes per row at most. With fp8 it serves attn_prefill_weights_fp8 too, which widens K rows
+    into it: 1 KiB per row."""
 
     def __init__(self, max_n: int, max_rows: int, fp8: bool = False, device="cuda"):
         self.max_n, self.max_rows = _count(max_n, "max_n"), _count(max_rows, "max_rows")

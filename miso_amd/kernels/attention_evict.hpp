@@ -799,13 +799,20 @@ struct AttnKeyWeightsCut {
   unsigned blocks, waves, groups, row_tiles, spans;
   unsigned long long span;
 };
+// Groups of 4 also keep within the bound of the sums: 9 to 11 of them up to 762000 rows or more.
 constexpr unsigned kWeightsCus = 256, kWeightsNearRows = 4096;
+// The (group, row) sums of a KV head, for a piece over `rows` rows: 8 groups' at least, so that a
+// streamed K serves them together (2.1 million rows, 256 tokens: 13.7 ms, in pieces of 4 groups 15.2).
+__host__ __device__ constexpr std::size_t attn_key_weights_most_sums(std::size_t rows) {
+  return 8 * rows > std::size_t{1} << 23 ? 8 * rows : std::size_t{1} << 23;
+}
 __host__ __device__ constexpr AttnKeyWeightsCut attn_key_weights_cut(unsigned pos0, unsigned n) {
   using namespace weights_detail;
   AttnKeyWeightsCut c{};
   c.blocks = div_up(n, kTokens);
   const unsigned rows = pos0 + n;
-  const bool fills = c.blocks < 64 && 27 * div_up(c.blocks, 4) < 50 * div_up(c.blocks, 8);
+  const bool fills = c.blocks < 64 && 27 * div_up(c.blocks, 4) < 50 * div_up(c.blocks, 8) &&
+                     std::size_t{div_up(c.blocks, 4)} * rows <= attn_key_weights_most_sums(rows);
   c.waves = rows <= kWeightsNearRows || fills ? 4 : 8;
   c.groups = div_up(c.blocks, c.waves);
   c.row_tiles = div_up(rows, kKeys);
@@ -817,10 +824,10 @@ __host__ __device__ constexpr AttnKeyWeightsCut attn_key_weights_cut(unsigned po
 }
 
 // A chunk runs in pieces of at most this many tokens, so that the groups' sums (8 bytes per group
-// and row) stay within 64 MiB over long caches.
+// and row) stay within 64 MiB, or 64 bytes a row beyond 2^20 rows (where the cache has 2048).
 __host__ __device__ constexpr unsigned attn_key_weights_tokens(unsigned rows) {
-  const unsigned groups = (1u << 23) / (rows < 64 ? 64 : rows);
-  return 32 * (groups < 8 ? 8 : groups);
+  const std::size_t few = rows < 64 ? 64 : rows;
+  return 32 * static_cast<unsigned>(attn_key_weights_most_sums(few) / few);
 }
 
 // The groups that a piece of up to `blocks` column blocks over up to `rows` rows has at most, where
@@ -828,14 +835,18 @@ __host__ __device__ constexpr unsigned attn_key_weights_tokens(unsigned rows) {
 __host__ __device__ constexpr std::size_t attn_key_weights_groups(std::size_t blocks) {
   return (blocks < 64 ? blocks / 4 : blocks < 120 ? 15 : blocks / 8) + 1;
 }
-// Floats of the groups' sums.
+// Floats of the groups' sums of pieces of up to `blocks` column blocks over up to `rows` rows (whole
+// tiles): never less for more blocks or rows. A piece's groups, 513 at most, times its rows are
+// within attn_key_weights_most_sums, so times its whole tiles' rows at most 2^14 above it.
 __host__ __device__ constexpr std::size_t attn_key_weights_sums(std::size_t blocks,
                                                                 std::size_t rows) {
   const std::size_t far = attn_key_weights_groups(blocks) * rows;
   const std::size_t near_blocks = blocks < kWeightsNearRows / 4 ? blocks : kWeightsNearRows / 4;
   const std::size_t near =
       (near_blocks / 4 + 1) * (rows < kWeightsNearRows ? rows : std::size_t{kWeightsNearRows});
-  return 2 * (far > near ? far : near);
+  const std::size_t most = attn_key_weights_most_sums(rows) + (1u << 14);
+  const std::size_t sums = far > near ? far : near;
+  return 2 * (sums < most ? sums : most);
 }
 
 // The workspace's parts, in bytes from its start, each 256-byte aligned.
@@ -875,16 +886,14 @@ __host__ __device__ constexpr AttnKeyWeightsLayout attn_key_weights_layout(unsig
 }
 
 // Bytes that serve every chunk of up to max_n tokens over up to max_rows rows. A piece has at most
-// 16384 tokens (its tokens times its rows, at least as many, are at most 2^28); its sums are those
-// of max_n at most, or of 2^23 group rows and 16 groups more.
+// 16384 tokens (its tokens times its rows, at least as many, are at most 2^28, or it has 256).
 __host__ __device__ constexpr std::size_t attn_key_weights_bytes(unsigned max_n, unsigned max_rows,
                                                                  bool fp8) {
   using namespace weights_detail;
   const std::size_t blocks = div_up(max_n < 16384 ? max_n : 16384, kTokens);
   const std::size_t rows = std::size_t{div_up(max_rows, kKeys)} * kKeys;
-  const std::size_t by_n = attn_key_weights_sums(blocks, rows);
-  const std::size_t by_rows = 2 * ((std::size_t{1} << 23) + 16 * (rows + 64));
-  return attn_key_weights_parts(blocks, by_n < by_rows ? by_n : by_rows, fp8 ? max_rows : 0).bytes;
+  return attn_key_weights_parts(blocks, attn_key_weights_sums(blocks, rows), fp8 ? max_rows : 0)
+      .bytes;
 }
 
 template <unsigned W>

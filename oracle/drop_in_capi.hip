@@ -1,10 +1,13 @@
 // Test infrastructure: extern "C" launchers for what the product's own library does not launch: the
 // engine drop-in (miso_amd/engine/attention.{hpp,hip} against engine_stub/), the 64 x 64 GEMM
 // kernel that the engine's own gemm() launches, GEMM batches of any mix, and the host's choices of
-// a form. Used only by GPU tests; never linked into the product.
+// a form and of a workspace's layout. Used only by tests; never linked into the product.
 
 #include "engine/attention.hip"
 
+#include "attention_evict.hpp"
+
+#include <algorithm>
 #include <cstring>
 
 namespace {
@@ -138,6 +141,23 @@ unsigned drop_qgemm_shape(unsigned count, const int* format, const unsigned* n_r
 // two row blocks (host only).
 unsigned drop_prefill_form(unsigned pos0, unsigned n, std::uint64_t workspace_bytes) {
   return static_cast<unsigned>(miso::kernels::attn_prefill_form(pos0, n, workspace_bytes));
+}
+
+// The prompt weights' workspace of one chunk: where its halves, scales, statistics, sums and widened
+// K begin, and its end (host only).
+void drop_key_weights_layout(unsigned pos0, unsigned n, int fp8, std::uint64_t* out) {
+  const auto l = miso::kernels::attn_key_weights_layout(pos0, n, fp8 != 0);
+  const std::size_t at[] = {l.halves, l.scale, l.stats, l.sums, l.k_wide, l.bytes};
+  std::copy(at, at + 6, out);
+}
+
+// How the piece of that chunk that begins with token t is cut: its tokens, column blocks, waves of a
+// workgroup, groups, tiles of rows, spans and tiles of a span (host only).
+void drop_key_weights_piece(unsigned pos0, unsigned n, unsigned t, std::uint64_t* out) {
+  const unsigned m = std::min(n - t, miso::kernels::attn_key_weights_tokens(pos0 + n));
+  const auto c = miso::kernels::attn_key_weights_cut(pos0 + t, m);
+  const std::uint64_t is[] = {m, c.blocks, c.waves, c.groups, c.row_tiles, c.spans, c.span};
+  std::copy(is, is + 7, out);
 }
 
 }  // extern "C"

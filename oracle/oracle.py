@@ -523,6 +523,8 @@ def drop_in():
             "drop_engine_step": (c_int, [V, c_int, V, V, V, U, c_float]),
             "drop_engine_read": (c_uint64, [V, ctypes.c_char_p, V, c_uint64]),
             "drop_prefill_form": (U, [U, U, c_uint64]),
+            "drop_key_weights_layout": (None, [U, U, c_int, V]),
+            "drop_key_weights_piece": (None, [U, U, U, V]),
             "drop_qgemm_kernel": (c_int, [c_int, V, V, V, V, U, U, U, U]),
             "drop_qgemm_batch": (c_int, [U, V, V, V, V, V, U, V, U, U]),
             "drop_qgemm_shape": (U, [U, V, V, U]),

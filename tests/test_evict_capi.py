@@ -2,6 +2,7 @@
 for a refused call), and that their workspaces cover every smaller call."""
 from __future__ import annotations
 
+import ctypes
 import random
 
 import pytest
@@ -71,6 +72,70 @@ def test_prefill_weights_workspace_covers_smaller_calls(lib):
                 m = rng.randint(1, n)
                 pos0 = rng.randint(0, rows - m)
                 assert lib.miso_attn_prefill_weights_workspace_bytes(m, pos0 + m, fp8) <= cap
+
+
+MIB = 1 << 20
+
+
+def test_prefill_weights_workspace_is_bounded_over_any_cache(lib):
+    """Beside 16 KiB of halves a token (of a piece: 16384 at most, rounded up to 4) there are at most 64
+    MiB of sums, or 64 bytes a row, and 4 MiB of scales and statistics, up to the most rows that a cache
+    may have; over e4m3 rows the widened K is 1 KiB a row more."""
+    for rows in (1 << 16, 1 << 20, (1 << 20) + 1, 3 << 20, 1 << 23, (1 << 24) + 5, 1 << 29):
+        for n in (1, 33, 256, 4096, 16384, 1 << 20):
+            halves = (min(n, 16384) + 3) * 16384
+            got = lib.miso_attn_prefill_weights_workspace_bytes(n, rows, 0)
+            assert got <= halves + max(64 * MIB, 64 * (rows + 31)) + 4 * MIB, (rows, n, got / MIB)
+            assert lib.miso_attn_prefill_weights_workspace_bytes(n, rows, 1) <= got + 1024 * (rows + 1)
+
+
+def key_weights_shapes():
+    rng = random.Random(5)
+    for pos0 in (0, 1, 31, 32, 33, 4000, 4095, 4096, 12001, 262143, 1 << 20):
+        for n in (1, 2, 4, 5, 16, 17, 32, 33, 64, 65, 300, 1000, 4096):
+            yield pos0, n
+    for _ in range(1500):
+        rows = int(2 ** rng.uniform(0, rng.choice([13, 19, 24, 29])))
+        n = min(rows, max(1, int(2 ** rng.uniform(0, 20))))
+        yield rng.choice([0, rows - n, rng.randint(0, rows - n)]), n
+
+
+def test_prefill_weights_workspace_covers_what_a_launch_uses(lib, O):
+    """The capacity holds the chunk's layout, and the layout what each piece's kernels index: the halves
+    and scales of its column blocks, the statistics of its spans and groups, and its groups' sums
+    (a single group has none)."""
+    host = O.drop_in()
+    layout, piece = (ctypes.c_uint64 * 6)(), (ctypes.c_uint64 * 7)()
+    rng = random.Random(6)
+    for pos0, n in key_weights_shapes():
+        rows = pos0 + n
+        for fp8 in (0, 1):
+            host.drop_key_weights_layout(pos0, n, fp8, layout)
+            halves, scale, stats, sums, wide, end = layout
+            assert all(x % 256 == 0 for x in layout)
+            assert end - wide >= (1024 * rows if fp8 else 0)
+            more = rng.randint(0, 5000)
+            for max_n, max_rows in ((n, rows), (n + more, rows + more), (n, rows + 100 * more)):
+                if max_rows <= 1 << 29:
+                    cap = lib.miso_attn_prefill_weights_workspace_bytes(max_n, max_rows, fp8)
+                    assert cap >= end, (pos0, n, max_n, max_rows)
+        host.drop_key_weights_piece(pos0, n, 0, piece)
+        most = piece[0]
+        count = -(-n // most)
+        for i in {0, 1, count // 2, count - 2, count - 1, rng.randrange(count)}:
+            if not 0 <= i < count:
+                continue
+            host.drop_key_weights_piece(pos0, n, i * most, piece)
+            m, blocks, waves, groups, row_tiles, spans, span = piece
+            at = (pos0, n, i)
+            assert m == min(most, n - i * most) and blocks == -(-m // 4), at
+            assert groups * waves >= blocks > (groups - 1) * waves and waves in (4, 8), at
+            assert 32 * row_tiles >= pos0 + i * most + m > 32 * (row_tiles - 1), at
+            assert 0 < spans <= 256 * (8 // waves) and span > 0, at
+            assert scale - halves >= 2 * blocks * 32768, at
+            assert stats - scale >= 2 * blocks * 4, at
+            assert sums - stats >= (spans + 2 * groups) * 32 * waves * 8, at
+            assert groups == 1 or wide - sums >= 2 * groups * row_tiles * 32 * 4, at
 
 
 def test_select_refusals(lib):

@@ -218,6 +218,20 @@ def test_prefill_weights_in_pieces(attn, fp8):
     check(w, torch.zeros_like(w), added, rel)
 
 
+@pytest.mark.parametrize("rows,n", [(1_000_000, 130), (1_100_001, 300), (4_200_000, 16)])
+def test_prefill_weights_over_a_million_rows(attn, rows, n):
+    """Groups that the bound of their sums makes larger, pieces of 8 groups with a rest, one group."""
+    g = gen(rows)
+    k = randn(g, KV, rows, D, dtype=torch.float16)
+    q = 2.0 * randn(g, n, H, D)
+    w = torch.zeros(KV, rows, device="cuda")
+    sc = attn.PrefillWeightsScratch(n, rows)
+    sc.ws.fill_(0xFF)  # a workspace of NaN
+    attn.attn_prefill_weights(q, k, w, rows - n, n, rows, sc)
+    added, rel = weights64(q, k.double(), rows - n)
+    check(w, torch.zeros_like(w), added, rel)
+
+
 @pytest.mark.parametrize("pos0,n", [(2500, 70), (5000, 300), (0, 200)])
 def test_prefill_weights_peaked(attn, pos0, n):
     """Few keys take nearly everything; rising scores lead the first tile's by far more and by less
