@@ -473,15 +473,19 @@ int miso_attn_decode_weights_fp8(const float* q, const float* qg, const uint8_t*
 uint64_t miso_attn_prefill_weights_workspace_bytes(uint32_t max_n, uint32_t max_rows, int fp8);
 
 /* The weights that n queries ([n][16][256], as the batched prep writes them) at rows pos0 .. give
- * the rows they see: row j gets the causal softmax weights of every token t with j <= pos0 + t, at
- * f32 precision (the queries as exact pairs of f16). Run beside miso_attn_prefill over the same
- * cache; the last tokens of a prompt alone may vote (q of those, pos0 their first row). Rejects
- * n == 0, pos0 + n > max_ctx, max_ctx > 2^29 and a workspace that is too small. */
+ * the rows they see: row j gets the causal softmax weights of every token t with j <= pos0 + t.
+ * Scores and sums are f32; a query element enters as a pair of f16, off by at most 2^-22 of itself
+ * or, where that is more, 2^-38 of the largest element of its block (8 query heads of a KV head,
+ * tokens 4 i .. 4 i + 3 of the call), which shares one power of two. Run beside miso_attn_prefill over
+ * the same cache; the last tokens of a prompt alone may vote (q of those, pos0 their first row).
+ * Rejects n == 0, pos0 + n > max_ctx, max_ctx > 2^29 and a workspace that is too small. */
 int miso_attn_prefill_weights(const float* q, const uint16_t* k_cache, float* weights,
                               uint32_t pos0, uint32_t n, uint32_t max_ctx, void* workspace,
                               uint64_t workspace_bytes, void* stream);
 
-/* The same over the e4m3-row cache, its K rows widened to f16 as miso_attn_prefill_fp8 does. */
+/* The same over the e4m3-row cache, its K rows widened to f16 as miso_attn_prefill_fp8 does: held
+ * within 65504, and off by up to 2^-25 where f16 is subnormal (row scales below 2^-15), where
+ * miso_attn_decode_weights_fp8 multiplies by the scale in f32. */
 int miso_attn_prefill_weights_fp8(const float* q, const uint8_t* k8, const float* k_scale,
                                   float* weights, uint32_t pos0, uint32_t n, uint32_t max_ctx,
                                   void* workspace, uint64_t workspace_bytes, void* stream);

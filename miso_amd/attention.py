@@ -570,7 +570,8 @@ def attn_prefill_weights(q, k_cache, weights, pos0: int, n: int, max_ctx: int,
 
 def attn_prefill_weights_fp8(q, cache: Fp8Cache, weights, pos0: int, n: int,
                              scratch: PrefillWeightsScratch, stream=None) -> None:
-    """attn_prefill_weights over an e4m3 cache (scratch made with fp8=True)."""
+    """attn_prefill_weights over an e4m3 cache (scratch made with fp8=True), its K rows widened to f16
+    as attn_prefill_fp8 does."""
     if not scratch.fp8:
         raise ValueError("the scratch was made without fp8=True")
     _need_fp8(cache)

@@ -223,7 +223,8 @@ __global__ void __launch_bounds__(64) attn_combine_weights_kernel(AttnWeightsPar
 // power of two that puts its largest element in [2^13, 2^14), and cut into f16 halves x = hi + lo,
 // exact to 2^-22 of x, or 2^-38 of the block's largest element where lo is subnormal (what counts
 // is a score's absolute error: beside a query element of 1000, that is 4e-9 per unit of K). hi k +
-// lo k are exact products summed in f32; the scale comes off in the exponent's fma. So a score
+// lo k are exact products summed in f32; the scale comes off in the exponent's fma (one per column
+// would take 16 registers more in the second pass, which has 4 left of its 256). So a score
 // costs 1024 flop of f16 matrix work per pass, and the passes are bound by it once there are some
 // hundred queries.
 //
@@ -352,7 +353,9 @@ struct AttnKWidenParams {
 };
 
 namespace weights_detail {
-// K codes widened to f16 (attn_kv_fp8_widen_kernel's values, K alone): workgroup `first` of
+// K codes widened to f16 (attn_kv_fp8_widen_kernel's values, K alone: the matrix cores take f16, a
+// code's 4 bits fit it exactly, and only row scales below 2^-15 make subnormals, off by 2^-25 at
+// most, which is below what f32 sums of ordinary scores lose): workgroup `first` of
 // `groups` of 4 waves, 8 codes a lane, 8 rows of a wave in flight.
 constexpr unsigned kWidenRows = 32;  // a workgroup's at a time
 __device__ __attribute__((always_inline)) inline void widen_rows(const AttnKWidenParams& p,

@@ -270,6 +270,90 @@ def test_prefill_weights_query_magnitudes(attn):
     check(w, torch.zeros_like(w), added, rel)
 
 
+def limit64(q, k, pos0, k_off=0.0):
+    """weights64's sums, and how far each may be off, query by query: a score in log2 units by
+      A (2^-22 + 40 2^-24) + (2^-38 B sum |k| + k_off sum |q|) log2(e) / 16
+    (A the sum of the magnitudes of its products as in the module's docstring; B the largest query element
+    of its block of 4 tokens x 8 heads, whose power of two the cut shares; k_off what a K element is off
+    by), its logarithmic sum by the largest of these, its weight by 2^(both) - 1 of itself, and by 2^-19
+    of itself for the exponential, the sums of the statistics and the scale's rounding."""
+    n, keys = q.shape[0], k.shape[1]
+    out = torch.zeros(KV, keys, dtype=torch.float64, device="cuda")
+    lim = torch.zeros_like(out)
+    hidden = torch.arange(keys, device="cuda")[None, :] > \
+        pos0 + torch.arange(n, device="cuda")[:, None]
+    top = q.abs().amax(dim=2).view(n, KV, G).amax(dim=2)
+    for h in range(H):
+        kk = k[h // G]
+        s = (q[:, h].double() @ kk.T) / math.sqrt(D)
+        p = torch.softmax(s.masked_fill_(hidden, -math.inf), dim=1)
+        out[h // G] += p.sum(dim=0)
+        block = torch.stack([top[t // 4 * 4:t // 4 * 4 + 4, h // G].max() for t in range(n)]).double()
+        off = (q[:, h].double().abs() @ kk.abs().T) * (2 ** -22 + 40 * 2 ** -24)
+        off += 2 ** -38 * block[:, None] * kk.abs().sum(dim=1)
+        off += k_off * q[:, h].double().abs().sum(dim=1)[:, None]
+        off = (off * (math.log2(math.e) / math.sqrt(D))).masked_fill_(hidden, 0.0)
+        off += off.amax(dim=1, keepdim=True)
+        lim[h // G] += (p * torch.expm1(off * math.log(2) + 2 ** -19)).clamp(max=1.0).sum(dim=0)
+    return out, lim + (n / 4 + 64) * 2 ** -24 * out + 1e-30
+
+
+@pytest.mark.parametrize("factor", [2.0 ** 10, 2.0 ** 16, 2.0 ** 22])
+@pytest.mark.parametrize("t,h", [(0, 0), (5, 3), (6, 12)])
+def test_prefill_weights_of_one_large_query(attn, factor, t, h):
+    """One head of one token far larger than the others: what it takes from the precision of its block's
+    queries is bounded, and those of other blocks keep theirs (limit64)."""
+    g = gen(t + h)
+    pos0, n = 190, 12
+    rows = pos0 + n
+    kc, _ = f16_cache(g, rows, rows)
+    q = randn(g, n, H, D)
+    q[t, h] *= factor
+    w = torch.zeros(KV, rows, device="cuda")
+    attn.attn_prefill_weights(q, kc, w, pos0, n, rows, attn.PrefillWeightsScratch(n, rows))
+    want, lim = limit64(q, kc.double(), pos0)
+    assert float(((w.double() - want).abs() / lim).max()) <= 1
+
+
+@pytest.mark.parametrize("pos0,n", [(0, 300), (700, 33), (4000, 300), (2000, 4)])
+def test_prefill_weights_of_low_halves(attn, pos0, n):
+    """Queries whose elements need more than f16: all of (1 + 2^-12) times a power of two. Without the
+    second half every score of a token would be 2^-12 of itself nearer to 0, for all tokens alike, and
+    weights off by up to 2^-12 times 32 of themselves, 46 times the tolerance."""
+    g = gen(n)
+    rows = pos0 + n
+    level = torch.rand(KV, rows, 1, generator=g, device="cuda") * 2 - 1
+    sign = torch.where(torch.rand(D, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    kc = (level * sign).half()
+    q = torch.exp2(torch.randint(-1, 2, (n, H, 1), generator=g, device="cuda").float())
+    q = q * (1 + 2 ** -12) * sign
+    w = torch.zeros(KV, rows, device="cuda")
+    attn.attn_prefill_weights(q, kc, w, pos0, n, rows, attn.PrefillWeightsScratch(n, rows))
+    added, rel = weights64(q, kc.double(), pos0)
+    check(w, torch.zeros_like(w), added, rel)
+
+
+@pytest.mark.parametrize("low,high,size", [(-30, -9, 50.0), (5, 11, 2.0 ** -13),
+                                           (12, 17, 2.0 ** -15)])
+@pytest.mark.parametrize("pos0,n", [(300, 40), (0, 33)])
+def test_prefill_weights_fp8_row_scales(attn, low, high, size, pos0, n):
+    """Rows of very small and very large scales: K as f16, its elements off by at most 2^-25 where f16 is
+    subnormal (4 bits of a code are exact elsewhere) and held within 65504."""
+    g = gen(low + n)
+    rows = pos0 + n
+    cache, k, _ = fp8_cache(attn, g, rows, rows)
+    more = torch.exp2(torch.randint(low, high, (KV, rows), generator=g, device="cuda").float())
+    cache.k_scale.mul_(more.view(-1))
+    k = k * more.double()[..., None]
+    assert (low == 12) == (float(k.abs().max()) > 65504)
+    q = size * randn(g, n, H, D)
+    w = torch.zeros(KV, rows, device="cuda")
+    attn.attn_prefill_weights_fp8(q, cache, w, pos0, n,
+                                  attn.PrefillWeightsScratch(n, rows, fp8=True))
+    want, lim = limit64(q, k.clamp(-65504.0, 65504.0), pos0, 2 ** -25)
+    assert float(((w.double() - want).abs() / lim).max()) <= 1
+
+
 def test_prefill_weights_of_one_token_equals_decode(attn):
     g = gen(12)
     n = 777
