@@ -875,21 +875,24 @@ def layer_decode_weights(layer: Layer, k_cache, v_cache, max_ctx: int, row: int,
 
 def layer_prefill_weights(layer: Layer, k_cache, v_cache, max_ctx: int, row0: int, pos0: int,
                           n: int, h, delta, y, eps: float, ws: LayerWorkspace, weights,
-                          scratch: PrefillWeightsScratch, voters: Optional[int] = None,
+                          scratch: Optional[PrefillWeightsScratch], voters: Optional[int] = None,
                           stream=None) -> None:
     """layer_prefill over a bounded cache: tokens of positions pos0 .. at rows row0 ..; the last
-    `voters` of them (None: all) add the weights they give the rows they see to weights."""
+    `voters` of them (None: all) add the weights they give the rows they see to weights. With 0
+    voters weights and scratch are not looked at and may be None."""
     for name, x in (("row0", row0), ("pos0", pos0), ("n", n), ("max_ctx", max_ctx)):
         _count(x, name)
     voters = n if voters is None else min(_count(voters, "voters"), n)
-    if voters > scratch.max_n or row0 + n > scratch.max_rows:
-        raise ValueError("voters or row0 + n exceeds the scratch capacity")
+    votes = (None, None, 0)
+    if voters:
+        if voters > scratch.max_n or row0 + n > scratch.max_rows:
+            raise ValueError("voters or row0 + n exceeds the scratch capacity")
+        _need(weights, "weights", torch.float32, KV_HEADS * max_ctx)
+        _here(weights, scratch.ws)
+        votes = (_ptr(weights), _ptr(scratch.ws), scratch.ws.numel())
     _rows(n, h=h, delta=delta, y=y)
-    _need(weights, "weights", torch.float32, KV_HEADS * max_ctx)
     kc, vc = _layer_cache(k_cache, v_cache, max_ctx)
-    _here(h, y, k_cache, v_cache, weights, scratch.ws, ws.prefill,
-          *(() if delta is None else (delta,)))
+    _here(h, y, k_cache, v_cache, ws.prefill, *(() if delta is None else (delta,)))
     _lib.check(_lib.load().miso_attn_layer_prefill_weights(
         ctypes.addressof(layer.c), kc, vc, row0, pos0, n, max_ctx, _ptr(h), _ptr(delta), _ptr(y),
-        eps, _ptr(ws.prefill), ws.max_tok, voters, _ptr(weights), _ptr(scratch.ws),
-        scratch.ws.numel(), _stream(stream)))
+        eps, _ptr(ws.prefill), ws.max_tok, voters, *votes, _stream(stream)))

@@ -127,6 +127,27 @@ def test_layer_prefill_weights(attn, layers, row0, n, voters):
     assert torch.equal(w[:, rows:], before[:, rows:])
 
 
+@pytest.mark.parametrize("how", ["small scratch", "none"])
+def test_layer_prefill_weights_without_voters(attn, layers, how):
+    """The chunks of a prompt before the one that votes: what only votes need is not asked for."""
+    g = gen(8)
+    row0, n = 40, 20
+    ctx = row0 + n + 2
+    k, v = f16_cache(g, row0, ctx)
+    h = randn(g, n * 2048)
+    got = [t.clone() for t in (h, k, v)]
+    ws = attn.LayerWorkspace(max_tok=32)
+    y, y0 = (torch.empty(n * 2048, device="cuda") for _ in range(2))
+    votes = (None, None) if how == "none" else \
+        (torch.empty(0, device="cuda"), attn.PrefillWeightsScratch(4, 8))
+    attn.layer_prefill_weights(layers["q4_k"], got[1], got[2], ctx, row0, row0, n, got[0], None, y, EPS,
+                               ws, *votes, voters=0)
+    attn.layer_prefill(layers["q4_k"], k, v, ctx, row0, n, h, None, y0, EPS, ws)
+    assert torch.equal(y, y0)
+    for a, b in zip(got, (h, k, v)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 @pytest.mark.parametrize("row0,pos0,n", [(0, 50, 20), (100, 5000, 33)])
 def test_layer_prefill_weights_at_another_row(attn, layers, row0, pos0, n):
     g = gen(pos0)
