@@ -435,6 +435,37 @@ def test_select_of_long_stretches(attn):
             assert np.array_equal(got[h], select_np(w[h], keep, sinks, recent)), (keep, h)
 
 
+def test_select_lengths_of_one_scratch(attn):
+    """One scratch, dirty at first, for selections of other numbers of workgroups in turn, of one launch
+    and of four, eager and replayed: where a workspace's parts lie goes with the length."""
+    rng = np.random.default_rng(6)
+    ctx, esc = 90000, attn.EvictScratch(90000)
+    esc.ws.fill_(0xFF)
+    w = np.exp(rng.standard_normal((KV, ctx))).astype(np.float32)
+    wd = torch.from_numpy(w).cuda()
+    calls = []
+    for n, keep in ((90000, 40001), (17000, 16999), (40000, 100), (16000, 9), (65537, 65000), (17408, 1)):
+        index = torch.full((KV, keep), -7, dtype=torch.int32, device="cuda")
+        want = np.stack([select_np(w[h, :n], keep, 3, 0 if keep < 10 else 5)
+                         if keep > 3 else select_np(w[h, :n], keep, 0, 0) for h in range(KV)])
+        args = (n, ctx, keep, 3 if keep > 3 else 0, 5 if keep >= 10 else 0, index)
+        calls.append((args, index, want))
+    graphs = []
+    for args, index, want in calls:
+        attn.attn_evict_select(wd, *args, esc)
+        assert np.array_equal(index.cpu().numpy(), want), args[:3]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            attn.attn_evict_select(wd, *args, esc)
+        graphs.append(graph)
+    for order in (range(6), (5, 0, 1, 4, 2, 3)):
+        for i in order:
+            calls[i][1].fill_(-7)
+            graphs[i].replay()
+        for args, index, want in calls:
+            assert np.array_equal(index.cpu().numpy(), want), args[:3]
+
+
 GATHERS = [(1, 1, 1), (5, 3, 3), (64, 64, 70), (1000, 257, 300), (4099, 1023, 5000),
            (33000, 16001, 16384)]
 
