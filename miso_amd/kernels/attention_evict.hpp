@@ -26,10 +26,11 @@ namespace miso::kernels {
 // key, both KV heads, beside the 2048 it reads) and the launch that merges the partials also turns
 // them into weights. The result of the attention is attn_decode's, bit for bit.
 //
-// Bound by the K and V stream, as attn_decode: 32768 keys take 19.9 us against 18.8 without
-// weights, 262144 103.9 against 89 (5.2 TB/s of what must move), of which 9 are the score stores
-// among the loads and 5.5 the merge's; 301 keys 11.3 against 9.9, two launches and the host's call.
-// 100003 e4m3 keys 30.2.
+// Bound by the K and V stream, as attn_decode: 32768 keys take 18.8 us against 18.4 without
+// weights, 262144 104 against 88.4 (5.2 TB/s of what must move), of which 5 are the merge's and the
+// others the score stores among the loads; 301 keys 11 to 12 against 9.4, two launches (8.7 on the
+// card) and the host's call. 100003 e4m3 keys 30.2 against 25.8: half the bytes of K and V, the same
+// scores (the split 26.6 against 22.5).
 // ------------------------------------------------------------------------------------------------
 
 // The scores' row length for len keys: the padding lets a span store whole groups of 4.
@@ -129,7 +130,7 @@ constexpr unsigned kWeightKeys = 256;  // keys per workgroup of the weights' par
 // Workgroups [0, 64): attn_combine_kernel's; with h, 8 more for the residual row; the others one
 // 256-key block of one KV head each: every lane forms the head statistics from the splits' and adds
 // 4 keys' weights, 64 apart (blocks of 64 threads, so that few keys still fill many CUs and the
-// scores are asked for before the statistics are joined). 3.6 us at 301 keys, 4.2 at 32768, 9.9 at
+// scores are asked for before the statistics are joined). 3.7 us at 301 keys, 4.2 at 32768, 9.9 at
 // 262144: the stream of the scores. Grid attn_combine_weights_grid, x 64.
 __host__ __device__ constexpr unsigned attn_combine_weights_grid(unsigned len, bool add) {
   return kCombineItems + (add ? 8 : 0) + 2 * (len / kWeightKeys + (len % kWeightKeys != 0));
@@ -217,7 +218,8 @@ __global__ void __launch_bounds__(64) attn_combine_weights_kernel(AttnWeightsPar
 // p[t][h][j], p the causal softmax over j <= pos0 + t. A weight needs its row's maximum and sum
 // before it can join its column's sum, so the products q k are formed twice: the first pass gives
 // each query's maximum and sum, the second sums 2^(s - lse) over the queries. (Keeping the scores
-// instead would move 64 bytes per token and key through memory twice, against 1024 flop.)
+// instead would move the 16 heads' 64 bytes per token and key through memory twice, 27 ps at a large
+// copy's rate, against 16 x 1024 flop, 14 ps at a large product's.)
 //
 // A query is 32 bits wide and the matrix cores take 16: each block of 32 columns is scaled by the
 // power of two that puts its largest element in [2^13, 2^14), and cut into f16 halves x = hi + lo,
@@ -240,11 +242,12 @@ __global__ void __launch_bounds__(64) attn_combine_weights_kernel(AttnWeightsPar
 // one per workgroup: causal groups differ in length, and a span takes up where the one before it
 // ends.
 //
-// Measured: 8192 tokens after 8192 in 2.55-2.65 ms, 1240-1300 TFLOP/s of f16 products (1.3 ms a
-// pass, the matrix units busy in 73 and 77% of the cycles; zeros for data take 1.88 ms, so the
-// card's power is what bounds it); 2048 tokens 96 us (passes of 42, the first 6 of them the start
-// of its spans, then tiles at the rate of the long chunk); 1001 after 5003 e4m3 rows 164; 33 after
-// 12001 37.4 us (four launches; passes of 15.5 and 19, 5 of them in tiles).
+// Measured: 8192 tokens after 8192 in 2.55-2.60 ms, 1270-1300 TFLOP/s of f16 products (1.3 ms a
+// pass, the matrix units busy in 73 and 77% of the cycles; zeros for data take as many cycles in 0.95
+// to 0.99 ms, so the card's power, which sets the clock, bounds it); 2048 tokens 95.3 us (passes of
+// 42, with zeros 37; the matrix units busy in 54 and 52% of the cycles: a span has 17 tiles behind a
+// start of 6 us); 1001 after 5003 e4m3 rows 156-160; 33 after 12001 37.5 us (four launches; passes of
+// 15.5 and 19, 5 of them in tiles).
 // ------------------------------------------------------------------------------------------------
 
 struct AttnKeyWeightsParams {
@@ -767,7 +770,7 @@ attn_key_weights_pass_kernel(AttnKeyWeightsParams p) {
 
 // weights += the groups' sums, in a fixed order: one workgroup per (KV head, tile of rows), 8
 // slices of the groups that hold the tile, joined in slice order. Bound by memory: 256 groups over
-// 16384 rows (8192 tokens after 8192, 25 MB of sums) 6.9 us.
+// 16384 rows (8192 tokens after 8192, 25 MB of sums) 6.6 us.
 template <unsigned W>
 __global__ void __launch_bounds__(256) attn_key_weights_join_kernel(AttnKeyWeightsParams p) {
   using namespace weights_detail;
@@ -794,10 +797,13 @@ __global__ void __launch_bounds__(256) attn_key_weights_join_kernel(AttnKeyWeigh
 
 // How a chunk is cut: column blocks, the waves W of a workgroup, the groups, and the spans of a
 // pass. W = 8 is one workgroup per CU, W = 4 two, which hide each other's starts and barriers but
-// stream K twice. Two are faster while K stays in an XCD's L2 (2048 tokens: 110 us against 120;
-// 1000 after 1000: 74.7 against 75.0), slower beyond (2048 after 12001: 855 against 794), except
-// for few blocks that fill groups of 4 better by more than that (33 tokens after 40000, 9 blocks:
-// 86 against 94; 17 after 40000, 5 blocks: 70 against 60).
+// stream K twice. Two while K stays in an XCD's L2 (us, W = 4 against 8: 300 tokens 18.1 against
+// 20.9, 2048 96 against 109, 4000 after 100 280 against 289; level with many rows before the chunk,
+// 1000 after 1000 68.6 against 68.8, and behind at the rule's edge, 2000 after 2000 188 against 180).
+// One beyond (2048 after 12001 731 against 690; 17 after 40000, 5 blocks, 56.6 against 50), except
+// for few blocks that fill groups of 4 better (33 after 40000, 9 blocks, 72 against 79.5; over fewer
+// rows it can be the other way, 33 after 12001 38.2 against 36.2, and 64 after 5000, 16 blocks, which
+// fill either, 30.2 against 33.1).
 struct AttnKeyWeightsCut {
   unsigned blocks, waves, groups, row_tiles, spans;
   unsigned long long span;
@@ -973,7 +979,7 @@ inline void attn_key_weights_launch(const float* q, const attn::half_t* k_cache,
 // count from the top reaches what is still to be kept. Then the rows above that rank are kept, and
 // of those equal to it the first ones. Counts are whole numbers, so their order does not matter.
 //
-// Bound by latencies, not bytes: 5.4 us for 2048 rows (one launch, the host's call), 22.6 for
+// Bound by latencies, not bytes: 6.3 us for 2048 rows (4.4 on the card, the host's call), 22.6 for
 // 262144 (2 MB, four launches). Joining all groups' histograms in every launch instead of adding
 // them up in memory took 35.6: 512 KiB to read per workgroup.
 // ------------------------------------------------------------------------------------------------
@@ -1448,8 +1454,8 @@ struct AttnEvictGatherParams {
 // A row of K or V is 32 (f16) or 16 (e4m3) lanes of 16 bytes; a thread moves its chunk of both, of
 // two rows over e4m3 rows (65535 rows: 30.3 us against 33.6; over f16 rows one is faster, 51.5
 // against 53.8). Rows [0, 2 keep) are moved, the 2 (out_ctx - keep) weights behind them cleared.
-// Grid-stride, x 256. Bound by memory: 8192 f16 rows of 32768 in 8.2 us (33.6 MB, 4.1 TB/s), 65535
-// e4m3 rows of 131072 in 30.2 (134 MB, 4.4 TB/s).
+// Grid-stride, x 256. Bound by memory: 8192 f16 rows of 32768 in 8.1 us (33.8 MB, 4.2 TB/s), 65535
+// e4m3 rows of 131072 in 30.2 (138 MB, 4.6 TB/s).
 template <bool kFp8>
 __global__ void __launch_bounds__(256) attn_evict_gather_kernel(AttnEvictGatherParams p) {
   constexpr unsigned kLanes = kFp8 ? 16 : 32, kRows = 256 / kLanes, kTwo = kFp8 ? 2 : 1;
