@@ -447,8 +447,9 @@ int miso_attn_layer_ingest(const miso_attn_layer* layer, uint16_t* k_cache, uint
  * weight that the head's 8 query heads have given the row, summed over the queries seen so far
  * (1 per query head and query in all). Operators add to rows [0, len); other rows are not touched.
  * weights and index need 4-byte alignment, workspaces 16-byte; the workspaces hold nothing between
- * calls. Sums are in a fixed order, so equal calls give equal bits. Queries and visible cache rows
- * are finite; what lies past the rows a query sees is not used, whatever it holds.
+ * calls. Sums are in a fixed order, so equal calls give equal bits. Queries, their scores in f32 and
+ * visible cache rows are finite, and the decodes' queries, as miso_attn_decode's, below 2^19; what lies
+ * past the rows a query sees is not used, whatever it holds.
  * ---------------------------------------------------------------------------------------------- */
 
 /* Bytes of the workspace of the decodes with weights, for len <= max_len and n_splits <= max_splits. */

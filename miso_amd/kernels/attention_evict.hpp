@@ -222,13 +222,15 @@ __global__ void __launch_bounds__(64) attn_combine_weights_kernel(AttnWeightsPar
 // copy's rate, against 16 x 1024 flop, 14 ps at a large product's.)
 //
 // A query is 32 bits wide and the matrix cores take 16: each block of 32 columns is scaled by the
-// power of two that puts its largest element in [2^13, 2^14), and cut into f16 halves x = hi + lo,
-// exact to 2^-22 of x, or 2^-38 of the block's largest element where lo is subnormal (what counts
-// is a score's absolute error: beside a query element of 1000, that is 4e-9 per unit of K). hi k +
-// lo k are exact products summed in f32; the scale comes off in the exponent's fma (one per column
-// would take 16 registers more in the second pass, which has 4 left of its 256). So a score
-// costs 1024 flop of f16 matrix work per pass, and the passes are bound by it once there are some
-// hundred queries.
+// power of two that puts its largest element in [2^13, 2^14), multiplied by log2(e), and cut into
+// f16 halves x = hi + lo, in all exact to 2^-22 of x, or 2^-38 of the block's largest element where lo
+// is subnormal (what counts is a score's absolute error: beside a query element of 1000, that is 4e-9
+// per unit of K). hi k + lo k are exact products summed in f32. What comes off in the exponent's fma is
+// a power of two, so that a maximum taken of scaled scores is the very number that the fma subtracts
+// from, however large the scores (a scale with log2(e) in it left its rounding, 2^-25 of a score, in
+// the exponent: infinite weights from scores of 2^32 on). A scale per column would take 16 registers
+// more in the second pass, which has 4 left of its 256. So a score costs 1024 flop of f16 matrix work
+// per pass, and the passes are bound by it once there are some hundred queries.
 //
 // A KV head's queries are columns c = 8 t + h % 8 in blocks of 32 (4 tokens). A wave holds one
 // block's halves in registers (128 VGPRs) and a workgroup of W waves, W blocks (a group), streams K
@@ -255,7 +257,7 @@ struct AttnKeyWeightsParams {
   const attn::half_t* k_cache;  // [2][k_ctx][256]
   float* weights;               // [2][max_ctx]
   attn::half_t* halves;         // [2][blocks][hi, lo][16][64][8], in the order of the operands
-  float* scale;                 // [2][blocks]: log2(e) / 16 over the block's power of two
+  float* scale;                 // [2][blocks]: 1 / 16 over the block's power of two
   float2* stats;                // [span + group][32 W]: a span's (maximum, sum) of a group's columns
   float* sums;                  // [2][groups][row_tiles][32]: a group's sums of its keys
   unsigned pos0, n, max_ctx, k_ctx;
@@ -447,7 +449,10 @@ __global__ void __launch_bounds__(256) attn_key_weights_cut_kernel(AttnKeyWeight
     cdna4::half4_t hi, lo;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float y = v[j] * up;  // a power of two: exact
+      float y = v[j] * up * decode_detail::kLog2e;  // up: a power of two, exact
+      // One value for both halves: the product must not be rounded to f16 within one instruction here
+      // and to f32 there, which near the middle of two f16 are a step of f16 apart.
+      asm("" : "+v"(y));
       hi[j] = static_cast<_Float16>(y);
       lo[j] = static_cast<_Float16>(y - static_cast<float>(hi[j]));
     }
@@ -464,7 +469,7 @@ __global__ void __launch_bounds__(256) attn_key_weights_cut_kernel(AttnKeyWeight
                                               at % 32 * 16);
   }
   if (t == 0)
-    p.scale[blockIdx.x] = __builtin_ldexpf(decode_detail::kLog2e / 16.0f, -e);
+    p.scale[blockIdx.x] = __builtin_ldexpf(1.0f / 16.0f, -e);
 }
 
 // One span of a pass (kSum: the second), x 64 W, one workgroup of 8 waves or two of 4 per CU.

@@ -315,6 +315,49 @@ def test_prefill_weights_of_one_large_query(attn, factor, t, h):
     assert float(((w.double() - want).abs() / lim).max()) <= 1
 
 
+def one_row_takes_all(g, pos0, n, size):
+    """Queries so large that each gives all its weight to one row: rows k = (a | b) s with s a vector of
+    signs and the levels a + b distinct whole numbers, queries +-size s. Scores are 8 size (a + b): they
+    lie 8 size apart, and at most 3000 times that from 0, so that f32 tells them apart. Returns q, K and
+    the weights, whole numbers."""
+    rows = pos0 + n
+    level = torch.stack([torch.randperm(6000, generator=g, device="cuda")[:rows] for _ in range(KV)])
+    a, b = level % 2000 - 1000, level // 2000 * 2000 - 2000
+    sign = torch.where(torch.rand(D, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    k = torch.stack([a, b], dim=2).repeat_interleave(D // 2, dim=2).float() * sign
+    way = torch.where(torch.rand(n, H, generator=g, device="cuda") < 0.5, -1, 1)
+    want = torch.zeros(KV, rows, device="cuda")
+    for t in range(n):
+        for h in range(H):
+            seen = (way[t, h] * (a + b)[h // G])[:pos0 + t + 1]
+            want[h // G, seen.argmax()] += 1
+    return size * way[..., None] * sign, k.half(), want
+
+
+SIZES = [2.0 ** 4, 2.0 ** 12, 2.0 ** 25, 2.0 ** 40, 2.0 ** 70, 2.0 ** 110]
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("pos0,n", [(300, 33), (0, 70), (5000, 9)])
+def test_prefill_weights_of_large_queries(attn, pos0, n, size):
+    """Scores up to 2^124: the largest one's weight is 1, the others' 0, no infinity and no NaN."""
+    q, k, want = one_row_takes_all(gen(n), pos0, n, size)
+    w = torch.zeros_like(want)
+    attn.attn_prefill_weights(q, k, w, pos0, n, pos0 + n, attn.PrefillWeightsScratch(n, pos0 + n))
+    assert torch.equal(w, want), (float(w.max()), float((w - want).abs().max()))
+
+
+@pytest.mark.parametrize("size", [2.0 ** 4, 2.0 ** 12, 2.0 ** 18])
+@pytest.mark.parametrize("n", [1, 70, 5009])
+def test_decode_weights_of_large_queries(attn, n, size):
+    """The decodes take queries below 2^19."""
+    q, k, want = one_row_takes_all(gen(n), n - 1, 1, size)
+    w = torch.zeros_like(want)
+    core, qg = torch.empty(H, D, device="cuda"), torch.zeros(H, 2, D, device="cuda")
+    attn.attn_decode_weights(q[0], qg, k, k, core, w, attn.DecodeWeightsScratch(64, n), n, n)
+    assert torch.equal(w, want), (float(w.max()), float((w - want).abs().max()))
+
+
 @pytest.mark.parametrize("pos0,n", [(0, 300), (700, 33), (4000, 300), (2000, 4)])
 def test_prefill_weights_of_low_halves(attn, pos0, n):
     """Queries whose elements need more than f16: all of (1 + 2^-12) times a power of two. Without the
