@@ -260,7 +260,8 @@ int miso_attn_decode_paged_ws(const float* q, const float* gate, const uint16_t*
  * is 256 OCP e4m3 codes in k8 / v8 [2][max_ctx][256] (uint8) plus one f32 power-of-two scale in
  * k_scale / v_scale [2][max_ctx]: value = scale * e4m3(code), scale = 2^(floor(log2 max|x|) - 7)
  * (rows whose max is below 2^-100 use 2^-107), codes rounded to nearest even, never saturated.
- * Readers also take a scale of 0: a row of zeros. Inputs must be finite. k8 / v8 need 16-byte alignment, the scale arrays 4-byte alignment.
+ * Readers also take a scale of 0: a row of zeros. Inputs must be finite. k8 / v8 need 16-byte
+ * alignment, the scale arrays 4-byte alignment.
  *
  * miso_attn_kv_encode_fp8: rows [pos0, pos0 + n) of both KV heads of an f16 cache -> e4m3 rows
  * (n == 0 is a no-op). Rejects pos0 + n > max_ctx. */
@@ -510,7 +511,7 @@ int miso_attn_evict_gather(const uint16_t* k_cache, const uint16_t* v_cache, con
                            uint32_t max_ctx, const int32_t* index, uint32_t keep, uint16_t* k_out,
                            uint16_t* v_out, float* weights_out, uint32_t out_ctx, void* stream);
 
-/* The same over the e4m3-row cache (codes and row scales). */
+/* The same over the e4m3-row cache (codes and row scales; a row of zeros has scale 0). */
 int miso_attn_evict_gather_fp8(const uint8_t* k8, const uint8_t* v8, const float* k_scale,
                                const float* v_scale, const float* weights, uint32_t max_ctx,
                                const int32_t* index, uint32_t keep, uint8_t* k8_out,
