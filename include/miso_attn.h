@@ -562,6 +562,97 @@ int miso_attn_layer_prefill_weights(const miso_attn_layer* layer, uint16_t* k_ca
                                     float* weights, void* workspace, uint64_t workspace_bytes,
                                     void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * A batch of requests over a KV page pool (no reference counterpart: the reference serves one
+ * sequence)
+ *
+ * A pool is k_pages and v_pages, page g [2 KV heads][page_size][256] f16 as miso_attn_decode_paged
+ * reads it, and a stack of free page ids. A slot (page * page_size + row in the page) names a row of
+ * both KV heads. page_size is a power of two in [8, 65536]. Integer arrays need 4-byte alignment.
+ * Prefix: all requests of a pool may share their first prefix_pages pages (prefix_table, whole pages);
+ * 0: they share none, prefix_table is not looked at.
+ * ---------------------------------------------------------------------------------------------- */
+
+/* One step's page tables, slots and positions, on the device (lens, n_new, ended, n_free: device
+ * arrays). Request s has lens[s] keys and gets n_new[s] tokens:
+ *   - ended[s] != 0 (ended may be NULL): the pages of its entries prefix_pages .. go back on the stack,
+ *     in the order of request and entry, and its length becomes 0; its place may start anew at once;
+ *   - a request of length 0 that gets tokens starts behind the prefix: entries 0 .. prefix_pages - 1
+ *     become prefix_table's and its length prefix_pages * page_size;
+ *   - pages come from the top of the stack, in the order of request and entry. A request that needs
+ *     pages gets them if the pages that it and all before it need are there; status 0.
+ * A request that does not fit keeps its length and its table row: status 1, too few free pages; 2, longer
+ * than its table row; 3, its tokens end behind max_tokens. What 2 and 3 would need is not counted.
+ * page_table [batch][max_pages] and free_pages [pool_pages] are updated in place; lens_out [batch] may
+ * be lens and n_free_out [1] may be n_free, no other arrays overlap. starts [batch + 1]: the first
+ * token of each request (the sum of n_new, refused requests' tokens counted). Per token t < max_tokens:
+ * slots, positions, rows (its request) and visible (position + 1, the keys it sees: `lens` of a decode
+ * whose entries are the step's tokens). Refused requests' tokens and those behind the last have slot -1,
+ * position 0 and visible 0 (the latter row 0). A page id outside [0, pool_pages) gives slot -1.
+ * The sum of n_new is below 2^32. Rejects batch == 0 or > 8192, max_tokens == 0 or >= 2^31, batch *
+ * max_pages, max_pages * page_size or pool_pages * page_size >= 2^31, prefix_pages > max_pages. */
+#define MISO_ATTN_PLAN_MAX_BATCH 8192
+int miso_attn_page_plan(const uint32_t* lens, const uint32_t* n_new, const uint32_t* ended,
+                        int32_t* page_table, uint32_t batch, uint32_t max_pages,
+                        uint32_t page_size, const int32_t* prefix_table, uint32_t prefix_pages,
+                        int32_t* free_pages, uint32_t pool_pages, const uint32_t* n_free,
+                        uint32_t* lens_out, uint32_t* n_free_out, int32_t* status,
+                        uint32_t* starts, int32_t* slots, uint32_t* positions, int32_t* rows,
+                        uint32_t* visible, uint32_t max_tokens, void* stream);
+
+/* miso_attn_prep_batch for tokens of many requests: token t is rotated for positions[t] and its K / V
+ * appended at slots[t] of the pool (device arrays, [n]); one whose slot is outside [0, pool_pages *
+ * page_size) is left out, its rows of q and gate stay as they are. Two tokens with one slot race.
+ * q [n][16][256]; gate [n][16][256] (or NULL): the gates of qg, dense, as the batched decodes take them.
+ * The first rope_dims dimensions (a multiple of 8, at most 256; 0: none) are rotated by positions[t] *
+ * inv_freq[i] (inv_freq [rope_dims / 2], 16-byte aligned), in pairs (i, i + rope_dims / 2) or, interleaved != 0,
+ * (2 i, 2 i + 1), cos and sin times rot_scale. Angles are formed and reduced in 64 bits (the other
+ * preps': in 32). n == 0 is a no-op. Rejects proj_stride < 9216 or not a multiple of 4 and
+ * pool_pages * page_size >= 2^31. */
+int miso_attn_prep_paged(const float* qg, const float* k, const float* v, const float* q_norm,
+                         const float* k_norm, const float* inv_freq, uint16_t* k_pages,
+                         uint16_t* v_pages, uint32_t pool_pages, uint32_t page_size,
+                         const int32_t* slots, const uint32_t* positions, float* q, float* gate,
+                         uint32_t n, uint32_t proj_stride, uint32_t rope_dims, int interleaved,
+                         float rot_scale, float eps, void* stream);
+
+/* Bytes of the workspace (16-byte aligned) of the two decodes below, for batch <= max_batch, max_own
+ * and prefixes of up to max_prefix keys. It holds nothing between calls. */
+uint64_t miso_attn_decode_shared_workspace_bytes(uint32_t max_batch, uint32_t max_own,
+                                                 uint32_t max_prefix);
+
+/* miso_attn_decode_paged where all entries share a prefix: the same attention, its keys [0,
+ * prefix_pages * page_size) read once for all entries, from prefix_table's pages; the entries' own
+ * keys from there on lie in pages prefix_pages .. of table row rows[s] (rows NULL: row s). lens[s]
+ * counts all keys of entry s, the prefix's too; one below the prefix sees its first lens[s] keys, 0
+ * gives core = 0. Entries may share a table row: a chunk of a request's prompt or drafted tokens are
+ * entries of rising lens (the chunk's K / V appended before). max_own: the longest part behind the
+ * prefix (a longer one still gets all of its keys); with 0 nothing behind the prefix is looked at.
+ * Precision as miso_attn_decode's: per-head relative L2 error <= 1e-5 over the same keys; equal calls
+ * give equal bits. Queries are finite and, as miso_attn_decode's, below 2^19; the prefix's rows are
+ * finite, also those that an entry does not see.
+ * Table entries and rows are not validated. Rejects batch == 0 or > 65536, page_size as above,
+ * prefix_pages > max_pages, max_pages * page_size >= 2^31 or < prefix_pages * page_size + max_own and a
+ * workspace that is too small. */
+int miso_attn_decode_paged_shared(const float* q, const float* gate, const uint16_t* k_pages,
+                                  const uint16_t* v_pages, const int32_t* page_table,
+                                  uint32_t max_pages, uint32_t page_size, const int32_t* rows,
+                                  const uint32_t* lens, uint32_t batch, uint32_t max_own,
+                                  const int32_t* prefix_table, uint32_t prefix_pages, float* core,
+                                  void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* miso_attn_decode_ragged behind a shared prefix of prefix_len keys of a contiguous cache (k_prefix,
+ * v_prefix: [2][prefix_ctx][256], as the preps and prefills above fill it). lens and kv_offsets: the
+ * sequences' own keys, as miso_attn_decode_ragged's; a sequence of none sees the prefix alone. Any
+ * prefix_len; 0: none, k_prefix and v_prefix are not looked at. Otherwise as the paged form. Rejects
+ * batch == 0 or > 65536, prefix_len > prefix_ctx or >= 2^31 and a workspace that is too small. */
+int miso_attn_decode_ragged_shared(const float* q, const float* gate, const uint16_t* k_cache,
+                                   const uint16_t* v_cache, const uint64_t* kv_offsets,
+                                   const uint32_t* lens, uint32_t batch, uint32_t max_own,
+                                   const uint16_t* k_prefix, const uint16_t* v_prefix,
+                                   uint32_t prefix_len, uint32_t prefix_ctx, float* core,
+                                   void* workspace, uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -99,6 +99,15 @@ SIGNATURES = {
     "miso_attn_prep_at_fp8": (c_int, [P] * 11 + [c_uint32, c_uint32, c_uint32, c_float, P]),
     "miso_attn_prep_batch_at_fp8": (c_int, [P] * 11 + [c_uint32, c_uint32, c_uint32, c_float,
                                                        c_uint32, c_uint32, P]),
+    "miso_attn_page_plan": (c_int, [P, P, P, P, c_uint32, c_uint32, c_uint32, P, c_uint32, P,
+                                    c_uint32, P, P, P, P, P, P, P, P, P, c_uint32, P]),
+    "miso_attn_prep_paged": (c_int, [P] * 8 + [c_uint32, c_uint32, P, P, P, P, c_uint32, c_uint32,
+                                               c_uint32, c_int, c_float, c_float, P]),
+    "miso_attn_decode_shared_workspace_bytes": (c_uint64, [c_uint32, c_uint32, c_uint32]),
+    "miso_attn_decode_paged_shared": (c_int, [P] * 5 + [c_uint32, c_uint32, P, P, c_uint32,
+                                                        c_uint32, P, c_uint32, P, P, c_uint64, P]),
+    "miso_attn_decode_ragged_shared": (c_int, [P] * 6 + [c_uint32, c_uint32, P, P, c_uint32,
+                                                         c_uint32, P, P, c_uint64, P]),
 }
 
 _lib = None

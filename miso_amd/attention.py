@@ -11,6 +11,7 @@ torch is used for device memory and streams only; all arithmetic runs in the HIP
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional
 
 import torch
@@ -639,6 +640,191 @@ def attn_evict_gather_fp8(cache: Fp8Cache, weights, index, keep: int, out: Fp8Ca
     _lib.check(_lib.load().miso_attn_evict_gather_fp8(
         *(_ptr(b) for b in cache.buffers()), _ptr(weights), cache.max_ctx, _ptr(index), keep,
         *(_ptr(b) for b in out.buffers()), _ptr(weights_out), out.max_ctx, _stream(stream)))
+
+
+# ------------------------------------------------------------------------------------------------
+# A batch of requests over a KV page pool: k_pages / v_pages (float16, page g [2][page][256]), a stack
+# of free page ids, page tables. A slot (page * page_size + row in the page) names a row of both heads.
+# ------------------------------------------------------------------------------------------------
+
+class PagePlan:
+    """What attn_page_plan says of a step of `batch` requests and up to max_tokens tokens: starts
+    [batch + 1] and status [batch]; per token slots, positions, rows (its request) and visible (the keys
+    it sees), [max_tokens]."""
+
+    def __init__(self, batch: int, max_tokens: int, device="cuda"):
+        self.batch, self.max_tokens = batch, max_tokens
+        self.starts, self.status, self.slots, self.positions, self.rows, self.visible = (
+            torch.zeros(n, dtype=torch.int32, device=device)
+            for n in (batch + 1, batch, max_tokens, max_tokens, max_tokens, max_tokens))
+
+
+def attn_page_plan(lens, n_new, page_table, page_size: int, free_pages, n_free, plan: PagePlan,
+                   lens_out=None, n_free_out=None, ended=None, prefix_table=None,
+                   prefix_pages: int = 0, stream=None) -> None:
+    """The tables, slots and positions of a step in which request s, of lens[s] keys, gets n_new[s]
+    tokens (int32, on the device): pages from the stack free_pages[:n_free[0]] into page_table
+    [batch][max_pages], and `plan`'s arrays. Requests with ended[s] != 0 give their pages back first;
+    one of length 0 that gets tokens starts behind the prefix (prefix_table's first prefix_pages pages).
+    plan.status[s]: 0, or why request s did not fit (1: free pages, 2: its table row, 3: max_tokens).
+    lens_out and n_free_out default to lens and n_free, which are then updated in place."""
+    batch, int32 = plan.batch, torch.int32
+    if page_table.dim() != 2 or page_table.shape[0] != batch:
+        raise ValueError("page_table must be [batch][max_pages]")
+    lens_out = lens if lens_out is None else lens_out
+    n_free_out = n_free if n_free_out is None else n_free_out
+    max_pages = int(page_table.shape[1])
+    for name, t, n in (("lens", lens, batch), ("n_new", n_new, batch), ("lens_out", lens_out, batch),
+                       ("page_table", page_table, batch * max_pages), ("n_free", n_free, 1),
+                       ("n_free_out", n_free_out, 1), ("free_pages", free_pages, 1)):
+        _need(t, name, int32, n)
+    if ended is not None:
+        _need(ended, "ended", int32, batch)
+    if prefix_pages:
+        _need(prefix_table, "prefix_table", int32, _count(prefix_pages, "prefix_pages"))
+    _here(lens, n_new, page_table, free_pages, n_free, lens_out, n_free_out, plan.slots,
+          *(t for t in (ended, prefix_table if prefix_pages else None) if t is not None))
+    _lib.check(_lib.load().miso_attn_page_plan(
+        lens.data_ptr(), n_new.data_ptr(), _ptr(ended), page_table.data_ptr(), batch, max_pages,
+        _count(page_size, "page_size"), prefix_table.data_ptr() if prefix_pages else None,
+        prefix_pages, free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(),
+        lens_out.data_ptr(), n_free_out.data_ptr(), plan.status.data_ptr(), plan.starts.data_ptr(),
+        plan.slots.data_ptr(), plan.positions.data_ptr(), plan.rows.data_ptr(),
+        plan.visible.data_ptr(), plan.max_tokens, _stream(stream)))
+
+
+def _pool_pages(k_pages, v_pages, page_size: int) -> int:
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        _need(t, name, _cache_dtype(t), 1)
+    if page_size <= 0:
+        raise ValueError("page_size must be positive")
+    return min(k_pages.numel(), v_pages.numel()) // (KV_HEADS * page_size * DIM)
+
+
+def rope_frequencies(rope_dims: int, base: float, factor: float = 1.0, scaling: str = "linear",
+                     original_ctx: int = 0, fast: float = 32.0, slow: float = 1.0, device="cuda"):
+    """(inv_freq, rot_scale) for attn_prep_paged: base ** (-2 i / rope_dims), computed in float64 and
+    rounded to float32, for contexts `factor` times as long as the model was trained on. "linear":
+    every frequency divided by factor. "yarn" (Peng et al., 2023): a frequency that turns more than
+    `fast` times over the original_ctx positions of training stays, one that turns less than `slow` times
+    is divided, those between by a linear ramp; rot_scale = 1 + 0.1 ln(factor) (1 for linear)."""
+    if rope_dims % 8 != 0 or not 0 <= rope_dims <= DIM:
+        raise ValueError("rope_dims must be a multiple of 8, at most 256")
+    if not (base > 0 and factor >= 1):
+        raise ValueError("base must be positive and factor at least 1")
+    freq = base ** (-torch.arange(0, rope_dims, 2, dtype=torch.float64) / max(rope_dims, 1))
+    if scaling == "linear":
+        return (freq / factor).to(device=device, dtype=torch.float32), 1.0
+    if scaling != "yarn":
+        raise ValueError("scaling must be 'linear' or 'yarn'")
+    if original_ctx <= 0 or not fast > slow:
+        raise ValueError("yarn needs original_ctx, and fast above slow")
+    turns = original_ctx * freq / (2 * math.pi)
+    stays = ((turns - slow) / (fast - slow)).clamp(0, 1)
+    freq = freq * (stays + (1 - stays) / factor)
+    return freq.to(device=device, dtype=torch.float32), 1.0 + 0.1 * math.log(factor)
+
+
+def attn_prep_paged(qg, k, v, q_norm, k_norm, inv_freq, k_pages, v_pages, page_size: int, slots,
+                    positions, q, n: int, proj_stride: int, eps: float, gate=None,
+                    rope_dims: int = 64, interleaved: bool = False, rot_scale: float = 1.0,
+                    stream=None) -> None:
+    """attn_prep_batch for tokens of many requests: token t is rotated for positions[t] and appended
+    at slots[t] of the page pool (int32, on the device); one without a slot in the pool is left out. qg /
+    k / v are views into a token-major projection buffer, rows proj_stride floats apart. With `gate`
+    ([n][16][256]) the gates are stored dense, as the batched decodes take them. The first rope_dims
+    dimensions are rotated by position * inv_freq (float32, rope_dims / 2; rope_frequencies makes them),
+    in pairs (i, i + rope_dims / 2) or neighbours (interleaved), cos and sin times rot_scale."""
+    f32 = torch.float32
+    n, proj_stride = _count(n, "n"), _count(proj_stride, "proj_stride")
+    for name, t, row in (("qg", qg, QG_STRIDE), ("k", k, KV_HEADS * DIM), ("v", v, KV_HEADS * DIM)):
+        _need(t.view(-1) if t.is_contiguous() else t, name, f32, (n - 1) * proj_stride + row if n else 0)
+    for name, t, m in (("q_norm", q_norm, DIM), ("k_norm", k_norm, DIM), ("q", q, n * Q_HEADS * DIM),
+                       ("inv_freq", inv_freq, _count(rope_dims, "rope_dims") // 2)):
+        _need(t, name, f32, m)
+    if gate is not None:
+        _need(gate, "gate", f32, n * Q_HEADS * DIM)
+    _need(slots, "slots", torch.int32, n)
+    _need(positions, "positions", torch.int32, n)
+    pages = _pool_pages(k_pages, v_pages, page_size)
+    _here(qg, k, v, q_norm, k_norm, inv_freq, k_pages, v_pages, slots, positions, q,
+          *(() if gate is None else (gate,)))
+    _lib.check(_lib.load().miso_attn_prep_paged(
+        qg.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
+        inv_freq.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page_size,
+        slots.data_ptr(), positions.data_ptr(), q.data_ptr(), _ptr(gate), n, proj_stride, rope_dims,
+        int(interleaved), rot_scale, eps, _stream(stream)))
+
+
+class SharedScratch:
+    """Workspace of the decodes behind a shared prefix: up to `batch` entries of max_own keys of their
+    own behind up to max_prefix keys."""
+
+    def __init__(self, batch: int, max_own: int, max_prefix: int, device="cuda"):
+        self.batch, self.max_own = _count(batch, "batch"), _count(max_own, "max_own")
+        self.max_prefix = _count(max_prefix, "max_prefix")
+        self.nbytes = int(_lib.load().miso_attn_decode_shared_workspace_bytes(batch, max_own,
+                                                                              max_prefix))
+        self.ws = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
+
+
+def _shared_args(q, gate, lens, core, scratch: SharedScratch, prefix: int) -> int:
+    batch = lens.numel()
+    if batch > scratch.batch or prefix > scratch.max_prefix:
+        raise ValueError("the batch or the prefix exceeds the scratch capacity")
+    for name, t in (("q", q), ("gate", gate), ("core", core)):
+        _need(t, name, torch.float32, batch * Q_HEADS * DIM)
+    _need(lens, "lens", torch.int32, batch)
+    _here(q, gate, lens, core, scratch.ws)
+    return batch
+
+
+def attn_decode_paged_shared(q, gate, k_pages, v_pages, page_table, page_size: int, lens,
+                             prefix_table, prefix_pages: int, core, scratch: SharedScratch,
+                             rows=None, stream=None) -> None:
+    """attn_decode_paged of lens.numel() entries whose first prefix_pages pages are prefix_table's: those
+    keys are read once for all entries, the others from entries prefix_pages .. of table row rows[s]
+    (None: row s; entries may share a row, as the tokens of a prompt's chunk do, each with its own
+    lens). lens counts all keys of an entry; 0 gives core = 0."""
+    prefix_pages = _count(prefix_pages, "prefix_pages")
+    batch = _shared_args(q, gate, lens, core, scratch, prefix_pages * page_size)
+    if page_table.dim() != 2 or (rows is None and page_table.shape[0] < batch):
+        raise ValueError("page_table must be [rows][max_pages], a row per entry without `rows`")
+    max_pages = int(page_table.shape[1])
+    _need(page_table, "page_table", torch.int32, 1)
+    if prefix_pages:
+        _need(prefix_table, "prefix_table", torch.int32, prefix_pages)
+    if rows is not None:
+        _need(rows, "rows", torch.int32, batch)
+    _pool_pages(k_pages, v_pages, page_size)
+    _here(k_pages, v_pages, page_table,
+          *(t for t in (rows, prefix_table if prefix_pages else None) if t is not None))
+    _lib.check(_lib.load().miso_attn_decode_paged_shared(
+        q.data_ptr(), gate.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+        page_table.data_ptr(), max_pages, _count(page_size, "page_size"), _ptr(rows),
+        lens.data_ptr(), batch,
+        min(scratch.max_own, max(0, (max_pages - prefix_pages) * page_size)),
+        prefix_table.data_ptr() if prefix_pages else None, prefix_pages, core.data_ptr(),
+        scratch.ws.data_ptr(), scratch.nbytes, _stream(stream)))
+
+
+def attn_decode_ragged_shared(q, gate, k_cache, v_cache, kv_offsets, lens, k_prefix, v_prefix,
+                              prefix_len: int, prefix_ctx: int, core, scratch: SharedScratch,
+                              stream=None) -> None:
+    """attn_decode_ragged of lens.numel() sequences behind a shared prefix, keys [0, prefix_len) of the
+    cache k_prefix / v_prefix ([2][prefix_ctx][256]); lens and kv_offsets: their own keys, 0 or more."""
+    prefix_len, prefix_ctx = _count(prefix_len, "prefix_len"), _count(prefix_ctx, "prefix_ctx")
+    batch = _shared_args(q, gate, lens, core, scratch, prefix_len)
+    _need(kv_offsets, "kv_offsets", torch.int64, batch)
+    for name, t, rows in (("k_cache", k_cache, 0), ("v_cache", v_cache, 0),
+                          ("k_prefix", k_prefix, prefix_ctx), ("v_prefix", v_prefix, prefix_ctx)):
+        _need(t, name, _cache_dtype(t), KV_HEADS * rows * DIM)
+    _here(k_cache, v_cache, kv_offsets, k_prefix, v_prefix)
+    _lib.check(_lib.load().miso_attn_decode_ragged_shared(
+        q.data_ptr(), gate.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        kv_offsets.data_ptr(), lens.data_ptr(), batch, scratch.max_own, k_prefix.data_ptr(),
+        v_prefix.data_ptr(), prefix_len, prefix_ctx, core.data_ptr(), scratch.ws.data_ptr(),
+        scratch.nbytes, _stream(stream)))
 
 
 # ------------------------------------------------------------------------------------------------

@@ -14,7 +14,9 @@
 #include "attention_decode.hpp"
 #include "attention_decode_fp8.hpp"
 #include "attention_evict.hpp"
+#include "attention_pages.hpp"
 #include "attention_prefill.hpp"
+#include "attention_shared.hpp"
 #include "q4k_gemv.hpp"
 #include "q6k_gemv.hpp"
 #include "attention_layer.hpp"
@@ -1339,6 +1341,186 @@ int miso_attn_layer_prefill_weights(const miso_attn_layer* layer, uint16_t* k_ca
                               w, as_half(k_cache), as_half(v_cache), row0, pos0, n, max_ctx, h,
                               delta, y, eps, k::layer::prefill_workspace(ws, max_tok), max_tok, m,
                               weights, workspace, as_stream(stream)));
+}
+
+}  // extern "C"
+
+namespace {
+
+// A batch of requests over a page pool.
+
+bool bad_page(uint32_t page_size) {
+  return page_size < 8 || page_size > 65536 || (page_size & (page_size - 1)) != 0;
+}
+constexpr const char* kBadPage = "page_size must be a power of two in [8, 65536]";
+constexpr uint64_t kInt32End = uint64_t{1} << 31;
+
+template <class... P>
+bool any_bad_words(const P*... p) {
+  return ((p == nullptr || (reinterpret_cast<uintptr_t>(p) & 3u) != 0) || ...);
+}
+
+}  // namespace
+
+extern "C" {
+
+int miso_attn_page_plan(const uint32_t* lens, const uint32_t* n_new, const uint32_t* ended,
+                        int32_t* page_table, uint32_t batch, uint32_t max_pages,
+                        uint32_t page_size, const int32_t* prefix_table, uint32_t prefix_pages,
+                        int32_t* free_pages, uint32_t pool_pages, const uint32_t* n_free,
+                        uint32_t* lens_out, uint32_t* n_free_out, int32_t* status,
+                        uint32_t* starts, int32_t* slots, uint32_t* positions, int32_t* rows,
+                        uint32_t* visible, uint32_t max_tokens, void* stream) {
+  constexpr const char* fn = "miso_attn_page_plan";
+  if (any_bad_words(lens, n_new, page_table, free_pages, n_free, lens_out, n_free_out, status,
+                    starts, slots, positions, rows, visible) ||
+      (reinterpret_cast<uintptr_t>(ended) & 3u) != 0 ||
+      (prefix_pages != 0 && any_bad_words(prefix_table)))
+    return fail(fn, "an array is NULL or not 4-byte aligned");
+  if (batch == 0 || batch > k::kAttnPlanMaxBatch)
+    return fail(fn, "batch must be in [1, 8192]");
+  if (bad_page(page_size))
+    return fail(fn, kBadPage);
+  if (max_pages == 0 || uint64_t{batch} * max_pages >= kInt32End ||
+      uint64_t{max_pages} * page_size >= kInt32End)
+    return fail(fn, "max_pages must be >= 1, batch and page_size times it below 2^31");
+  if (pool_pages == 0 || uint64_t{pool_pages} * page_size >= kInt32End)
+    return fail(fn, "pool_pages must be >= 1, pool_pages * page_size below 2^31");
+  if (prefix_pages > max_pages)
+    return fail(fn, "prefix_pages exceeds max_pages");
+  if (max_tokens == 0 || max_tokens >= kInt32End)
+    return fail(fn, "max_tokens must be in [1, 2^31)");
+  k::attn_page_plan_launch(
+      {lens, n_new, ended, page_table, prefix_table, free_pages, n_free, lens_out, n_free_out,
+       status, starts, slots, positions, rows, visible, batch, max_pages,
+       static_cast<unsigned>(__builtin_ctz(page_size)), prefix_pages, pool_pages, max_tokens},
+      as_stream(stream));
+  return launched(fn);
+}
+
+int miso_attn_prep_paged(const float* qg, const float* kx, const float* v, const float* q_norm,
+                         const float* k_norm, const float* inv_freq, uint16_t* k_pages,
+                         uint16_t* v_pages, uint32_t pool_pages, uint32_t page_size,
+                         const int32_t* slots, const uint32_t* positions, float* q, float* gate,
+                         uint32_t n, uint32_t proj_stride, uint32_t rope_dims, int interleaved,
+                         float rot_scale, float eps, void* stream) {
+  constexpr const char* fn = "miso_attn_prep_paged";
+  if (n == 0)
+    return 0;
+  if (any_bad(qg, kx, v, q_norm, k_norm, k_pages, v_pages, q) ||
+      (rope_dims != 0 && bad_ptr(inv_freq)) || (gate != nullptr && bad_ptr(gate)))
+    return fail(fn, kBadPtr);
+  if (any_bad_words(slots, positions))
+    return fail(fn, "slots or positions is NULL or not 4-byte aligned");
+  if (bad_page(page_size))
+    return fail(fn, kBadPage);
+  if (pool_pages == 0 || uint64_t{pool_pages} * page_size >= kInt32End)
+    return fail(fn, "pool_pages must be >= 1, pool_pages * page_size below 2^31");
+  if (n >= kInt32End)
+    return fail(fn, "n must be below 2^31");
+  if (proj_stride < 9216 || proj_stride % 4 != 0)
+    return fail(fn, "proj_stride must be >= 9216 and a multiple of 4");
+  if (rope_dims > 256 || rope_dims % 8 != 0)
+    return fail(fn, "rope_dims must be a multiple of 8, at most 256");
+  const k::AttnPrepPagedParams p{
+      qg,    kx,        v,           q_norm, k_norm, inv_freq, as_half(k_pages), as_half(v_pages),
+      slots, positions, q,           gate,   n,      proj_stride,
+      static_cast<unsigned>(__builtin_ctz(page_size)), pool_pages * page_size, rope_dims, rot_scale,
+      eps};
+  if (interleaved != 0)
+    k::attn_prep_paged_kernel<true><<<n, 384, 0, as_stream(stream)>>>(p);
+  else
+    k::attn_prep_paged_kernel<false><<<n, 384, 0, as_stream(stream)>>>(p);
+  return launched(fn);
+}
+
+uint64_t miso_attn_decode_shared_workspace_bytes(uint32_t max_batch, uint32_t max_own,
+                                                 uint32_t max_prefix) {
+  return k::attn_shared_layout(max_batch, max_own, max_prefix).bytes;
+}
+
+// Why a shared decode's batch and workspace are refused, or nullptr.
+static const char* bad_shared(uint32_t batch, uint32_t max_own, uint64_t prefix,
+                              const void* workspace, uint64_t bytes) {
+  if (batch == 0 || batch > 65536)
+    return "batch must be in [1, 65536]";
+  if (prefix >= kInt32End)
+    return "the prefix must be shorter than 2^31 keys";
+  if (max_own >= kInt32End)
+    return "max_own must be below 2^31";
+  if (bad_ptr(workspace))
+    return "workspace must be a non-null, 16-byte aligned device pointer";
+  if (bytes < miso_attn_decode_shared_workspace_bytes(batch, max_own,
+                                                      static_cast<uint32_t>(prefix)))
+    return "workspace smaller than miso_attn_decode_shared_workspace_bytes(batch, max_own, prefix)";
+  return nullptr;
+}
+
+static int decode_shared(const char* fn, const k::AttnSharedParams& p, const k::AttnSharedOwn& own,
+                         uint32_t max_own, void* workspace, void* stream) {
+  const unsigned cus = device_cus();
+  k::attn_shared_launch(p, own, max_own, static_cast<char*>(workspace),
+                        cus != 0 ? cus : k::kAttnSharedCus, as_stream(stream));
+  return launched(fn);
+}
+
+int miso_attn_decode_paged_shared(const float* q, const float* gate, const uint16_t* k_pages,
+                                  const uint16_t* v_pages, const int32_t* page_table,
+                                  uint32_t max_pages, uint32_t page_size, const int32_t* rows,
+                                  const uint32_t* lens, uint32_t batch, uint32_t max_own,
+                                  const int32_t* prefix_table, uint32_t prefix_pages, float* core,
+                                  void* workspace, uint64_t workspace_bytes, void* stream) {
+  constexpr const char* fn = "miso_attn_decode_paged_shared";
+  if (any_bad(q, gate, k_pages, v_pages, core))
+    return fail(fn, kBadPtr);
+  if (any_bad_words(page_table, lens) || (reinterpret_cast<uintptr_t>(rows) & 3u) != 0 ||
+      (prefix_pages != 0 && any_bad_words(prefix_table)))
+    return fail(fn, "an array is NULL or not 4-byte aligned");
+  if (bad_page(page_size))
+    return fail(fn, kBadPage);
+  if (max_pages == 0 || uint64_t{max_pages} * page_size >= kInt32End)
+    return fail(fn, "max_pages must be >= 1, max_pages * page_size below 2^31");
+  if (prefix_pages > max_pages)
+    return fail(fn, "prefix_pages exceeds max_pages");
+  const uint32_t prefix = prefix_pages * page_size, own_cap = max_pages * page_size - prefix;
+  if (max_own > own_cap)
+    return fail(fn, "max_pages * page_size < prefix_pages * page_size + max_own");
+  if (const char* err = bad_shared(batch, max_own, prefix, workspace, workspace_bytes))
+    return fail(fn, err);
+  const unsigned log2_page = static_cast<unsigned>(__builtin_ctz(page_size));
+  k::AttnSharedParams p{};
+  p.q = q, p.gate = gate, p.core = core, p.lens = lens;
+  p.prefix = {as_half(k_pages), as_half(v_pages), prefix_table, 0, log2_page, prefix};
+  p.batch = batch, p.whole = true, p.own_cap = own_cap;
+  const k::AttnSharedOwn own{as_half(k_pages), as_half(v_pages), page_table + prefix_pages, rows,
+                             max_pages,        log2_page,        nullptr};
+  return decode_shared(fn, p, own, max_own, workspace, stream);
+}
+
+int miso_attn_decode_ragged_shared(const float* q, const float* gate, const uint16_t* k_cache,
+                                   const uint16_t* v_cache, const uint64_t* kv_offsets,
+                                   const uint32_t* lens, uint32_t batch, uint32_t max_own,
+                                   const uint16_t* k_prefix, const uint16_t* v_prefix,
+                                   uint32_t prefix_len, uint32_t prefix_ctx, float* core,
+                                   void* workspace, uint64_t workspace_bytes, void* stream) {
+  constexpr const char* fn = "miso_attn_decode_ragged_shared";
+  if (any_bad(q, gate, core) || (max_own != 0 && any_bad(k_cache, v_cache)) ||
+      (prefix_len != 0 && any_bad(k_prefix, v_prefix)))
+    return fail(fn, kBadPtr);
+  if (any_bad_words(lens) ||
+      (max_own != 0 && (kv_offsets == nullptr || (reinterpret_cast<uintptr_t>(kv_offsets) & 7u))))
+    return fail(fn, "lens or kv_offsets is NULL or not aligned to its elements");
+  if (prefix_len > prefix_ctx)
+    return fail(fn, "prefix_len exceeds prefix_ctx");
+  if (const char* err = bad_shared(batch, max_own, prefix_len, workspace, workspace_bytes))
+    return fail(fn, err);
+  k::AttnSharedParams p{};
+  p.q = q, p.gate = gate, p.core = core, p.lens = lens;
+  p.prefix = {as_half(k_prefix), as_half(v_prefix), nullptr, prefix_ctx, 0, prefix_len};
+  p.batch = batch, p.whole = false, p.own_cap = 0xFFFFFFFFu;
+  const k::AttnSharedOwn own{as_half(k_cache), as_half(v_cache), nullptr, nullptr, 0, 0,
+                             kv_offsets};
+  return decode_shared(fn, p, own, max_own, workspace, stream);
 }
 
 }  // extern "C"

@@ -2892,6 +2892,15 @@ struct PagedStreamSource {
   }
 };
 
+// Keys of sequence s (a source whose lens count other keys too overloads it).
+template <class Src>
+__device__ __attribute__((always_inline)) inline unsigned stream_length(const Src&,
+                                                                        const StreamBatch& p,
+                                                                        unsigned s) {
+  const unsigned len = p.lens[s];
+  return len < p.len_cap ? len : p.len_cap;
+}
+
 // The streaming split over the batch's items (attn_ragged_stream_kernel's description), with
 // the tiles where Src says they are.
 template <class Src>
@@ -2914,8 +2923,8 @@ __device__ __attribute__((always_inline)) inline void stream_items(const StreamB
       if (cdna4::kLanes * i >= p.batch)  // uniform
         break;
       const unsigned s_ = cdna4::kLanes * i + lane;
-      const unsigned len = p.lens[s_ < p.batch ? s_ : p.batch - 1];
-      lens[i] = s_ >= p.batch ? 0u : len < p.len_cap ? len : p.len_cap;
+      const unsigned len = stream_length(src, p, s_ < p.batch ? s_ : p.batch - 1);
+      lens[i] = s_ >= p.batch ? 0u : len;
     }
     unsigned chunk = p.chunk;
     if (wave == 1) {
@@ -2962,7 +2971,7 @@ __device__ __attribute__((always_inline)) inline void stream_items(const StreamB
     }
     const unsigned r = k - prefix[lo], n = (prefix[lo + 1] - prefix[lo]) / 2;
     const unsigned kvh = r >= n ? 1u : 0u, split = r - kvh * n;
-    const unsigned len = p.lens[lo] < p.len_cap ? p.lens[lo] : p.len_cap;
+    const unsigned len = stream_length(src, p, lo);
     const AttnSpan span = attn_split_span(len, n, split);
     src.describe(lo, kvh, len);
     it_begin = span.begin;

@@ -1,0 +1,641 @@
+#pragma once
+
+// Batched decode behind a prefix that all sequences share, for MI355X (gfx950 / CDNA4); no reference
+// counterpart (the reference is batch-1). The ragged and paged decodes (attention_decode.hpp) read the
+// prefix once per sequence: 64 sequences behind 32768 keys stream 4.3 GB. Here the queries of all
+// sequences meet the prefix's keys together, so that K and V are read once per 16 sequences:
+//   attn_shared_prefix_kernel: partials of 8 query rows per sequence and KV head over spans of the prefix
+//   attn_shared_own_kernel:    the streaming split over each sequence's own keys behind it
+//   attn_shared_merge_kernel:  both partials joined, the gate applied
+// Precision is the decodes': every f32 operand (queries, numerators) enters the matrix units as a pair
+// of f16, sums are f32.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstddef>
+#include <cstdint>
+
+#include "attention_decode.hpp"
+#include "attention_evict.hpp"
+#include "attention_prefill.hpp"
+#include "cdna4_wave.hpp"
+
+namespace miso::kernels {
+
+// The prefix's rows: contiguous, K and V [2][ctx][256], or pages of a pool.
+struct AttnSharedPrefix {
+  const attn::half_t* k;
+  const attn::half_t* v;
+  const int32_t* table;  // nullptr: contiguous
+  std::size_t ctx;       // rows of a KV head where contiguous
+  unsigned log2_page;
+  unsigned len;  // keys
+};
+
+struct AttnSharedParams {
+  const float* q;     // [batch][16][256] (unscaled)
+  const float* gate;  // [batch][16][256]
+  float* core;        // [batch][16][256]
+  const uint32_t* lens;  // [batch]: own keys, or (whole) all keys, the prefix's among them
+  AttnSharedPrefix prefix;
+  float4* part_o;    // [span][KV head][row block][dimension block of 32][4][64 lanes]
+  float2* part_ml;   // [span][KV head][row of 8 batch, padded]: reference (log2 units), sum
+  unsigned batch;
+  unsigned spans, span_tiles;  // of the prefix; 0: no prefix
+  unsigned blocks;             // row blocks (of 32 rows: 4 sequences x 8 heads)
+  bool whole;
+  // The own keys' partials, [batch][2][s_max][8] and 256 times that, as the ragged decode's.
+  float* own_m;
+  float* own_l;
+  float* own_o;
+  unsigned s_max, chunk, own_cap;  // s_max 0: nobody has own keys
+  unsigned* balanced;
+};
+
+namespace shared_detail {
+
+using cdna4::float16_t;
+using cdna4::half8_t;
+using decode_detail::kGroup;
+using weights_detail::mfma32;
+
+constexpr unsigned kKeys = 32, kSteps = 16, kStages = 5;
+constexpr unsigned kTileBytes = kKeys * attn::kDim * 2;    // K or V of a tile
+constexpr unsigned kStageBytes = 2 * kTileBytes;           // K, then V
+constexpr unsigned kBlockRows = 32;                        // of the matrix instruction's columns
+constexpr unsigned kSeqs = kBlockRows / kGroup;            // sequences of a row block
+constexpr float kNoScore = -3e38f;  // below every score, and finite: differences stay numbers
+// Numerators are 2^(s - m) with m kLead below the first tile's maximum, and m follows when a lane's
+// numerators of a tile sum to more than kMost: below f16's 65504, and the f16 pair of a numerator of 1
+// relative to the row's largest keeps 2^-25 / 2^6 of it.
+constexpr float kLead = 6.0f, kMost = 32768.0f;
+
+struct alignas(1024) PrefixShared {
+  unsigned char ring[kStages * kStageBytes];
+};
+static_assert(sizeof(PrefixShared) == 160 * 1024, "the CU's LDS");
+
+// Keys of the prefix that a sequence sees.
+__device__ __attribute__((always_inline)) inline unsigned prefix_keys(const AttnSharedParams& p,
+                                                                      unsigned seq) {
+  if (seq >= p.batch)
+    return 0;
+  return p.whole ? min(p.lens[seq], p.prefix.len) : p.prefix.len;
+}
+
+}  // namespace shared_detail
+
+// One workgroup per (span, KV head, group of kRowBlocks row blocks). kRowBlocks waves side by side
+// hold 32 rows each: their queries as f16 pairs in 128 registers, a tile's scores S^T = K Q^T by 32
+// MFMAs, each K operand read serving both halves; and each of the 4 / kRowBlocks waves of a row block
+// adds P V for its share of the 256 dimensions (all 8 blocks of 32 dimensions: 32 MFMAs). So a wave's
+// tile is 64, 48 or 40 MFMAs of 32 cycles for 4, 2 and 1 row blocks: with few rows the memory sets the
+// pace (32 KiB a tile and CU), with many the matrix units.
+template <unsigned kRowBlocks>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
+attn_shared_prefix_kernel(AttnSharedParams p) {
+  using namespace shared_detail;
+  constexpr unsigned kParts = 4 / kRowBlocks;       // waves of a row block
+  constexpr unsigned kDimBlocks = 8 / kParts;       // of 32 dimensions, per wave
+  constexpr unsigned kStageRows = 32 / kParts;      // query rows that a wave lays out
+  __shared__ PrefixShared sh;
+  const unsigned lane = threadIdx.x & 63u, col = lane & 31u, hi = lane >> 5;
+  const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Row groups of one (span, KV head) on one XCD: its L2 serves them the same tiles.
+  const unsigned groups = (p.blocks + kRowBlocks - 1) / kRowBlocks;
+  const unsigned combo = blockIdx.x % 8 + 8 * (blockIdx.x / 8 / groups);
+  const unsigned group = blockIdx.x / 8 % groups;
+  if (combo >= 2 * p.spans)
+    return;
+  const unsigned kvh = combo % 2, span = combo / 2;
+  const unsigned t0 = span * p.span_tiles;
+  const unsigned t1 = min(t0 + p.span_tiles, (p.prefix.len + kKeys - 1) / kKeys);
+  const unsigned lds = cdna4::lds_offset(sh.ring);
+  const unsigned local = wave / kParts, part = wave % kParts;
+  const unsigned block = group * kRowBlocks + local;  // this wave's row block
+  const bool active = block < p.blocks;               // wave-uniform
+
+  // ---- Tiles: this wave copies rows 8 wave .. + 7 of K and V.
+  unsigned koff[4], voff[4];
+#pragma unroll
+  for (unsigned i = 0; i < 4; ++i) {
+    const unsigned row = 8 * wave + 2 * i + (lane >> 5), r = 2 * i + (lane >> 5);
+    koff[i] = r * 512 + 16 * prefill_detail::swz_k(row, lane & 31u) - 1024 * i;
+    voff[i] = r * 512 + 16 * prefill_detail::swz_v(row, lane & 31u) - 1024 * i;
+  }
+  int pages = 0;  // lane i: the page of this wave's rows of tile page0 + i
+  unsigned page0 = t0 - 64;
+  auto row_at = [&](unsigned row) __attribute__((always_inline)) {  // in halves
+    if (p.prefix.table == nullptr)
+      return (std::size_t{kvh} * p.prefix.ctx + row) * attn::kDim;
+    const unsigned page =
+        static_cast<unsigned>(__builtin_amdgcn_readlane(pages, row / kKeys - page0));
+    return (((std::size_t{page} * attn::kKvHeads + kvh) << p.prefix.log2_page) +
+            (row & ((1u << p.prefix.log2_page) - 1u))) * attn::kDim;
+  };
+  auto issue = [&](unsigned ti) __attribute__((always_inline)) {
+    const unsigned slot = lds + (ti - t0 + kStages - 1) % kStages * kStageBytes + 4096 * wave;
+    const unsigned row = ti * kKeys + 8 * wave, last = p.prefix.len - 1;
+    if (p.prefix.table != nullptr && ti - page0 >= 64u) {  // uniform
+      page0 = ti;
+      const unsigned r = min((ti + lane) * kKeys + 8 * wave, last);
+      pages = p.prefix.table[r >> p.prefix.log2_page];
+    }
+    if (row + 7 <= last) {
+      const std::size_t at = row_at(row);
+      prefill_detail::copy_tile(decode_detail::uniform(p.prefix.k + at),
+                                decode_detail::uniform(p.prefix.v + at), koff, voff, slot,
+                                slot + kTileBytes);
+    } else {  // the prefix ends here: rows past its last one repeat it (masked at use)
+      const unsigned from = min(row, last);
+      const std::size_t at = row_at(from);
+#pragma unroll
+      for (unsigned i = 0; i < 4; ++i) {
+        const unsigned r = 2 * i + (lane >> 5), x = lane & 31u;
+        const std::size_t a = at + static_cast<std::size_t>(min(r, last - from)) * attn::kDim;
+        cdna4::lds_load16(p.prefix.k + a + 8 * prefill_detail::swz_k(8 * wave + r, x),
+                          slot + 1024 * i);
+        cdna4::lds_load16(p.prefix.v + a + 8 * prefill_detail::swz_v(8 * wave + r, x),
+                          slot + kTileBytes + 1024 * i);
+      }
+    }
+  };
+  issue(t0);  // into the last stage: the queries pass through the others
+
+  // ---- Queries: row r of a block is sequence 4 block + r / 8, head 8 kvh + r % 8. Each row times
+  // log2(e) and a power of two of its own (its largest element near 2^14) is cut into f16 halves
+  // hi + lo (2^-22 of an element, 2^-38 of the row's largest), laid out in LDS (512-byte rows, chunk c
+  // of row r at c ^ (r % 16)) and read back as B operands.
+  half8_t qh[kSteps], ql[kSteps];
+  float scale = 1.0f;  // of the scores of this lane's row
+  const unsigned area = lds + 32768 * local;
+  {
+    float4 x[kStageRows];
+#pragma unroll
+    for (unsigned i = 0; i < kStageRows; ++i) {
+      const unsigned r = kStageRows * part + i, seq = min(kSeqs * block + r / kGroup, p.batch - 1);
+      x[i] = *reinterpret_cast<const float4*>(
+          p.q + (std::size_t{seq} * attn::kQHeads + kvh * kGroup + r % kGroup) * attn::kDim +
+          4 * lane);
+    }
+#pragma unroll
+    for (unsigned i = 0; i < kStageRows; ++i) {
+      const unsigned r = kStageRows * part + i;
+      const float top = cdna4::wave_allmax(fmaxf(fmaxf(__builtin_fabsf(x[i].x), __builtin_fabsf(x[i].y)),
+                                                 fmaxf(__builtin_fabsf(x[i].z), __builtin_fabsf(x[i].w))));
+      int e = 13 - (static_cast<int>(cdna4::as_uint(top) >> 23) - 127);
+      e = top == 0.0f || !(top < __builtin_inff()) ? 0 : (e < 100 ? e : 100);
+      const float up = __builtin_ldexpf(1.0f, e);
+      const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      cdna4::half4_t h, l;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float y = v[j] * up * decode_detail::kLog2e;
+        asm("" : "+v"(y));  // one rounding for both halves
+        h[j] = static_cast<_Float16>(y);
+        l[j] = static_cast<_Float16>(y - static_cast<float>(h[j]));
+      }
+      const unsigned at = area + 512 * r + 16 * ((lane / 2) ^ (r & 15u)) + 8 * (lane & 1u);
+      *reinterpret_cast<__attribute__((address_space(3))) cdna4::half4_t*>(at) = h;
+      *reinterpret_cast<__attribute__((address_space(3))) cdna4::half4_t*>(at + 16384) = l;
+      const float down = __builtin_ldexpf(1.0f / 16.0f, -e);
+      if constexpr (kParts == 1) {
+        scale = col == r ? down : scale;
+      } else if (lane == 0) {
+        *reinterpret_cast<__attribute__((address_space(3))) float*>(lds + 32768 * kRowBlocks +
+                                                                    128 * local + 4 * r) = down;
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (unsigned s = 0; s < kSteps; ++s) {
+    const unsigned at = area + 512 * col + 16 * ((2 * s + hi) ^ (col & 15u));
+    qh[s] = decode_detail::lds_b128(at);
+    ql[s] = decode_detail::lds_b128(at + 16384);
+  }
+  if constexpr (kParts != 1)
+    scale = *reinterpret_cast<const __attribute__((address_space(3))) float*>(
+        lds + 32768 * kRowBlocks + 128 * local + 4 * col);
+  __syncthreads();  // every wave has its operands: the ring takes the space
+#pragma unroll
+  for (unsigned i = 1; i < kStages - 1; ++i)
+    if (t0 + i < t1)
+      issue(t0 + i);
+
+  // ---- Keys this lane's row sees, and whether every row of the wave sees the whole span.
+  const unsigned seq = kSeqs * block + col / kGroup;
+  const unsigned sees = prefix_keys(p, seq);
+  const bool full = __builtin_amdgcn_ballot_w64(seq < p.batch && sees < t1 * kKeys) == 0;
+
+  // ---- Operand addresses of a stage (attention_prefill.hpp: the same tiles and swizzles).
+  const unsigned kb = col * 512 + 16 * (hi ^ (col & 15u));
+  unsigned vb[4];
+  {
+    const unsigned g = lane >> 4, j = lane & 15u;
+    const unsigned vrow = 4 * (g >> 1) + j / 4, vchunk = 2 * (g & 1u) + (j % 4) / 2;
+    const unsigned base = vrow * 512 + 8 * (j & 1u) + 16 * prefill_detail::swz_v(vrow, vchunk);
+#pragma unroll
+    for (unsigned c = 0; c < 4; ++c)
+      vb[c] = base ^ (64u * c);
+  }
+
+  float16_t o[kDimBlocks];
+#pragma unroll
+  for (unsigned b = 0; b < kDimBlocks; ++b)
+    o[b] = float16_t{};
+  float m = kNoScore, l = 0.0f;
+
+  for (unsigned ti = t0; ti < t1; ++ti) {
+    // Tile ti has landed (this wave's share by the count, the others' by the barrier), and every wave
+    // is done with tile ti - 1, whose stage the next copy takes.
+    const unsigned behind = min(t1 - 1 - ti, kStages - 2);
+    if (behind >= 3)
+      cdna4::wait_vmcnt<24>();
+    else if (behind == 2)
+      cdna4::wait_vmcnt<16>();
+    else if (behind == 1)
+      cdna4::wait_vmcnt<8>();
+    else
+      cdna4::wait_vmcnt<0>();
+    decode_detail::tile_barrier();
+    if (ti + kStages - 1 < t1)
+      issue(ti + kStages - 1);
+    if (!active)
+      continue;
+    const unsigned slot = lds + (ti - t0 + kStages - 1) % kStages * kStageBytes;
+    float16_t s = {};
+#pragma unroll
+    for (unsigned k = 0; k < kSteps; ++k) {
+      const half8_t a = decode_detail::lds_b128((slot + kb) ^ (32u * k));
+      s = mfma32(a, qh[k], s);
+      s = mfma32(a, ql[k], s);
+    }
+    float x[16];
+#pragma unroll
+    for (unsigned i = 0; i < 16; ++i) {
+      x[i] = s[i];
+      if (!full)  // uniform
+        x[i] = ti * kKeys + weights_detail::tile_row(lane, i) < sees ? x[i] : -__builtin_inff();
+    }
+    float w[16], sum = 0.0f;
+    auto numerators = [&]() __attribute__((always_inline)) {
+      sum = 0.0f;
+#pragma unroll
+      for (unsigned i = 0; i < 16; ++i) {
+        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], scale, -m));
+        sum += w[i];
+      }
+    };
+    numerators();
+    if (__builtin_amdgcn_ballot_w64(sum > kMost) != 0) {  // rare, and the first tile
+      float top = x[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i)
+        top = fmaxf(top, x[i]);
+      top = fmaxf(m, cdna4::max_xor32(top) * scale - kLead);
+      const float corr = __builtin_amdgcn_exp2f(m - top);
+      m = top;
+      l *= corr;
+#pragma unroll
+      for (unsigned b = 0; b < kDimBlocks; ++b)
+        o[b] *= corr;
+      numerators();
+    }
+    l += sum;
+    half8_t ph[2], pl[2];
+#pragma unroll
+    for (unsigned i = 0; i < 16; ++i) {
+      const _Float16 h = static_cast<_Float16>(w[i]);
+      ph[i / 8][i % 8] = h;
+      pl[i / 8][i % 8] = static_cast<_Float16>(w[i] - static_cast<float>(h));
+    }
+#pragma unroll
+    for (unsigned step = 0; step < 2; ++step)
+#pragma unroll
+      for (unsigned d = 0; d < kDimBlocks; ++d) {
+        // Dimension block part kDimBlocks + d: 64 (block % 4) by the XOR, 256 (block / 4) bytes.
+        const unsigned b = kParts == 4 ? d + 2 * (part & 1u) : d % 4;
+        const unsigned upper = kParts == 4 ? part >> 1 : kParts == 2 ? part : d / 4;
+        const unsigned at = slot + kTileBytes + (kParts == 4 ? vb[0] ^ (64u * b) : vb[d % 4]) +
+                            256u * upper + 8192u * step;
+        const cdna4::half4_t lo = prefill_detail::read_tr(at);
+        const cdna4::half4_t up = prefill_detail::read_tr(upper ? at + 4096u - 256u
+                                                                : at + 4096u + 256u);
+        const half8_t a = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
+        o[d] = mfma32(a, ph[step], o[d]);
+        o[d] = mfma32(a, pl[step], o[d]);
+      }
+  }
+  if (!active)
+    return;
+  // ---- The partial, relative to 2^m, in the accumulators' order (whole 1 KiB a store).
+  const std::size_t at = (std::size_t{span} * attn::kKvHeads + kvh) * p.blocks + block;
+  float4* out = p.part_o + (at * 8 + part * kDimBlocks) * 256 + lane;
+#pragma unroll
+  for (unsigned b = 0; b < kDimBlocks; ++b)
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i)
+      out[256 * b + 64 * i] = float4{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]};
+  const float all = cdna4::sum_xor32(l);
+  if (part == 0 && hi == 0)
+    p.part_ml[at * kBlockRows + col] = float2{m, all};
+}
+
+// ------------------------------------------------------------------------------------------------
+// Own keys: the streaming split of the ragged and paged decode over what lies behind the prefix.
+// ------------------------------------------------------------------------------------------------
+
+namespace decode_detail {
+
+// Pages behind the prefix: sequence s's own keys are in table row rows[s] (row s without rows), their
+// number is lens[s] less the prefix's.
+struct SharedPagedSource {
+  PagedStreamSource base;
+  const int32_t* rows;
+  unsigned prefix_len, table_row = 0;  // lane j: item j's row
+  __device__ __attribute__((always_inline)) void describe(unsigned seq, unsigned, unsigned) {
+    table_row = rows != nullptr ? static_cast<unsigned>(rows[seq]) : seq;
+  }
+  __device__ __attribute__((always_inline)) void prepare(unsigned, unsigned kvh, unsigned k0,
+                                                         unsigned last_row, unsigned j) {
+    base.prepare(lane_value(table_row, j), kvh, k0, last_row, j);
+  }
+  template <bool kV>
+  __device__ __attribute__((always_inline)) void issue(unsigned j, unsigned k0, unsigned last_row,
+                                                       unsigned lds, const WaveCopy& cp,
+                                                       unsigned lane) const {
+    base.template issue<kV>(j, k0, last_row, lds, cp, lane);
+  }
+};
+__device__ __attribute__((always_inline)) inline unsigned stream_length(
+    const SharedPagedSource& src, const StreamBatch& p, unsigned s) {
+  const unsigned len = p.lens[s], mine = len > src.prefix_len ? len - src.prefix_len : 0;
+  return mine < p.len_cap ? mine : p.len_cap;
+}
+
+}  // namespace decode_detail
+
+// Where the own keys lie: pages, or contiguous as the ragged decode's (page_table nullptr).
+struct AttnSharedOwn {
+  const attn::half_t* k;
+  const attn::half_t* v;
+  const int32_t* page_table;  // [..][max_pages], from the first entry behind the prefix
+  const int32_t* rows;        // [batch] table rows, or nullptr: 0 .. batch - 1
+  unsigned max_pages, log2_page;
+  const uint64_t* kv_offsets;
+};
+
+template <int = 0>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
+attn_shared_own_paged_kernel(AttnSharedParams p, AttnSharedOwn g) {
+  __shared__ decode_detail::StreamShared sh;
+  decode_detail::SharedPagedSource src{
+      {g.k, g.v, g.page_table, g.max_pages, g.log2_page}, g.rows, p.prefix.len};
+  decode_detail::stream_items(
+      decode_detail::StreamBatch{p.q, p.own_m, p.own_l, p.own_o, p.lens, p.batch, p.s_max,
+                                 p.own_cap, p.chunk, p.balanced},
+      src, sh);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Merge: a workgroup per (KV head, row block, 32 dimensions). Its waves take the prefix's spans in
+// turn, each lane the row of its column as the partials lie (M the largest reference, O and L summed
+// relative to 2^M in span order), and meet in LDS; then a thread per (row, 4 dimensions) adds the
+// waves' sums and the own keys' splits in order, divides and applies the gate. The order is fixed.
+// ------------------------------------------------------------------------------------------------
+
+template <int = 0>
+__global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams p) {
+  using namespace shared_detail;
+  constexpr unsigned kBatch = 4, kRow = 33;  // floats of a staged row: 32 and one apart
+  __shared__ float rows[4][kBlockRows * kRow];
+  __shared__ float2 ml[4][kBlockRows];
+  const unsigned t = threadIdx.x, lane = t & 63u, wave = t >> 6, col = lane & 31u, hi = lane >> 5;
+  const unsigned d = blockIdx.x % 8, kvh = blockIdx.x / 8 % 2, block = blockIdx.x / 16;
+  // This wave's spans of the prefix.
+  float m = kNoScore, l = 0.0f;
+  float4 o[4] = {};
+  for (unsigned s0 = wave; s0 < p.spans; s0 += 4 * kBatch) {
+    float2 x[kBatch];
+    float4 y[kBatch][4];
+#pragma unroll
+    for (unsigned i = 0; i < kBatch; ++i) {
+      const unsigned s = min(s0 + 4 * i, p.spans - 1);
+      const std::size_t at = (std::size_t{s} * attn::kKvHeads + kvh) * p.blocks + block;
+      x[i] = p.part_ml[at * kBlockRows + col];
+      x[i] = s0 + 4 * i < p.spans ? x[i] : float2{kNoScore, 0.0f};
+#pragma unroll
+      for (unsigned j = 0; j < 4; ++j)
+        y[i][j] = p.part_o[(at * 8 + d) * 256 + 64 * j + lane];
+    }
+    float top = m;
+#pragma unroll
+    for (unsigned i = 0; i < kBatch; ++i)
+      top = fmaxf(top, x[i].x);
+    const float old = __builtin_amdgcn_exp2f(m - top);
+    m = top;
+    l *= old;
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j)
+      o[j] = float4{o[j].x * old, o[j].y * old, o[j].z * old, o[j].w * old};
+#pragma unroll
+    for (unsigned i = 0; i < kBatch; ++i) {
+      if (s0 + 4 * i >= p.spans)  // uniform: a repeated span is left out (0 x infinity is NaN)
+        break;
+      const float e = __builtin_amdgcn_exp2f(x[i].x - top);
+      l = __builtin_fmaf(x[i].y, e, l);
+#pragma unroll
+      for (unsigned j = 0; j < 4; ++j) {
+        o[j].x = __builtin_fmaf(y[i][j].x, e, o[j].x);
+        o[j].y = __builtin_fmaf(y[i][j].y, e, o[j].y);
+        o[j].z = __builtin_fmaf(y[i][j].z, e, o[j].z);
+        o[j].w = __builtin_fmaf(y[i][j].w, e, o[j].w);
+      }
+    }
+  }
+#pragma unroll
+  for (unsigned j = 0; j < 4; ++j) {  // dimensions 8 j + 4 hi .. + 3 of the block
+    float* at = &rows[wave][col * kRow + 8 * j + 4 * hi];
+    at[0] = o[j].x, at[1] = o[j].y, at[2] = o[j].z, at[3] = o[j].w;
+  }
+  if (hi == 0)
+    ml[wave][col] = float2{m, l};
+  __syncthreads();
+
+  const unsigned row = t / 8, dim = 4 * (t % 8), seq = kSeqs * block + row / kGroup;
+  if (seq >= p.batch)
+    return;
+  const std::size_t out =
+      (std::size_t{seq} * attn::kQHeads + kvh * kGroup + row % kGroup) * attn::kDim + 32 * d + dim;
+  const float4 g = *reinterpret_cast<const float4*>(p.gate + out);
+  float top = kNoScore;
+#pragma unroll
+  for (unsigned w = 0; w < 4; ++w)
+    top = fmaxf(top, ml[w][row].x);
+  float all = 0.0f, v[4] = {};
+#pragma unroll
+  for (unsigned w = 0; w < 4; ++w) {
+    const float e = __builtin_amdgcn_exp2f(ml[w][row].x - top);
+    all = __builtin_fmaf(ml[w][row].y, e, all);
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j)
+      v[j] = __builtin_fmaf(rows[w][row * kRow + dim + j], e, v[j]);
+  }
+  if (p.s_max != 0) {
+    const unsigned len = p.lens[seq], skip = p.whole ? p.prefix.len : 0;
+    const unsigned mine = min(len > skip ? len - skip : 0u, p.own_cap);
+    const unsigned chunk = p.balanced != nullptr ? *p.balanced : p.chunk;
+    const unsigned n = attn_ragged_seq_splits(mine, p.s_max, chunk);
+    const std::size_t at0 =
+        ((std::size_t{seq} * attn::kKvHeads + kvh) * p.s_max) * kGroup + row % kGroup;
+    for (unsigned s0 = 0; s0 < n; s0 += kBatch) {
+      float sm[kBatch], sl[kBatch];
+      float4 so[kBatch];
+#pragma unroll
+      for (unsigned i = 0; i < kBatch; ++i) {
+        const std::size_t at = at0 + static_cast<std::size_t>(min(s0 + i, n - 1)) * kGroup;
+        sm[i] = p.own_m[at] * decode_detail::kLog2e;
+        sl[i] = p.own_l[at];
+        so[i] = *reinterpret_cast<const float4*>(p.own_o + at * attn::kDim + 32 * d + dim);
+      }
+#pragma unroll
+      for (unsigned i = 0; i < kBatch; ++i) {
+        if (s0 + i >= n)
+          break;
+        if (!(sl[i] != 0.0f))  // an empty span
+          continue;
+        const float next = fmaxf(top, sm[i]);
+        const float a = __builtin_amdgcn_exp2f(top - next), b = __builtin_amdgcn_exp2f(sm[i] - next);
+        top = next;
+        all = __builtin_fmaf(sl[i], b, all * a);
+        v[0] = __builtin_fmaf(so[i].x, b, v[0] * a);
+        v[1] = __builtin_fmaf(so[i].y, b, v[1] * a);
+        v[2] = __builtin_fmaf(so[i].z, b, v[2] * a);
+        v[3] = __builtin_fmaf(so[i].w, b, v[3] * a);
+      }
+    }
+  }
+  const float inv = all != 0.0f ? 1.0f / all : 0.0f;
+  const float gv[4] = {g.x, g.y, g.z, g.w};
+  float r[4];
+#pragma unroll
+  for (unsigned j = 0; j < 4; ++j)
+    r[j] = v[j] * inv / (1.0f + __expf(-gv[j]));
+  *reinterpret_cast<float4*>(p.core + out) = float4{r[0], r[1], r[2], r[3]};
+}
+
+// ------------------------------------------------------------------------------------------------
+// Launch
+// ------------------------------------------------------------------------------------------------
+
+constexpr unsigned kAttnSharedCus = 256;
+
+__host__ __device__ constexpr unsigned attn_shared_row_blocks(unsigned batch) {  // of a workgroup
+  return batch <= 4 ? 1 : batch <= 8 ? 2 : 4;
+}
+
+struct AttnSharedCut {
+  unsigned spans, span_tiles, blocks;
+};
+__host__ __device__ constexpr AttnSharedCut attn_shared_cut(unsigned batch, unsigned prefix) {
+  const unsigned rb = attn_shared_row_blocks(batch), blocks = (batch + 3) / 4;
+  const unsigned groups = (blocks + rb - 1) / rb, tiles = prefix / 32 + (prefix % 32 != 0);
+  if (tiles == 0)
+    return AttnSharedCut{0, 0, blocks};
+  unsigned spans = kAttnSharedCus / (2 * groups);
+  spans = spans == 0 ? 1 : spans;
+  const unsigned each = (tiles + spans - 1) / spans;
+  return AttnSharedCut{(tiles + each - 1) / each, each, blocks};
+}
+
+// Row blocks x spans of a KV head's partials: no less than any smaller batch or shorter prefix takes.
+__host__ __device__ constexpr std::size_t attn_shared_part_blocks(unsigned batch, unsigned prefix) {
+  const std::size_t blocks = (std::size_t{batch} + 3) / 4, tiles = (std::size_t{prefix} + 31) / 32;
+  const std::size_t most = blocks <= 1 ? 128 : blocks <= 2 ? 256 : blocks < 512 ? 512 : blocks;
+  return most < blocks * tiles ? most : blocks * tiles;
+}
+
+// The workspace: the prefix's partials, then the own keys' (as the ragged decode's balanced scratch).
+struct AttnSharedLayout {
+  std::size_t part_ml, own_m, own_l, own_o, bytes;  // part_o first
+};
+__host__ __device__ constexpr AttnSharedLayout attn_shared_layout(unsigned batch, unsigned max_own,
+                                                                  unsigned prefix) {
+  const std::size_t blocks = attn::kKvHeads * attn_shared_part_blocks(batch, prefix);
+  const std::size_t own = attn_ragged_balanced_rows(batch, max_own) * attn::kQHeads + 4;
+  AttnSharedLayout a{};
+  a.part_ml = blocks * 32 * attn::kDim * sizeof(float);
+  a.own_o = a.part_ml + blocks * 32 * sizeof(float2);
+  a.own_m = a.own_o + own * attn::kDim * sizeof(float);
+  a.own_l = a.own_m + own * sizeof(float);
+  a.bytes = a.own_l + own * sizeof(float);
+  return a;
+}
+
+// p: q, gate, core, lens, prefix, batch, whole and own_cap given; the workspace holds
+// attn_shared_layout(batch, max_own, p.prefix.len).
+inline void attn_shared_launch(AttnSharedParams p, const AttnSharedOwn& own, unsigned max_own,
+                               char* ws, unsigned cus, hipStream_t stream) {
+  const AttnSharedLayout at = attn_shared_layout(p.batch, max_own, p.prefix.len);
+  const AttnSharedCut cut = attn_shared_cut(p.batch, p.prefix.len);
+  p.part_o = reinterpret_cast<float4*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + at.part_ml);
+  p.own_m = reinterpret_cast<float*>(ws + at.own_m);
+  p.own_l = reinterpret_cast<float*>(ws + at.own_l);
+  p.own_o = reinterpret_cast<float*>(ws + at.own_o);
+  p.spans = cut.spans;
+  p.span_tiles = cut.span_tiles;
+  p.blocks = cut.blocks;
+  if (cut.spans != 0) {
+    const unsigned rb = attn_shared_row_blocks(p.batch), groups = (cut.blocks + rb - 1) / rb;
+    const unsigned grid = 8 * ((2 * cut.spans + 7) / 8) * groups;
+    if (rb == 1)
+      attn_shared_prefix_kernel<1><<<grid, 256, 0, stream>>>(p);
+    else if (rb == 2)
+      attn_shared_prefix_kernel<2><<<grid, 256, 0, stream>>>(p);
+    else
+      attn_shared_prefix_kernel<4><<<grid, 256, 0, stream>>>(p);
+  }
+  if (max_own != 0) {
+    // At most one streaming launch's sequences and items at a time.
+    const unsigned most_items = kRaggedStreamMaxItems * cus;
+    p.s_max = std::min(attn_ragged_balanced_splits(p.batch, max_own),
+                       most_items / attn::kKvHeads);
+    p.chunk = attn_ragged_chunk(p.batch, max_own, cus);
+    const std::size_t items = std::size_t{p.batch} * attn::kKvHeads * p.s_max;
+    const unsigned grid = static_cast<unsigned>(std::min<std::size_t>(cus, items));
+    unsigned step = p.batch;
+    if (attn_ragged_balanced(p.batch, max_own, cus, grid))
+      p.balanced = reinterpret_cast<unsigned*>(p.own_l) - 4;
+    else
+      step = std::min(kRaggedStreamMaxBatch,
+                      std::max(1u, kRaggedStreamMaxItems * grid / (attn::kKvHeads * p.s_max)));
+    for (unsigned s = 0; s < p.batch; s += step) {
+      const std::size_t row = std::size_t{s} * attn::kKvHeads * p.s_max * decode_detail::kGroup;
+      AttnSharedParams a = p;
+      a.batch = std::min(step, p.batch - s);
+      a.q += std::size_t{s} * attn::kQHeads * attn::kDim;
+      a.lens += s;
+      a.own_m += row;
+      a.own_l += row;
+      a.own_o += row * attn::kDim;
+      if (own.page_table != nullptr) {
+        AttnSharedOwn g = own;
+        if (g.rows != nullptr)
+          g.rows += s;
+        else
+          g.page_table += std::size_t{s} * g.max_pages;
+        attn_shared_own_paged_kernel<<<grid, 256, 0, stream>>>(a, g);
+      } else {
+        attn_ragged_stream_kernel<256><<<grid, 256, 0, stream>>>(AttnRaggedParams{
+            a.q, nullptr, own.k, own.v, own.kv_offsets + s, a.lens, nullptr, a.own_m, a.own_l,
+            a.own_o, a.batch, a.s_max, a.own_cap, a.chunk, a.balanced});
+      }
+    }
+  }
+  attn_shared_merge_kernel<<<16 * cut.blocks, 256, 0, stream>>>(p);
+}
+
+}  // namespace miso::kernels

@@ -1,0 +1,409 @@
+"""Decode behind a shared prefix on the GPU (no reference counterpart): paged and ragged against float64
+over the same keys, at the decodes' precision, and a batch served from page plan to attention."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from conftest import REF_REL_L2
+
+pytestmark = pytest.mark.gpu
+
+H, KV, D, GROUP = 16, 2, 256, 8
+
+
+def dev(torch, a, dtype=None):
+    return torch.from_numpy(np.ascontiguousarray(a)).to(dtype or torch.int32).cuda()
+
+
+def attention(torch, q, gate, k, v):
+    """[16][256] in float64: one entry's gated attention over k, v [2][n][256]."""
+    if k.shape[1] == 0:
+        return torch.zeros(H, D, dtype=torch.float64, device="cuda")
+    x = q.double().view(KV, GROUP, D)
+    s = torch.matmul(x, k.double().transpose(1, 2).contiguous()) / 16
+    return (torch.matmul(torch.softmax(s, -1), v.double()).view(H, D) *
+            torch.sigmoid(gate.double()))
+
+
+def check(torch, core, ref, what=""):
+    err = (core.double() - ref).norm(dim=-1) / ref.norm(dim=-1).clamp(min=1e-300)
+    err = torch.where(ref.abs().amax(-1) == 0, core.double().abs().amax(-1), err)
+    assert torch.isfinite(core).all(), what
+    assert err.max() <= REF_REL_L2, (what, float(err.max()))
+
+
+class Paged:
+    """Entries over a pool whose pages lie in random order; unused table entries and pages are bad."""
+
+    def __init__(self, torch, page, prefix_pages, lens, seed, rows=None, q_scale=2.0, room=None):
+        self.torch, self.page, self.pp = torch, page, prefix_pages
+        rng = np.random.default_rng(seed)
+        g = torch.Generator(device="cuda")
+        g.manual_seed(seed)
+        self.lens = np.asarray(lens)
+        b = len(self.lens)
+        self.rows = np.arange(b) if rows is None else np.asarray(rows)
+        n_rows = int(self.rows.max()) + 1
+        most = np.zeros(n_rows, np.int64)
+        np.maximum.at(most, self.rows, np.maximum(self.lens - prefix_pages * page, 0))
+        own = -(-most // page)
+        self.room = room or prefix_pages + max(1, int(own.max()))
+        total = prefix_pages + int(own.sum())
+        ids = rng.permutation(total + 4)
+        self.table = np.full((n_rows, self.room), -(2 ** 31) + 5, np.int64)
+        at = prefix_pages
+        for r in range(n_rows):
+            self.table[r, :prefix_pages] = ids[:prefix_pages]
+            self.table[r, prefix_pages:prefix_pages + own[r]] = ids[at:at + own[r]]
+            at += own[r]
+        self.prefix = ids[:prefix_pages]
+        shape = (total + 4, KV, page, D)
+        self.k = torch.randn(*shape, generator=g, device="cuda", dtype=torch.float16)
+        self.v = torch.randn(*shape, generator=g, device="cuda", dtype=torch.float16)
+        # Rows that nobody sees: the spare pages, and what lies behind a row's last key.
+        for x in (self.k, self.v):
+            x[torch.from_numpy(ids[total:]).cuda()] = float("nan")
+            for r in range(n_rows):
+                if own[r] and most[r] % page:
+                    x[int(self.table[r, prefix_pages + own[r] - 1]), :, most[r] % page:] = (
+                        float("inf"))
+        self.q = q_scale * torch.randn(b, H, D, generator=g, device="cuda")
+        self.gate = torch.randn(b, H, D, generator=g, device="cuda")
+        self.core = torch.full((b, H, D), 777.25, device="cuda")
+        self.max_own = int(most.max())
+        self.d = dict(lens=dev(torch, self.lens), table=dev(torch, self.table),
+                      prefix=dev(torch, self.prefix),
+                      rows=None if rows is None else dev(torch, self.rows))
+
+    def scratch(self, attn, **kw):
+        sc = attn.SharedScratch(**{**dict(batch=len(self.lens), max_own=self.max_own,
+                                          max_prefix=self.pp * self.page), **kw})
+        sc.ws.fill_(255)  # NaN everywhere
+        return sc
+
+    def run(self, attn, sc=None, **kw):
+        attn.attn_decode_paged_shared(self.q, self.gate, self.k, self.v, self.d["table"], self.page,
+                                      self.d["lens"], self.d["prefix"], self.pp, self.core,
+                                      sc or self.scratch(attn), rows=self.d["rows"], **kw)
+        self.torch.cuda.synchronize()
+        return self.core
+
+    def keys(self, x, e):
+        n, page = int(self.lens[e]), self.page
+        table = self.table[self.rows[e]].copy()
+        table[:self.pp] = self.prefix
+        pages = self.torch.from_numpy(table[:-(-n // page)]).cuda()
+        return x[pages].transpose(0, 1).reshape(KV, -1, D)[:, :n]
+
+    def ref(self):
+        return self.torch.stack([attention(self.torch, self.q[e], self.gate[e],
+                                           self.keys(self.k, e), self.keys(self.v, e))
+                                 for e in range(len(self.lens))])
+
+
+def lengths(rng, batch, prefix, own, zeros=True):
+    lens = prefix + rng.integers(0, own + 1, batch)
+    if zeros and batch > 3:
+        lens[rng.integers(0, batch)] = 0
+        lens[rng.integers(0, batch)] = max(prefix // 2, 1)
+        lens[rng.integers(0, batch)] = prefix
+    lens[0] = prefix + own
+    return lens
+
+
+@pytest.mark.parametrize("batch,page,prefix_pages,own", [
+    (1, 8, 1, 1), (1, 16, 40, 5), (2, 16, 0, 70), (3, 8, 3, 33), (4, 16, 130, 513), (5, 32, 1, 100),
+    (7, 64, 9, 31), (8, 16, 17, 1030), (9, 8, 5, 8), (16, 128, 3, 300), (17, 16, 70, 64),
+    (33, 16, 21, 700), (64, 8, 300, 129), (100, 256, 2, 40), (3, 4096, 1, 100), (20, 65536, 1, 9)])
+def test_paged(torch_mod, attn, batch, page, prefix_pages, own):
+    rng = np.random.default_rng(batch * 1000 + page)
+    c = Paged(torch_mod, page, prefix_pages, lengths(rng, batch, prefix_pages * page, own), batch)
+    first = c.run(attn).clone()
+    check(torch_mod, first, c.ref())
+    c.core.fill_(-5.0)
+    assert torch_mod.equal(c.run(attn), first)  # the same bits over another dirty workspace
+
+
+def test_paged_equals_the_paged_decode(torch_mod, attn):
+    """The keys of attn_decode_paged on the same tables; entries without keys give zeros in both."""
+    rng = np.random.default_rng(2)
+    lens = lengths(rng, 21, 320, 300)
+    c = Paged(torch_mod, 16, 20, lens, 21)
+    c.d["table"].clamp_(min=0)  # (that call reads no bad entry either, but says so of fewer)
+    got = c.run(attn).clone()
+    other = torch_mod.empty_like(got)
+    attn.attn_decode_paged(c.q, c.gate, c.k, c.v, c.d["table"], 16, c.d["lens"], other,
+                           attn.RaggedScratch(21, int(lens.max())))
+    check(torch_mod, got, other.double())
+    empty = torch_mod.from_numpy(lens == 0).cuda()
+    assert (got[empty] == 0).all() and empty.any()
+
+
+@pytest.mark.parametrize("batch,seqs,prefix_pages", [(6, 1, 2), (40, 1, 30), (203, 1, 12),
+                                                     (24, 3, 5), (9, 2, 0)])
+def test_chunks_share_a_table_row(torch_mod, attn, batch, seqs, prefix_pages):
+    """Entries of one row with rising lengths: the causal attention of a chunk of each request."""
+    page = 16
+    rows = np.arange(batch) * seqs // batch
+    count = np.bincount(rows)
+    index = np.arange(batch) - np.concatenate([[0], np.cumsum(count)])[rows]
+    lens = prefix_pages * page + 11 * rows + index + 1
+    c = Paged(torch_mod, page, prefix_pages, lens, batch, rows=rows)
+    check(torch_mod, c.run(attn), c.ref())
+
+
+@pytest.mark.parametrize("batch,own", [(513, 40), (1100, 5), (600, 700)])
+def test_many_entries(torch_mod, attn, batch, own):
+    """Above the entries of one streaming launch."""
+    rng = np.random.default_rng(batch)
+    c = Paged(torch_mod, 16, 3, lengths(rng, batch, 48, own), batch)
+    check(torch_mod, c.run(attn), c.ref())
+
+
+def test_own_keys_beyond_max_own(torch_mod, attn):
+    """lens above the capacity the scratch was made for: still all keys, in longer spans."""
+    c = Paged(torch_mod, 8, 4, [32 + 2049, 32 + 5, 32], 3)
+    sc = c.scratch(attn, max_own=600)
+    check(torch_mod, c.run(attn, sc), c.ref())
+
+
+def test_max_own_of_zero_looks_at_the_prefix_alone(torch_mod, attn):
+    c = Paged(torch_mod, 8, 6, [48, 48, 20, 0, 48], 4, room=6)
+    c.table[:] = -1
+    check(torch_mod, c.run(attn, c.scratch(attn, max_own=0)), c.ref())
+
+
+def test_scratch_serves_smaller_calls(torch_mod, attn):
+    rng = np.random.default_rng(8)
+    sc = attn.SharedScratch(64, 900, 4096)
+    for batch, pp, own in ((64, 256, 900), (1, 256, 900), (13, 3, 40), (64, 1, 1), (9, 255, 700)):
+        c = Paged(torch_mod, 16, pp, lengths(rng, batch, 16 * pp, own), batch)
+        check(torch_mod, c.run(attn, sc), c.ref(), (batch, pp, own))
+
+
+def test_spans_longer_than_the_page_ids_a_wave_holds(torch_mod, attn):
+    """More than 64 tiles a span: its pages are read again, and tiles wrap the ring many times."""
+    lens = 90112 + np.arange(30) % 7
+    lens[3] = 50001  # ends inside a span
+    c = Paged(torch_mod, 16, 5632, lens, 30)
+    check(torch_mod, c.run(attn), c.ref())
+
+
+def test_extreme_scores(torch_mod, attn):
+    """Queries of 2^-20 .. 2^16 (2^20 over the prefix alone: the split over own keys takes those below
+    2^19) and rising keys: references move late in a span, weights of 0 and 1."""
+    torch = torch_mod
+    for scale, own in ((2.0 ** -20, 90), (30.0, 90), (2.0 ** 16, 90), (2.0 ** 20, 0)):
+        c = Paged(torch, 16, 16, lengths(np.random.default_rng(1), 19, 256, own, zeros=False), 6,
+                  q_scale=scale)
+        if scale == 30.0:
+            ramp = torch.linspace(0.01, 1.5, 256, device="cuda", dtype=torch.float16)
+            pages = torch.from_numpy(c.prefix).cuda()
+            c.k[pages] = (c.k[pages].transpose(1, 2) * ramp.view(16, 16, 1, 1)).transpose(1, 2)
+        got, ref = c.run(attn), c.ref()
+        # A score s is off by 2^-22 of |q| |k| / 16 (pairs) and 2^-23 (sums), its weight by that factor.
+        if scale <= 30.0:
+            size = float(c.q.norm(dim=-1).max()) * float(c.k[~c.k.isnan() & ~c.k.isinf()].abs().max())
+            err = ((got.double() - ref).norm(dim=-1) / ref.norm(dim=-1)).max()
+            assert err <= REF_REL_L2 + 2.0 ** -21 * size, float(err)
+        else:  # one key has all the weight, unless two scores lie within rounding
+            assert torch.isfinite(got).all()
+            assert ((got.double() - ref).norm(dim=-1) <= 1e-4 * ref.norm(dim=-1)).float().mean() > 0.98
+
+
+def test_rows_are_independent(torch_mod, attn):
+    """NaN and infinities in the queries of an entry stay in its rows; queries of zero weigh evenly."""
+    torch = torch_mod
+    c = Paged(torch, 16, 10, lengths(np.random.default_rng(4), 18, 160, 60, zeros=False), 18)
+    c.q[5] = 0
+    good = c.run(attn).clone()
+    check(torch, good, c.ref())
+    c.q[3] = float("nan")
+    c.q[7, 2] = float("inf")
+    c.q[12] = 3e38
+    got = c.run(attn)
+    keep = torch.ones(18, H, dtype=torch.bool, device="cuda")
+    keep[3] = keep[12] = keep[7, 2] = False
+    assert torch.equal(got[keep], good[keep])
+
+
+def test_padding_entries_read_nothing(torch_mod, attn):
+    """Entries of length 0 with NaN queries, rows outside the table's use: zeros, the others whole."""
+    torch = torch_mod
+    lens = np.array([200, 0, 0, 161, 0, 160, 190, 0, 0, 0])
+    c = Paged(torch, 16, 10, lens, 5, rows=np.array([0, 0, 0, 1, 0, 2, 3, 0, 0, 0]))
+    ref = c.ref()
+    for e in np.flatnonzero(lens == 0):
+        c.q[e] = float("nan")
+        c.d["rows"][int(e)] = 2 ** 30
+    got = c.run(attn)
+    check(torch, got, ref)
+    assert (got[torch.from_numpy(lens == 0).cuda()] == 0).all()
+
+
+def test_pool_beyond_4_gib(torch_mod, attn):
+    torch, page, pp = torch_mod, 64, 20
+    c = Paged(torch, page, pp, [pp * page + 100, pp * page + 7, pp * page], 31)
+    pages = 80000  # 5.2 GB each
+    far = np.random.default_rng(1).permutation(4000)[:len(c.k)] + pages - 4000
+    k, v = (torch.empty(pages, KV, page, D, device="cuda", dtype=torch.float16) for _ in range(2))
+    at = torch.from_numpy(far).cuda()
+    k[at], v[at] = c.k, c.v
+    ref = c.ref()
+    table = np.where(c.table >= 0, far[np.clip(c.table, 0, len(far) - 1)], -1)
+    c.k, c.v = k, v
+    c.d["table"], c.d["prefix"] = dev(torch, table), dev(torch, far[c.prefix])
+    check(torch, c.run(attn), ref)
+
+
+def ragged(torch, batch, prefix, own, seed, ctx_spare=13):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    rng = np.random.default_rng(seed)
+    held = rng.integers(0, own + 1, batch)
+    held[0] = own
+    first = np.concatenate([[0], np.cumsum(held)[:-1]]) * KV * D
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda", dtype=torch.float16)  # noqa: E731
+    total, ctx = max(int(held.sum()), 1), prefix + ctx_spare
+    c = dict(held=held, q=2 * torch.randn(batch, H, D, generator=g, device="cuda"),
+             gate=torch.randn(batch, H, D, generator=g, device="cuda"), k=rand(total * KV * D),
+             v=rand(total * KV * D), kp=rand(KV, ctx, D), vp=rand(KV, ctx, D), first=first,
+             prefix=prefix, ctx=ctx, core=torch.full((batch, H, D), -3.5, device="cuda"))
+    c["kp"][:, prefix:], c["vp"][:, prefix:] = float("nan"), float("inf")
+    return c
+
+
+def run_ragged(torch, attn, c, sc=None):
+    sc = sc or attn.SharedScratch(len(c["held"]), int(c["held"].max()), c["prefix"])
+    attn.attn_decode_ragged_shared(c["q"], c["gate"], c["k"], c["v"],
+                                   dev(torch, c["first"], torch.int64), dev(torch, c["held"]),
+                                   c["kp"], c["vp"], c["prefix"], c["ctx"], c["core"], sc)
+    ref = []
+    for e, n in enumerate(c["held"]):
+        n, at = int(n), int(c["first"][e])
+        kv = [torch.cat([p[:, :c["prefix"]], x[at:at + KV * n * D].view(KV, n, D)], dim=1)
+              for p, x in ((c["kp"], c["k"]), (c["vp"], c["v"]))]
+        ref.append(attention(torch, c["q"][e], c["gate"][e], *kv))
+    return c["core"], torch.stack(ref)
+
+
+@pytest.mark.parametrize("batch,prefix,own", [
+    (1, 1, 0), (1, 31, 3), (2, 32, 40), (3, 33, 1), (4, 1000, 600), (6, 257, 10), (8, 4097, 64),
+    (13, 65, 900), (16, 0, 50), (33, 5003, 100), (70, 511, 17), (530, 63, 9)])
+def test_ragged(torch_mod, attn, batch, prefix, own):
+    c = ragged(torch_mod, batch, prefix, own, batch + prefix)
+    core, ref = run_ragged(torch_mod, attn, c)
+    check(torch_mod, core, ref)
+
+
+def test_ragged_prefix_beyond_4_gib(torch_mod, attn):
+    """A cache of 4.3 million rows a head: the second head's rows lie past 32-bit byte and half offsets."""
+    torch = torch_mod
+    c = ragged(torch, 5, 700, 20, 3)
+    ctx = 9_000_000  # 4.6 GB a head
+    for x in ("kp", "vp"):
+        far = torch.empty(KV, ctx, D, device="cuda", dtype=torch.float16)
+        far[:, :700] = c[x][:, :700]
+        c[x] = far
+    c["ctx"] = ctx
+    core, ref = run_ragged(torch, attn, c)
+    check(torch, core, ref)
+
+
+def test_two_streams_and_graphs(torch_mod, attn):
+    """Two calls at once over scratches of their own, and a captured call replayed over new lengths."""
+    torch = torch_mod
+    a = Paged(torch, 16, 40, lengths(np.random.default_rng(1), 12, 640, 200), 1)
+    b = Paged(torch, 8, 9, lengths(np.random.default_rng(2), 40, 72, 90), 2)
+    sa, sb = a.scratch(attn), b.scratch(attn)
+    ra, rb = a.run(attn, sa).clone(), b.run(attn, sb).clone()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        a.core.zero_()
+        b.core.zero_()
+        torch.cuda.synchronize()
+        for c, sc, s in ((a, sa, streams[0]), (b, sb, streams[1])):
+            attn.attn_decode_paged_shared(c.q, c.gate, c.k, c.v, c.d["table"], c.page, c.d["lens"],
+                                          c.d["prefix"], c.pp, c.core, sc, stream=s)
+        torch.cuda.synchronize()
+        assert torch.equal(a.core, ra) and torch.equal(b.core, rb)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attn.attn_decode_paged_shared(a.q, a.gate, a.k, a.v, a.d["table"], a.page, a.d["lens"],
+                                      a.d["prefix"], a.pp, a.core, sa)
+    for step in range(4):
+        a.lens = np.minimum(lengths(np.random.default_rng(step), 12, 640, 200), a.lens)
+        a.d["lens"].copy_(dev(torch, a.lens))
+        a.q.normal_()
+        sa.ws.fill_(255)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(torch, a.core, a.ref(), step)
+
+
+def test_a_batch_served(torch_mod, attn):
+    """Steps of a server: plan, prep and attention over one pool, requests behind a shared prefix that
+    start with prompts, go on by one token and end; every step's outputs against float64 over the keys
+    that the prep wrote, and the keys against a record of what each request was given."""
+    torch = torch_mod
+    rng = np.random.default_rng(21)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    b, page, pp, room, pool, most = 12, 8, 6, 20, 170, 96
+    stride = 9216
+    k_pages, v_pages = (torch.zeros(pool, KV, page, D, device="cuda", dtype=torch.float16)
+                        for _ in range(2))
+    ids = rng.permutation(pool)
+    prefix = dev(torch, ids[:pp])
+    k_pages[prefix.long()] = torch.randn(pp, KV, page, D, generator=g, device="cuda").half()
+    v_pages[prefix.long()] = torch.randn(pp, KV, page, D, generator=g, device="cuda").half()
+    lens, table = dev(torch, np.zeros(b)), dev(torch, np.full((b, room), -1))
+    stack, n_free = dev(torch, np.concatenate([ids[pp:], np.full(pp, -1)])), dev(torch, [pool - pp])
+    q_norm, k_norm = (1 + 0.1 * torch.randn(D, generator=g, device="cuda") for _ in range(2))
+    freq, scale = attn.rope_frequencies(64, 1e7, factor=4, scaling="yarn", original_ctx=32768)
+    plan = attn.PagePlan(b, most)
+    q, gate, core = (torch.full((most, H, D), 5.0, device="cuda") for _ in range(3))
+    sc = attn.SharedScratch(most, (room - pp) * page, pp * page)
+    given = [[] for _ in range(b)]  # per request: (step, token) of its keys behind the prefix
+    projs = []
+    held = np.zeros(b, np.int64)
+    for step in range(9):
+        ended = (rng.random(b) < 0.15) & (held > 0)
+        new = np.where(held == 0, rng.integers(0, 15, b), 1)
+        new[ended] = rng.integers(0, 2, b)[ended] * 9
+        proj = torch.randn(most, stride, generator=g, device="cuda")
+        projs.append(proj)
+        attn.attn_page_plan(lens, dev(torch, new), table, page, stack, n_free, plan,
+                            ended=dev(torch, ended), prefix_table=prefix, prefix_pages=pp)
+        flat = proj.view(-1)
+        attn.attn_prep_paged(flat, flat[8192:], flat[8704:], q_norm, k_norm, freq, k_pages, v_pages,
+                             page, plan.slots, plan.positions, q, most, stride, 1e-6, gate=gate,
+                             rot_scale=scale)
+        attn.attn_decode_paged_shared(q, gate, k_pages, v_pages, table, page, plan.visible, prefix,
+                                      pp, core, sc, rows=plan.rows)
+        torch.cuda.synchronize()
+        status, starts = plan.status.cpu().numpy(), plan.starts.cpu().numpy()
+        for r in range(b):
+            if ended[r]:
+                given[r], held[r] = [], 0
+            if new[r] and status[r] == 0:
+                given[r] += [(step, t) for t in range(starts[r], starts[r + 1])]
+                held[r] = pp * page + len(given[r])
+        assert np.array_equal(lens.cpu().numpy(), held)
+        rows, sees = plan.rows.cpu().numpy(), plan.visible.cpu().numpy()
+        t_of = table.cpu().numpy()
+        for t in range(most):
+            if sees[t] == 0:
+                assert (core[t] == 0).all()
+                continue
+            pages = torch.from_numpy(np.concatenate([ids[:pp], t_of[rows[t]][pp:]])[
+                :-(-sees[t] // page)]).cuda().long()
+            k = k_pages[pages].transpose(0, 1).reshape(KV, -1, D)[:, :sees[t]]
+            v = v_pages[pages].transpose(0, 1).reshape(KV, -1, D)[:, :sees[t]]
+            check(torch, core[t][None], attention(torch, q[t], gate[t], k, v)[None], (step, t))
+            if t == starts[rows[t] + 1] - 1:  # V rows are the given tokens', in order
+                mine = torch.stack([projs[s][i, 8704:].view(KV, D) for s, i in given[rows[t]]], 1)
+                assert torch.equal(v[:, pp * page:], mine.half())
+    assert held.max() > 0
