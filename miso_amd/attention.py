@@ -66,6 +66,20 @@ def _here(*tensors: torch.Tensor) -> None:
             raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{device}")
 
 
+def _need_all(*specs) -> None:
+    """_need of every (name, tensor, dtype, numel) and _here of their tensors, in one pass: most of a
+    short call's time on the host."""
+    name, t, dtype, numel = specs[0]
+    if not t.is_cuda:
+        _need(t, name, dtype, numel)
+    device = torch.cuda.current_device() if _device is None else _device()
+    for name, t, dtype, numel in specs:
+        if (t.dtype is not dtype or t.get_device() != device or t.numel() < numel
+                or not t.is_contiguous()):
+            _need(t, name, dtype, numel)
+            _here(t)
+
+
 def _cache_dtype(t: torch.Tensor) -> torch.dtype:
     return torch.float16 if t.dtype == torch.float16 else torch.int16
 
@@ -673,29 +687,27 @@ def attn_page_plan(lens, n_new, page_table, page_size: int, free_pages, n_free, 
         raise ValueError("page_table must be [batch][max_pages]")
     lens_out = lens if lens_out is None else lens_out
     n_free_out = n_free if n_free_out is None else n_free_out
-    max_pages = int(page_table.shape[1])
-    for name, t, n in (("lens", lens, batch), ("n_new", n_new, batch), ("lens_out", lens_out, batch),
-                       ("page_table", page_table, batch * max_pages), ("n_free", n_free, 1),
-                       ("n_free_out", n_free_out, 1), ("free_pages", free_pages, 1)):
-        _need(t, name, int32, n)
+    _count(page_size, "page_size"), _count(prefix_pages, "prefix_pages")
+    _need_all(("lens", lens, int32, batch), ("n_new", n_new, int32, batch),
+              ("lens_out", lens_out, int32, batch), ("page_table", page_table, int32, 0),
+              ("n_free", n_free, int32, 1), ("n_free_out", n_free_out, int32, 1),
+              ("free_pages", free_pages, int32, 1), ("plan.slots", plan.slots, int32, 0))
     if ended is not None:
-        _need(ended, "ended", int32, batch)
+        _need_all(("ended", ended, int32, batch))
     if prefix_pages:
-        _need(prefix_table, "prefix_table", int32, _count(prefix_pages, "prefix_pages"))
-    _here(lens, n_new, page_table, free_pages, n_free, lens_out, n_free_out, plan.slots,
-          *(t for t in (ended, prefix_table if prefix_pages else None) if t is not None))
+        _need_all(("prefix_table", prefix_table, int32, prefix_pages))
     _lib.check(_lib.load().miso_attn_page_plan(
-        lens.data_ptr(), n_new.data_ptr(), _ptr(ended), page_table.data_ptr(), batch, max_pages,
-        _count(page_size, "page_size"), prefix_table.data_ptr() if prefix_pages else None,
-        prefix_pages, free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(),
-        lens_out.data_ptr(), n_free_out.data_ptr(), plan.status.data_ptr(), plan.starts.data_ptr(),
-        plan.slots.data_ptr(), plan.positions.data_ptr(), plan.rows.data_ptr(),
-        plan.visible.data_ptr(), plan.max_tokens, _stream(stream)))
+        lens.data_ptr(), n_new.data_ptr(), None if ended is None else ended.data_ptr(),
+        page_table.data_ptr(), batch, page_table.shape[1], page_size,
+        prefix_table.data_ptr() if prefix_pages else None, prefix_pages, free_pages.data_ptr(),
+        free_pages.numel(), n_free.data_ptr(), lens_out.data_ptr(), n_free_out.data_ptr(),
+        plan.status.data_ptr(), plan.starts.data_ptr(), plan.slots.data_ptr(),
+        plan.positions.data_ptr(), plan.rows.data_ptr(), plan.visible.data_ptr(),
+        plan.max_tokens, _stream(stream)))
 
 
 def _pool_pages(k_pages, v_pages, page_size: int) -> int:
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        _need(t, name, _cache_dtype(t), 1)
+    """Pages that both pools hold."""
     if page_size <= 0:
         raise ValueError("page_size must be positive")
     return min(k_pages.numel(), v_pages.numel()) // (KV_HEADS * page_size * DIM)
@@ -735,25 +747,22 @@ def attn_prep_paged(qg, k, v, q_norm, k_norm, inv_freq, k_pages, v_pages, page_s
     ([n][16][256]) the gates are stored dense, as the batched decodes take them. The first rope_dims
     dimensions are rotated by position * inv_freq (float32, rope_dims / 2; rope_frequencies makes them),
     in pairs (i, i + rope_dims / 2) or neighbours (interleaved), cos and sin times rot_scale."""
-    f32 = torch.float32
-    n, proj_stride = _count(n, "n"), _count(proj_stride, "proj_stride")
-    for name, t, row in (("qg", qg, QG_STRIDE), ("k", k, KV_HEADS * DIM), ("v", v, KV_HEADS * DIM)):
-        _need(t.view(-1) if t.is_contiguous() else t, name, f32, (n - 1) * proj_stride + row if n else 0)
-    for name, t, m in (("q_norm", q_norm, DIM), ("k_norm", k_norm, DIM), ("q", q, n * Q_HEADS * DIM),
-                       ("inv_freq", inv_freq, _count(rope_dims, "rope_dims") // 2)):
-        _need(t, name, f32, m)
-    if gate is not None:
-        _need(gate, "gate", f32, n * Q_HEADS * DIM)
-    _need(slots, "slots", torch.int32, n)
-    _need(positions, "positions", torch.int32, n)
-    pages = _pool_pages(k_pages, v_pages, page_size)
-    _here(qg, k, v, q_norm, k_norm, inv_freq, k_pages, v_pages, slots, positions, q,
-          *(() if gate is None else (gate,)))
+    f32, int32, cache = torch.float32, torch.int32, _cache_dtype(k_pages)
+    rows = (_count(n, "n") - 1) * _count(proj_stride, "proj_stride") if n else -QG_STRIDE
+    heads = n * Q_HEADS * DIM
+    _need_all(("qg", qg, f32, rows + QG_STRIDE), ("k", k, f32, rows + KV_HEADS * DIM),
+              ("v", v, f32, rows + KV_HEADS * DIM), ("q_norm", q_norm, f32, DIM),
+              ("k_norm", k_norm, f32, DIM),
+              ("inv_freq", inv_freq, f32, _count(rope_dims, "rope_dims") // 2),
+              ("k_pages", k_pages, cache, 1), ("v_pages", v_pages, cache, 1),
+              ("slots", slots, int32, n), ("positions", positions, int32, n),
+              ("q", q, f32, heads), ("gate", q if gate is None else gate, f32, heads))
     _lib.check(_lib.load().miso_attn_prep_paged(
         qg.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
-        inv_freq.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page_size,
-        slots.data_ptr(), positions.data_ptr(), q.data_ptr(), _ptr(gate), n, proj_stride, rope_dims,
-        int(interleaved), rot_scale, eps, _stream(stream)))
+        inv_freq.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+        _pool_pages(k_pages, v_pages, page_size), page_size, slots.data_ptr(),
+        positions.data_ptr(), q.data_ptr(), None if gate is None else gate.data_ptr(), n,
+        proj_stride, rope_dims, int(interleaved), rot_scale, eps, _stream(stream)))
 
 
 class SharedScratch:
@@ -768,14 +777,10 @@ class SharedScratch:
         self.ws = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
 
 
-def _shared_args(q, gate, lens, core, scratch: SharedScratch, prefix: int) -> int:
+def _shared_batch(lens, scratch: SharedScratch, prefix: int) -> int:
     batch = lens.numel()
     if batch > scratch.batch or prefix > scratch.max_prefix:
         raise ValueError("the batch or the prefix exceeds the scratch capacity")
-    for name, t in (("q", q), ("gate", gate), ("core", core)):
-        _need(t, name, torch.float32, batch * Q_HEADS * DIM)
-    _need(lens, "lens", torch.int32, batch)
-    _here(q, gate, lens, core, scratch.ws)
     return batch
 
 
@@ -786,24 +791,25 @@ def attn_decode_paged_shared(q, gate, k_pages, v_pages, page_table, page_size: i
     keys are read once for all entries, the others from entries prefix_pages .. of table row rows[s]
     (None: row s; entries may share a row, as the tokens of a prompt's chunk do, each with its own
     lens). lens counts all keys of an entry; 0 gives core = 0."""
-    prefix_pages = _count(prefix_pages, "prefix_pages")
-    batch = _shared_args(q, gate, lens, core, scratch, prefix_pages * page_size)
+    prefix = _count(prefix_pages, "prefix_pages") * _count(page_size, "page_size")
+    batch = _shared_batch(lens, scratch, prefix)
     if page_table.dim() != 2 or (rows is None and page_table.shape[0] < batch):
         raise ValueError("page_table must be [rows][max_pages], a row per entry without `rows`")
-    max_pages = int(page_table.shape[1])
-    _need(page_table, "page_table", torch.int32, 1)
+    max_pages = page_table.shape[1]
+    f32, int32, cache = torch.float32, torch.int32, _cache_dtype(k_pages)
+    heads = batch * Q_HEADS * DIM
+    _need_all(("q", q, f32, heads), ("gate", gate, f32, heads), ("core", core, f32, heads),
+              ("k_pages", k_pages, cache, 1), ("v_pages", v_pages, cache, 1),
+              ("page_table", page_table, int32, 1), ("lens", lens, int32, batch),
+              ("scratch", scratch.ws, torch.uint8, 0))
     if prefix_pages:
-        _need(prefix_table, "prefix_table", torch.int32, prefix_pages)
+        _need_all(("prefix_table", prefix_table, int32, prefix_pages))
     if rows is not None:
-        _need(rows, "rows", torch.int32, batch)
-    _pool_pages(k_pages, v_pages, page_size)
-    _here(k_pages, v_pages, page_table,
-          *(t for t in (rows, prefix_table if prefix_pages else None) if t is not None))
+        _need_all(("rows", rows, int32, batch))
     _lib.check(_lib.load().miso_attn_decode_paged_shared(
         q.data_ptr(), gate.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-        page_table.data_ptr(), max_pages, _count(page_size, "page_size"), _ptr(rows),
-        lens.data_ptr(), batch,
-        min(scratch.max_own, max(0, (max_pages - prefix_pages) * page_size)),
+        page_table.data_ptr(), max_pages, page_size, None if rows is None else rows.data_ptr(),
+        lens.data_ptr(), batch, min(scratch.max_own, max(0, max_pages * page_size - prefix)),
         prefix_table.data_ptr() if prefix_pages else None, prefix_pages, core.data_ptr(),
         scratch.ws.data_ptr(), scratch.nbytes, _stream(stream)))
 
@@ -813,13 +819,14 @@ def attn_decode_ragged_shared(q, gate, k_cache, v_cache, kv_offsets, lens, k_pre
                               stream=None) -> None:
     """attn_decode_ragged of lens.numel() sequences behind a shared prefix, keys [0, prefix_len) of the
     cache k_prefix / v_prefix ([2][prefix_ctx][256]); lens and kv_offsets: their own keys, 0 or more."""
-    prefix_len, prefix_ctx = _count(prefix_len, "prefix_len"), _count(prefix_ctx, "prefix_ctx")
-    batch = _shared_args(q, gate, lens, core, scratch, prefix_len)
-    _need(kv_offsets, "kv_offsets", torch.int64, batch)
-    for name, t, rows in (("k_cache", k_cache, 0), ("v_cache", v_cache, 0),
-                          ("k_prefix", k_prefix, prefix_ctx), ("v_prefix", v_prefix, prefix_ctx)):
-        _need(t, name, _cache_dtype(t), KV_HEADS * rows * DIM)
-    _here(k_cache, v_cache, kv_offsets, k_prefix, v_prefix)
+    rows = KV_HEADS * _count(prefix_ctx, "prefix_ctx") * DIM
+    batch = _shared_batch(lens, scratch, _count(prefix_len, "prefix_len"))
+    f32, cache, heads = torch.float32, _cache_dtype(k_cache), batch * Q_HEADS * DIM
+    _need_all(("q", q, f32, heads), ("gate", gate, f32, heads), ("core", core, f32, heads),
+              ("k_cache", k_cache, cache, 0), ("v_cache", v_cache, cache, 0),
+              ("k_prefix", k_prefix, cache, rows), ("v_prefix", v_prefix, cache, rows),
+              ("kv_offsets", kv_offsets, torch.int64, batch), ("lens", lens, torch.int32, batch),
+              ("scratch", scratch.ws, torch.uint8, 0))
     _lib.check(_lib.load().miso_attn_decode_ragged_shared(
         q.data_ptr(), gate.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
         kv_offsets.data_ptr(), lens.data_ptr(), batch, scratch.max_own, k_prefix.data_ptr(),

@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <cstddef>
 #include <cstdint>
+#include <type_traits>
 
 #include "attention_decode.hpp"
 #include "attention_evict.hpp"
@@ -76,6 +77,69 @@ struct alignas(1024) PrefixShared {
 };
 static_assert(sizeof(PrefixShared) == 160 * 1024, "the CU's LDS");
 
+// S += A B for the lo halves of the queries, which lie in AGPRs beside O (64 and 128 registers; the hi
+// halves and the scores in VGPRs). These MFMAs and prefill_detail's are assembly, so that the compiler
+// keeps each block where it is (with the builtins it spilled 66 registers around 1670 moves). Back-to-back
+// accumulation into one register block chains in hardware. The compiler does not know their other wait
+// states, also where it copies a block by itself: they stand at the start and the end of each step.
+__device__ __attribute__((always_inline)) inline void score_lo(float16_t& s, const half8_t& a,
+                                                               const half8_t& b) {
+  asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "a"(b));
+}
+
+// o *= c element by element in the AGPRs, inside the caller's rare branch (attention_prefill.hpp's
+// scale_acc for fewer blocks). The no-ops cover the last MFMA's result.
+template <unsigned N>
+__device__ __attribute__((always_inline)) inline void scale_values(float16_t (&o)[N], float c) {
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+#pragma unroll
+  for (unsigned b = 0; b < N; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float x = o[b][r], tmp;
+      asm volatile(
+          "v_accvgpr_read_b32 %1, %0\n\t"
+          "v_mul_f32 %1, %1, %2\n\t"
+          "v_accvgpr_write_b32 %0, %1"
+          : "+a"(x), "=&v"(tmp)
+          : "v"(c));
+      o[b][r] = x;
+    }
+}
+
+// Four copies of copy_tile: rows 2 i + lane / 32 of the 8 at `row`, lane offsets `off` less 1024 i.
+__device__ __attribute__((always_inline)) inline void copy_rows(const attn::half_t* row,
+                                                                const unsigned (&off)[4],
+                                                                unsigned to) {
+  unsigned saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %6\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %5\n\t"
+      "global_load_lds_dwordx4 %2, %5 offset:1024\n\t"
+      "global_load_lds_dwordx4 %3, %5 offset:2048\n\t"
+      "global_load_lds_dwordx4 %4, %5 offset:3072\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(row), "s"(to)
+      : "memory");
+}
+
+// Wait states behind the last MFMA of O, tied to its registers: what the compiler copies of them, it
+// copies after these.
+template <unsigned N>
+__device__ __attribute__((always_inline)) inline void drain_values(float16_t (&o)[N]) {
+  if constexpr (N == 2)
+    asm volatile("s_nop 7\n\ts_nop 7" : "+a"(o[0]), "+a"(o[1]));
+  else if constexpr (N == 4)
+    asm volatile("s_nop 7\n\ts_nop 7" : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]));
+  else
+    asm volatile("s_nop 7\n\ts_nop 7"
+                 : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]), "+a"(o[4]), "+a"(o[5]),
+                   "+a"(o[6]), "+a"(o[7]));
+}
+
 // Keys of the prefix that a sequence sees.
 __device__ __attribute__((always_inline)) inline unsigned prefix_keys(const AttnSharedParams& p,
                                                                       unsigned seq) {
@@ -92,7 +156,7 @@ __device__ __attribute__((always_inline)) inline unsigned prefix_keys(const Attn
 // adds P V for its share of the 256 dimensions (all 8 blocks of 32 dimensions: 32 MFMAs). So a wave's
 // tile is 64, 48 or 40 MFMAs of 32 cycles for 4, 2 and 1 row blocks: with few rows the memory sets the
 // pace (32 KiB a tile and CU), with many the matrix units.
-template <unsigned kRowBlocks>
+template <unsigned kRowBlocks, bool kPaged>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
 attn_shared_prefix_kernel(AttnSharedParams p) {
   using namespace shared_detail;
@@ -102,66 +166,82 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
   __shared__ PrefixShared sh;
   const unsigned lane = threadIdx.x & 63u, col = lane & 31u, hi = lane >> 5;
   const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Row groups of one (span, KV head) on one XCD: its L2 serves them the same tiles.
+  // Workgroups go to the XCDs round robin: neighbours of the list (span, KV head, row group), whose
+  // row groups read the same tiles, on one XCD, so that its L2 serves them.
   const unsigned groups = (p.blocks + kRowBlocks - 1) / kRowBlocks;
-  const unsigned combo = blockIdx.x % 8 + 8 * (blockIdx.x / 8 / groups);
-  const unsigned group = blockIdx.x / 8 % groups;
+  const unsigned place = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+  const unsigned combo = place / groups, group = place % groups;
   if (combo >= 2 * p.spans)
     return;
   const unsigned kvh = combo % 2, span = combo / 2;
-  const unsigned t0 = span * p.span_tiles;
-  const unsigned t1 = min(t0 + p.span_tiles, (p.prefix.len + kKeys - 1) / kKeys);
+  const unsigned t0 = span * p.span_tiles, last = p.prefix.len - 1;
+  const unsigned t1 = min(t0 + p.span_tiles, last / kKeys + 1);
   const unsigned lds = cdna4::lds_offset(sh.ring);
   const unsigned local = wave / kParts, part = wave % kParts;
   const unsigned block = group * kRowBlocks + local;  // this wave's row block
   const bool active = block < p.blocks;               // wave-uniform
 
-  // ---- Tiles: this wave copies rows 8 wave .. + 7 of K and V.
+  // ---- Tiles: this wave copies rows 8 wave .. + 7 of K and V (instruction i rows 2 i + lane / 32 of
+  // them, chunks swizzled as attention_prefill.hpp's tiles). Rows past the prefix's last one repeat it
+  // (they are masked at use). The lane offsets are unsigned, and a repeated row lies up to 3072 bytes
+  // below its instruction's: offsets are that much larger, their base that much lower.
+  constexpr unsigned kBelow = 3072;
   unsigned koff[4], voff[4];
 #pragma unroll
   for (unsigned i = 0; i < 4; ++i) {
-    const unsigned row = 8 * wave + 2 * i + (lane >> 5), r = 2 * i + (lane >> 5);
-    koff[i] = r * 512 + 16 * prefill_detail::swz_k(row, lane & 31u) - 1024 * i;
-    voff[i] = r * 512 + 16 * prefill_detail::swz_v(row, lane & 31u) - 1024 * i;
+    const unsigned r = 2 * i + (lane >> 5);
+    koff[i] = kBelow + 512 * r + 16 * prefill_detail::swz_k(8 * wave + r, lane & 31u) - 1024 * i;
+    voff[i] = kBelow + 512 * r + 16 * prefill_detail::swz_v(8 * wave + r, lane & 31u) - 1024 * i;
   }
   int pages = 0;  // lane i: the page of this wave's rows of tile page0 + i
   unsigned page0 = t0 - 64;
-  auto row_at = [&](unsigned row) __attribute__((always_inline)) {  // in halves
-    if (p.prefix.table == nullptr)
-      return (std::size_t{kvh} * p.prefix.ctx + row) * attn::kDim;
-    const unsigned page =
-        static_cast<unsigned>(__builtin_amdgcn_readlane(pages, row / kKeys - page0));
-    return (((std::size_t{page} * attn::kKvHeads + kvh) << p.prefix.log2_page) +
-            (row & ((1u << p.prefix.log2_page) - 1u))) * attn::kDim;
+  struct Place {
+    const attn::half_t* k;
+    const attn::half_t* v;
+    unsigned most;  // the last of the 8 rows that exists
   };
-  auto issue = [&](unsigned ti) __attribute__((always_inline)) {
-    const unsigned slot = lds + (ti - t0 + kStages - 1) % kStages * kStageBytes + 4096 * wave;
-    const unsigned row = ti * kKeys + 8 * wave, last = p.prefix.len - 1;
-    if (p.prefix.table != nullptr && ti - page0 >= 64u) {  // uniform
-      page0 = ti;
-      const unsigned r = min((ti + lane) * kKeys + 8 * wave, last);
-      pages = p.prefix.table[r >> p.prefix.log2_page];
+  auto place_of = [&](unsigned ti) __attribute__((always_inline)) {
+    const unsigned want = ti * kKeys + 8 * wave, row = want < last ? want : last;
+    std::size_t at;  // of the row, in halves
+    if constexpr (kPaged) {
+      if (ti - page0 >= 64u) {  // uniform
+        page0 = ti;
+        const unsigned r = (ti + lane) * kKeys + 8 * wave;
+        pages = p.prefix.table[(r < last ? r : last) >> p.prefix.log2_page];
+      }
+      const unsigned page = decode_detail::lane_value(static_cast<unsigned>(pages), ti - page0);
+      at = (((std::size_t{page} * attn::kKvHeads + kvh) << p.prefix.log2_page) +
+            (row & ((1u << p.prefix.log2_page) - 1u))) * attn::kDim;
+    } else {
+      at = (std::size_t{kvh} * p.prefix.ctx + row) * attn::kDim;
     }
-    if (row + 7 <= last) {
-      const std::size_t at = row_at(row);
-      prefill_detail::copy_tile(decode_detail::uniform(p.prefix.k + at),
-                                decode_detail::uniform(p.prefix.v + at), koff, voff, slot,
-                                slot + kTileBytes);
-    } else {  // the prefix ends here: rows past its last one repeat it (masked at use)
-      const unsigned from = min(row, last);
-      const std::size_t at = row_at(from);
+    const std::size_t base = 2 * at - kBelow;  // in bytes
+    return Place{decode_detail::uniform(reinterpret_cast<const attn::half_t*>(
+                     reinterpret_cast<std::uintptr_t>(p.prefix.k) + base)),
+                 decode_detail::uniform(reinterpret_cast<const attn::half_t*>(
+                     reinterpret_cast<std::uintptr_t>(p.prefix.v) + base)),
+                 last - row};
+  };
+  auto copy = [&](const Place& from, unsigned to, bool is_v) __attribute__((always_inline)) {
+    unsigned off[4];
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i)
+      off[i] = is_v ? voff[i] : koff[i];
+    if (from.most < 7)  // uniform
 #pragma unroll
       for (unsigned i = 0; i < 4; ++i) {
-        const unsigned r = 2 * i + (lane >> 5), x = lane & 31u;
-        const std::size_t a = at + static_cast<std::size_t>(min(r, last - from)) * attn::kDim;
-        cdna4::lds_load16(p.prefix.k + a + 8 * prefill_detail::swz_k(8 * wave + r, x),
-                          slot + 1024 * i);
-        cdna4::lds_load16(p.prefix.v + a + 8 * prefill_detail::swz_v(8 * wave + r, x),
-                          slot + kTileBytes + 1024 * i);
+        const unsigned r = 2 * i + (lane >> 5);
+        off[i] -= 512 * (r > from.most ? r - from.most : 0);
       }
-    }
+    copy_rows(is_v ? from.v : from.k, off, to + 4096 * wave + (is_v ? kTileBytes : 0));
   };
-  issue(t0);  // into the last stage: the queries pass through the others
+  // Stages are named by their offset in the ring; tile t0 takes the last one.
+  auto issue = [&](unsigned ti, unsigned to) __attribute__((always_inline)) {
+    const Place from = place_of(ti);
+    copy(from, lds + to, false);
+    copy(from, lds + to, true);
+  };
+  issue(t0, (kStages - 1) * kStageBytes);  // the last stage: the queries pass through the others
 
   // ---- Queries: row r of a block is sequence 4 block + r / 8, head 8 kvh + r % 8. Each row times
   // log2(e) and a power of two of its own (its largest element near 2^14) is cut into f16 halves
@@ -220,9 +300,9 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
         lds + 32768 * kRowBlocks + 128 * local + 4 * col);
   __syncthreads();  // every wave has its operands: the ring takes the space
 #pragma unroll
-  for (unsigned i = 1; i < kStages - 1; ++i)
+  for (unsigned i = 1; i < 3; ++i)
     if (t0 + i < t1)
-      issue(t0 + i);
+      issue(t0 + i, (i - 1) * kStageBytes);
 
   // ---- Keys this lane's row sees, and whether every row of the wave sees the whole span.
   const unsigned seq = kSeqs * block + col / kGroup;
@@ -246,49 +326,53 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
   for (unsigned b = 0; b < kDimBlocks; ++b)
     o[b] = float16_t{};
   float m = kNoScore, l = 0.0f;
+  float16_t cur;       // the scores of a tile under way
+  float x[16];         // those of the tile before
+  half8_t a[4];        // the K operands of the next four k-steps
+  unsigned ph[8], pl[8];  // a tile's numerators, pairs of hi and of lo halves
+  float w[16];
+  // Stages: of the tile before the current one, the current, the next; of the copy under way.
+  unsigned before = 0, here = lds + (kStages - 1) * kStageBytes, after = lds,
+           spare = lds + 2 * kStageBytes;
+  auto rotate = [&]() __attribute__((always_inline)) {
+    before = here;
+    here = after;
+    after = after == lds + (kStages - 1) * kStageBytes ? lds : after + kStageBytes;
+    spare = spare == lds + (kStages - 1) * kStageBytes ? lds : spare + kStageBytes;
+  };
 
-  for (unsigned ti = t0; ti < t1; ++ti) {
-    // Tile ti has landed (this wave's share by the count, the others' by the barrier), and every wave
-    // is done with tile ti - 1, whose stage the next copy takes.
-    const unsigned behind = min(t1 - 1 - ti, kStages - 2);
-    if (behind >= 3)
-      cdna4::wait_vmcnt<24>();
-    else if (behind == 2)
-      cdna4::wait_vmcnt<16>();
-    else if (behind == 1)
+  // Tile ti + 1 has landed: this wave's copies by the count, every wave's by the barrier, which also
+  // says that every wave is done with tile ti - 2, whose stage the next copy takes.
+  auto turn = [&](unsigned ti) __attribute__((always_inline)) {
+    if (ti + 2 < t1)
       cdna4::wait_vmcnt<8>();
     else
       cdna4::wait_vmcnt<0>();
     decode_detail::tile_barrier();
-    if (ti + kStages - 1 < t1)
-      issue(ti + kStages - 1);
-    if (!active)
-      continue;
-    const unsigned slot = lds + (ti - t0 + kStages - 1) % kStages * kStageBytes;
-    float16_t s = {};
+  };
+  auto read = [&](unsigned base, unsigned k) __attribute__((always_inline)) {
+    return decode_detail::lds_b128((base + kb) ^ (32u * k));
+  };
+  auto mask = [&](unsigned ti) __attribute__((always_inline)) {
+    if (full)  // uniform
+      return;
 #pragma unroll
-    for (unsigned k = 0; k < kSteps; ++k) {
-      const half8_t a = decode_detail::lds_b128((slot + kb) ^ (32u * k));
-      s = mfma32(a, qh[k], s);
-      s = mfma32(a, ql[k], s);
-    }
-    float x[16];
-#pragma unroll
-    for (unsigned i = 0; i < 16; ++i) {
-      x[i] = s[i];
-      if (!full)  // uniform
-        x[i] = ti * kKeys + weights_detail::tile_row(lane, i) < sees ? x[i] : -__builtin_inff();
-    }
-    float w[16], sum = 0.0f;
-    auto numerators = [&]() __attribute__((always_inline)) {
-      sum = 0.0f;
-#pragma unroll
-      for (unsigned i = 0; i < 16; ++i) {
-        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], scale, -m));
-        sum += w[i];
-      }
-    };
-    numerators();
+    for (unsigned i = 0; i < 16; ++i)
+      x[i] = ti * kKeys + weights_detail::tile_row(lane, i) < sees ? x[i] : -__builtin_inff();
+  };
+  // Numerators i, i + 1 as halves: hi rounded towards zero, lo what is left (2^-21 of the numerator, or
+  // 2^-25). Pinned: the compiler would move them below the MFMAs that they stand between.
+  auto pair = [&](unsigned i) __attribute__((always_inline)) {
+    const cdna4::half2_t h = __builtin_bit_cast(cdna4::half2_t,
+                                                __builtin_amdgcn_cvt_pkrtz(w[i], w[i + 1]));
+    const cdna4::half2_t r = {static_cast<_Float16>(w[i] - static_cast<float>(h[0])),
+                              static_cast<_Float16>(w[i + 1] - static_cast<float>(h[1]))};
+    ph[i / 2] = cdna4::as_uint(h);
+    pl[i / 2] = cdna4::as_uint(r);
+    asm volatile("" : "+v"(ph[i / 2]), "+v"(pl[i / 2]));
+  };
+  // After a tile's numerators w (their sum given): the reference follows where they are too large.
+  auto settle = [&](float sum) __attribute__((always_inline)) {
     if (__builtin_amdgcn_ballot_w64(sum > kMost) != 0) {  // rare, and the first tile
       float top = x[0];
 #pragma unroll
@@ -298,38 +382,160 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
       const float corr = __builtin_amdgcn_exp2f(m - top);
       m = top;
       l *= corr;
+      scale_values(o, corr);
+      sum = 0.0f;
 #pragma unroll
-      for (unsigned b = 0; b < kDimBlocks; ++b)
-        o[b] *= corr;
-      numerators();
+      for (unsigned i = 0; i < 16; ++i) {
+        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], scale, -m));
+        sum += w[i];
+      }
+#pragma unroll
+      for (unsigned i = 0; i < 16; i += 2)
+        pair(i);
     }
     l += sum;
-    half8_t ph[2], pl[2];
+  };
+  // O += P V of the tile in stage `base`. Dimension block part kDimBlocks + d of 8: 64 bytes (block
+  // % 4) by the XOR, 256 (block / 4) further.
+  auto values = [&](unsigned base, unsigned i) __attribute__((always_inline)) {
+    const unsigned step = i / kDimBlocks, d = i % kDimBlocks;
+    const unsigned upper = kParts == 4 ? part >> 1 : kParts == 2 ? part : d / 4;
+    const unsigned v = kParts == 4 ? vb[0] ^ (64u * (d + 2 * (part & 1u))) : vb[d % 4];
+    const unsigned at = base + kTileBytes + v + 256u * upper + 8192u * step;
+    const cdna4::half4_t lo = prefill_detail::read_tr(at);
+    const cdna4::half4_t up = prefill_detail::read_tr(upper ? at + 4096u - 256u
+                                                            : at + 4096u + 256u);
+    return half8_t{lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
+  };
+  constexpr unsigned kValues = 2 * kDimBlocks, kAhead = kValues < 4 ? kValues : 4;
+  half8_t va[kAhead];
+  auto add_values = [&](unsigned base, bool more) __attribute__((always_inline)) {
+    half8_t bh[2], bl[2];
+#pragma unroll
+    for (unsigned i = 0; i < 2; ++i) {
+      bh[i] = __builtin_bit_cast(half8_t, cdna4::u32x4_t{ph[4 * i], ph[4 * i + 1], ph[4 * i + 2],
+                                                         ph[4 * i + 3]});
+      bl[i] = __builtin_bit_cast(half8_t, cdna4::u32x4_t{pl[4 * i], pl[4 * i + 1], pl[4 * i + 2],
+                                                         pl[4 * i + 3]});
+    }
+    asm volatile("s_nop 4" : "+v"(bh[0]), "+v"(bh[1]), "+v"(bl[0]), "+v"(bl[1]));  // VALU to MFMA
+#pragma unroll
+    for (unsigned i = 0; i < kValues; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      const unsigned step = i / kDimBlocks, d = i % kDimBlocks;
+      half8_t next = va[i % kAhead];
+      if (i + kAhead < kValues)
+        next = values(base, i + kAhead);
+      prefill_detail::pv_mfma(o[d], va[i % kAhead], bh[step]);
+      if (more && i != 0)  // the next tile's scores, done since the first MFMA above
+#pragma unroll
+        for (unsigned j = (i - 1) * 16 / (kValues - 1); j < i * 16 / (kValues - 1); ++j) {
+          x[j] = cur[j];
+          asm volatile("" : "+v"(x[j]));
+        }
+      prefill_detail::pv_mfma(o[d], va[i % kAhead], bl[step]);
+      va[i % kAhead] = next;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    drain_values(o);
+  };
+  turn(t0);
+  if (t0 + 3 < t1)
+    issue(t0 + 3, 2 * kStageBytes);
+  if (!active) {
+    for (unsigned ti = t0 + 1; ti < t1; ++ti) {
+      rotate();
+      turn(ti);
+      if (ti + 3 < t1)
+        issue(ti + 3, spare - lds);
+    }
+    return;
+  }
+#pragma unroll
+  for (unsigned k = 0; k < 4; ++k)
+    a[k] = read(here, k);
+  asm volatile("s_nop 4" ::: "memory");
+#pragma unroll
+  for (unsigned k = 0; k < kSteps; ++k) {
+    const half8_t next = k + 4 < kSteps ? read(here, k + 4) : read(after, k + 4 - kSteps);
+    if (k == 0)
+      prefill_detail::s_mfma_first(cur, a[0], qh[0]);
+    else
+      prefill_detail::s_mfma(cur, a[k % 4], qh[k]);
+    score_lo(cur, a[k % 4], ql[k]);
+    a[k % 4] = next;
+  }
+  prefill_detail::drain_scores(cur);
+#pragma unroll
+  for (unsigned i = 0; i < 16; ++i)
+    x[i] = cur[i];
+
+  // Step ti: the scores of tile ti into cur, beside them the numerators of tile ti - 1 (x), then its
+  // P V. Between two score MFMAs stand one fma, one exponential, one sum and half a pair of neighbouring
+  // numerators, so that none waits for another; the copy of tile ti + 3 goes behind the first ones.
+  for (unsigned ti = t0 + 1; ti < t1; ++ti) {
+    turn(ti);
+    rotate();
+    mask(ti - 1);
+    asm volatile("s_nop 4" ::: "memory");
+    Place from{};
+    const bool more = ti + 3 < t1;  // uniform
+    float sum[2] = {0.0f, 0.0f}, x1 = 0.0f;
+#pragma unroll
+    for (unsigned k = 0; k < kSteps; ++k) {
+      __builtin_amdgcn_sched_barrier(0);
+      const half8_t next = k + 4 < kSteps ? read(here, k + 4) : read(after, k + 4 - kSteps);
+      if (k == 0)
+        prefill_detail::s_mfma_first(cur, a[0], qh[0]);
+      else
+        prefill_detail::s_mfma(cur, a[k % 4], qh[k]);
+      const float x0 = __builtin_fmaf(x[k], scale, -m);
+      if (k > 0)
+        w[k - 1] = __builtin_amdgcn_exp2f(x1);
+      score_lo(cur, a[k % 4], ql[k]);
+      if (k > 1)
+        sum[k % 2] += w[k - 2];
+      if (k > 3 && k % 2 == 0)
+        pair(k - 4);
+      a[k % 4] = next;
+      x1 = x0;
+      if (more) {
+        if (k == 0)
+          from = place_of(ti + 3);
+        if (k == 1)
+          copy(from, spare, false);
+        if (k == 2)
+          copy(from, spare, true);
+      }
+      if (k + kAhead >= kSteps)
+        va[k + kAhead - kSteps] = values(before, k + kAhead - kSteps);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    w[15] = __builtin_amdgcn_exp2f(x1);
+    sum[0] += w[14];
+    sum[1] += w[15];
+    pair(12);
+    pair(14);
+    settle(sum[0] + sum[1]);
+    add_values(before, true);
+  }
+  {  // the last tile
+    mask(t1 - 1);
+    float sum = 0.0f;
 #pragma unroll
     for (unsigned i = 0; i < 16; ++i) {
-      const _Float16 h = static_cast<_Float16>(w[i]);
-      ph[i / 8][i % 8] = h;
-      pl[i / 8][i % 8] = static_cast<_Float16>(w[i] - static_cast<float>(h));
+      w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], scale, -m));
+      sum += w[i];
     }
 #pragma unroll
-    for (unsigned step = 0; step < 2; ++step)
+    for (unsigned i = 0; i < 16; i += 2)
+      pair(i);
+    settle(sum);
 #pragma unroll
-      for (unsigned d = 0; d < kDimBlocks; ++d) {
-        // Dimension block part kDimBlocks + d: 64 (block % 4) by the XOR, 256 (block / 4) bytes.
-        const unsigned b = kParts == 4 ? d + 2 * (part & 1u) : d % 4;
-        const unsigned upper = kParts == 4 ? part >> 1 : kParts == 2 ? part : d / 4;
-        const unsigned at = slot + kTileBytes + (kParts == 4 ? vb[0] ^ (64u * b) : vb[d % 4]) +
-                            256u * upper + 8192u * step;
-        const cdna4::half4_t lo = prefill_detail::read_tr(at);
-        const cdna4::half4_t up = prefill_detail::read_tr(upper ? at + 4096u - 256u
-                                                                : at + 4096u + 256u);
-        const half8_t a = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
-        o[d] = mfma32(a, ph[step], o[d]);
-        o[d] = mfma32(a, pl[step], o[d]);
-      }
+    for (unsigned i = 0; i < kAhead; ++i)
+      va[i] = values(here, i);
+    add_values(here, false);
   }
-  if (!active)
-    return;
   // ---- The partial, relative to 2^m, in the accumulators' order (whole 1 KiB a store).
   const std::size_t at = (std::size_t{span} * attn::kKvHeads + kvh) * p.blocks + block;
   float4* out = p.part_o + (at * 8 + part * kDimBlocks) * 256 + lane;
@@ -590,13 +796,20 @@ inline void attn_shared_launch(AttnSharedParams p, const AttnSharedOwn& own, uns
   p.blocks = cut.blocks;
   if (cut.spans != 0) {
     const unsigned rb = attn_shared_row_blocks(p.batch), groups = (cut.blocks + rb - 1) / rb;
-    const unsigned grid = 8 * ((2 * cut.spans + 7) / 8) * groups;
-    if (rb == 1)
-      attn_shared_prefix_kernel<1><<<grid, 256, 0, stream>>>(p);
-    else if (rb == 2)
-      attn_shared_prefix_kernel<2><<<grid, 256, 0, stream>>>(p);
+    const unsigned grid = 8 * ((2 * cut.spans * groups + 7) / 8);
+    const auto launch = [&](auto paged) {
+      constexpr bool kPaged = decltype(paged)::value;
+      if (rb == 1)
+        attn_shared_prefix_kernel<1, kPaged><<<grid, 256, 0, stream>>>(p);
+      else if (rb == 2)
+        attn_shared_prefix_kernel<2, kPaged><<<grid, 256, 0, stream>>>(p);
+      else
+        attn_shared_prefix_kernel<4, kPaged><<<grid, 256, 0, stream>>>(p);
+    };
+    if (p.prefix.table != nullptr)
+      launch(std::true_type{});
     else
-      attn_shared_prefix_kernel<4><<<grid, 256, 0, stream>>>(p);
+      launch(std::false_type{});
   }
   if (max_own != 0) {
     // At most one streaming launch's sequences and items at a time.

@@ -182,6 +182,17 @@ def test_scratch_serves_smaller_calls(torch_mod, attn):
         check(torch_mod, c.run(attn, sc), c.ref(), (batch, pp, own))
 
 
+@pytest.mark.parametrize("batch", [2, 7, 16, 17])
+@pytest.mark.parametrize("tiles", [1, 2, 3, 4, 5, 6, 7, 12])
+def test_every_count_of_tiles_in_a_span(torch_mod, attn, batch, tiles):
+    """The streaming loop's start, ring and end, by one, two and four row blocks a workgroup (128 spans,
+    64 for 17 entries), the last span shorter."""
+    keys = tiles * 32 * (128 if batch <= 16 else 64) - 24
+    c = Paged(torch_mod, 8, keys // 8, [keys + 1 if e % 3 else keys - 5 * e for e in range(batch)],
+              tiles)
+    check(torch_mod, c.run(attn), c.ref())
+
+
 def test_spans_longer_than_the_page_ids_a_wave_holds(torch_mod, attn):
     """More than 64 tiles a span: its pages are read again, and tiles wrap the ring many times."""
     lens = 90112 + np.arange(30) % 7
