@@ -2902,15 +2902,16 @@ __device__ __attribute__((always_inline)) inline unsigned stream_length(const Sr
 }
 
 // The streaming split over the batch's items (attn_ragged_stream_kernel's description), with
-// the tiles where Src says they are.
+// the tiles where Src says they are, by the launch's workgroups from `first` on.
 template <class Src>
 __device__ __attribute__((always_inline)) inline void stream_items(const StreamBatch& p, Src& src,
-                                                                  StreamShared& sh) {
+                                                                  StreamShared& sh,
+                                                                  unsigned first = 0) {
   using cdna4::half8_t;
   constexpr unsigned kBlock = 256;
   const unsigned t = threadIdx.x, lane = t & 63u;
   const unsigned wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const unsigned G = gridDim.x, w = blockIdx.x;
+  const unsigned G = gridDim.x - first, w = blockIdx.x - first;
   StreamLists& ls = *reinterpret_cast<StreamLists*>(sh.merge);
 
   // Sequence starts of the item list, by wave 0. In a balanced launch wave 1 chooses the span

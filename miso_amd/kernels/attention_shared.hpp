@@ -4,9 +4,9 @@
 // counterpart (the reference is batch-1). The ragged and paged decodes (attention_decode.hpp) read the
 // prefix once per sequence: 64 sequences behind 32768 keys stream 4.3 GB. Here the queries of all
 // sequences meet the prefix's keys together, so that K and V are read once per 16 sequences:
-//   attn_shared_prefix_kernel: partials of 8 query rows per sequence and KV head over spans of the prefix
-//   attn_shared_own_kernel:    the streaming split over each sequence's own keys behind it
-//   attn_shared_merge_kernel:  both partials joined, the gate applied
+//   attn_shared_split_kernel: partials of 8 query rows per sequence and KV head over spans of the prefix,
+//                             and the streaming split over each sequence's own keys behind it
+//   attn_shared_merge_kernel: both partials joined, the gate applied
 // Precision is the decodes': every f32 operand (queries, numerators) enters the matrix units as a pair
 // of f16, sums are f32.
 
@@ -52,6 +52,7 @@ struct AttnSharedParams {
   float* own_o;
   unsigned s_max, chunk, own_cap;  // s_max 0: nobody has own keys
   unsigned* balanced;
+  unsigned prefix_grid, own_batch;  // of a split launch
 };
 
 namespace shared_detail {
@@ -140,6 +141,37 @@ __device__ __attribute__((always_inline)) inline void drain_values(float16_t (&o
                    "+a"(o[6]), "+a"(o[7]));
 }
 
+// Wait states between the queries' way into their registers and the first MFMA that reads them.
+__device__ __attribute__((always_inline)) inline void settle_operands(half8_t (&h)[kSteps],
+                                                                      half8_t (&l)[kSteps]) {
+  static_assert(kSteps == 16);
+#pragma unroll
+  for (unsigned i = 0; i < kSteps; i += 8) {
+    asm volatile("s_nop 4"
+                 : "+v"(h[i]), "+v"(h[i + 1]), "+v"(h[i + 2]), "+v"(h[i + 3]), "+v"(h[i + 4]),
+                   "+v"(h[i + 5]), "+v"(h[i + 6]), "+v"(h[i + 7]));
+    asm volatile("s_nop 4"
+                 : "+a"(l[i]), "+a"(l[i + 1]), "+a"(l[i + 2]), "+a"(l[i + 3]), "+a"(l[i + 4]),
+                   "+a"(l[i + 5]), "+a"(l[i + 6]), "+a"(l[i + 7]));
+  }
+}
+
+// Two numerators as halves: hi rounded towards zero, lo what is left (2^-21 of the numerator, or 2^-25).
+// Volatile: the compiler would move them below the MFMAs that they stand between. The no-op: the
+// numerators come from exponentials, whose results need a wait state.
+__device__ __attribute__((always_inline)) inline void numerator_pair(float a, float b, unsigned& h,
+                                                                     unsigned& l) {
+  float rest;
+  asm volatile(
+      "s_nop 0\n\t"
+      "v_cvt_pkrtz_f16_f32 %0, %3, %4\n\t"
+      "v_fma_mix_f32 %1, %0, -1.0, %3 op_sel_hi:[1,0,0]\n\t"
+      "v_fma_mix_f32 %2, %0, -1.0, %4 op_sel:[1,0,0] op_sel_hi:[1,0,0]\n\t"
+      "v_cvt_pk_f16_f32 %1, %1, %2"
+      : "=&v"(h), "=&v"(l), "=&v"(rest)
+      : "v"(a), "v"(b));
+}
+
 // Keys of the prefix that a sequence sees.
 __device__ __attribute__((always_inline)) inline unsigned prefix_keys(const AttnSharedParams& p,
                                                                       unsigned seq) {
@@ -156,20 +188,19 @@ __device__ __attribute__((always_inline)) inline unsigned prefix_keys(const Attn
 // adds P V for its share of the 256 dimensions (all 8 blocks of 32 dimensions: 32 MFMAs). So a wave's
 // tile is 64, 48 or 40 MFMAs of 32 cycles for 4, 2 and 1 row blocks: with few rows the memory sets the
 // pace (32 KiB a tile and CU), with many the matrix units.
+namespace shared_detail {
 template <unsigned kRowBlocks, bool kPaged>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
-attn_shared_prefix_kernel(AttnSharedParams p) {
-  using namespace shared_detail;
+__device__ __attribute__((always_inline)) inline void prefix_span(const AttnSharedParams& p,
+                                                                 PrefixShared& sh) {
   constexpr unsigned kParts = 4 / kRowBlocks;       // waves of a row block
   constexpr unsigned kDimBlocks = 8 / kParts;       // of 32 dimensions, per wave
   constexpr unsigned kStageRows = 32 / kParts;      // query rows that a wave lays out
-  __shared__ PrefixShared sh;
   const unsigned lane = threadIdx.x & 63u, col = lane & 31u, hi = lane >> 5;
   const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups go to the XCDs round robin: neighbours of the list (span, KV head, row group), whose
   // row groups read the same tiles, on one XCD, so that its L2 serves them.
   const unsigned groups = (p.blocks + kRowBlocks - 1) / kRowBlocks;
-  const unsigned place = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+  const unsigned place = blockIdx.x % 8 * (p.prefix_grid / 8) + blockIdx.x / 8;
   const unsigned combo = place / groups, group = place % groups;
   if (combo >= 2 * p.spans)
     return;
@@ -208,6 +239,8 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
         page0 = ti;
         const unsigned r = (ti + lane) * kKeys + 8 * wave;
         pages = p.prefix.table[(r < last ? r : last) >> p.prefix.log2_page];
+        // Here and not where the paths meet: there it would wait for the copies under way in every step.
+        __builtin_amdgcn_s_waitcnt(weights_detail::kVmcnt0);
       }
       const unsigned page = decode_detail::lane_value(static_cast<unsigned>(pages), ti - page0);
       at = (((std::size_t{page} * attn::kKvHeads + kvh) << p.prefix.log2_page) +
@@ -241,68 +274,76 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
     copy(from, lds + to, false);
     copy(from, lds + to, true);
   };
-  issue(t0, (kStages - 1) * kStageBytes);  // the last stage: the queries pass through the others
-
-  // ---- Queries: row r of a block is sequence 4 block + r / 8, head 8 kvh + r % 8. Each row times
-  // log2(e) and a power of two of its own (its largest element near 2^14) is cut into f16 halves
-  // hi + lo (2^-22 of an element, 2^-38 of the row's largest), laid out in LDS (512-byte rows, chunk c
-  // of row r at c ^ (r % 16)) and read back as B operands.
+  // ---- Queries: row r of a block is sequence 4 block + r / 8, head 8 kvh + r % 8. The waves of a block
+  // copy its rows to LDS (1 KiB each, 16-byte chunk c of row r at c ^ (r % 16)) and every lane reads the
+  // 128 dimensions of its row that its B operands hold. Times log2(e) and a power of two of the row's own
+  // (its largest element near 2^13) they are cut into f16 halves hi + lo (2^-21 of an element, 2^-38 of
+  // the row's largest).
+  // They pass through the stages that the first tiles leave: with four row blocks all but the first's.
+  const unsigned area = lds + 32768 * (4 - kRowBlocks + local);
+  constexpr unsigned kEarly = kRowBlocks == 4 ? 1 : 3;  // tiles under way meanwhile
+#pragma unroll
+  for (unsigned i = 0; i < kStageRows; ++i) {
+    const unsigned r = kStageRows * part + i, seq = min(kSeqs * block + r / kGroup, p.batch - 1);
+    cdna4::lds_load16(p.q + (std::size_t{seq} * attn::kQHeads + kvh * kGroup + r % kGroup) *
+                                attn::kDim + 4 * (lane ^ (r & 15u)),
+                      area + 1024 * r);
+  }
+  // Tile t0 takes the last stage, the next ones those from the first on.
+  issue(t0, (kStages - 1) * kStageBytes);
+  if (kEarly > 1 && t0 + 1 < t1)
+    issue(t0 + 1, 0);
+  if (kEarly > 2 && t0 + 2 < t1)
+    issue(t0 + 2, kStageBytes);
+  if (kEarly > 2 && t0 + 2 < t1)
+    cdna4::wait_vmcnt<24>();
+  else if (kEarly > 1 && t0 + 1 < t1)
+    cdna4::wait_vmcnt<16>();
+  else
+    cdna4::wait_vmcnt<8>();
+  decode_detail::tile_barrier();
   half8_t qh[kSteps], ql[kSteps];
-  float scale = 1.0f;  // of the scores of this lane's row
-  const unsigned area = lds + 32768 * local;
+  float scale;  // of the scores of this lane's row
   {
-    float4 x[kStageRows];
+    const unsigned at = area + 1024 * col + 16 * ((2 * hi) ^ (col & 15u));
+    cdna4::float4_t v[2 * kSteps];
 #pragma unroll
-    for (unsigned i = 0; i < kStageRows; ++i) {
-      const unsigned r = kStageRows * part + i, seq = min(kSeqs * block + r / kGroup, p.batch - 1);
-      x[i] = *reinterpret_cast<const float4*>(
-          p.q + (std::size_t{seq} * attn::kQHeads + kvh * kGroup + r % kGroup) * attn::kDim +
-          4 * lane);
-    }
+    for (unsigned c = 0; c < 2 * kSteps; ++c)
+      v[c] = *reinterpret_cast<const __attribute__((address_space(3))) cdna4::float4_t*>(
+          at ^ (64u * (c / 2) + 16u * (c % 2)));
+    float top = 0.0f;
 #pragma unroll
-    for (unsigned i = 0; i < kStageRows; ++i) {
-      const unsigned r = kStageRows * part + i;
-      const float top = cdna4::wave_allmax(fmaxf(fmaxf(__builtin_fabsf(x[i].x), __builtin_fabsf(x[i].y)),
-                                                 fmaxf(__builtin_fabsf(x[i].z), __builtin_fabsf(x[i].w))));
-      int e = 13 - (static_cast<int>(cdna4::as_uint(top) >> 23) - 127);
-      e = top == 0.0f || !(top < __builtin_inff()) ? 0 : (e < 100 ? e : 100);
-      const float up = __builtin_ldexpf(1.0f, e);
-      const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      cdna4::half4_t h, l;
+    for (unsigned c = 0; c < 2 * kSteps; ++c)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float y = v[j] * up * decode_detail::kLog2e;
-        asm("" : "+v"(y));  // one rounding for both halves
-        h[j] = static_cast<_Float16>(y);
-        l[j] = static_cast<_Float16>(y - static_cast<float>(h[j]));
+      for (int j = 0; j < 4; ++j)
+        top = fmaxf(top, __builtin_fabsf(v[c][j]));
+    top = cdna4::max_xor32(top);
+    int e = 13 - (static_cast<int>(cdna4::as_uint(top) >> 23) - 127);
+    e = top == 0.0f || !(top < __builtin_inff()) ? 0 : (e < 100 ? e : 100);
+    const float up = __builtin_ldexpf(1.0f, e);
+    scale = __builtin_ldexpf(1.0f / 16.0f, -e);
+#pragma unroll
+    for (unsigned c = 0; c < 2 * kSteps; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        const float y0 = v[c][j] * up * decode_detail::kLog2e;
+        const float y1 = v[c][j + 1] * up * decode_detail::kLog2e;
+        const cdna4::half2_t h =
+            __builtin_bit_cast(cdna4::half2_t, __builtin_amdgcn_cvt_pkrtz(y0, y1));
+        const unsigned k = 4 * (c % 2) + j;
+        qh[c / 2][k] = h[0];
+        qh[c / 2][k + 1] = h[1];
+        ql[c / 2][k] = static_cast<_Float16>(y0 - static_cast<float>(h[0]));
+        ql[c / 2][k + 1] = static_cast<_Float16>(y1 - static_cast<float>(h[1]));
       }
-      const unsigned at = area + 512 * r + 16 * ((lane / 2) ^ (r & 15u)) + 8 * (lane & 1u);
-      *reinterpret_cast<__attribute__((address_space(3))) cdna4::half4_t*>(at) = h;
-      *reinterpret_cast<__attribute__((address_space(3))) cdna4::half4_t*>(at + 16384) = l;
-      const float down = __builtin_ldexpf(1.0f / 16.0f, -e);
-      if constexpr (kParts == 1) {
-        scale = col == r ? down : scale;
-      } else if (lane == 0) {
-        *reinterpret_cast<__attribute__((address_space(3))) float*>(lds + 32768 * kRowBlocks +
-                                                                    128 * local + 4 * r) = down;
-      }
-    }
   }
-  __syncthreads();
+  if constexpr (kEarly == 1) {
+    decode_detail::tile_barrier();  // every wave has its operands: the ring takes the space
 #pragma unroll
-  for (unsigned s = 0; s < kSteps; ++s) {
-    const unsigned at = area + 512 * col + 16 * ((2 * s + hi) ^ (col & 15u));
-    qh[s] = decode_detail::lds_b128(at);
-    ql[s] = decode_detail::lds_b128(at + 16384);
+    for (unsigned i = 1; i < 3; ++i)
+      if (t0 + i < t1)
+        issue(t0 + i, (i - 1) * kStageBytes);
   }
-  if constexpr (kParts != 1)
-    scale = *reinterpret_cast<const __attribute__((address_space(3))) float*>(
-        lds + 32768 * kRowBlocks + 128 * local + 4 * col);
-  __syncthreads();  // every wave has its operands: the ring takes the space
-#pragma unroll
-  for (unsigned i = 1; i < 3; ++i)
-    if (t0 + i < t1)
-      issue(t0 + i, (i - 1) * kStageBytes);
 
   // ---- Keys this lane's row sees, and whether every row of the wave sees the whole span.
   const unsigned seq = kSeqs * block + col / kGroup;
@@ -326,11 +367,12 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
   for (unsigned b = 0; b < kDimBlocks; ++b)
     o[b] = float16_t{};
   float m = kNoScore, l = 0.0f;
-  float16_t cur;       // the scores of a tile under way
-  float x[16];         // those of the tile before
-  half8_t a[4];        // the K operands of the next four k-steps
-  unsigned ph[8], pl[8];  // a tile's numerators, pairs of hi and of lo halves
-  float w[16];
+  float16_t cur;  // the scores of a tile under way
+  float x[16];    // those of the tile before
+  float w[16];    // its numerators
+  half8_t a[4];   // the K operands of the next four k-steps
+  half8_t va[4];  // the V operands of the next four products
+  unsigned ka[8];  // where the current tile's K operands k and k + 8 (256 bytes on) lie
   // Stages: of the tile before the current one, the current, the next; of the copy under way.
   unsigned before = 0, here = lds + (kStages - 1) * kStageBytes, after = lds,
            spare = lds + 2 * kStageBytes;
@@ -340,18 +382,36 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
     after = after == lds + (kStages - 1) * kStageBytes ? lds : after + kStageBytes;
     spare = spare == lds + (kStages - 1) * kStageBytes ? lds : spare + kStageBytes;
   };
-
-  // Tile ti + 1 has landed: this wave's copies by the count, every wave's by the barrier, which also
-  // says that every wave is done with tile ti - 2, whose stage the next copy takes.
+  // Tile ti has landed: this wave's copies by the count (two tiles more are under way), every wave's by
+  // the barrier, which also says that every wave has read tile ti - 2, whose stage the next copy takes.
   auto turn = [&](unsigned ti) __attribute__((always_inline)) {
-    if (ti + 2 < t1)
+    const unsigned behind = t1 - 1 - ti;
+    if (behind >= 2)
+      cdna4::wait_vmcnt<16>();
+    else if (behind == 1)
       cdna4::wait_vmcnt<8>();
     else
       cdna4::wait_vmcnt<0>();
     decode_detail::tile_barrier();
   };
-  auto read = [&](unsigned base, unsigned k) __attribute__((always_inline)) {
-    return decode_detail::lds_b128((base + kb) ^ (32u * k));
+  auto first_operands = [&](unsigned base) __attribute__((always_inline)) {
+#pragma unroll
+    for (unsigned k = 0; k < 8; ++k)
+      ka[k] = (base + kb) ^ (32u * k);
+#pragma unroll
+    for (unsigned k = 0; k < 4; ++k)
+      a[k] = decode_detail::lds_b128(ka[k]);
+  };
+  // Two score MFMAs of k-step k, and the operand four steps on.
+  auto score_hi = [&](unsigned k) __attribute__((always_inline)) {
+    if (k == 0)
+      prefill_detail::s_mfma_first(cur, a[0], qh[0]);
+    else
+      prefill_detail::s_mfma(cur, a[k % 4], qh[k]);
+  };
+  auto operand = [&](unsigned k) __attribute__((always_inline)) {
+    return k + 4 < kSteps ? decode_detail::lds_b128(ka[(k + 4) % 8] + 256u * ((k + 4) / 8))
+                          : a[k % 4];
   };
   auto mask = [&](unsigned ti) __attribute__((always_inline)) {
     if (full)  // uniform
@@ -360,16 +420,9 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
     for (unsigned i = 0; i < 16; ++i)
       x[i] = ti * kKeys + weights_detail::tile_row(lane, i) < sees ? x[i] : -__builtin_inff();
   };
-  // Numerators i, i + 1 as halves: hi rounded towards zero, lo what is left (2^-21 of the numerator, or
-  // 2^-25). Pinned: the compiler would move them below the MFMAs that they stand between.
+  unsigned ph[8], pl[8];  // pairs of numerators, hi and lo halves
   auto pair = [&](unsigned i) __attribute__((always_inline)) {
-    const cdna4::half2_t h = __builtin_bit_cast(cdna4::half2_t,
-                                                __builtin_amdgcn_cvt_pkrtz(w[i], w[i + 1]));
-    const cdna4::half2_t r = {static_cast<_Float16>(w[i] - static_cast<float>(h[0])),
-                              static_cast<_Float16>(w[i + 1] - static_cast<float>(h[1]))};
-    ph[i / 2] = cdna4::as_uint(h);
-    pl[i / 2] = cdna4::as_uint(r);
-    asm volatile("" : "+v"(ph[i / 2]), "+v"(pl[i / 2]));
+    numerator_pair(w[i], w[i + 1], ph[i / 2], pl[i / 2]);
   };
   // After a tile's numerators w (their sum given): the reference follows where they are too large.
   auto settle = [&](float sum) __attribute__((always_inline)) {
@@ -390,13 +443,13 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
         sum += w[i];
       }
 #pragma unroll
-      for (unsigned i = 0; i < 16; i += 2)
+      for (unsigned i = 0; i < 8; i += 2)
         pair(i);
     }
     l += sum;
   };
-  // O += P V of the tile in stage `base`. Dimension block part kDimBlocks + d of 8: 64 bytes (block
-  // % 4) by the XOR, 256 (block / 4) further.
+  // V operand i of the tile in stage `base`: key step i / kDimBlocks, dimension block part kDimBlocks + d
+  // of 8: 64 bytes (block % 4) by the XOR, 256 (block / 4) further.
   auto values = [&](unsigned base, unsigned i) __attribute__((always_inline)) {
     const unsigned step = i / kDimBlocks, d = i % kDimBlocks;
     const unsigned upper = kParts == 4 ? part >> 1 : kParts == 2 ? part : d / 4;
@@ -407,38 +460,42 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
                                                             : at + 4096u + 256u);
     return half8_t{lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
   };
-  constexpr unsigned kValues = 2 * kDimBlocks, kAhead = kValues < 4 ? kValues : 4;
-  half8_t va[kAhead];
-  auto add_values = [&](unsigned base, bool more) __attribute__((always_inline)) {
-    half8_t bh[2], bl[2];
-#pragma unroll
-    for (unsigned i = 0; i < 2; ++i) {
-      bh[i] = __builtin_bit_cast(half8_t, cdna4::u32x4_t{ph[4 * i], ph[4 * i + 1], ph[4 * i + 2],
-                                                         ph[4 * i + 3]});
-      bl[i] = __builtin_bit_cast(half8_t, cdna4::u32x4_t{pl[4 * i], pl[4 * i + 1], pl[4 * i + 2],
-                                                         pl[4 * i + 3]});
-    }
-    asm volatile("s_nop 4" : "+v"(bh[0]), "+v"(bh[1]), "+v"(bl[0]), "+v"(bl[1]));  // VALU to MFMA
+  constexpr unsigned kValues = 2 * kDimBlocks;
+  static_assert(kValues >= 4);
+  auto halves = [&](const unsigned (&h)[8], unsigned step) __attribute__((always_inline)) {
+    return __builtin_bit_cast(half8_t, cdna4::u32x4_t{h[4 * step], h[4 * step + 1],
+                                                      h[4 * step + 2], h[4 * step + 3]});
+  };
+  // O += P V of the tile in stage `base`, two MFMAs an operand, numerators 0 .. 7 in pairs already and
+  // the others made beside the first half; `beside(i)` goes between the two MFMAs of operand i.
+  auto add_values = [&](unsigned base, auto beside) __attribute__((always_inline)) {
+    half8_t bh, bl;
 #pragma unroll
     for (unsigned i = 0; i < kValues; ++i) {
       __builtin_amdgcn_sched_barrier(0);
       const unsigned step = i / kDimBlocks, d = i % kDimBlocks;
-      half8_t next = va[i % kAhead];
-      if (i + kAhead < kValues)
-        next = values(base, i + kAhead);
-      prefill_detail::pv_mfma(o[d], va[i % kAhead], bh[step]);
-      if (more && i != 0)  // the next tile's scores, done since the first MFMA above
+      if (i % kDimBlocks == 0) {
+        bh = halves(ph, step);
+        bl = halves(pl, step);
+        asm volatile("s_nop 4" : "+v"(bh), "+v"(bl));  // VALU to MFMA
+      }
+      half8_t next = va[i % 4];
+      if (i + 4 < kValues)
+        next = values(base, i + 4);
+      prefill_detail::pv_mfma(o[d], va[i % 4], bh);
+      __builtin_amdgcn_sched_barrier(0);
+      if (step == 0)
 #pragma unroll
-        for (unsigned j = (i - 1) * 16 / (kValues - 1); j < i * 16 / (kValues - 1); ++j) {
-          x[j] = cur[j];
-          asm volatile("" : "+v"(x[j]));
-        }
-      prefill_detail::pv_mfma(o[d], va[i % kAhead], bl[step]);
-      va[i % kAhead] = next;
+        for (unsigned j = 8 + 8 * d / kDimBlocks / 2 * 2; j < 8 + 8 * (d + 1) / kDimBlocks / 2 * 2;
+             j += 2)
+          pair(j);
+      beside(i);
+      prefill_detail::pv_mfma(o[d], va[i % 4], bl);
+      va[i % 4] = next;
     }
     __builtin_amdgcn_sched_barrier(0);
-    drain_values(o);
   };
+
   turn(t0);
   if (t0 + 3 < t1)
     issue(t0 + 3, 2 * kStageBytes);
@@ -451,17 +508,12 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
     }
     return;
   }
-#pragma unroll
-  for (unsigned k = 0; k < 4; ++k)
-    a[k] = read(here, k);
-  asm volatile("s_nop 4" ::: "memory");
+  first_operands(here);
+  settle_operands(qh, ql);
 #pragma unroll
   for (unsigned k = 0; k < kSteps; ++k) {
-    const half8_t next = k + 4 < kSteps ? read(here, k + 4) : read(after, k + 4 - kSteps);
-    if (k == 0)
-      prefill_detail::s_mfma_first(cur, a[0], qh[0]);
-    else
-      prefill_detail::s_mfma(cur, a[k % 4], qh[k]);
+    const half8_t next = operand(k);
+    score_hi(k);
     score_lo(cur, a[k % 4], ql[k]);
     a[k % 4] = next;
   }
@@ -471,53 +523,73 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
     x[i] = cur[i];
 
   // Step ti: the scores of tile ti into cur, beside them the numerators of tile ti - 1 (x), then its
-  // P V. Between two score MFMAs stand one fma, one exponential, one sum and half a pair of neighbouring
-  // numerators, so that none waits for another; the copy of tile ti + 3 goes behind the first ones.
-  for (unsigned ti = t0 + 1; ti < t1; ++ti) {
-    turn(ti);
-    rotate();
-    mask(ti - 1);
-    asm volatile("s_nop 4" ::: "memory");
-    Place from{};
-    const bool more = ti + 3 < t1;  // uniform
-    float sum[2] = {0.0f, 0.0f}, x1 = 0.0f;
+  // P V; tile ti + 3 is copied meanwhile. Between two score MFMAs stand an fma, an exponential and a sum
+  // of different numerators, so that none waits for another, and the last ones are done before the last
+  // MFMAs; between those of P V the other half's pairs, the moves of cur to x, and behind the last V
+  // operand the barrier and the next tile's first operands.
+  if (t0 + 1 < t1) {
+    turn(t0 + 1);
+    first_operands(after);
+    for (unsigned ti = t0 + 1;;) {
+      rotate();
+      mask(ti - 1);
+      Place from{};
+      const bool more = ti + 3 < t1, next_tile = ti + 1 < t1;  // uniform
+      float sum[2] = {0.0f, 0.0f}, e[16];
+      // Numerators of k-step k: 16 in 13 steps.
+      constexpr auto at = [](unsigned k) { return k >= 13 ? 16u : (16 * k + 12) / 13; };
 #pragma unroll
-    for (unsigned k = 0; k < kSteps; ++k) {
-      __builtin_amdgcn_sched_barrier(0);
-      const half8_t next = k + 4 < kSteps ? read(here, k + 4) : read(after, k + 4 - kSteps);
-      if (k == 0)
-        prefill_detail::s_mfma_first(cur, a[0], qh[0]);
-      else
-        prefill_detail::s_mfma(cur, a[k % 4], qh[k]);
-      const float x0 = __builtin_fmaf(x[k], scale, -m);
-      if (k > 0)
-        w[k - 1] = __builtin_amdgcn_exp2f(x1);
-      score_lo(cur, a[k % 4], ql[k]);
-      if (k > 1)
-        sum[k % 2] += w[k - 2];
-      if (k > 3 && k % 2 == 0)
-        pair(k - 4);
-      a[k % 4] = next;
-      x1 = x0;
-      if (more) {
-        if (k == 0)
-          from = place_of(ti + 3);
-        if (k == 1)
-          copy(from, spare, false);
-        if (k == 2)
-          copy(from, spare, true);
+      for (unsigned k = 0; k < kSteps; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        const half8_t next = operand(k);
+        score_hi(k);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (unsigned i = at(k); i < at(k + 1); ++i)
+          e[i] = __builtin_fmaf(x[i], scale, -m);
+        if (k > 0)
+#pragma unroll
+          for (unsigned i = at(k - 1); i < at(k); ++i)
+            w[i] = __builtin_amdgcn_exp2f(e[i]);
+        score_lo(cur, a[k % 4], ql[k]);
+        if (k > 1)
+#pragma unroll
+          for (unsigned i = at(k - 2); i < at(k - 1); ++i)
+            sum[i % 2] += w[i];
+        if (k >= 9 && k < 13)
+          pair(2 * (k - 9));
+        a[k % 4] = next;
+        if (more) {
+          if (k == 0)
+            from = place_of(ti + 3);
+          if (k == 2)
+            copy(from, spare, false);
+          if (k == 4)
+            copy(from, spare, true);
+        }
+        if (k >= kSteps - 4)
+          va[k + 4 - kSteps] = values(before, k + 4 - kSteps);
       }
-      if (k + kAhead >= kSteps)
-        va[k + kAhead - kSteps] = values(before, k + kAhead - kSteps);
+      __builtin_amdgcn_sched_barrier(0);
+      settle(sum[0] + sum[1]);
+      add_values(before, [&](unsigned i) __attribute__((always_inline)) {
+        // The next tile's scores, done since the first MFMA of P V.
+        if (i != 0)
+#pragma unroll
+          for (unsigned j = (i - 1) * 16 / (kValues - 1); j < i * 16 / (kValues - 1); ++j) {
+            x[j] = cur[j];
+            asm volatile("" : "+v"(x[j]));
+          }
+        if (i == kValues - 3 && next_tile) {  // the V operands are here
+          turn(ti + 1);
+          first_operands(after);
+        }
+      });
+      if (++ti >= t1) {
+        drain_values(o);
+        break;
+      }
     }
-    __builtin_amdgcn_sched_barrier(0);
-    w[15] = __builtin_amdgcn_exp2f(x1);
-    sum[0] += w[14];
-    sum[1] += w[15];
-    pair(12);
-    pair(14);
-    settle(sum[0] + sum[1]);
-    add_values(before, true);
   }
   {  // the last tile
     mask(t1 - 1);
@@ -528,13 +600,14 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
       sum += w[i];
     }
 #pragma unroll
-    for (unsigned i = 0; i < 16; i += 2)
+    for (unsigned i = 0; i < 8; i += 2)
       pair(i);
     settle(sum);
 #pragma unroll
-    for (unsigned i = 0; i < kAhead; ++i)
+    for (unsigned i = 0; i < 4; ++i)
       va[i] = values(here, i);
-    add_values(here, false);
+    add_values(here, [](unsigned) {});
+    drain_values(o);
   }
   // ---- The partial, relative to 2^m, in the accumulators' order (whole 1 KiB a store).
   const std::size_t at = (std::size_t{span} * attn::kKvHeads + kvh) * p.blocks + block;
@@ -548,6 +621,7 @@ attn_shared_prefix_kernel(AttnSharedParams p) {
   if (part == 0 && hi == 0)
     p.part_ml[at * kBlockRows + col] = float2{m, all};
 }
+}  // namespace shared_detail
 
 // ------------------------------------------------------------------------------------------------
 // Own keys: the streaming split of the ragged and paged decode over what lies behind the prefix.
@@ -575,6 +649,8 @@ struct SharedPagedSource {
     base.template issue<kV>(j, k0, last_row, lds, cp, lane);
   }
 };
+// Contiguous own keys: the ragged decode's. (A type of its own: its launch's workgroups start elsewhere.)
+struct SharedRaggedSource : RaggedStreamSource {};
 __device__ __attribute__((always_inline)) inline unsigned stream_length(
     const SharedPagedSource& src, const StreamBatch& p, unsigned s) {
   const unsigned len = p.lens[s], mine = len > src.prefix_len ? len - src.prefix_len : 0;
@@ -593,39 +669,57 @@ struct AttnSharedOwn {
   const uint64_t* kv_offsets;
 };
 
-template <int = 0>
+// The first p.prefix_grid workgroups take the prefix's spans, the others the sequences' own keys: in one
+// launch they fill the CUs side by side, and the second set starts where the first leaves a CU.
+template <unsigned kRowBlocks, bool kPaged>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
-attn_shared_own_paged_kernel(AttnSharedParams p, AttnSharedOwn g) {
+attn_shared_split_kernel(AttnSharedParams p, AttnSharedOwn own) {
   __shared__ decode_detail::StreamShared sh;
-  decode_detail::SharedPagedSource src{
-      {g.k, g.v, g.page_table, g.max_pages, g.log2_page}, g.rows, p.prefix.len};
-  decode_detail::stream_items(
-      decode_detail::StreamBatch{p.q, p.own_m, p.own_l, p.own_o, p.lens, p.batch, p.s_max,
-                                 p.own_cap, p.chunk, p.balanced},
-      src, sh);
+  static_assert(sizeof(sh) >= sizeof(shared_detail::PrefixShared));
+  if (blockIdx.x < p.prefix_grid) {  // uniform
+    shared_detail::prefix_span<kRowBlocks, kPaged>(
+        p, reinterpret_cast<shared_detail::PrefixShared&>(sh));
+    return;
+  }
+  const decode_detail::StreamBatch batch{p.q,     p.own_m, p.own_l,   p.own_o, p.lens,
+                                         p.own_batch, p.s_max, p.own_cap, p.chunk, p.balanced};
+  if constexpr (kPaged) {
+    decode_detail::SharedPagedSource src{
+        {own.k, own.v, own.page_table, own.max_pages, own.log2_page}, own.rows, p.prefix.len};
+    decode_detail::stream_items(batch, src, sh, p.prefix_grid);
+  } else {
+    decode_detail::SharedRaggedSource src{{own.k, own.v, own.kv_offsets}};
+    decode_detail::stream_items(batch, src, sh, p.prefix_grid);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
-// Merge: a workgroup per (KV head, row block, 32 dimensions). Its waves take the prefix's spans in
+// Merge: a workgroup per (KV head, row block, 8 kQuads dimensions). Its waves take the prefix's spans in
 // turn, each lane the row of its column as the partials lie (M the largest reference, O and L summed
 // relative to 2^M in span order), and meet in LDS; then a thread per (row, 4 dimensions) adds the
 // waves' sums and the own keys' splits in order, divides and applies the gate. The order is fixed.
+// Bound by the partials it reads, 1 KiB a row and span; a CU takes in only so much of them, so with
+// few row blocks their dimensions are spread over four times the workgroups.
 // ------------------------------------------------------------------------------------------------
 
-template <int = 0>
+template <unsigned kQuads>
 __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams p) {
   using namespace shared_detail;
-  constexpr unsigned kBatch = 4, kRow = 33;  // floats of a staged row: 32 and one apart
+  static_assert(kQuads == 1 || kQuads == 4);
+  constexpr unsigned kBatch = 16 / kQuads, kDims = 8 * kQuads;  // spans, dimensions at a time
+  constexpr unsigned kRow = kDims + 1;  // floats of a staged row
+  constexpr unsigned kPieces = attn::kDim / kDims;
   __shared__ float rows[4][kBlockRows * kRow];
   __shared__ float2 ml[4][kBlockRows];
   const unsigned t = threadIdx.x, lane = t & 63u, wave = t >> 6, col = lane & 31u, hi = lane >> 5;
-  const unsigned d = blockIdx.x % 8, kvh = blockIdx.x / 8 % 2, block = blockIdx.x / 16;
+  const unsigned d = blockIdx.x % kPieces, kvh = blockIdx.x / kPieces % 2;
+  const unsigned block = blockIdx.x / (2 * kPieces);
   // This wave's spans of the prefix.
   float m = kNoScore, l = 0.0f;
-  float4 o[4] = {};
+  float4 o[kQuads] = {};
   for (unsigned s0 = wave; s0 < p.spans; s0 += 4 * kBatch) {
     float2 x[kBatch];
-    float4 y[kBatch][4];
+    float4 y[kBatch][kQuads];
 #pragma unroll
     for (unsigned i = 0; i < kBatch; ++i) {
       const unsigned s = min(s0 + 4 * i, p.spans - 1);
@@ -633,8 +727,8 @@ __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams
       x[i] = p.part_ml[at * kBlockRows + col];
       x[i] = s0 + 4 * i < p.spans ? x[i] : float2{kNoScore, 0.0f};
 #pragma unroll
-      for (unsigned j = 0; j < 4; ++j)
-        y[i][j] = p.part_o[(at * 8 + d) * 256 + 64 * j + lane];
+      for (unsigned j = 0; j < kQuads; ++j)
+        y[i][j] = p.part_o[at * 8 * 256 + 64 * (kQuads * d + j) + lane];
     }
     float top = m;
 #pragma unroll
@@ -644,7 +738,7 @@ __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams
     m = top;
     l *= old;
 #pragma unroll
-    for (unsigned j = 0; j < 4; ++j)
+    for (unsigned j = 0; j < kQuads; ++j)
       o[j] = float4{o[j].x * old, o[j].y * old, o[j].z * old, o[j].w * old};
 #pragma unroll
     for (unsigned i = 0; i < kBatch; ++i) {
@@ -653,7 +747,7 @@ __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams
       const float e = __builtin_amdgcn_exp2f(x[i].x - top);
       l = __builtin_fmaf(x[i].y, e, l);
 #pragma unroll
-      for (unsigned j = 0; j < 4; ++j) {
+      for (unsigned j = 0; j < kQuads; ++j) {
         o[j].x = __builtin_fmaf(y[i][j].x, e, o[j].x);
         o[j].y = __builtin_fmaf(y[i][j].y, e, o[j].y);
         o[j].z = __builtin_fmaf(y[i][j].z, e, o[j].z);
@@ -662,7 +756,7 @@ __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams
     }
   }
 #pragma unroll
-  for (unsigned j = 0; j < 4; ++j) {  // dimensions 8 j + 4 hi .. + 3 of the block
+  for (unsigned j = 0; j < kQuads; ++j) {  // dimensions 8 j + 4 hi .. + 3 of the piece
     float* at = &rows[wave][col * kRow + 8 * j + 4 * hi];
     at[0] = o[j].x, at[1] = o[j].y, at[2] = o[j].z, at[3] = o[j].w;
   }
@@ -670,11 +764,12 @@ __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams
     ml[wave][col] = float2{m, l};
   __syncthreads();
 
-  const unsigned row = t / 8, dim = 4 * (t % 8), seq = kSeqs * block + row / kGroup;
-  if (seq >= p.batch)
+  const unsigned row = t / (2 * kQuads), dim = 4 * (t % (2 * kQuads));
+  const unsigned seq = kSeqs * block + row / kGroup;
+  if (row >= kBlockRows || seq >= p.batch)
     return;
   const std::size_t out =
-      (std::size_t{seq} * attn::kQHeads + kvh * kGroup + row % kGroup) * attn::kDim + 32 * d + dim;
+      (std::size_t{seq} * attn::kQHeads + kvh * kGroup + row % kGroup) * attn::kDim + kDims * d + dim;
   const float4 g = *reinterpret_cast<const float4*>(p.gate + out);
   float top = kNoScore;
 #pragma unroll
@@ -696,18 +791,19 @@ __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams
     const unsigned n = attn_ragged_seq_splits(mine, p.s_max, chunk);
     const std::size_t at0 =
         ((std::size_t{seq} * attn::kKvHeads + kvh) * p.s_max) * kGroup + row % kGroup;
-    for (unsigned s0 = 0; s0 < n; s0 += kBatch) {
-      float sm[kBatch], sl[kBatch];
-      float4 so[kBatch];
+    constexpr unsigned kSplits = 4;
+    for (unsigned s0 = 0; s0 < n; s0 += kSplits) {
+      float sm[kSplits], sl[kSplits];
+      float4 so[kSplits];
 #pragma unroll
-      for (unsigned i = 0; i < kBatch; ++i) {
+      for (unsigned i = 0; i < kSplits; ++i) {
         const std::size_t at = at0 + static_cast<std::size_t>(min(s0 + i, n - 1)) * kGroup;
         sm[i] = p.own_m[at] * decode_detail::kLog2e;
         sl[i] = p.own_l[at];
-        so[i] = *reinterpret_cast<const float4*>(p.own_o + at * attn::kDim + 32 * d + dim);
+        so[i] = *reinterpret_cast<const float4*>(p.own_o + at * attn::kDim + kDims * d + dim);
       }
 #pragma unroll
-      for (unsigned i = 0; i < kBatch; ++i) {
+      for (unsigned i = 0; i < kSplits; ++i) {
         if (s0 + i >= n)
           break;
         if (!(sl[i] != 0.0f))  // an empty span
@@ -794,23 +890,9 @@ inline void attn_shared_launch(AttnSharedParams p, const AttnSharedOwn& own, uns
   p.spans = cut.spans;
   p.span_tiles = cut.span_tiles;
   p.blocks = cut.blocks;
-  if (cut.spans != 0) {
-    const unsigned rb = attn_shared_row_blocks(p.batch), groups = (cut.blocks + rb - 1) / rb;
-    const unsigned grid = 8 * ((2 * cut.spans * groups + 7) / 8);
-    const auto launch = [&](auto paged) {
-      constexpr bool kPaged = decltype(paged)::value;
-      if (rb == 1)
-        attn_shared_prefix_kernel<1, kPaged><<<grid, 256, 0, stream>>>(p);
-      else if (rb == 2)
-        attn_shared_prefix_kernel<2, kPaged><<<grid, 256, 0, stream>>>(p);
-      else
-        attn_shared_prefix_kernel<4, kPaged><<<grid, 256, 0, stream>>>(p);
-    };
-    if (p.prefix.table != nullptr)
-      launch(std::true_type{});
-    else
-      launch(std::false_type{});
-  }
+  const unsigned rb = attn_shared_row_blocks(p.batch), groups = (cut.blocks + rb - 1) / rb;
+  p.prefix_grid = 8 * ((2 * cut.spans * groups + 7) / 8);
+  unsigned grid = 0, step = p.batch;  // of the own keys: workgroups, sequences of one launch
   if (max_own != 0) {
     // At most one streaming launch's sequences and items at a time.
     const unsigned most_items = kRaggedStreamMaxItems * cus;
@@ -818,37 +900,56 @@ inline void attn_shared_launch(AttnSharedParams p, const AttnSharedOwn& own, uns
                        most_items / attn::kKvHeads);
     p.chunk = attn_ragged_chunk(p.batch, max_own, cus);
     const std::size_t items = std::size_t{p.batch} * attn::kKvHeads * p.s_max;
-    const unsigned grid = static_cast<unsigned>(std::min<std::size_t>(cus, items));
-    unsigned step = p.batch;
+    // The CUs that the prefix leaves, all of them where it leaves less than half.
+    const unsigned free = 2 * p.prefix_grid <= cus ? cus - p.prefix_grid : cus;
+    grid = static_cast<unsigned>(std::min<std::size_t>(free, items));
     if (attn_ragged_balanced(p.batch, max_own, cus, grid))
       p.balanced = reinterpret_cast<unsigned*>(p.own_l) - 4;
     else
       step = std::min(kRaggedStreamMaxBatch,
                       std::max(1u, kRaggedStreamMaxItems * grid / (attn::kKvHeads * p.s_max)));
-    for (unsigned s = 0; s < p.batch; s += step) {
-      const std::size_t row = std::size_t{s} * attn::kKvHeads * p.s_max * decode_detail::kGroup;
-      AttnSharedParams a = p;
-      a.batch = std::min(step, p.batch - s);
+  }
+  const auto launch = [&](const AttnSharedParams& a, const AttnSharedOwn& o) {
+    const auto as = [&](auto paged) {
+      constexpr bool kPaged = decltype(paged)::value;
+      const unsigned all = a.prefix_grid + grid;
+      if (rb == 1)
+        attn_shared_split_kernel<1, kPaged><<<all, 256, 0, stream>>>(a, o);
+      else if (rb == 2)
+        attn_shared_split_kernel<2, kPaged><<<all, 256, 0, stream>>>(a, o);
+      else
+        attn_shared_split_kernel<4, kPaged><<<all, 256, 0, stream>>>(a, o);
+    };
+    if (own.page_table != nullptr)
+      as(std::true_type{});
+    else
+      as(std::false_type{});
+  };
+  for (unsigned s = 0; (p.prefix_grid != 0 || grid != 0) && s < p.batch; s += step) {
+    const std::size_t row = std::size_t{s} * attn::kKvHeads * p.s_max * decode_detail::kGroup;
+    AttnSharedParams a = p;
+    AttnSharedOwn o = own;
+    a.own_batch = std::min(step, p.batch - s);
+    if (s != 0) {  // the own keys of more sequences
+      a.prefix_grid = 0;
       a.q += std::size_t{s} * attn::kQHeads * attn::kDim;
       a.lens += s;
       a.own_m += row;
       a.own_l += row;
       a.own_o += row * attn::kDim;
-      if (own.page_table != nullptr) {
-        AttnSharedOwn g = own;
-        if (g.rows != nullptr)
-          g.rows += s;
-        else
-          g.page_table += std::size_t{s} * g.max_pages;
-        attn_shared_own_paged_kernel<<<grid, 256, 0, stream>>>(a, g);
-      } else {
-        attn_ragged_stream_kernel<256><<<grid, 256, 0, stream>>>(AttnRaggedParams{
-            a.q, nullptr, own.k, own.v, own.kv_offsets + s, a.lens, nullptr, a.own_m, a.own_l,
-            a.own_o, a.batch, a.s_max, a.own_cap, a.chunk, a.balanced});
-      }
+      if (own.page_table == nullptr)
+        o.kv_offsets += s;
+      else if (own.rows != nullptr)
+        o.rows += s;
+      else
+        o.page_table += std::size_t{s} * own.max_pages;
     }
+    launch(a, o);
   }
-  attn_shared_merge_kernel<<<16 * cut.blocks, 256, 0, stream>>>(p);
+  if (16 * cut.blocks < cus)
+    attn_shared_merge_kernel<1><<<64 * cut.blocks, 256, 0, stream>>>(p);
+  else
+    attn_shared_merge_kernel<4><<<16 * cut.blocks, 256, 0, stream>>>(p);
 }
 
 }  // namespace miso::kernels
