@@ -52,8 +52,82 @@ struct AttnSharedParams {
   float* own_o;
   unsigned s_max, chunk, own_cap;  // s_max 0: nobody has own keys
   unsigned* balanced;
-  unsigned prefix_grid, own_batch;  // of a split launch
+  // Of a split launch: workgroups of the prefix, the first of the own keys, sequences.
+  unsigned prefix_grid, own_first, own_batch;
+  unsigned* chosen;    // word for the spans where the kernel chooses them (AttnSharedCut), or nullptr
+  unsigned own_least;  // and the workgroups that the own keys take at least
 };
+
+// Where a split launch cuts the prefix.
+struct AttnSharedCut {
+  unsigned spans, span_tiles, grid;  // grid: the prefix's workgroups, a multiple of 8
+  bool both;                         // the own keys are every workgroup's, behind its span
+};
+
+// Row blocks of a workgroup of the prefix.
+__host__ __device__ constexpr unsigned attn_shared_row_blocks(unsigned batch) {
+  return batch <= 4 ? 1 : batch <= 8 ? 2 : 4;
+}
+
+// What the tiles of a launch cost on `cus` CUs, a workgroup each, in us without the fixed part: the
+// slower side, or the span and its share of the `own` tiles of own keys (both heads') one after the
+// other. A tile of a span behind 64 sequences takes 1.5 us (32768 keys of 40 tiles a span: 70 us), behind
+// 8 1.0 (9 tiles: 23 us, 12: 26), behind 3 0.9; of the own keys 1.4 (48 workgroups: 72 us, 32: 97); the
+// own keys' start behind a span 7.
+template <unsigned kRowBlocks>
+constexpr float kAttnSharedTile = kRowBlocks == 4 ? 1.5f : kRowBlocks == 2 ? 1.0f : 0.9f;
+constexpr float kAttnSharedOwnTile = 1.5f, kAttnSharedOwnStart = 7.0f;
+template <unsigned kRowBlocks>
+__host__ __device__ constexpr float attn_shared_cost(const AttnSharedCut& c, unsigned own,
+                                                     unsigned cus) {
+  const float prefix = kAttnSharedTile<kRowBlocks> * static_cast<float>(c.span_tiles);
+  const float keys = kAttnSharedOwnTile * static_cast<float>(own) /
+                     static_cast<float>(c.both ? cus : cus - c.grid);
+  return c.both ? prefix + kAttnSharedOwnStart + keys : prefix < keys ? keys : prefix;
+}
+
+// The cut of `tiles` tiles for `pairs` (group of row blocks, KV head) pairs that costs least: beside the
+// own keys on CUs of their own, `least` or more, or on all CUs. 8 sequences behind 32768 keys, 300 own
+// keys each: 23.7 us of 9 tiles a span with 28 CUs for the own keys, 34.4 of 8 with all CUs and the
+// own keys behind them; 256 behind 8192, 256 each: 79 of 43 with 64 CUs, 94 of 32.
+// Spans shorter than 4 tiles only add partials: 8 behind 8192 22.0 us of 4, 24.1 of 3 (the merge's
+// time among them).
+template <unsigned kRowBlocks>
+__host__ __device__ constexpr AttnSharedCut attn_shared_cut(unsigned tiles, unsigned pairs, unsigned own,
+                                                            unsigned cus, unsigned least) {
+  constexpr unsigned kFewTiles = 4;
+  if (tiles == 0)
+    return AttnSharedCut{0, 0, 0, false};
+  const auto cut = [=](unsigned spans, bool both) {
+    const unsigned each = (tiles + spans - 1) / spans;
+    spans = (tiles + each - 1) / each;
+    return AttnSharedCut{spans, each, 8 * ((pairs * spans + 7) / 8), both};
+  };
+  unsigned most = cus / pairs;
+  most = most < tiles / kFewTiles ? most : tiles / kFewTiles;
+  most = most < 1 ? 1 : most;
+  if (own == 0 || cut(most, false).grid > cus)
+    return cut(most, false);
+  AttnSharedCut best = cut(most, true);
+  float cost = attn_shared_cost<kRowBlocks>(best, own, cus);
+  // The spans with which both sides end together, and one more.
+  const float prefix = kAttnSharedTile<kRowBlocks> * static_cast<float>(tiles);
+  const float keys = kAttnSharedOwnTile * static_cast<float>(own);
+  const unsigned even = static_cast<unsigned>(prefix * static_cast<float>(cus) /
+                                              (keys + prefix * static_cast<float>(pairs)));
+  for (unsigned i = 0; i < 2; ++i) {
+    const unsigned spans = even + i < most ? even + i : most;
+    const AttnSharedCut c = cut(spans < 1 ? 1 : spans, false);
+    if (c.grid + least > cus)
+      continue;
+    const float cost_c = attn_shared_cost<kRowBlocks>(c, own, cus);
+    if (cost_c < cost) {
+      cost = cost_c;
+      best = c;
+    }
+  }
+  return best;
+}
 
 namespace shared_detail {
 
@@ -178,6 +252,13 @@ __device__ __attribute__((always_inline)) inline unsigned prefix_keys(const Attn
   if (seq >= p.batch)
     return 0;
   return p.whole ? min(p.lens[seq], p.prefix.len) : p.prefix.len;
+}
+
+// And its own, seq < batch.
+__device__ __attribute__((always_inline)) inline unsigned own_keys(const AttnSharedParams& p,
+                                                                   unsigned seq) {
+  const unsigned len = p.lens[seq], skip = p.whole ? p.prefix.len : 0;
+  return min(len > skip ? len - skip : 0u, p.own_cap);
 }
 
 }  // namespace shared_detail
@@ -669,27 +750,46 @@ struct AttnSharedOwn {
   const uint64_t* kv_offsets;
 };
 
-// The first p.prefix_grid workgroups take the prefix's spans, the others the sequences' own keys: in one
-// launch they fill the CUs side by side, and the second set starts where the first leaves a CU.
+// The first p.prefix_grid workgroups take the prefix's spans, those from p.own_first on the sequences' own
+// keys. Where the lengths decide on how many CUs either does best, which only the device knows, each wave
+// makes the choice before anything else.
 template <unsigned kRowBlocks, bool kPaged>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
 attn_shared_split_kernel(AttnSharedParams p, AttnSharedOwn own) {
   __shared__ decode_detail::StreamShared sh;
   static_assert(sizeof(sh) >= sizeof(shared_detail::PrefixShared));
+  if (p.chosen != nullptr) {  // uniform
+    float tiles = 0.0f;
+    for (unsigned s = threadIdx.x & 63u; s < p.batch; s += 64)
+      tiles += __builtin_ceilf(static_cast<float>(shared_detail::own_keys(p, s)) * (1.0f / 32.0f));
+    const unsigned all = __builtin_amdgcn_readfirstlane(
+        static_cast<unsigned>(fminf(2.0f * cdna4::wave_allsum(tiles), 0x1p30f)));
+    const AttnSharedCut cut = attn_shared_cut<kRowBlocks>(
+        (p.prefix.len - 1) / 32 + 1, 2 * ((p.blocks + kRowBlocks - 1) / kRowBlocks), all, gridDim.x,
+        p.own_least);
+    p.spans = __builtin_amdgcn_readfirstlane(cut.spans);
+    p.span_tiles = __builtin_amdgcn_readfirstlane(cut.span_tiles);
+    p.prefix_grid = __builtin_amdgcn_readfirstlane(cut.grid);
+    p.own_first = __builtin_amdgcn_readfirstlane(cut.both ? 0u : cut.grid);
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+      *p.chosen = p.spans;
+  }
   if (blockIdx.x < p.prefix_grid) {  // uniform
     shared_detail::prefix_span<kRowBlocks, kPaged>(
         p, reinterpret_cast<shared_detail::PrefixShared&>(sh));
-    return;
+    if (blockIdx.x < p.own_first || p.s_max == 0)
+      return;
+    __syncthreads();  // the ring's space is the stream's
   }
   const decode_detail::StreamBatch batch{p.q,     p.own_m, p.own_l,   p.own_o, p.lens,
                                          p.own_batch, p.s_max, p.own_cap, p.chunk, p.balanced};
   if constexpr (kPaged) {
     decode_detail::SharedPagedSource src{
         {own.k, own.v, own.page_table, own.max_pages, own.log2_page}, own.rows, p.prefix.len};
-    decode_detail::stream_items(batch, src, sh, p.prefix_grid);
+    decode_detail::stream_items(batch, src, sh, p.own_first);
   } else {
     decode_detail::SharedRaggedSource src{{own.k, own.v, own.kv_offsets}};
-    decode_detail::stream_items(batch, src, sh, p.prefix_grid);
+    decode_detail::stream_items(batch, src, sh, p.own_first);
   }
 }
 
@@ -715,17 +815,18 @@ __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams
   const unsigned d = blockIdx.x % kPieces, kvh = blockIdx.x / kPieces % 2;
   const unsigned block = blockIdx.x / (2 * kPieces);
   // This wave's spans of the prefix.
+  const unsigned spans = p.chosen != nullptr ? *p.chosen : p.spans;
   float m = kNoScore, l = 0.0f;
   float4 o[kQuads] = {};
-  for (unsigned s0 = wave; s0 < p.spans; s0 += 4 * kBatch) {
+  for (unsigned s0 = wave; s0 < spans; s0 += 4 * kBatch) {
     float2 x[kBatch];
     float4 y[kBatch][kQuads];
 #pragma unroll
     for (unsigned i = 0; i < kBatch; ++i) {
-      const unsigned s = min(s0 + 4 * i, p.spans - 1);
+      const unsigned s = min(s0 + 4 * i, spans - 1);
       const std::size_t at = (std::size_t{s} * attn::kKvHeads + kvh) * p.blocks + block;
       x[i] = p.part_ml[at * kBlockRows + col];
-      x[i] = s0 + 4 * i < p.spans ? x[i] : float2{kNoScore, 0.0f};
+      x[i] = s0 + 4 * i < spans ? x[i] : float2{kNoScore, 0.0f};
 #pragma unroll
       for (unsigned j = 0; j < kQuads; ++j)
         y[i][j] = p.part_o[at * 8 * 256 + 64 * (kQuads * d + j) + lane];
@@ -742,7 +843,7 @@ __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams
       o[j] = float4{o[j].x * old, o[j].y * old, o[j].z * old, o[j].w * old};
 #pragma unroll
     for (unsigned i = 0; i < kBatch; ++i) {
-      if (s0 + 4 * i >= p.spans)  // uniform: a repeated span is left out (0 x infinity is NaN)
+      if (s0 + 4 * i >= spans)  // uniform: a repeated span is left out (0 x infinity is NaN)
         break;
       const float e = __builtin_amdgcn_exp2f(x[i].x - top);
       l = __builtin_fmaf(x[i].y, e, l);
@@ -785,8 +886,7 @@ __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams
       v[j] = __builtin_fmaf(rows[w][row * kRow + dim + j], e, v[j]);
   }
   if (p.s_max != 0) {
-    const unsigned len = p.lens[seq], skip = p.whole ? p.prefix.len : 0;
-    const unsigned mine = min(len > skip ? len - skip : 0u, p.own_cap);
+    const unsigned mine = own_keys(p, seq);
     const unsigned chunk = p.balanced != nullptr ? *p.balanced : p.chunk;
     const unsigned n = attn_ragged_seq_splits(mine, p.s_max, chunk);
     const std::size_t at0 =
@@ -833,24 +933,7 @@ __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams
 // ------------------------------------------------------------------------------------------------
 
 constexpr unsigned kAttnSharedCus = 256;
-
-__host__ __device__ constexpr unsigned attn_shared_row_blocks(unsigned batch) {  // of a workgroup
-  return batch <= 4 ? 1 : batch <= 8 ? 2 : 4;
-}
-
-struct AttnSharedCut {
-  unsigned spans, span_tiles, blocks;
-};
-__host__ __device__ constexpr AttnSharedCut attn_shared_cut(unsigned batch, unsigned prefix) {
-  const unsigned rb = attn_shared_row_blocks(batch), blocks = (batch + 3) / 4;
-  const unsigned groups = (blocks + rb - 1) / rb, tiles = prefix / 32 + (prefix % 32 != 0);
-  if (tiles == 0)
-    return AttnSharedCut{0, 0, blocks};
-  unsigned spans = kAttnSharedCus / (2 * groups);
-  spans = spans == 0 ? 1 : spans;
-  const unsigned each = (tiles + spans - 1) / spans;
-  return AttnSharedCut{(tiles + each - 1) / each, each, blocks};
-}
+constexpr unsigned kAttnSharedOwnLeast = 16;  // workgroups of the own keys beside the prefix's
 
 // Row blocks x spans of a KV head's partials: no less than any smaller batch or shorter prefix takes.
 __host__ __device__ constexpr std::size_t attn_shared_part_blocks(unsigned batch, unsigned prefix) {
@@ -878,60 +961,77 @@ __host__ __device__ constexpr AttnSharedLayout attn_shared_layout(unsigned batch
 
 // p: q, gate, core, lens, prefix, batch, whole and own_cap given; the workspace holds
 // attn_shared_layout(batch, max_own, p.prefix.len).
-inline void attn_shared_launch(AttnSharedParams p, const AttnSharedOwn& own, unsigned max_own,
-                               char* ws, unsigned cus, hipStream_t stream) {
+template <unsigned kRowBlocks, bool kPaged>
+inline void attn_shared_launch_as(AttnSharedParams p, const AttnSharedOwn& own, unsigned max_own,
+                                  char* ws, unsigned cus, hipStream_t stream) {
   const AttnSharedLayout at = attn_shared_layout(p.batch, max_own, p.prefix.len);
-  const AttnSharedCut cut = attn_shared_cut(p.batch, p.prefix.len);
   p.part_o = reinterpret_cast<float4*>(ws);
   p.part_ml = reinterpret_cast<float2*>(ws + at.part_ml);
   p.own_m = reinterpret_cast<float*>(ws + at.own_m);
   p.own_l = reinterpret_cast<float*>(ws + at.own_l);
   p.own_o = reinterpret_cast<float*>(ws + at.own_o);
-  p.spans = cut.spans;
-  p.span_tiles = cut.span_tiles;
-  p.blocks = cut.blocks;
-  const unsigned rb = attn_shared_row_blocks(p.batch), groups = (cut.blocks + rb - 1) / rb;
-  p.prefix_grid = 8 * ((2 * cut.spans * groups + 7) / 8);
-  unsigned grid = 0, step = p.batch;  // of the own keys: workgroups, sequences of one launch
+  unsigned* const words = reinterpret_cast<unsigned*>(p.own_l) - 4;
+  p.blocks = (p.batch + 3) / 4;
+  const unsigned tiles = p.prefix.len / 32 + (p.prefix.len % 32 != 0);
+  const unsigned pairs = 2 * ((p.blocks + kRowBlocks - 1) / kRowBlocks);
+  const unsigned shared_cus = std::min(cus, kAttnSharedCus);
+  AttnSharedCut cut = attn_shared_cut<kRowBlocks>(tiles, pairs, 0, shared_cus, 0);
+  unsigned own_grid = 0, step = p.batch;  // of the own keys: workgroups, sequences of one launch
+  unsigned grid = cut.grid;
   if (max_own != 0) {
-    // At most one streaming launch's sequences and items at a time.
-    const unsigned most_items = kRaggedStreamMaxItems * cus;
+    // The CUs that the prefix leaves, all of them where it leaves less than half; at most one streaming
+    // launch's sequences and items at a time.
+    own_grid = 2 * cut.grid <= cus ? cus - cut.grid : cus;
     p.s_max = std::min(attn_ragged_balanced_splits(p.batch, max_own),
-                       most_items / attn::kKvHeads);
+                       kRaggedStreamMaxItems * own_grid / attn::kKvHeads);
     p.chunk = attn_ragged_chunk(p.batch, max_own, cus);
     const std::size_t items = std::size_t{p.batch} * attn::kKvHeads * p.s_max;
-    // The CUs that the prefix leaves, all of them where it leaves less than half.
-    const unsigned free = 2 * p.prefix_grid <= cus ? cus - p.prefix_grid : cus;
-    grid = static_cast<unsigned>(std::min<std::size_t>(free, items));
-    if (attn_ragged_balanced(p.batch, max_own, cus, grid))
-      p.balanced = reinterpret_cast<unsigned*>(p.own_l) - 4;
-    else
-      step = std::min(kRaggedStreamMaxBatch,
-                      std::max(1u, kRaggedStreamMaxItems * grid / (attn::kKvHeads * p.s_max)));
+    const std::size_t least = (items + kRaggedStreamMaxItems - 1) / kRaggedStreamMaxItems;
+    own_grid = static_cast<unsigned>(std::min<std::size_t>(own_grid, items));
+    if (tiles != 0 && cut.grid <= shared_cus && p.batch <= kRaggedStreamMaxBatch &&
+        least <= shared_cus) {
+      // One round of workgroups, cut for few own keys; where that could cost much beside the cut for
+      // max_own, the kernel chooses (1 us: 16 sequences behind 4096 keys, 1024 each, 17.3 us of this cut,
+      // 18.6 of a chosen one).
+      constexpr float kMuch = 3.0f;
+      p.own_least = static_cast<unsigned>(
+          std::min(items, std::max<std::size_t>(least, kAttnSharedOwnLeast)));
+      const unsigned most = static_cast<unsigned>(std::min<std::size_t>(
+          std::size_t{p.batch} * attn::kKvHeads * (max_own / 32 + 1), 1u << 30));
+      const auto as = [&](unsigned own_tiles) {
+        return attn_shared_cut<kRowBlocks>(tiles, pairs, own_tiles, shared_cus, p.own_least);
+      };
+      const auto cost = [&](const AttnSharedCut& c) {
+        return attn_shared_cost<kRowBlocks>(c, most, shared_cus);
+      };
+      cut = as(1);
+      if (cost(cut) > cost(as(most)) + kMuch)
+        p.chosen = words + 1;
+      own_grid = cut.both ? shared_cus
+                          : static_cast<unsigned>(std::min<std::size_t>(shared_cus - cut.grid, items));
+      grid = cut.both || p.chosen != nullptr ? shared_cus : cut.grid + own_grid;
+      p.own_first = cut.both ? 0 : cut.grid;
+    } else {  // the own keys' workgroups follow the prefix's
+      p.own_first = cut.grid;
+      grid = cut.grid + own_grid;
+      if (p.batch > kRaggedStreamMaxBatch || least > own_grid)
+        step = std::min(kRaggedStreamMaxBatch,
+                        std::max(1u, kRaggedStreamMaxItems * own_grid / (attn::kKvHeads * p.s_max)));
+    }
+    if (step >= p.batch &&
+        attn_ragged_balanced(p.batch, max_own, cus, p.chosen != nullptr ? p.own_least : own_grid))
+      p.balanced = words;
   }
-  const auto launch = [&](const AttnSharedParams& a, const AttnSharedOwn& o) {
-    const auto as = [&](auto paged) {
-      constexpr bool kPaged = decltype(paged)::value;
-      const unsigned all = a.prefix_grid + grid;
-      if (rb == 1)
-        attn_shared_split_kernel<1, kPaged><<<all, 256, 0, stream>>>(a, o);
-      else if (rb == 2)
-        attn_shared_split_kernel<2, kPaged><<<all, 256, 0, stream>>>(a, o);
-      else
-        attn_shared_split_kernel<4, kPaged><<<all, 256, 0, stream>>>(a, o);
-    };
-    if (own.page_table != nullptr)
-      as(std::true_type{});
-    else
-      as(std::false_type{});
-  };
-  for (unsigned s = 0; (p.prefix_grid != 0 || grid != 0) && s < p.batch; s += step) {
+  p.spans = cut.spans;
+  p.span_tiles = cut.span_tiles;
+  p.prefix_grid = cut.grid;
+  for (unsigned s = 0; grid != 0 && s < p.batch; s += step) {
     const std::size_t row = std::size_t{s} * attn::kKvHeads * p.s_max * decode_detail::kGroup;
     AttnSharedParams a = p;
     AttnSharedOwn o = own;
     a.own_batch = std::min(step, p.batch - s);
     if (s != 0) {  // the own keys of more sequences
-      a.prefix_grid = 0;
+      a.prefix_grid = a.own_first = 0;
       a.q += std::size_t{s} * attn::kQHeads * attn::kDim;
       a.lens += s;
       a.own_m += row;
@@ -944,12 +1044,28 @@ inline void attn_shared_launch(AttnSharedParams p, const AttnSharedOwn& own, uns
       else
         o.page_table += std::size_t{s} * own.max_pages;
     }
-    launch(a, o);
+    attn_shared_split_kernel<kRowBlocks, kPaged>
+        <<<s == 0 ? grid : own_grid, 256, 0, stream>>>(a, o);
   }
-  if (16 * cut.blocks < cus)
-    attn_shared_merge_kernel<1><<<64 * cut.blocks, 256, 0, stream>>>(p);
+  if (16 * p.blocks < cus)
+    attn_shared_merge_kernel<1><<<64 * p.blocks, 256, 0, stream>>>(p);
   else
-    attn_shared_merge_kernel<4><<<16 * cut.blocks, 256, 0, stream>>>(p);
+    attn_shared_merge_kernel<4><<<16 * p.blocks, 256, 0, stream>>>(p);
+}
+
+inline void attn_shared_launch(const AttnSharedParams& p, const AttnSharedOwn& own, unsigned max_own,
+                               char* ws, unsigned cus, hipStream_t stream) {
+  const auto as = [&](auto paged) {
+    constexpr bool kPaged = decltype(paged)::value;
+    const unsigned rb = attn_shared_row_blocks(p.batch);
+    (rb == 1   ? attn_shared_launch_as<1, kPaged>
+     : rb == 2 ? attn_shared_launch_as<2, kPaged>
+               : attn_shared_launch_as<4, kPaged>)(p, own, max_own, ws, cus, stream);
+  };
+  if (own.page_table != nullptr)
+    as(std::true_type{});
+  else
+    as(std::false_type{});
 }
 
 }  // namespace miso::kernels
