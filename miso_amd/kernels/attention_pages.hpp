@@ -72,18 +72,51 @@ __device__ __attribute__((always_inline)) inline unsigned pages_of(unsigned long
   return static_cast<unsigned>((keys + (1ull << log2_page) - 1) >> log2_page);
 }
 
-// The first request whose running sum exceeds k (n if none).
-__device__ __attribute__((always_inline)) inline unsigned owner_of(const unsigned* sums, unsigned n,
-                                                                   unsigned k) {
-  unsigned lo = 0, hi = n;
-  while (lo < hi) {
-    const unsigned mid = (lo + hi) / 2;
-    if (sums[mid] <= k)
-      lo = mid + 1;
-    else
-      hi = mid;
+// For each k the first request whose running sum exceeds it (n if none): kMany searches side by side, since
+// one waits for LDS at each of its steps.
+template <unsigned kMany>
+__device__ __attribute__((always_inline)) inline void owners_of(const unsigned* sums, unsigned n,
+                                                                const unsigned (&k)[kMany],
+                                                                unsigned (&owner)[kMany]) {
+#pragma unroll
+  for (unsigned i = 0; i < kMany; ++i)
+    owner[i] = 0;
+  for (unsigned step = 1u << (31 - __builtin_clz(n)); step != 0; step /= 2) {
+    unsigned sum[kMany];
+#pragma unroll
+    for (unsigned i = 0; i < kMany; ++i)
+      sum[i] = sums[min(owner[i] + step, n) - 1];
+#pragma unroll
+    for (unsigned i = 0; i < kMany; ++i)
+      owner[i] += owner[i] + step <= n && sum[i] <= k[i] ? step : 0u;
   }
-  return lo;
+}
+
+// visit(k, s, place of k among request s's) for k = first, first + stride, .. below n; kMany at a time.
+template <unsigned kMany, typename Visit>
+__device__ __attribute__((always_inline)) inline void each_of_many(const unsigned* sums, unsigned batch,
+                                                                   unsigned first, unsigned stride,
+                                                                   unsigned n, Visit visit) {
+  for (unsigned k0 = first; k0 < n; k0 += kMany * stride) {
+    unsigned k[kMany], s[kMany];
+#pragma unroll
+    for (unsigned i = 0; i < kMany; ++i)
+      k[i] = min(k0 + i * stride, n - 1);
+    owners_of(sums, batch, k, s);
+#pragma unroll
+    for (unsigned i = 0; i < kMany; ++i)
+      if (k0 + i * stride < n)
+        visit(k[i], s[i], k[i] - (s[i] != 0 ? sums[s[i] - 1] : 0u));
+  }
+}
+template <typename Visit>
+__device__ __attribute__((always_inline)) inline void each_of(const unsigned* sums, unsigned batch,
+                                                              unsigned first, unsigned stride,
+                                                              unsigned n, Visit visit) {
+  if (n <= stride)  // uniform
+    each_of_many<1>(sums, batch, first, stride, n, visit);
+  else
+    each_of_many<4>(sums, batch, first, stride, n, visit);
 }
 
 // The sum of x over the threads before this one, and over all (in `all`); `words`: one per wave, not
@@ -106,31 +139,66 @@ __device__ __attribute__((always_inline)) inline unsigned scan_threads(unsigned 
   return before + incl - x;
 }
 
-// Token t of the step, its request's running sums and base given.
-__device__ __attribute__((always_inline)) inline void put_token(const AttnPagePlanParams& p,
-                                                                unsigned t, unsigned row,
-                                                                unsigned first, unsigned base) {
-  int32_t slot = -1;
-  unsigned pos = 0, sees = 0;
-  if (row < p.batch && base != kNotHere &&
-      ((base + (t - first)) >> p.log2_page) < p.max_pages) {  // (sums beyond 32 bits may break order)
-    pos = base + (t - first);
-    const unsigned page = static_cast<unsigned>(
-        p.page_table[std::size_t{row} * p.max_pages + (pos >> p.log2_page)]);
-    if (page < p.pool_pages)
-      slot = static_cast<int32_t>((page << p.log2_page) + (pos & ((1u << p.log2_page) - 1u)));
-    sees = pos + 1;
+// The step's tokens first, first + stride, .. of kMany x stride (a part of max_tokens): ends, need: running
+// sums of tokens and of pages handed out; base: lengths before; the pages handed out lie below `top`.
+template <unsigned kMany>
+__device__ __attribute__((always_inline)) inline void put_tokens(
+    const AttnPagePlanParams& p, unsigned t0, unsigned stride, const unsigned* ends,
+    const unsigned* need, const unsigned* base, unsigned top) {
+  unsigned t[kMany], s[kMany], at[kMany], seen[kMany];
+  int32_t page[kMany];
+#pragma unroll
+  for (unsigned i = 0; i < kMany; ++i)
+    t[i] = t0 + i * stride;
+  owners_of(ends, p.batch, t, s);
+#pragma unroll
+  for (unsigned i = 0; i < kMany; ++i) {
+    const bool any = s[i] < p.batch;
+    const unsigned row = any ? s[i] : 0u, before = row != 0 ? row - 1 : 0u;
+    const unsigned from = base[row], pos = from + (t[i] - (row != 0 ? ends[before] : 0u));
+    const unsigned entry = pos >> p.log2_page, held = pages_of(from, p.log2_page);
+    const unsigned taken = (row != 0 ? need[before] : 0u) + (entry - held);
+    // (A sum of n_new beyond 32 bits breaks the order: entries and stack are checked.)
+    const bool good = any && from != kNotHere && t[i] < p.max_tokens && entry < p.max_pages &&
+                      (entry < held || taken < top);
+    page[i] = -1;
+    if (good)
+      page[i] = entry < held ? p.page_table[std::size_t{row} * p.max_pages + entry]
+                             : p.free_pages[top - 1 - taken];
+    s[i] = row;
+    at[i] = good ? pos : 0u;
+    seen[i] = good ? pos + 1 : 0u;
   }
-  p.slots[t] = slot;
-  p.positions[t] = pos;
-  p.rows[t] = row < p.batch ? static_cast<int32_t>(row) : 0;
-  p.visible[t] = sees;
+#pragma unroll
+  for (unsigned i = 0; i < kMany; ++i) {
+    if (t[i] >= p.max_tokens)
+      break;
+    const bool good = static_cast<unsigned>(page[i]) < p.pool_pages;
+    p.slots[t[i]] = good ? (page[i] << p.log2_page) +
+                               static_cast<int32_t>(at[i] & ((1u << p.log2_page) - 1u))
+                         : -1;
+    p.positions[t[i]] = at[i];
+    p.rows[t[i]] = static_cast<int32_t>(s[i]);
+    p.visible[t[i]] = seen[i];
+  }
+}
+
+// Entries of the pages handed out, by `stride` threads.
+__device__ __attribute__((always_inline)) inline void put_pages(const AttnPagePlanParams& p,
+                                                                unsigned thread, unsigned stride,
+                                                                const unsigned* need,
+                                                                const unsigned* base, unsigned top,
+                                                                unsigned taken) {
+  each_of(need, p.batch, thread, stride, taken, [&](unsigned k, unsigned s, unsigned at) {
+    p.page_table[std::size_t{s} * p.max_pages + pages_of(base[s], p.log2_page) + at] =
+        p.free_pages[top - 1 - k];
+  });
 }
 
 }  // namespace pages_detail
 
-// Steps 1 to 3 (and 4, kTokens: the step's tokens too), one workgroup; a thread holds kPer requests
-// in order.
+// The lengths, the stack and the prefix's entries, one workgroup, a thread holding kPer requests in order;
+// kTokens: the pages handed out and the step's tokens too, which attn_page_tokens_kernel does otherwise.
 template <unsigned kPer, bool kTokens>
 __global__ void __launch_bounds__(pages_detail::kThreads) attn_page_plan_kernel(
     AttnPagePlanParams p) {
@@ -187,18 +255,15 @@ __global__ void __launch_bounds__(pages_detail::kThreads) attn_page_plan_kernel(
     }
   }
   __syncthreads();  // sh.back whole, and the scans' words free again
-  for (unsigned k = t; k < all_back; k += kThreads) {
-    const unsigned s = owner_of(sh.back, p.batch, k);
-    const unsigned before = s != 0 ? sh.back[s - 1] : 0u;
+  each_of(sh.back, p.batch, t, kThreads, all_back, [&](unsigned k, unsigned s, unsigned at) {
     if (free0 + k < p.pool_pages)
-      p.free_pages[free0 + k] =
-          p.page_table[std::size_t{s} * p.max_pages + p.prefix_pages + (k - before)];
-  }
+      p.free_pages[free0 + k] = p.page_table[std::size_t{s} * p.max_pages + p.prefix_pages + at];
+  });
   unsigned all_need;
   unsigned at_need = scan_threads(n_need, sh.wave[0], all_need);  // its barrier: the stack is whole
 
   unsigned taken = 0;  // pages handed out, up to this thread's last request that got some
-  unsigned long long starting = 0;
+  unsigned long long starting[kPer];  // of the wave's lanes: those whose request starts
 #pragma unroll
   for (unsigned i = 0; i < kPer; ++i) {
     const unsigned s = t * kPer + i;
@@ -214,20 +279,23 @@ __global__ void __launch_bounds__(pages_detail::kThreads) attn_page_plan_kernel(
       sh.need[s] = at_need;
       sh.base[s] = grows ? base[i] : kNotHere;
     }
-    // Requests that start: the wave copies the prefix's entries for each of them.
-    starting = __builtin_amdgcn_ballot_w64(s < p.batch && grows && len[i] == 0);
-    while (starting != 0) {
-      const unsigned l = static_cast<unsigned>(__builtin_ctzll(starting));
-      starting &= starting - 1;
-      const std::size_t row = std::size_t{(t - lane + l) * kPer + i} * p.max_pages;
-      for (unsigned j = lane; j < p.prefix_pages; j += 64)
-        p.page_table[row + j] = p.prefix_table[j];
-    }
+    starting[i] = __builtin_amdgcn_ballot_w64(s < p.batch && grows && len[i] == 0);
     if (s < p.batch) {
       p.lens_out[s] = grows ? base[i] + grow[i] : len[i];
       p.status[s] = why[i];
       p.starts[s + 1] = first[i] + grow[i];
     }
+  }
+  // The prefix's entries of the requests that start, a wave at a time.
+  for (unsigned j = lane; j - lane < p.prefix_pages; j += 64) {
+    const int32_t page = p.prefix_table[min(j, p.prefix_pages - 1)];
+#pragma unroll
+    for (unsigned i = 0; i < kPer; ++i)
+      for (unsigned long long left = starting[i]; left != 0; left &= left - 1) {
+        const unsigned s = (t - lane + static_cast<unsigned>(__builtin_ctzll(left))) * kPer + i;
+        if (j < p.prefix_pages)
+          p.page_table[std::size_t{s} * p.max_pages + j] = page;
+      }
   }
 #pragma unroll
   for (unsigned o = 1; o < 64; o *= 2)
@@ -239,49 +307,57 @@ __global__ void __launch_bounds__(pages_detail::kThreads) attn_page_plan_kernel(
 #pragma unroll
   for (unsigned o = 1; o < kWaves; o *= 2)
     taken = max(taken, static_cast<unsigned>(__shfl_xor(static_cast<int>(taken), o)));
-  for (unsigned k = t; k < taken; k += kThreads) {
-    const unsigned s = owner_of(sh.need, p.batch, k);
-    const unsigned before = s != 0 ? sh.need[s - 1] : 0u;
-    const unsigned at = pages_of(sh.base[s], p.log2_page) + (k - before);
-    p.page_table[std::size_t{s} * p.max_pages + at] = p.free_pages[top - 1 - k];
-  }
   if (t == 0) {
     p.starts[0] = 0;
     *p.n_free_out = top - taken;
   }
   if constexpr (kTokens) {
-    __syncthreads();  // the tables are whole
-    for (unsigned i = t; i < p.max_tokens; i += kThreads) {
-      const unsigned s = i < all_tokens ? owner_of(sh.tokens, p.batch, i) : p.batch;
-      put_token(p, i, s, s != 0 && s < p.batch ? sh.tokens[s - 1] : 0u,
-                s < p.batch ? sh.base[s] : kNotHere);
+    put_pages(p, t, kThreads, sh.need, sh.base, top, taken);
+    if (p.max_tokens <= kThreads) {
+      if (t < p.max_tokens)
+        put_tokens<1>(p, t, kThreads, sh.tokens, sh.need, sh.base, top);
+    } else {
+      for (unsigned t0 = t; t0 < p.max_tokens; t0 += 4 * kThreads)
+        put_tokens<4>(p, t0, kThreads, sh.tokens, sh.need, sh.base, top);
     }
   }
 }
 
-// Step 4 of many tokens, 1024 a workgroup, behind the launch above.
+// The pages handed out and the step's tokens where those are many, 1024 tokens a workgroup, behind the
+// launch above: what that one knew of the requests follows from what it left.
 template <int = 0>
 __global__ void __launch_bounds__(256) attn_page_tokens_kernel(AttnPagePlanParams p) {
   using namespace pages_detail;
-  __shared__ unsigned ends[kAttnPlanMaxBatch];
-  for (unsigned s = threadIdx.x; s < p.batch; s += 256)
-    ends[s] = p.starts[s + 1];
-  __syncthreads();
-  const unsigned all = ends[p.batch - 1];
-#pragma unroll
-  for (unsigned j = 0; j < 4; ++j) {
-    const unsigned i = 1024 * blockIdx.x + 256 * j + threadIdx.x;
-    if (i >= p.max_tokens)
-      return;
-    const unsigned s = i < all ? owner_of(ends, p.batch, i) : p.batch;
-    unsigned first = 0, base = kNotHere;
-    if (s < p.batch) {
-      first = s != 0 ? ends[s - 1] : 0u;
-      if (p.status[s] == kFits)
-        base = p.lens_out[s] - (ends[s] - first);
-    }
-    put_token(p, i, s, first, base);
+  __shared__ unsigned ends[kAttnPlanMaxBatch], need[kAttnPlanMaxBatch], base[kAttnPlanMaxBatch];
+  __shared__ unsigned words[4];
+  const unsigned t = threadIdx.x, lane = t & 63u;
+  for (unsigned s = t; s < p.batch; s += 256) {
+    const unsigned end = p.starts[s + 1], grow = end - p.starts[s];
+    const unsigned len = p.lens_out[s], from = len - grow;
+    const bool here = grow != 0 && p.status[s] == kFits;
+    ends[s] = end;
+    base[s] = here ? from : kNotHere;
+    need[s] = here ? pages_of(len, p.log2_page) - pages_of(from, p.log2_page) : 0u;
   }
+  __syncthreads();
+  // need's running sums, each thread's share of the requests in order.
+  const unsigned per = (p.batch + 255) / 256, s0 = min(t * per, p.batch), s1 = min(s0 + per, p.batch);
+  unsigned mine = 0;
+  for (unsigned s = s0; s < s1; ++s)
+    mine += need[s];
+  const unsigned incl = decode_detail::wave_prefix_sum(mine);
+  if (lane == 63)
+    words[t >> 6] = incl;
+  __syncthreads();
+  unsigned sum = incl - mine;
+  for (unsigned w = 0; w < t >> 6; ++w)
+    sum += words[w];
+  for (unsigned s = s0; s < s1; ++s)
+    need[s] = sum += need[s];
+  __syncthreads();
+  const unsigned taken = need[p.batch - 1], top = *p.n_free_out + taken;
+  put_tokens<4>(p, 1024 * blockIdx.x + t, 256, ends, need, base, top);
+  put_pages(p, 256 * blockIdx.x + t, 256 * gridDim.x, need, base, top, taken);
 }
 
 // Up to this many tokens are placed by the first launch.
