@@ -131,6 +131,16 @@ def test_plan_equals_a_loop(torch_mod, attn, batch, page, prefix, most_len, most
     same(run_plan(torch_mod, attn, s, in_place, with_ended=False), plan_ref(s))
 
 
+@pytest.mark.parametrize("batch,prefix,most_len,most_new,short", [
+    (300, 70, 1200, 40, False), (300, 70, 1200, 40, True), (2000, 66, 300, 3, True),
+    (1500, 130, 90, 30, False), (64, 64, 6000, 1, False), (2, 65, 50000, 9000, False)])
+def test_plan_of_many_pages(torch_mod, attn, batch, prefix, most_len, most_new, short):
+    """Long prefixes, thousands of pages that go back, prompts of more tokens than one launch places."""
+    s = scenario(np.random.default_rng(batch + prefix), batch, 8, prefix, most_len, most_new, short)
+    s["ended"][0] = s["lens"][0] > 0
+    same(run_plan(torch_mod, attn, s, True), plan_ref(s))
+
+
 def test_plan_refuses_requests_alone(torch_mod, attn):
     """A row too long for its table, tokens behind max_tokens, no pages: the others go on."""
     s = dict(lens=np.array([30, 5, 0, 16, 8, 3]), new=np.array([3, 2, 9, 1, 8, 4]),

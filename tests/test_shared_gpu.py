@@ -193,6 +193,22 @@ def test_every_count_of_tiles_in_a_span(torch_mod, attn, batch, tiles):
     check(torch_mod, c.run(attn), c.ref())
 
 
+@pytest.mark.parametrize("batch,prefix_pages", [(3, 300), (7, 300), (24, 128), (150, 600), (490, 160)])
+def test_cut_by_the_lengths(torch_mod, attn, batch, prefix_pages):
+    """A scratch for 4000 own keys and batches that have far fewer, or nearly those: the CUs of the prefix
+    and of the own keys, and the spans with them, follow the lengths; one scratch serves all."""
+    rng = np.random.default_rng(batch)
+    sc = None
+    for own in (0, 1, 40, 300, 3990 if batch < 100 else 900):
+        c = Paged(torch_mod, 16, prefix_pages, lengths(rng, batch, 16 * prefix_pages, own), batch,
+                  room=prefix_pages + 250)
+        sc = sc or c.scratch(attn, max_own=4000)
+        first = c.run(attn, sc).clone()
+        check(torch_mod, first, c.ref(), own)
+        sc.ws.fill_(255)
+        assert torch_mod.equal(c.run(attn, sc), first), own
+
+
 def test_spans_longer_than_the_page_ids_a_wave_holds(torch_mod, attn):
     """More than 64 tiles a span: its pages are read again, and tiles wrap the ring many times."""
     lens = 90112 + np.arange(30) % 7
