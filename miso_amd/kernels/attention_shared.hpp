@@ -230,11 +230,11 @@ __device__ __attribute__((always_inline)) inline void settle_operands(half8_t (&
   }
 }
 
-// Two numerators as halves: hi rounded towards zero, lo what is left (2^-21 of the numerator, or 2^-25).
-// Volatile: the compiler would move them below the MFMAs that they stand between. The no-op: the
-// numerators come from exponentials, whose results need a wait state.
-__device__ __attribute__((always_inline)) inline void numerator_pair(float a, float b, unsigned& h,
-                                                                     unsigned& l) {
+// Two values as halves: hi rounded towards zero, lo what is left (2^-21 of the value, or 2^-25).
+// Volatile: the compiler would move a tile's numerators below the MFMAs that they stand between. The
+// no-op: they come from exponentials, whose results need a wait state.
+__device__ __attribute__((always_inline)) inline void half_pair(float a, float b, unsigned& h,
+                                                                unsigned& l) {
   float rest;
   asm volatile(
       "s_nop 0\n\t"
@@ -401,22 +401,20 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
     top = cdna4::max_xor32(top);
     int e = 13 - (static_cast<int>(cdna4::as_uint(top) >> 23) - 127);
     e = top == 0.0f || !(top < __builtin_inff()) ? 0 : (e < 100 ? e : 100);
-    const float up = __builtin_ldexpf(1.0f, e);
+    const float up = __builtin_ldexpf(decode_detail::kLog2e, e);
     scale = __builtin_ldexpf(1.0f / 16.0f, -e);
 #pragma unroll
-    for (unsigned c = 0; c < 2 * kSteps; ++c)
+    for (unsigned k = 0; k < kSteps; ++k) {
+      struct alignas(16) Halves {
+        unsigned w[4];
+      } h, l;
 #pragma unroll
-      for (int j = 0; j < 4; j += 2) {
-        const float y0 = v[c][j] * up * decode_detail::kLog2e;
-        const float y1 = v[c][j + 1] * up * decode_detail::kLog2e;
-        const cdna4::half2_t h =
-            __builtin_bit_cast(cdna4::half2_t, __builtin_amdgcn_cvt_pkrtz(y0, y1));
-        const unsigned k = 4 * (c % 2) + j;
-        qh[c / 2][k] = h[0];
-        qh[c / 2][k + 1] = h[1];
-        ql[c / 2][k] = static_cast<_Float16>(y0 - static_cast<float>(h[0]));
-        ql[c / 2][k + 1] = static_cast<_Float16>(y1 - static_cast<float>(h[1]));
-      }
+      for (unsigned j = 0; j < 4; ++j)
+        half_pair(v[2 * k + j / 2][2 * (j % 2)] * up, v[2 * k + j / 2][2 * (j % 2) + 1] * up, h.w[j],
+                  l.w[j]);
+      qh[k] = __builtin_bit_cast(half8_t, h);
+      ql[k] = __builtin_bit_cast(half8_t, l);
+    }
   }
   if constexpr (kEarly == 1) {
     decode_detail::tile_barrier();  // every wave has its operands: the ring takes the space
@@ -503,7 +501,7 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
   };
   unsigned ph[8], pl[8];  // pairs of numerators, hi and lo halves
   auto pair = [&](unsigned i) __attribute__((always_inline)) {
-    numerator_pair(w[i], w[i + 1], ph[i / 2], pl[i / 2]);
+    half_pair(w[i], w[i + 1], ph[i / 2], pl[i / 2]);
   };
   // After a tile's numerators w (their sum given): the reference follows where they are too large.
   auto settle = [&](float sum) __attribute__((always_inline)) {
