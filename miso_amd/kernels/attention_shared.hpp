@@ -182,23 +182,37 @@ __device__ __attribute__((always_inline)) inline void scale_values(float16_t (&o
     }
 }
 
-// Four copies of copy_tile: rows 2 i + lane / 32 of the 8 at `row`, lane offsets `off` less 1024 i.
-__device__ __attribute__((always_inline)) inline void copy_rows(const attn::half_t* row,
-                                                                const unsigned (&off)[4],
-                                                                unsigned to) {
-  unsigned saved;
+// Rows 2 i and 2 i + 1 of the 8 at `row` to LDS (attention_decode.hpp's copy_tile, one instruction of it),
+// the lane offset `off` less 1024 i: the instruction's offset counts on both sides. `lanes`: all, or none
+// (a branch would part what the compiler places between the MFMAs).
+template <unsigned kI>
+__device__ __attribute__((always_inline)) inline void copy_rows_at(const attn::half_t* row,
+                                                                   unsigned off, unsigned to,
+                                                                   unsigned long long lanes) {
+  unsigned m0;
+  unsigned long long exec;
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %6\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, %5\n\t"
-      "global_load_lds_dwordx4 %2, %5 offset:1024\n\t"
-      "global_load_lds_dwordx4 %3, %5 offset:2048\n\t"
-      "global_load_lds_dwordx4 %4, %5 offset:3072\n\t"
+      "s_mov_b32 m0, %4\n\t"
+      "s_and_saveexec_b64 %1, %5\n\t"
+      "global_load_lds_dwordx4 %2, %3 offset:%6\n\t"
+      "s_mov_b64 exec, %1\n\t"
       "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(row), "s"(to)
-      : "memory");
+      : "=&s"(m0), "=&s"(exec)
+      : "v"(off), "s"(row), "s"(to), "s"(lanes), "n"(1024 * kI)
+      : "memory", "scc");
+}
+__device__ __attribute__((always_inline)) inline void copy_rows(const attn::half_t* row, unsigned off,
+                                                                unsigned to, unsigned i,
+                                                                unsigned long long lanes) {
+  if (i == 0)
+    copy_rows_at<0>(row, off, to, lanes);
+  else if (i == 1)
+    copy_rows_at<1>(row, off, to, lanes);
+  else if (i == 2)
+    copy_rows_at<2>(row, off, to, lanes);
+  else
+    copy_rows_at<3>(row, off, to, lanes);
 }
 
 // Wait states behind the last MFMA of O, tied to its registers: what the compiler copies of them, it
@@ -295,8 +309,9 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
 
   // ---- Tiles: this wave copies rows 8 wave .. + 7 of K and V (instruction i rows 2 i + lane / 32 of
   // them, chunks swizzled as attention_prefill.hpp's tiles). Rows past the prefix's last one repeat it
-  // (they are masked at use). The lane offsets are unsigned, and a repeated row lies up to 3072 bytes
-  // below its instruction's: offsets are that much larger, their base that much lower.
+  // (they are masked at use): the last tile's, so that its offsets can take the place of the others'. The
+  // lane offsets are unsigned, and a repeated row lies up to 3072 bytes below its instruction's: offsets
+  // are that much larger, their base that much lower.
   constexpr unsigned kBelow = 3072;
   unsigned koff[4], voff[4];
 #pragma unroll
@@ -310,10 +325,17 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
   struct Place {
     const attn::half_t* k;
     const attn::half_t* v;
-    unsigned most;  // the last of the 8 rows that exists
   };
   auto place_of = [&](unsigned ti) __attribute__((always_inline)) {
     const unsigned want = ti * kKeys + 8 * wave, row = want < last ? want : last;
+    if (last - row < 7) {  // uniform
+#pragma unroll
+      for (unsigned i = 0; i < 4; ++i) {
+        const unsigned r = 2 * i + (lane >> 5), past = r > last - row ? r - (last - row) : 0u;
+        koff[i] -= 512 * past;
+        voff[i] -= 512 * past;
+      }
+    }
     std::size_t at;  // of the row, in halves
     if constexpr (kPaged) {
       if (ti - page0 >= 64u) {  // uniform
@@ -333,27 +355,22 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
     return Place{decode_detail::uniform(reinterpret_cast<const attn::half_t*>(
                      reinterpret_cast<std::uintptr_t>(p.prefix.k) + base)),
                  decode_detail::uniform(reinterpret_cast<const attn::half_t*>(
-                     reinterpret_cast<std::uintptr_t>(p.prefix.v) + base)),
-                 last - row};
+                     reinterpret_cast<std::uintptr_t>(p.prefix.v) + base))};
   };
-  auto copy = [&](const Place& from, unsigned to, bool is_v) __attribute__((always_inline)) {
-    unsigned off[4];
-#pragma unroll
-    for (unsigned i = 0; i < 4; ++i)
-      off[i] = is_v ? voff[i] : koff[i];
-    if (from.most < 7)  // uniform
-#pragma unroll
-      for (unsigned i = 0; i < 4; ++i) {
-        const unsigned r = 2 * i + (lane >> 5);
-        off[i] -= 512 * (r > from.most ? r - from.most : 0);
-      }
-    copy_rows(is_v ? from.v : from.k, off, to + 4096 * wave + (is_v ? kTileBytes : 0));
+  // Copy j < 8 of a tile to its stage: two rows of K, then of V.
+  auto copy = [&](const Place& from, unsigned to, unsigned j, unsigned long long lanes = ~0ull)
+      __attribute__((always_inline)) {
+    if (j < 4)
+      copy_rows(from.k, koff[j], to + 4096 * wave, j, lanes);
+    else
+      copy_rows(from.v, voff[j - 4], to + 4096 * wave + kTileBytes, j - 4, lanes);
   };
   // Stages are named by their offset in the ring; tile t0 takes the last one.
   auto issue = [&](unsigned ti, unsigned to) __attribute__((always_inline)) {
     const Place from = place_of(ti);
-    copy(from, lds + to, false);
-    copy(from, lds + to, true);
+#pragma unroll
+    for (unsigned j = 0; j < 8; ++j)
+      copy(from, lds + to, j);
   };
   // ---- Queries: row r of a block is sequence 4 block + r / 8, head 8 kvh + r % 8. The waves of a block
   // copy its rows to LDS (1 KiB each, 16-byte chunk c of row r at c ^ (r % 16)) and every lane reads the
@@ -503,14 +520,18 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
   auto pair = [&](unsigned i) __attribute__((always_inline)) {
     half_pair(w[i], w[i + 1], ph[i / 2], pl[i / 2]);
   };
+  // The reference for scores x.
+  auto reference = [&]() __attribute__((always_inline)) {
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i)
+      top = fmaxf(top, x[i]);
+    return fmaxf(m, cdna4::max_xor32(top) * scale - kLead);
+  };
   // After a tile's numerators w (their sum given): the reference follows where they are too large.
   auto settle = [&](float sum) __attribute__((always_inline)) {
-    if (__builtin_amdgcn_ballot_w64(sum > kMost) != 0) {  // rare, and the first tile
-      float top = x[0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i)
-        top = fmaxf(top, x[i]);
-      top = fmaxf(m, cdna4::max_xor32(top) * scale - kLead);
+    if (__builtin_amdgcn_ballot_w64(sum > kMost) != 0) {  // rare
+      const float top = reference();
       const float corr = __builtin_amdgcn_exp2f(m - top);
       m = top;
       l *= corr;
@@ -600,6 +621,8 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
 #pragma unroll
   for (unsigned i = 0; i < 16; ++i)
     x[i] = cur[i];
+  mask(t0);
+  m = reference();
 
   // Step ti: the scores of tile ti into cur, beside them the numerators of tile ti - 1 (x), then its
   // P V; tile ti + 3 is copied meanwhile. Between two score MFMAs stand an fma, an exponential and a sum
@@ -614,7 +637,10 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
       mask(ti - 1);
       Place from{};
       const bool more = ti + 3 < t1, next_tile = ti + 1 < t1;  // uniform
+      unsigned long long lanes;  // more ? ~0 : 0 (as C++ the compiler takes it through VGPRs)
+      asm("s_cmp_lt_u32 %1, %2\n\ts_cselect_b64 %0, -1, 0" : "=s"(lanes) : "s"(ti + 3), "s"(t1) : "scc");
       float sum[2] = {0.0f, 0.0f}, e[16];
+      constexpr unsigned kCopy = 2;  // the k-step of the first copy, one each
       // Numerators of k-step k: 16 in 13 steps.
       constexpr auto at = [](unsigned k) { return k >= 13 ? 16u : (16 * k + 12) / 13; };
 #pragma unroll
@@ -638,14 +664,10 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
         if (k >= 9 && k < 13)
           pair(2 * (k - 9));
         a[k % 4] = next;
-        if (more) {
-          if (k == 0)
-            from = place_of(ti + 3);
-          if (k == 2)
-            copy(from, spare, false);
-          if (k == 4)
-            copy(from, spare, true);
-        }
+        if (k == 0 && more)
+          from = place_of(ti + 3);
+        if (k >= kCopy && k < kCopy + 8)
+          copy(from, spare, k - kCopy, lanes);
         if (k >= kSteps - 4)
           va[k + 4 - kSteps] = values(before, k + 4 - kSteps);
       }
