@@ -640,7 +640,6 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
       unsigned long long lanes;  // more ? ~0 : 0 (as C++ the compiler takes it through VGPRs)
       asm("s_cmp_lt_u32 %1, %2\n\ts_cselect_b64 %0, -1, 0" : "=s"(lanes) : "s"(ti + 3), "s"(t1) : "scc");
       float sum[2] = {0.0f, 0.0f}, e[16];
-      constexpr unsigned kCopy = 2;  // the k-step of the first copy, one each
       // Numerators of k-step k: 16 in 13 steps.
       constexpr auto at = [](unsigned k) { return k >= 13 ? 16u : (16 * k + 12) / 13; };
 #pragma unroll
@@ -656,6 +655,8 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
 #pragma unroll
           for (unsigned i = at(k - 1); i < at(k); ++i)
             w[i] = __builtin_amdgcn_exp2f(e[i]);
+        if (k % 2 == 1)
+          copy(from, spare, k / 2, lanes);
         score_lo(cur, a[k % 4], ql[k]);
         if (k > 1)
 #pragma unroll
@@ -666,8 +667,6 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
         a[k % 4] = next;
         if (k == 0 && more)
           from = place_of(ti + 3);
-        if (k >= kCopy && k < kCopy + 8)
-          copy(from, spare, k - kCopy, lanes);
         if (k >= kSteps - 4)
           va[k + 4 - kSteps] = values(before, k + 4 - kSteps);
       }
