@@ -28,7 +28,11 @@ namespace miso::kernels {
 //      (pages, its table row, the step's tokens) keeps its length; status says why.
 //   4. Token t of the step (request by request): its request, position, slot and the keys it sees.
 // Nothing here is more than a few words per request and token: the launches and the dependent steps
-// (two scans, the pages, the tokens behind them) are its time.
+// (loads, three scans, a search per page and token) are its time. One workgroup does it, since the
+// steps depend on sums over all requests; with more than kAttnPlanOneLaunch tokens a second launch spreads
+// the pages and tokens over the CUs. 64 requests of a token each: 4.9 us. 512 with prompts, 66 thousand
+// tokens, some ending: 9.8 + 7.3 us (13.4 + 7.0 with the pages handed out by the first launch and one
+// search at a time).
 // ------------------------------------------------------------------------------------------------
 
 struct AttnPagePlanParams {
@@ -360,7 +364,8 @@ __global__ void __launch_bounds__(256) attn_page_tokens_kernel(AttnPagePlanParam
   put_pages(p, 256 * blockIdx.x + t, 256 * gridDim.x, need, base, top, taken);
 }
 
-// Up to this many tokens are placed by the first launch.
+// Up to this many tokens are placed by the first launch: 64 requests with 3523 tokens 6.8 us there, 3.7 +
+// 4.7 in two; 512 with 2434 12.7 and 9.2 + 5.8, with 4450 15.0 and 9.2 + 6.5.
 constexpr unsigned kAttnPlanOneLaunch = 4096;
 
 inline void attn_page_plan_launch(const AttnPagePlanParams& p, hipStream_t stream) {
@@ -390,7 +395,13 @@ inline void attn_page_plan_launch(const AttnPagePlanParams& p, hipStream_t strea
 // the pool)) is left out: nothing of it is read or written.
 //
 // The angle is formed and reduced to (-pi, pi] in 64 bits: pos x inv_freq in f32 is off by up to 0.008
-// rad at position 262143, and the rotation by as much.
+// rad at position 262143, and the rotation by as much. K and V are rounded to f16, half a step, as the caches
+// hold them; all else is f32.
+//
+// A workgroup per token, a head a wave at a time (64 lanes x 4 dimensions), three heads a wave with all
+// loads in flight before the first use: the rotation's partners lie in the same wave, its sines are
+// computed once for the token. Bound by memory: 70 KiB a token. 4096 tokens 55.9 us, 5.2 TB/s of those
+// bytes (the caches keep some of them); 1001 11.7; 64 3.9; 1 2.7, a launch.
 // ------------------------------------------------------------------------------------------------
 
 struct AttnPrepPagedParams {

@@ -58,6 +58,11 @@ struct AttnSharedParams {
   unsigned own_least;  // and the workgroups that the own keys take at least
 };
 
+// Own keys of one sequence in tiles, as attn_shared_cost counts them: both heads, four waves.
+__host__ __device__ constexpr unsigned attn_shared_own_tiles(unsigned keys) {
+  return 8 * (keys / 128 + (keys % 128 != 0));
+}
+
 // Where a split launch cuts the prefix.
 struct AttnSharedCut {
   unsigned spans, span_tiles, grid;  // grid: the prefix's workgroups, a multiple of 8
@@ -72,11 +77,12 @@ __host__ __device__ constexpr unsigned attn_shared_row_blocks(unsigned batch) {
 // What the tiles of a launch cost on `cus` CUs, a workgroup each, in us without the fixed part: the
 // slower side, or the span and its share of the `own` tiles of own keys (both heads') one after the
 // other. A tile of a span behind 64 sequences takes 1.5 us (32768 keys of 40 tiles a span: 70 us), behind
-// 8 1.0 (9 tiles: 23 us, 12: 26), behind 3 0.9; of the own keys 1.4 (48 workgroups: 72 us, 32: 97); the
-// own keys' start behind a span 7.
+// 8 1.0 (9 tiles: 23 us, 12: 26), behind 3 0.9; of the own keys 1.4 (48 workgroups: 72 us, 32: 97), four
+// at a time, a wave each: a sequence of 5 keys counts as four tiles (106 of them on 32 CUs: 45 us); the own
+// keys' start behind a span 14 (256 behind 8192 keys, 256 each: 92 us of 32 tiles and 12, 80 of 43 beside 48).
 template <unsigned kRowBlocks>
 constexpr float kAttnSharedTile = kRowBlocks == 4 ? 1.5f : kRowBlocks == 2 ? 1.0f : 0.9f;
-constexpr float kAttnSharedOwnTile = 1.5f, kAttnSharedOwnStart = 7.0f;
+constexpr float kAttnSharedOwnTile = 1.5f, kAttnSharedOwnStart = 14.0f;
 template <unsigned kRowBlocks>
 __host__ __device__ constexpr float attn_shared_cost(const AttnSharedCut& c, unsigned own,
                                                      unsigned cus) {
@@ -110,13 +116,17 @@ __host__ __device__ constexpr AttnSharedCut attn_shared_cut(unsigned tiles, unsi
     return cut(most, false);
   AttnSharedCut best = cut(most, true);
   float cost = attn_shared_cost<kRowBlocks>(best, own, cus);
-  // The spans with which both sides end together, and one more.
+  // The spans with which both sides end together, and one more; no more than leave `least` CUs.
   const float prefix = kAttnSharedTile<kRowBlocks> * static_cast<float>(tiles);
   const float keys = kAttnSharedOwnTile * static_cast<float>(own);
   const unsigned even = static_cast<unsigned>(prefix * static_cast<float>(cus) /
                                               (keys + prefix * static_cast<float>(pairs)));
+  const unsigned room = cus > least + 7 ? (cus - least) / 8 * 8 / pairs : 0;
+  const unsigned top = room < most ? room : most;
+  if (top == 0)
+    return best;
   for (unsigned i = 0; i < 2; ++i) {
-    const unsigned spans = even + i < most ? even + i : most;
+    const unsigned spans = even + i < top ? even + i : top;
     const AttnSharedCut c = cut(spans < 1 ? 1 : spans, false);
     if (c.grid + least > cus)
       continue;
@@ -282,7 +292,18 @@ __device__ __attribute__((always_inline)) inline unsigned own_keys(const AttnSha
 // MFMAs, each K operand read serving both halves; and each of the 4 / kRowBlocks waves of a row block
 // adds P V for its share of the 256 dimensions (all 8 blocks of 32 dimensions: 32 MFMAs). So a wave's
 // tile is 64, 48 or 40 MFMAs of 32 cycles for 4, 2 and 1 row blocks: with few rows the memory sets the
-// pace (32 KiB a tile and CU), with many the matrix units.
+// pace (32 KiB a tile and CU), with many the matrix units. More rows a workgroup would read the tiles less
+// often, but 32 rows a wave take all its registers (O 128, queries 128, scores and numerators 48).
+//
+// Softmax in one pass: per row a reference m (log2 units), the sum of numerators 2^(s - m), and O relative
+// to 2^m; m starts kLead below the first tile's maximum and moves only when numerators grow too large.
+// Tiles come through a ring of five stages, three under way; a step adds the scores of a tile while the
+// numerators of the one before are formed between its MFMAs, then that one's P V.
+//
+// 64 sequences behind 131072 keys: 1.75 us a tile and CU, 1230 TFLOP/s of f16 products (an 8192^3 library
+// product: 1076), 2960 cycles for 2048 of MFMAs at 1.65 GHz. There the power sets the pace: with 4% fewer
+// cycles (the copies placed elsewhere) the clock fell by as much. 8 behind 32768 keys: 22.3 us, 3.2 TB/s,
+// 11 of them in the loop at 5.2 TB/s, 5 before it (queries from memory and cut, three tiles on their way).
 namespace shared_detail {
 template <unsigned kRowBlocks, bool kPaged>
 __device__ __attribute__((always_inline)) inline void prefix_span(const AttnSharedParams& p,
@@ -770,8 +791,9 @@ struct AttnSharedOwn {
 };
 
 // The first p.prefix_grid workgroups take the prefix's spans, those from p.own_first on the sequences' own
-// keys. Where the lengths decide on how many CUs either does best, which only the device knows, each wave
-// makes the choice before anything else.
+// keys: one launch, side by side (3 sequences behind 512 keys 10.5 us, in two launches 17). Where the
+// lengths decide on how many CUs either does best, which only the device knows, each wave makes the choice
+// before anything else, 1.1 us.
 template <unsigned kRowBlocks, bool kPaged>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
 attn_shared_split_kernel(AttnSharedParams p, AttnSharedOwn own) {
@@ -780,9 +802,9 @@ attn_shared_split_kernel(AttnSharedParams p, AttnSharedOwn own) {
   if (p.chosen != nullptr) {  // uniform
     float tiles = 0.0f;
     for (unsigned s = threadIdx.x & 63u; s < p.batch; s += 64)
-      tiles += __builtin_ceilf(static_cast<float>(shared_detail::own_keys(p, s)) * (1.0f / 32.0f));
+      tiles += static_cast<float>(attn_shared_own_tiles(shared_detail::own_keys(p, s)));
     const unsigned all = __builtin_amdgcn_readfirstlane(
-        static_cast<unsigned>(fminf(2.0f * cdna4::wave_allsum(tiles), 0x1p30f)));
+        static_cast<unsigned>(fminf(cdna4::wave_allsum(tiles), 0x1p30f)));
     const AttnSharedCut cut = attn_shared_cut<kRowBlocks>(
         (p.prefix.len - 1) / 32 + 1, 2 * ((p.blocks + kRowBlocks - 1) / kRowBlocks), all, gridDim.x,
         p.own_least);
@@ -818,7 +840,8 @@ attn_shared_split_kernel(AttnSharedParams p, AttnSharedOwn own) {
 // relative to 2^M in span order), and meet in LDS; then a thread per (row, 4 dimensions) adds the
 // waves' sums and the own keys' splits in order, divides and applies the gate. The order is fixed.
 // Bound by the partials it reads, 1 KiB a row and span; a CU takes in only so much of them, so with
-// few row blocks their dimensions are spread over four times the workgroups.
+// few row blocks their dimensions are spread over four times the workgroups (8 sequences, 114 spans: 6.6 us;
+// 12 with all dimensions of 32 in a workgroup). 3 sequences, 4 spans: 3.9 us, 64 and 26: 8.6, 256 and 6: 9.0.
 // ------------------------------------------------------------------------------------------------
 
 template <unsigned kQuads>
@@ -1009,22 +1032,23 @@ inline void attn_shared_launch_as(AttnSharedParams p, const AttnSharedOwn& own, 
     own_grid = static_cast<unsigned>(std::min<std::size_t>(own_grid, items));
     if (tiles != 0 && cut.grid <= shared_cus && p.batch <= kRaggedStreamMaxBatch &&
         least <= shared_cus) {
-      // One round of workgroups, cut for few own keys; where that could cost much beside the cut for
-      // max_own, the kernel chooses (1 us: 16 sequences behind 4096 keys, 1024 each, 17.3 us of this cut,
-      // 18.6 of a chosen one).
+      // One round of workgroups, cut for no own keys or for max_own of every sequence; where either could
+      // cost much beside the other, the kernel chooses (1.1 us: 16 sequences behind 4096 keys, 1024 each,
+      // 17.3 us of the first cut, 18.6 of a chosen one).
       constexpr float kMuch = 3.0f;
       p.own_least = static_cast<unsigned>(
           std::min(items, std::max<std::size_t>(least, kAttnSharedOwnLeast)));
       const unsigned most = static_cast<unsigned>(std::min<std::size_t>(
-          std::size_t{p.batch} * attn::kKvHeads * (max_own / 32 + 1), 1u << 30));
+          std::size_t{p.batch} * attn_shared_own_tiles(max_own), 1u << 30));
       const auto as = [&](unsigned own_tiles) {
         return attn_shared_cut<kRowBlocks>(tiles, pairs, own_tiles, shared_cus, p.own_least);
       };
-      const auto cost = [&](const AttnSharedCut& c) {
-        return attn_shared_cost<kRowBlocks>(c, most, shared_cus);
+      const auto cost = [&](const AttnSharedCut& c, unsigned own_tiles) {
+        return attn_shared_cost<kRowBlocks>(c, own_tiles, shared_cus);
       };
-      cut = as(1);
-      if (cost(cut) > cost(as(most)) + kMuch)
+      const AttnSharedCut few = as(1), many = as(most);
+      cut = cost(few, most) <= cost(many, most) + kMuch ? few : many;
+      if (cost(cut, 1) > cost(few, 1) + kMuch)
         p.chosen = words + 1;
       own_grid = cut.both ? shared_cus
                           : static_cast<unsigned>(std::min<std::size_t>(shared_cus - cut.grid, items));
