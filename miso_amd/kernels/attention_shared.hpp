@@ -56,11 +56,14 @@ struct AttnSharedParams {
   unsigned prefix_grid, own_first, own_batch;
   unsigned* chosen;    // word for the spans where the kernel chooses them (AttnSharedCut), or nullptr
   unsigned own_least;  // and the workgroups that the own keys take at least
+  bool own_waves;      // sequences of few own keys may be a wave's each
 };
 
-// Own keys of one sequence in tiles, as attn_shared_cost counts them: both heads, four waves.
-__host__ __device__ constexpr unsigned attn_shared_own_tiles(unsigned keys) {
-  return 8 * (keys / 128 + (keys % 128 != 0));
+// Own keys of one sequence in tiles, as attn_shared_cost counts them, both heads': four waves at a time, or
+// a wave each (wave_items).
+__host__ __device__ constexpr float attn_shared_own_tiles(unsigned keys, bool waves) {
+  const unsigned n = waves ? 32 : 128, rounds = keys / n + (keys % n != 0);
+  return waves ? 1.5f * static_cast<float>(rounds) : 8.0f * static_cast<float>(rounds);
 }
 
 // Where a split launch cuts the prefix.
@@ -84,11 +87,9 @@ template <unsigned kRowBlocks>
 constexpr float kAttnSharedTile = kRowBlocks == 4 ? 1.5f : kRowBlocks == 2 ? 1.0f : 0.9f;
 constexpr float kAttnSharedOwnTile = 1.5f, kAttnSharedOwnStart = 14.0f;
 template <unsigned kRowBlocks>
-__host__ __device__ constexpr float attn_shared_cost(const AttnSharedCut& c, unsigned own,
-                                                     unsigned cus) {
+__host__ __device__ constexpr float attn_shared_cost(const AttnSharedCut& c, float own, unsigned cus) {
   const float prefix = kAttnSharedTile<kRowBlocks> * static_cast<float>(c.span_tiles);
-  const float keys = kAttnSharedOwnTile * static_cast<float>(own) /
-                     static_cast<float>(c.both ? cus : cus - c.grid);
+  const float keys = kAttnSharedOwnTile * own / static_cast<float>(c.both ? cus : cus - c.grid);
   return c.both ? prefix + kAttnSharedOwnStart + keys : prefix < keys ? keys : prefix;
 }
 
@@ -99,7 +100,7 @@ __host__ __device__ constexpr float attn_shared_cost(const AttnSharedCut& c, uns
 // Spans shorter than 4 tiles only add partials: 8 behind 8192 22.0 us of 4, 24.1 of 3 (the merge's
 // time among them).
 template <unsigned kRowBlocks>
-__host__ __device__ constexpr AttnSharedCut attn_shared_cut(unsigned tiles, unsigned pairs, unsigned own,
+__host__ __device__ constexpr AttnSharedCut attn_shared_cut(unsigned tiles, unsigned pairs, float own,
                                                             unsigned cus, unsigned least) {
   constexpr unsigned kFewTiles = 4;
   if (tiles == 0)
@@ -112,13 +113,13 @@ __host__ __device__ constexpr AttnSharedCut attn_shared_cut(unsigned tiles, unsi
   unsigned most = cus / pairs;
   most = most < tiles / kFewTiles ? most : tiles / kFewTiles;
   most = most < 1 ? 1 : most;
-  if (own == 0 || cut(most, false).grid > cus)
+  if (own == 0.0f || cut(most, false).grid > cus)
     return cut(most, false);
   AttnSharedCut best = cut(most, true);
   float cost = attn_shared_cost<kRowBlocks>(best, own, cus);
   // The spans with which both sides end together, and one more; no more than leave `least` CUs.
   const float prefix = kAttnSharedTile<kRowBlocks> * static_cast<float>(tiles);
-  const float keys = kAttnSharedOwnTile * static_cast<float>(own);
+  const float keys = kAttnSharedOwnTile * own;
   const unsigned even = static_cast<unsigned>(prefix * static_cast<float>(cus) /
                                               (keys + prefix * static_cast<float>(pairs)));
   const unsigned room = cus > least + 7 ? (cus - least) / 8 * 8 / pairs : 0;
@@ -138,6 +139,10 @@ __host__ __device__ constexpr AttnSharedCut attn_shared_cut(unsigned tiles, unsi
   }
   return best;
 }
+
+// Sequences of up to kAttnSharedWaveKeys own keys, kAttnSharedWaveBatch or more of them, may be a wave's each
+// (wave_items): longer ones would leave one wave to work when the others are done, fewer leave waves idle.
+constexpr unsigned kAttnSharedWaveKeys = 256, kAttnSharedWaveBatch = 64;
 
 namespace shared_detail {
 
@@ -778,6 +783,141 @@ __device__ __attribute__((always_inline)) inline unsigned stream_length(
   return mine < p.len_cap ? mine : p.len_cap;
 }
 
+// The streaming split where every sequence has few keys: an item (sequence, KV head) is one wave's, its
+// tiles one after the other, since four waves on it would each take a tile or none and wait for one another:
+// 6 us a round of four tiles, here 3.6 a tile of each wave. 490 sequences of at most 5 keys behind 2560 (the
+// whole split): 68 us with four waves an item, 54 here; 300 of at most 60 behind 2048: 43 and 34; 203 of 1 ..
+// 203 behind 12000: 90 either way. Each wave for itself: item j of wave w is w + j times the launch's waves; a
+// K and a V tile and the queries of an item in LDS, the next tile's copies issued as soon as the operands of the
+// one before are in registers. Partials as the streaming split's, of one span.
+template <class Src>
+__device__ __attribute__((always_inline)) inline void wave_items(const StreamBatch& p, Src& src,
+                                                                StreamShared& sh, unsigned first) {
+  using cdna4::half8_t;
+  const unsigned t = threadIdx.x, lane = t & 63u;
+  const unsigned wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const unsigned stride = 4 * (gridDim.x - first), w = 4 * (blockIdx.x - first) + wave;
+  if (p.balanced != nullptr && w == 0 && lane == 0)
+    *p.balanced = p.chunk;
+  const unsigned all = attn::kKvHeads * p.batch, n_items = w < all ? (all - w + stride - 1) / stride : 0;
+  unsigned it_len = 0, it_seq = 0, it_kvh = 0;  // lane j: item j
+  if (lane < n_items) {
+    const unsigned k = w + lane * stride;
+    it_seq = k / attn::kKvHeads;
+    it_kvh = k % attn::kKvHeads;
+    it_len = stream_length(src, p, it_seq);
+    src.describe(it_seq, it_kvh, it_len);
+  }
+  auto next_item = [&](unsigned j) __attribute__((always_inline)) {  // first with keys >= j
+    while (j < n_items && lane_value(it_len, j) == 0)
+      ++j;
+    return j;
+  };
+  // The waits count as in stream_items.
+  unsigned issued = 0;
+  const unsigned k_lds = cdna4::lds_offset(sh.k[wave]), v_lds = cdna4::lds_offset(sh.v[wave]);
+  // The queries' 8 KiB a wave take the place of sh.q and, behind it, sh.merge.
+  static_assert(offsetof(StreamShared, merge) == offsetof(StreamShared, q) + sizeof(sh.q) &&
+                sizeof(sh.q) + sizeof(sh.merge) == 4 * sizeof(sh.q[0]));
+  float(*const q)[attn::kDim] = reinterpret_cast<float(*)[attn::kDim]>(
+      reinterpret_cast<unsigned char*>(&sh) + offsetof(StreamShared, q) + sizeof(sh.q[0]) * wave);
+  const unsigned q_lds = cdna4::lds_offset(q);
+  const WaveCopy cp = wave_copy_offsets(lane);
+  auto prepare = [&](unsigned j, unsigned ti) __attribute__((always_inline)) {
+    src.prepare(lane_value(it_seq, j), lane_value(it_kvh, j), ti * kTileKeys,
+                lane_value(it_len, j) - 1, j);
+  };
+  auto issue_k = [&](unsigned j, unsigned ti) __attribute__((always_inline)) {
+    src.template issue<false>(j, ti * kTileKeys, lane_value(it_len, j) - 1, k_lds, cp, lane);
+    issued += 16;
+  };
+  auto issue_v = [&](unsigned j, unsigned ti) __attribute__((always_inline)) {
+    src.template issue<true>(j, ti * kTileKeys, lane_value(it_len, j) - 1, v_lds, cp, lane);
+    issued += 16;
+  };
+  auto issue_q = [&](unsigned j) __attribute__((always_inline)) {
+    const float* from = p.q + (std::size_t{lane_value(it_seq, j)} * attn::kQHeads +
+                               lane_value(it_kvh, j) * kGroup) * attn::kDim;
+#pragma unroll
+    for (unsigned h = 0; h < kGroup; ++h)
+      cdna4::lds_load16(from + h * attn::kDim + 4 * lane, q_lds + h * attn::kDim * 4);
+    issued += kGroup;
+  };
+  unsigned jc = next_item(0);
+  if (jc >= n_items)  // uniform
+    return;
+  issue_q(jc);
+  unsigned mark_q = issued;
+  prepare(jc, 0);
+  issue_k(jc, 0);
+  unsigned mark_k = issued;
+  issue_v(jc, 0);
+  unsigned mark_v = issued;
+  const TileLane tln = tile_lane(lane);
+  const WaveOperands op = wave_operands(lane);
+  WaveTileState st;
+  for (;;) {
+    wait_vm_at_most(issued - mark_q);
+    wave_start(st, q, lane, tln);
+    const unsigned jn = next_item(jc + 1), end = lane_value(it_len, jc);
+    if (jn < n_items) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the queries are in registers
+      issue_q(jn);
+      mark_q = issued;
+    }
+    for (unsigned k0 = 0; k0 < end; k0 += kTileKeys) {
+      const unsigned mk = mark_k, mv = mark_v;
+      const bool last = k0 + kTileKeys >= end, next = !last || jn < n_items;
+      const unsigned nj = last ? jn : jc, nt = last ? 0 : k0 / kTileKeys + 1;
+      if (next)
+        prepare(nj, nt);
+      wait_vm_at_most(issued - mk);
+      half8_t ka[2][8];
+      read_k(ka, k_lds + op.kl);
+      __builtin_amdgcn_sched_barrier(0);
+      f32x4 s[2];
+      wave_scores(s, ka, st);
+      if (next) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the K operands are in registers
+        issue_k(nj, nt);
+        mark_k = issued;
+      }
+      wait_vm_at_most(issued - mv);
+      half8_t va[16];
+      read_v_all(va, v_lds, op.vl);
+      __builtin_amdgcn_sched_barrier(0);
+      TileSoftmax sm;
+      wave_softmax(sm, st, s, k0, end, k0 == 0, lane, tln);
+      if (next) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the V operands are in registers
+        issue_v(nj, nt);
+        mark_v = issued;
+      }
+      wave_pv(st, sm, va);
+    }
+    WaveResult r;
+    wave_result(r, st, true);
+    const unsigned g = lane >> 4, c = lane & 15u;
+    if (c < kGroup) {  // lane (g, c): head c, dimensions 4 (4 b + g) ..
+      const std::size_t row =
+          (std::size_t{lane_value(it_seq, jc)} * attn::kKvHeads + lane_value(it_kvh, jc)) * p.s_max *
+              kGroup + c;
+#pragma unroll
+      for (unsigned b = 0; b < 16; ++b)
+        *reinterpret_cast<float4*>(p.part_o + row * attn::kDim + 4 * (4 * b + g)) =
+            float4{r.o[b][0], r.o[b][1], r.o[b][2], r.o[b][3]};
+      if (g == 0) {
+        p.part_m[row] = r.mt * kLn2;
+        p.part_l[row] = r.l;
+      }
+    }
+    issued += 8;  // stores, at least
+    jc = jn;
+    if (jc >= n_items)
+      break;
+  }
+}
+
 }  // namespace decode_detail
 
 // Where the own keys lie: pages, or contiguous as the ragged decode's (page_table nullptr).
@@ -790,6 +930,20 @@ struct AttnSharedOwn {
   const uint64_t* kv_offsets;
 };
 
+// The cut for `own` tiles of own keys (AttnSharedCut), in the launch's own workgroups.
+template <unsigned kRowBlocks>
+__device__ __attribute__((always_inline)) inline void choose_cut(AttnSharedParams& p, float own) {
+  const AttnSharedCut cut = attn_shared_cut<kRowBlocks>(
+      (p.prefix.len - 1) / 32 + 1, 2 * ((p.blocks + kRowBlocks - 1) / kRowBlocks), own, gridDim.x,
+      p.own_least);
+  p.spans = __builtin_amdgcn_readfirstlane(cut.spans);
+  p.span_tiles = __builtin_amdgcn_readfirstlane(cut.span_tiles);
+  p.prefix_grid = __builtin_amdgcn_readfirstlane(cut.grid);
+  p.own_first = __builtin_amdgcn_readfirstlane(cut.both ? 0u : cut.grid);
+  if (blockIdx.x == 0 && threadIdx.x == 0)
+    *p.chosen = p.spans;
+}
+
 // The first p.prefix_grid workgroups take the prefix's spans, those from p.own_first on the sequences' own
 // keys: one launch, side by side (3 sequences behind 512 keys 10.5 us, in two launches 17). Where the
 // lengths decide on how many CUs either does best, which only the device knows, each wave makes the choice
@@ -799,21 +953,20 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
 attn_shared_split_kernel(AttnSharedParams p, AttnSharedOwn own) {
   __shared__ decode_detail::StreamShared sh;
   static_assert(sizeof(sh) >= sizeof(shared_detail::PrefixShared));
-  if (p.chosen != nullptr) {  // uniform
-    float tiles = 0.0f;
-    for (unsigned s = threadIdx.x & 63u; s < p.batch; s += 64)
-      tiles += static_cast<float>(attn_shared_own_tiles(shared_detail::own_keys(p, s)));
-    const unsigned all = __builtin_amdgcn_readfirstlane(
-        static_cast<unsigned>(fminf(cdna4::wave_allsum(tiles), 0x1p30f)));
-    const AttnSharedCut cut = attn_shared_cut<kRowBlocks>(
-        (p.prefix.len - 1) / 32 + 1, 2 * ((p.blocks + kRowBlocks - 1) / kRowBlocks), all, gridDim.x,
-        p.own_least);
-    p.spans = __builtin_amdgcn_readfirstlane(cut.spans);
-    p.span_tiles = __builtin_amdgcn_readfirstlane(cut.span_tiles);
-    p.prefix_grid = __builtin_amdgcn_readfirstlane(cut.grid);
-    p.own_first = __builtin_amdgcn_readfirstlane(cut.both ? 0u : cut.grid);
-    if (blockIdx.x == 0 && threadIdx.x == 0)
-      *p.chosen = p.spans;
+  bool waves = false;  // uniform
+  if (p.chosen != nullptr || p.own_waves) {
+    float fours = 0.0f, ones = 0.0f;
+    unsigned most = 0;
+    for (unsigned s = threadIdx.x & 63u; s < p.batch; s += 64) {
+      const unsigned n = shared_detail::own_keys(p, s);
+      fours += attn_shared_own_tiles(n, false);
+      ones += attn_shared_own_tiles(n, true);
+      most = max(most, n);
+    }
+    waves = p.own_waves && __builtin_amdgcn_ballot_w64(most > kAttnSharedWaveKeys) == 0;
+    ones = cdna4::wave_allsum(waves ? ones : fours);
+    if (p.chosen != nullptr)
+      choose_cut<kRowBlocks>(p, ones);
   }
   if (blockIdx.x < p.prefix_grid) {  // uniform
     shared_detail::prefix_span<kRowBlocks, kPaged>(
@@ -822,15 +975,22 @@ attn_shared_split_kernel(AttnSharedParams p, AttnSharedOwn own) {
       return;
     __syncthreads();  // the ring's space is the stream's
   }
+  waves = waves && p.own_batch >= gridDim.x - p.own_first;  // two items a workgroup
   const decode_detail::StreamBatch batch{p.q,     p.own_m, p.own_l,   p.own_o, p.lens,
                                          p.own_batch, p.s_max, p.own_cap, p.chunk, p.balanced};
   if constexpr (kPaged) {
     decode_detail::SharedPagedSource src{
         {own.k, own.v, own.page_table, own.max_pages, own.log2_page}, own.rows, p.prefix.len};
-    decode_detail::stream_items(batch, src, sh, p.own_first);
+    if (waves)
+      decode_detail::wave_items(batch, src, sh, p.own_first);
+    else
+      decode_detail::stream_items(batch, src, sh, p.own_first);
   } else {
     decode_detail::SharedRaggedSource src{{own.k, own.v, own.kv_offsets}};
-    decode_detail::stream_items(batch, src, sh, p.own_first);
+    if (waves)
+      decode_detail::wave_items(batch, src, sh, p.own_first);
+    else
+      decode_detail::stream_items(batch, src, sh, p.own_first);
   }
 }
 
@@ -1017,7 +1177,7 @@ inline void attn_shared_launch_as(AttnSharedParams p, const AttnSharedOwn& own, 
   const unsigned tiles = p.prefix.len / 32 + (p.prefix.len % 32 != 0);
   const unsigned pairs = 2 * ((p.blocks + kRowBlocks - 1) / kRowBlocks);
   const unsigned shared_cus = std::min(cus, kAttnSharedCus);
-  AttnSharedCut cut = attn_shared_cut<kRowBlocks>(tiles, pairs, 0, shared_cus, 0);
+  AttnSharedCut cut = attn_shared_cut<kRowBlocks>(tiles, pairs, 0.0f, shared_cus, 0);
   unsigned own_grid = 0, step = p.batch;  // of the own keys: workgroups, sequences of one launch
   unsigned grid = cut.grid;
   if (max_own != 0) {
@@ -1038,17 +1198,18 @@ inline void attn_shared_launch_as(AttnSharedParams p, const AttnSharedOwn& own, 
       constexpr float kMuch = 3.0f;
       p.own_least = static_cast<unsigned>(
           std::min(items, std::max<std::size_t>(least, kAttnSharedOwnLeast)));
-      const unsigned most = static_cast<unsigned>(std::min<std::size_t>(
-          std::size_t{p.batch} * attn_shared_own_tiles(max_own), 1u << 30));
-      const auto as = [&](unsigned own_tiles) {
+      p.own_waves = p.batch >= kAttnSharedWaveBatch;
+      const float most = static_cast<float>(p.batch) *
+                         attn_shared_own_tiles(max_own, p.own_waves && max_own <= kAttnSharedWaveKeys);
+      const auto as = [&](float own_tiles) {
         return attn_shared_cut<kRowBlocks>(tiles, pairs, own_tiles, shared_cus, p.own_least);
       };
-      const auto cost = [&](const AttnSharedCut& c, unsigned own_tiles) {
+      const auto cost = [&](const AttnSharedCut& c, float own_tiles) {
         return attn_shared_cost<kRowBlocks>(c, own_tiles, shared_cus);
       };
-      const AttnSharedCut few = as(1), many = as(most);
+      const AttnSharedCut few = as(1.0f), many = as(most);
       cut = cost(few, most) <= cost(many, most) + kMuch ? few : many;
-      if (cost(cut, 1) > cost(few, 1) + kMuch)
+      if (cost(cut, 1.0f) > cost(few, 1.0f) + kMuch)
         p.chosen = words + 1;
       own_grid = cut.both ? shared_cus
                           : static_cast<unsigned>(std::min<std::size_t>(shared_cus - cut.grid, items));

@@ -209,6 +209,25 @@ def test_cut_by_the_lengths(torch_mod, attn, batch, prefix_pages):
         assert torch_mod.equal(c.run(attn, sc), first), own
 
 
+@pytest.mark.parametrize("batch", [63, 64, 130, 512])
+@pytest.mark.parametrize("own", [1, 33, 256, 257])
+def test_few_own_keys(torch_mod, attn, batch, own):
+    """Around the lengths and batches whose own keys are a wave's each, paged and ragged; one workspace for
+    rising and falling lengths."""
+    torch = torch_mod
+    rng = np.random.default_rng(batch + own)
+    for pp in (4, 90):
+        lens = 16 * pp + rng.choice([0, 1, 31, 32, 33, own, rng.integers(0, own + 1)], batch)
+        lens = np.minimum(lens, 16 * pp + own)
+        lens[5], lens[6] = 0, 16 * pp + own
+        c = Paged(torch, 16, pp, lens, batch)
+        sc = c.scratch(attn, max_own=2000 if own == 33 else own)
+        check(torch, c.run(attn, sc), c.ref(), pp)
+    r = ragged(torch, batch, 300, own, own)
+    core, ref = run_ragged(torch, attn, r)
+    check(torch, core, ref)
+
+
 def test_spans_longer_than_the_page_ids_a_wave_holds(torch_mod, attn):
     """More than 64 tiles a span: its pages are read again, and tiles wrap the ring many times."""
     lens = 90112 + np.arange(30) % 7
