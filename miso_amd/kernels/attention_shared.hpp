@@ -298,17 +298,17 @@ __device__ __attribute__((always_inline)) inline unsigned own_keys(const AttnSha
 // adds P V for its share of the 256 dimensions (all 8 blocks of 32 dimensions: 32 MFMAs). So a wave's
 // tile is 64, 48 or 40 MFMAs of 32 cycles for 4, 2 and 1 row blocks: with few rows the memory sets the
 // pace (32 KiB a tile and CU), with many the matrix units. More rows a workgroup would read the tiles less
-// often, but 32 rows a wave take all its registers (O 128, queries 128, scores and numerators 48).
+// often, but 32 rows a wave take 420 of its 512 registers (O 128, queries 128, scores and numerators 48).
 //
 // Softmax in one pass: per row a reference m (log2 units), the sum of numerators 2^(s - m), and O relative
 // to 2^m; m starts kLead below the first tile's maximum and moves only when numerators grow too large.
 // Tiles come through a ring of five stages, three under way; a step adds the scores of a tile while the
 // numerators of the one before are formed between its MFMAs, then that one's P V.
 //
-// 64 sequences behind 131072 keys: 1.75 us a tile and CU, 1230 TFLOP/s of f16 products (an 8192^3 library
-// product: 1076), 2960 cycles for 2048 of MFMAs at 1.65 GHz. There the power sets the pace: with 4% fewer
-// cycles (the copies placed elsewhere) the clock fell by as much. 8 behind 32768 keys: 22.3 us, 3.2 TB/s,
-// 11 of them in the loop at 5.2 TB/s, 5 before it (queries from memory and cut, three tiles on their way).
+// 64 sequences behind 131072 keys: 1.77 us a tile and CU, 1210 TFLOP/s of f16 products (an 8192^3 library
+// product: 1076), 2860 cycles for 2048 of MFMAs at 1.62 GHz. There the power sets the pace: 2980 cycles, with
+// the copies elsewhere, ran at 1.68 GHz. 8 behind 32768 keys: 22.5 us, 3.1 TB/s, 11 of them in the loop at 5.2
+// TB/s, 5 before it (queries from memory and cut, three tiles on their way).
 namespace shared_detail {
 template <unsigned kRowBlocks, bool kPaged>
 __device__ __attribute__((always_inline)) inline void prefix_span(const AttnSharedParams& p,
@@ -336,9 +336,9 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
   // ---- Tiles: this wave copies rows 8 wave .. + 7 of K and V (instruction i rows 2 i + lane / 32 of
   // them, chunks swizzled as attention_prefill.hpp's tiles). Rows past the prefix's last one repeat it
   // (they are masked at use): the last tile's, so that its offsets can take the place of the others'. The
-  // lane offsets are unsigned, and a repeated row lies up to 3072 bytes below its instruction's: offsets
+  // lane offsets are unsigned, and a repeated row lies up to 3 KiB below its instruction's: offsets
   // are that much larger, their base that much lower.
-  constexpr unsigned kBelow = 3072;
+  constexpr unsigned kBelow = 3 * 1024;
   unsigned koff[4], voff[4];
 #pragma unroll
   for (unsigned i = 0; i < 4; ++i) {
