@@ -141,6 +141,16 @@ def test_plan_of_many_pages(torch_mod, attn, batch, prefix, most_len, most_new, 
     same(run_plan(torch_mod, attn, s, True), plan_ref(s))
 
 
+@pytest.mark.parametrize("tokens", [1, 1023, 4096, 4097, 9000])
+def test_plan_with_too_few_tokens(torch_mod, attn, tokens):
+    """Requests whose tokens end behind max_tokens, by either number of launches."""
+    s = scenario(np.random.default_rng(tokens), 700, 8, 2, 90, 40)
+    s["tokens"] = tokens
+    want = plan_ref(s)
+    assert (want["status"] == 3).any() and (tokens == 1 or (want["status"] == 0).any())
+    same(run_plan(torch_mod, attn, s, True), want)
+
+
 def test_plan_refuses_requests_alone(torch_mod, attn):
     """A row too long for its table, tokens behind max_tokens, no pages: the others go on."""
     s = dict(lens=np.array([30, 5, 0, 16, 8, 3]), new=np.array([3, 2, 9, 1, 8, 4]),

@@ -161,6 +161,29 @@ def test_many_entries(torch_mod, attn, batch, own):
     check(torch_mod, c.run(attn), c.ref())
 
 
+def test_many_entries_of_few_rows(torch_mod, attn):
+    """Chunks of two requests, more entries than one streaming launch takes."""
+    rows = np.arange(700) // 400
+    lens = 64 + 1 + np.arange(700) % 400
+    c = Paged(torch_mod, 16, 4, lens, 700, rows=rows)
+    check(torch_mod, c.run(attn), c.ref())
+
+
+def test_thousands_of_entries(torch_mod, attn):
+    """More row groups than CUs; some entries against float64, those of equal queries against each other."""
+    torch = torch_mod
+    rng = np.random.default_rng(3)
+    lens = lengths(rng, 9000, 64, 3)
+    c = Paged(torch, 16, 4, lens, 9000)
+    c.core = torch.full((9002, H, D), 777.25, device="cuda")
+    got = c.run(attn)
+    assert (got[9000:] == 777.25).all()  # behind the last entry
+    for e in [0, 1, 2047, 2048, 4095, 4096, 8191, 8192, 8999, *rng.integers(0, 9000, 40)]:
+        ref = attention(torch, c.q[e], c.gate[e], c.keys(c.k, e), c.keys(c.v, e))
+        check(torch, got[e][None], ref[None], e)
+    assert (got[:9000][torch.from_numpy(lens == 0).cuda()] == 0).all()
+
+
 def test_own_keys_beyond_max_own(torch_mod, attn):
     """lens above the capacity the scratch was made for: still all keys, in longer spans."""
     c = Paged(torch_mod, 8, 4, [32 + 2049, 32 + 5, 32], 3)
@@ -387,6 +410,32 @@ def test_two_streams_and_graphs(torch_mod, attn):
         graph.replay()
         torch.cuda.synchronize()
         check(torch, a.core, a.ref(), step)
+
+
+def test_two_graphs_share_a_workspace(torch_mod, attn):
+    """Calls of different batches, prefixes and lengths captured over one scratch, replayed in turn with eager
+    work between."""
+    torch = torch_mod
+    cases = [Paged(torch, 16, 200, lengths(np.random.default_rng(1), 9, 3200, 700), 1),
+             Paged(torch, 8, 5, lengths(np.random.default_rng(2), 90, 40, 30), 2),
+             Paged(torch, 32, 40, lengths(np.random.default_rng(3), 30, 1280, 500), 3)]
+    sc = attn.SharedScratch(90, 1000, 3200)
+    graphs, refs = [], []
+    for c in cases:
+        c.run(attn, sc)
+        refs.append(c.core.clone())
+        check(torch, c.core, c.ref())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            attn.attn_decode_paged_shared(c.q, c.gate, c.k, c.v, c.d["table"], c.page, c.d["lens"],
+                                          c.d["prefix"], c.pp, c.core, sc)
+        graphs.append(graph)
+    for i in (0, 1, 2, 1, 0, 2, 2, 0, 1):
+        cases[i].core.zero_()
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(cases[i].core, refs[i]), i
+        sc.ws[::7].add_(1)
 
 
 def test_a_batch_served(torch_mod, attn):
