@@ -72,11 +72,6 @@ struct AttnSharedCut {
   bool both;                         // the own keys are every workgroup's, behind its span
 };
 
-// Row blocks of a workgroup of the prefix.
-__host__ __device__ constexpr unsigned attn_shared_row_blocks(unsigned batch) {
-  return batch <= 4 ? 1 : batch <= 8 ? 2 : 4;
-}
-
 // What the tiles of a launch cost on `cus` CUs, a workgroup each, in us without the fixed part: the
 // slower side, or the span and its share of the `own` tiles of own keys (both heads') one after the
 // other. A tile of a span behind 64 sequences takes 1.5 us (32768 keys of 40 tiles a span: 70 us), behind
@@ -93,6 +88,19 @@ __host__ __device__ constexpr float attn_shared_cost(const AttnSharedCut& c, flo
   return c.both ? prefix + kAttnSharedOwnStart + keys : prefix < keys ? keys : prefix;
 }
 
+// Row blocks of a workgroup of the prefix. More share a tile's way from memory, fewer make its time shorter
+// and the workgroups more. 4 sequences: 11.4 us of one behind 4096 keys, 12.2 of two, 12.8 of four; 20.3, 19.8,
+// 21.8 behind 32768. 8: 28.9, 22.9, 23.8 behind 32768. Above, two where the shortest spans fill half of the CUs
+// at most: 64 behind 512 13.1 against 15.0 of four, 16 behind 4096 14.6 and 15.1; beyond that four: 32 behind 4096
+// 16.9 against 18.8 of two, 12 behind 32768 27.4 and 33.3.
+constexpr unsigned kAttnSharedFewTiles = 4;  // of a span, at least
+__host__ __device__ constexpr unsigned attn_shared_row_blocks(unsigned batch, unsigned prefix,
+                                                              unsigned cus) {
+  constexpr std::size_t kSpan = 32 * kAttnSharedFewTiles;
+  const std::size_t spans = (std::size_t{prefix} + kSpan - 1) / kSpan, pairs = 2 * ((std::size_t{batch} + 7) / 8);
+  return batch <= 4 ? 1 : batch <= 8 || 2 * pairs * spans <= cus ? 2 : 4;
+}
+
 // The cut of `tiles` tiles for `pairs` (group of row blocks, KV head) pairs that costs least: beside the
 // own keys on CUs of their own, `least` or more, or on all CUs. 8 sequences behind 32768 keys, 300 own
 // keys each: 23.7 us of 9 tiles a span with 28 CUs for the own keys, 34.4 of 8 with all CUs and the
@@ -102,7 +110,6 @@ __host__ __device__ constexpr float attn_shared_cost(const AttnSharedCut& c, flo
 template <unsigned kRowBlocks>
 __host__ __device__ constexpr AttnSharedCut attn_shared_cut(unsigned tiles, unsigned pairs, float own,
                                                             unsigned cus, unsigned least) {
-  constexpr unsigned kFewTiles = 4;
   if (tiles == 0)
     return AttnSharedCut{0, 0, 0, false};
   const auto cut = [=](unsigned spans, bool both) {
@@ -111,7 +118,7 @@ __host__ __device__ constexpr AttnSharedCut attn_shared_cut(unsigned tiles, unsi
     return AttnSharedCut{spans, each, 8 * ((pairs * spans + 7) / 8), both};
   };
   unsigned most = cus / pairs;
-  most = most < tiles / kFewTiles ? most : tiles / kFewTiles;
+  most = most < tiles / kAttnSharedFewTiles ? most : tiles / kAttnSharedFewTiles;
   most = most < 1 ? 1 : most;
   if (own == 0.0f || cut(most, false).grid > cus)
     return cut(most, false);
@@ -141,7 +148,9 @@ __host__ __device__ constexpr AttnSharedCut attn_shared_cut(unsigned tiles, unsi
 }
 
 // Sequences of up to kAttnSharedWaveKeys own keys, kAttnSharedWaveBatch or more of them, may be a wave's each
-// (wave_items): longer ones would leave one wave to work when the others are done, fewer leave waves idle.
+// (wave_items): longer ones would leave one wave to work when the others are done, fewer leave waves idle. Of up
+// to 250 own keys behind 4096: 48 sequences 19.9 us with four waves an item, 20.3 with one; 64 26.3 and 22.3;
+// 200 51.8 and 48.8.
 constexpr unsigned kAttnSharedWaveKeys = 256, kAttnSharedWaveBatch = 64;
 
 namespace shared_detail {
@@ -1261,7 +1270,7 @@ inline void attn_shared_launch(const AttnSharedParams& p, const AttnSharedOwn& o
                                char* ws, unsigned cus, hipStream_t stream) {
   const auto as = [&](auto paged) {
     constexpr bool kPaged = decltype(paged)::value;
-    const unsigned rb = attn_shared_row_blocks(p.batch);
+    const unsigned rb = attn_shared_row_blocks(p.batch, p.prefix.len, cus);
     (rb == 1   ? attn_shared_launch_as<1, kPaged>
      : rb == 2 ? attn_shared_launch_as<2, kPaged>
                : attn_shared_launch_as<4, kPaged>)(p, own, max_own, ws, cus, stream);
