@@ -1010,18 +1010,19 @@ attn_shared_split_kernel(AttnSharedParams p, AttnSharedOwn own) {
 // waves' sums and the own keys' splits in order, divides and applies the gate. The order is fixed.
 // Bound by the partials it reads, 1 KiB a row and span; a CU takes in only so much of them, so with
 // few row blocks their dimensions are spread over four times the workgroups (8 sequences, 114 spans: 6.6 us;
-// 12 with all dimensions of 32 in a workgroup). 3 sequences, 4 spans: 3.9 us, 64 and 26: 8.6, 256 and 6: 9.0.
+// 12 with 32 dimensions a workgroup), and where that leaves CUs, over twice the waves (6.0; with 33
+// sequences and 20 spans 7.7 against 5.9). 3 sequences, 4 spans: 3.9 us, 64 and 26: 8.4, 256 and 6: 9.0.
 // ------------------------------------------------------------------------------------------------
 
-template <unsigned kQuads>
-__global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams p) {
+template <unsigned kQuads, unsigned kWaves>
+__global__ void __launch_bounds__(64 * kWaves) attn_shared_merge_kernel(AttnSharedParams p) {
   using namespace shared_detail;
   static_assert(kQuads == 1 || kQuads == 4);
   constexpr unsigned kBatch = 16 / kQuads, kDims = 8 * kQuads;  // spans, dimensions at a time
   constexpr unsigned kRow = kDims + 1;  // floats of a staged row
   constexpr unsigned kPieces = attn::kDim / kDims;
-  __shared__ float rows[4][kBlockRows * kRow];
-  __shared__ float2 ml[4][kBlockRows];
+  __shared__ float rows[kWaves][kBlockRows * kRow];
+  __shared__ float2 ml[kWaves][kBlockRows];
   const unsigned t = threadIdx.x, lane = t & 63u, wave = t >> 6, col = lane & 31u, hi = lane >> 5;
   const unsigned d = blockIdx.x % kPieces, kvh = blockIdx.x / kPieces % 2;
   const unsigned block = blockIdx.x / (2 * kPieces);
@@ -1029,15 +1030,15 @@ __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams
   const unsigned spans = p.chosen != nullptr ? *p.chosen : p.spans;
   float m = kNoScore, l = 0.0f;
   float4 o[kQuads] = {};
-  for (unsigned s0 = wave; s0 < spans; s0 += 4 * kBatch) {
+  for (unsigned s0 = wave; s0 < spans; s0 += kWaves * kBatch) {
     float2 x[kBatch];
     float4 y[kBatch][kQuads];
 #pragma unroll
     for (unsigned i = 0; i < kBatch; ++i) {
-      const unsigned s = min(s0 + 4 * i, spans - 1);
+      const unsigned s = min(s0 + kWaves * i, spans - 1);
       const std::size_t at = (std::size_t{s} * attn::kKvHeads + kvh) * p.blocks + block;
       x[i] = p.part_ml[at * kBlockRows + col];
-      x[i] = s0 + 4 * i < spans ? x[i] : float2{kNoScore, 0.0f};
+      x[i] = s0 + kWaves * i < spans ? x[i] : float2{kNoScore, 0.0f};
 #pragma unroll
       for (unsigned j = 0; j < kQuads; ++j)
         y[i][j] = p.part_o[at * 8 * 256 + 64 * (kQuads * d + j) + lane];
@@ -1054,7 +1055,7 @@ __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams
       o[j] = float4{o[j].x * old, o[j].y * old, o[j].z * old, o[j].w * old};
 #pragma unroll
     for (unsigned i = 0; i < kBatch; ++i) {
-      if (s0 + 4 * i >= spans)  // uniform: a repeated span is left out (0 x infinity is NaN)
+      if (s0 + kWaves * i >= spans)  // uniform: a repeated span is left out (0 x infinity is NaN)
         break;
       const float e = __builtin_amdgcn_exp2f(x[i].x - top);
       l = __builtin_fmaf(x[i].y, e, l);
@@ -1085,11 +1086,11 @@ __global__ void __launch_bounds__(256) attn_shared_merge_kernel(AttnSharedParams
   const float4 g = *reinterpret_cast<const float4*>(p.gate + out);
   float top = kNoScore;
 #pragma unroll
-  for (unsigned w = 0; w < 4; ++w)
+  for (unsigned w = 0; w < kWaves; ++w)
     top = fmaxf(top, ml[w][row].x);
   float all = 0.0f, v[4] = {};
 #pragma unroll
-  for (unsigned w = 0; w < 4; ++w) {
+  for (unsigned w = 0; w < kWaves; ++w) {
     const float e = __builtin_amdgcn_exp2f(ml[w][row].x - top);
     all = __builtin_fmaf(ml[w][row].y, e, all);
 #pragma unroll
@@ -1260,10 +1261,12 @@ inline void attn_shared_launch_as(AttnSharedParams p, const AttnSharedOwn& own, 
     attn_shared_split_kernel<kRowBlocks, kPaged>
         <<<s == 0 ? grid : own_grid, 256, 0, stream>>>(a, o);
   }
-  if (16 * p.blocks < cus)
-    attn_shared_merge_kernel<1><<<64 * p.blocks, 256, 0, stream>>>(p);
+  if (64 * p.blocks <= cus)
+    attn_shared_merge_kernel<1, 8><<<64 * p.blocks, 512, 0, stream>>>(p);
+  else if (16 * p.blocks < cus)
+    attn_shared_merge_kernel<1, 4><<<64 * p.blocks, 256, 0, stream>>>(p);
   else
-    attn_shared_merge_kernel<4><<<16 * p.blocks, 256, 0, stream>>>(p);
+    attn_shared_merge_kernel<4, 4><<<16 * p.blocks, 256, 0, stream>>>(p);
 }
 
 inline void attn_shared_launch(const AttnSharedParams& p, const AttnSharedOwn& own, unsigned max_own,
