@@ -1171,6 +1171,74 @@ __host__ __device__ constexpr AttnSharedLayout attn_shared_layout(unsigned batch
   return a;
 }
 
+// What a call launches.
+struct AttnSharedRule {
+  AttnSharedCut cut;               // of the prefix, unless the kernel chooses it (chosen)
+  unsigned grid;                   // workgroups of the first split launch; 0: none
+  unsigned own_first, own_grid;    // of the own keys: the first workgroup, their number
+  unsigned own_least;              // AttnSharedParams'
+  unsigned s_max, chunk;           // AttnSharedParams'
+  unsigned step;                   // sequences of a split launch
+  bool chosen, balanced, own_waves;
+};
+template <unsigned kRowBlocks>
+inline AttnSharedRule attn_shared_rule(unsigned batch, unsigned prefix, unsigned max_own, unsigned cus) {
+  AttnSharedRule r{};
+  const unsigned blocks = (batch + 3) / 4;
+  const unsigned tiles = prefix / 32 + (prefix % 32 != 0);
+  const unsigned pairs = 2 * ((blocks + kRowBlocks - 1) / kRowBlocks);
+  const unsigned shared_cus = std::min(cus, kAttnSharedCus);
+  r.cut = attn_shared_cut<kRowBlocks>(tiles, pairs, 0.0f, shared_cus, 0);
+  r.step = batch;
+  r.grid = r.cut.grid;
+  if (max_own == 0)
+    return r;
+  // The CUs that the prefix leaves, all of them where it leaves less than half; at most one streaming
+  // launch's sequences and items at a time.
+  r.own_grid = 2 * r.cut.grid <= cus ? cus - r.cut.grid : cus;
+  r.s_max = std::min(attn_ragged_balanced_splits(batch, max_own),
+                     kRaggedStreamMaxItems * r.own_grid / attn::kKvHeads);
+  r.chunk = attn_ragged_chunk(batch, max_own, cus);
+  const std::size_t items = std::size_t{batch} * attn::kKvHeads * r.s_max;
+  const std::size_t least = (items + kRaggedStreamMaxItems - 1) / kRaggedStreamMaxItems;
+  r.own_grid = static_cast<unsigned>(std::min<std::size_t>(r.own_grid, items));
+  if (tiles != 0 && r.cut.grid <= shared_cus && batch <= kRaggedStreamMaxBatch &&
+      least <= shared_cus) {
+    // One round of workgroups, cut for no own keys or for max_own of every sequence; where either could
+    // cost much beside the other, the kernel chooses (1.1 us: 16 sequences behind 4096 keys, 1024 each,
+    // 17.3 us of the first cut, 18.6 of a chosen one).
+    constexpr float kMuch = 3.0f;
+    r.own_least = static_cast<unsigned>(
+        std::min(items, std::max<std::size_t>(least, kAttnSharedOwnLeast)));
+    r.own_waves = batch >= kAttnSharedWaveBatch;
+    const float most = static_cast<float>(batch) *
+                       attn_shared_own_tiles(max_own, r.own_waves && max_own <= kAttnSharedWaveKeys);
+    const auto as = [&](float own_tiles) {
+      return attn_shared_cut<kRowBlocks>(tiles, pairs, own_tiles, shared_cus, r.own_least);
+    };
+    const auto cost = [&](const AttnSharedCut& c, float own_tiles) {
+      return attn_shared_cost<kRowBlocks>(c, own_tiles, shared_cus);
+    };
+    const AttnSharedCut few = as(1.0f), many = as(most);
+    r.cut = cost(few, most) <= cost(many, most) + kMuch ? few : many;
+    r.chosen = cost(r.cut, 1.0f) > cost(few, 1.0f) + kMuch;
+    r.own_grid = r.cut.both
+                     ? shared_cus
+                     : static_cast<unsigned>(std::min<std::size_t>(shared_cus - r.cut.grid, items));
+    r.grid = r.cut.both || r.chosen ? shared_cus : r.cut.grid + r.own_grid;
+    r.own_first = r.cut.both ? 0 : r.cut.grid;
+  } else {  // the own keys' workgroups follow the prefix's
+    r.own_first = r.cut.grid;
+    r.grid = r.cut.grid + r.own_grid;
+    if (batch > kRaggedStreamMaxBatch || least > r.own_grid)
+      r.step = std::min(kRaggedStreamMaxBatch,
+                        std::max(1u, kRaggedStreamMaxItems * r.own_grid / (attn::kKvHeads * r.s_max)));
+  }
+  r.balanced = r.step >= batch &&
+               attn_ragged_balanced(batch, max_own, cus, r.chosen ? r.own_least : r.own_grid);
+  return r;
+}
+
 // p: q, gate, core, lens, prefix, batch, whole and own_cap given; the workspace holds
 // attn_shared_layout(batch, max_own, p.prefix.len).
 template <unsigned kRowBlocks, bool kPaged>
@@ -1184,66 +1252,22 @@ inline void attn_shared_launch_as(AttnSharedParams p, const AttnSharedOwn& own, 
   p.own_o = reinterpret_cast<float*>(ws + at.own_o);
   unsigned* const words = reinterpret_cast<unsigned*>(p.own_l) - 4;
   p.blocks = (p.batch + 3) / 4;
-  const unsigned tiles = p.prefix.len / 32 + (p.prefix.len % 32 != 0);
-  const unsigned pairs = 2 * ((p.blocks + kRowBlocks - 1) / kRowBlocks);
-  const unsigned shared_cus = std::min(cus, kAttnSharedCus);
-  AttnSharedCut cut = attn_shared_cut<kRowBlocks>(tiles, pairs, 0.0f, shared_cus, 0);
-  unsigned own_grid = 0, step = p.batch;  // of the own keys: workgroups, sequences of one launch
-  unsigned grid = cut.grid;
-  if (max_own != 0) {
-    // The CUs that the prefix leaves, all of them where it leaves less than half; at most one streaming
-    // launch's sequences and items at a time.
-    own_grid = 2 * cut.grid <= cus ? cus - cut.grid : cus;
-    p.s_max = std::min(attn_ragged_balanced_splits(p.batch, max_own),
-                       kRaggedStreamMaxItems * own_grid / attn::kKvHeads);
-    p.chunk = attn_ragged_chunk(p.batch, max_own, cus);
-    const std::size_t items = std::size_t{p.batch} * attn::kKvHeads * p.s_max;
-    const std::size_t least = (items + kRaggedStreamMaxItems - 1) / kRaggedStreamMaxItems;
-    own_grid = static_cast<unsigned>(std::min<std::size_t>(own_grid, items));
-    if (tiles != 0 && cut.grid <= shared_cus && p.batch <= kRaggedStreamMaxBatch &&
-        least <= shared_cus) {
-      // One round of workgroups, cut for no own keys or for max_own of every sequence; where either could
-      // cost much beside the other, the kernel chooses (1.1 us: 16 sequences behind 4096 keys, 1024 each,
-      // 17.3 us of the first cut, 18.6 of a chosen one).
-      constexpr float kMuch = 3.0f;
-      p.own_least = static_cast<unsigned>(
-          std::min(items, std::max<std::size_t>(least, kAttnSharedOwnLeast)));
-      p.own_waves = p.batch >= kAttnSharedWaveBatch;
-      const float most = static_cast<float>(p.batch) *
-                         attn_shared_own_tiles(max_own, p.own_waves && max_own <= kAttnSharedWaveKeys);
-      const auto as = [&](float own_tiles) {
-        return attn_shared_cut<kRowBlocks>(tiles, pairs, own_tiles, shared_cus, p.own_least);
-      };
-      const auto cost = [&](const AttnSharedCut& c, float own_tiles) {
-        return attn_shared_cost<kRowBlocks>(c, own_tiles, shared_cus);
-      };
-      const AttnSharedCut few = as(1.0f), many = as(most);
-      cut = cost(few, most) <= cost(many, most) + kMuch ? few : many;
-      if (cost(cut, 1.0f) > cost(few, 1.0f) + kMuch)
-        p.chosen = words + 1;
-      own_grid = cut.both ? shared_cus
-                          : static_cast<unsigned>(std::min<std::size_t>(shared_cus - cut.grid, items));
-      grid = cut.both || p.chosen != nullptr ? shared_cus : cut.grid + own_grid;
-      p.own_first = cut.both ? 0 : cut.grid;
-    } else {  // the own keys' workgroups follow the prefix's
-      p.own_first = cut.grid;
-      grid = cut.grid + own_grid;
-      if (p.batch > kRaggedStreamMaxBatch || least > own_grid)
-        step = std::min(kRaggedStreamMaxBatch,
-                        std::max(1u, kRaggedStreamMaxItems * own_grid / (attn::kKvHeads * p.s_max)));
-    }
-    if (step >= p.batch &&
-        attn_ragged_balanced(p.batch, max_own, cus, p.chosen != nullptr ? p.own_least : own_grid))
-      p.balanced = words;
-  }
-  p.spans = cut.spans;
-  p.span_tiles = cut.span_tiles;
-  p.prefix_grid = cut.grid;
-  for (unsigned s = 0; grid != 0 && s < p.batch; s += step) {
+  const AttnSharedRule r = attn_shared_rule<kRowBlocks>(p.batch, p.prefix.len, max_own, cus);
+  p.s_max = r.s_max;
+  p.chunk = r.chunk;
+  p.own_first = r.own_first;
+  p.own_least = r.own_least;
+  p.own_waves = r.own_waves;
+  p.balanced = r.balanced ? words : nullptr;
+  p.chosen = r.chosen ? words + 1 : nullptr;
+  p.spans = r.cut.spans;
+  p.span_tiles = r.cut.span_tiles;
+  p.prefix_grid = r.cut.grid;
+  for (unsigned s = 0; r.grid != 0 && s < p.batch; s += r.step) {
     const std::size_t row = std::size_t{s} * attn::kKvHeads * p.s_max * decode_detail::kGroup;
     AttnSharedParams a = p;
     AttnSharedOwn o = own;
-    a.own_batch = std::min(step, p.batch - s);
+    a.own_batch = std::min(r.step, p.batch - s);
     if (s != 0) {  // the own keys of more sequences
       a.prefix_grid = a.own_first = 0;
       a.q += std::size_t{s} * attn::kQHeads * attn::kDim;
@@ -1259,7 +1283,7 @@ inline void attn_shared_launch_as(AttnSharedParams p, const AttnSharedOwn& own, 
         o.page_table += std::size_t{s} * own.max_pages;
     }
     attn_shared_split_kernel<kRowBlocks, kPaged>
-        <<<s == 0 ? grid : own_grid, 256, 0, stream>>>(a, o);
+        <<<s == 0 ? r.grid : r.own_grid, 256, 0, stream>>>(a, o);
   }
   if (64 * p.blocks <= cus)
     attn_shared_merge_kernel<1, 8><<<64 * p.blocks, 512, 0, stream>>>(p);

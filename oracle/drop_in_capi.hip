@@ -6,6 +6,7 @@
 #include "engine/attention.hip"
 
 #include "attention_evict.hpp"
+#include "attention_shared.hpp"
 
 #include <algorithm>
 #include <cstring>
@@ -158,6 +159,31 @@ void drop_key_weights_piece(unsigned pos0, unsigned n, unsigned t, std::uint64_t
   const auto c = miso::kernels::attn_key_weights_cut(pos0 + t, m);
   const std::uint64_t is[] = {m, c.blocks, c.waves, c.groups, c.row_tiles, c.spans, c.span};
   std::copy(is, is + 7, out);
+}
+
+// What a decode behind a shared prefix launches: row blocks of a workgroup, spans and tiles of a span (as
+// the host cuts them), workgroups of the prefix and of the launch, whether the kernel chooses the cut and the
+// own keys' span, and the workgroups of the prefix if it finds no own keys (host only).
+void drop_shared_rule(unsigned batch, unsigned prefix, unsigned max_own, unsigned cus,
+                      std::uint64_t* out) {
+  namespace K = miso::kernels;
+  const unsigned rb = K::attn_shared_row_blocks(batch, prefix, cus);
+  const auto as = [&](auto row_blocks) {
+    constexpr unsigned kRowBlocks = decltype(row_blocks)::value;
+    const auto r = K::attn_shared_rule<kRowBlocks>(batch, prefix, max_own, cus);
+    const unsigned pairs = 2 * (((batch + 3) / 4 + kRowBlocks - 1) / kRowBlocks);
+    const auto none = K::attn_shared_cut<kRowBlocks>((prefix + 31) / 32, pairs, 0.0f, r.grid,
+                                                     r.own_least);
+    const std::uint64_t is[] = {rb,     r.cut.spans, r.cut.span_tiles, r.cut.grid,
+                                r.grid, r.chosen,    r.balanced,       none.grid};
+    std::copy(is, is + 8, out);
+  };
+  if (rb == 1)
+    as(std::integral_constant<unsigned, 1>{});
+  else if (rb == 2)
+    as(std::integral_constant<unsigned, 2>{});
+  else
+    as(std::integral_constant<unsigned, 4>{});
 }
 
 }  // extern "C"
