@@ -66,6 +66,14 @@ __host__ __device__ constexpr float attn_shared_own_tiles(unsigned keys, bool wa
   return waves ? 1.5f * static_cast<float>(rounds) : 8.0f * static_cast<float>(rounds);
 }
 
+// Partials of a sequence of `mine` own keys. Without any, `chunk` may be a word that nobody wrote: the cut
+// that the kernel chooses for a batch of no own keys can take every workgroup for the prefix, and then none
+// is left to choose the own keys' span.
+__host__ __device__ inline unsigned attn_shared_own_splits(unsigned mine, unsigned s_max,
+                                                           unsigned chunk) {
+  return mine != 0 ? attn_ragged_seq_splits(mine, s_max, chunk) : 0;
+}
+
 // Where a split launch cuts the prefix.
 struct AttnSharedCut {
   unsigned spans, span_tiles, grid;  // grid: the prefix's workgroups, a multiple of 8
@@ -1100,7 +1108,7 @@ __global__ void __launch_bounds__(64 * kWaves) attn_shared_merge_kernel(AttnShar
   if (p.s_max != 0) {
     const unsigned mine = own_keys(p, seq);
     const unsigned chunk = p.balanced != nullptr ? *p.balanced : p.chunk;
-    const unsigned n = attn_ragged_seq_splits(mine, p.s_max, chunk);
+    const unsigned n = attn_shared_own_splits(mine, p.s_max, chunk);
     const std::size_t at0 =
         ((std::size_t{seq} * attn::kKvHeads + kvh) * p.s_max) * kGroup + row % kGroup;
     constexpr unsigned kSplits = 4;

@@ -161,6 +161,11 @@ void drop_key_weights_piece(unsigned pos0, unsigned n, unsigned t, std::uint64_t
   std::copy(is, is + 7, out);
 }
 
+// Partials of a sequence's own keys as the merge counts them, `chunk` what it found in the workspace.
+unsigned drop_shared_own_splits(unsigned mine, unsigned s_max, unsigned chunk) {
+  return miso::kernels::attn_shared_own_splits(mine, s_max, chunk);
+}
+
 // What a decode behind a shared prefix launches: row blocks of a workgroup, spans and tiles of a span (as
 // the host cuts them), workgroups of the prefix and of the launch, whether the kernel chooses the cut and the
 // own keys' span, and the workgroups of the prefix if it finds no own keys (host only).

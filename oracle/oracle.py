@@ -525,6 +525,7 @@ def drop_in():
             "drop_prefill_form": (U, [U, U, c_uint64]),
             "drop_key_weights_layout": (None, [U, U, c_int, V]),
             "drop_key_weights_piece": (None, [U, U, U, V]),
+            "drop_shared_own_splits": (U, [U, U, U]),
             "drop_shared_rule": (None, [U, U, U, U, V]),
             "drop_qgemm_kernel": (c_int, [c_int, V, V, V, V, U, U, U, U]),
             "drop_qgemm_batch": (c_int, [U, V, V, V, V, V, U, V, U, U]),

@@ -251,6 +251,25 @@ def test_few_own_keys(torch_mod, attn, batch, own):
     check(torch, core, ref)
 
 
+@pytest.mark.parametrize("batch,prefix,max_own", [(8, 32768, 7988), (8, 16384, 4096),
+                                                  (16, 32768, 1024), (24, 8192, 1024)])
+def test_no_own_keys_leave_no_workgroup_for_them(torch_mod, attn, batch, prefix, max_own):
+    """The kernel gives the whole launch to the prefix, so that nobody chooses the own keys' span: over a
+    workspace of zeros, of ones and of an earlier call's words, and with own keys again after it."""
+    c = Paged(torch_mod, 16, prefix // 16, [prefix] * (batch - 2) + [0, prefix - 100], batch,
+              room=prefix // 16 + -(-max_own // 16))
+    sc = c.scratch(attn, max_own=max_own)
+    ref = c.ref()
+    for fill in (0, 255, 1):
+        sc.ws.fill_(fill)
+        c.core.fill_(777.25)
+        check(torch_mod, c.run(attn, sc), ref, fill)
+    other = Paged(torch_mod, 16, prefix // 16, [prefix + 90 + 31 * e for e in range(batch)], batch)
+    check(torch_mod, other.run(attn, sc), other.ref())
+    c.core.fill_(777.25)
+    check(torch_mod, c.run(attn, sc), ref)
+
+
 def test_spans_longer_than_the_page_ids_a_wave_holds(torch_mod, attn):
     """More than 64 tiles a span: its pages are read again, and tiles wrap the ring many times."""
     lens = 90112 + np.arange(30) % 7
