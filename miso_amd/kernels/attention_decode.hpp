@@ -1923,11 +1923,12 @@ __device__ __attribute__((always_inline)) inline void wave_merge_out(
       wave_merge_o(ms, o);
 }
 
+// unit: of part_m in log2 units, kLn2 for natural ones.
 template <class Scores = NoScores>
 __device__ __attribute__((always_inline)) inline void wave_merge_ml_out(
     const WaveMergeScale& ms, unsigned h, float* part_m, float* part_l, std::size_t base,
-    const Scores& scores = Scores{}) {
-  part_m[base * kGroup + h] = ms.m * kLn2;  // -inf stays -inf for an empty item
+    const Scores& scores = Scores{}, float unit = kLn2) {
+  part_m[base * kGroup + h] = ms.m * unit;  // -inf stays -inf for an empty item
   part_l[base * kGroup + h] = ms.l;
   if constexpr (Scores::kOn)
     scores.m2[base * kGroup + h] = ms.m;
@@ -2892,6 +2893,12 @@ struct PagedStreamSource {
   }
 };
 
+// What a source's maxima are multiplied by in the partials: natural units, unless the source says otherwise.
+template <class Src, class = void>
+constexpr float kStreamUnit = kLn2;
+template <class Src>
+constexpr float kStreamUnit<Src, std::void_t<decltype(Src::kUnit)>> = Src::kUnit;
+
 // Keys of sequence s (a source whose lens count other keys too overloads it).
 template <class Src>
 __device__ __attribute__((always_inline)) inline unsigned stream_length(const Src&,
@@ -3121,7 +3128,7 @@ __device__ __attribute__((always_inline)) inline void stream_items(const StreamB
       const WaveMergeScale ms = wave_merge_load_scale(ml, 16, h);
       wave_merge_out(&sh.merge[0][0], 32 * kGroup * 4, ms, d, d, h, p.part_o, part);
       if (d == 0)
-        wave_merge_ml_out(ms, h, p.part_m, p.part_l, part);
+        wave_merge_ml_out(ms, h, p.part_m, p.part_l, part, NoScores{}, kStreamUnit<Src>);
       tile_barrier();
       wave_merge_store(sh.merge[wave], nullptr, r, lane, 8, 8);
       tile_barrier();

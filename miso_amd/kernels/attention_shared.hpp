@@ -46,7 +46,8 @@ struct AttnSharedParams {
   unsigned spans, span_tiles;  // of the prefix; 0: no prefix
   unsigned blocks;             // row blocks (of 32 rows: 4 sequences x 8 heads)
   bool whole;
-  // The own keys' partials, [batch][2][s_max][8] and 256 times that, as the ragged decode's.
+  // The own keys' partials, [batch][2][s_max][8] and 256 times that, as the ragged decode's, but the maxima
+  // in log2 units: to natural ones and back a maximum of 1000 moves by 6e-5, the weights with it.
   float* own_m;
   float* own_l;
   float* own_o;
@@ -775,6 +776,7 @@ namespace decode_detail {
 // Pages behind the prefix: sequence s's own keys are in table row rows[s] (row s without rows), their
 // number is lens[s] less the prefix's.
 struct SharedPagedSource {
+  static constexpr float kUnit = 1.0f;  // maxima stay in log2 units, as the prefix's references
   PagedStreamSource base;
   const int32_t* rows;
   unsigned prefix_len, table_row = 0;  // lane j: item j's row
@@ -793,7 +795,9 @@ struct SharedPagedSource {
   }
 };
 // Contiguous own keys: the ragged decode's. (A type of its own: its launch's workgroups start elsewhere.)
-struct SharedRaggedSource : RaggedStreamSource {};
+struct SharedRaggedSource : RaggedStreamSource {
+  static constexpr float kUnit = 1.0f;
+};
 __device__ __attribute__((always_inline)) inline unsigned stream_length(
     const SharedPagedSource& src, const StreamBatch& p, unsigned s) {
   const unsigned len = p.lens[s], mine = len > src.prefix_len ? len - src.prefix_len : 0;
@@ -924,7 +928,7 @@ __device__ __attribute__((always_inline)) inline void wave_items(const StreamBat
         *reinterpret_cast<float4*>(p.part_o + row * attn::kDim + 4 * (4 * b + g)) =
             float4{r.o[b][0], r.o[b][1], r.o[b][2], r.o[b][3]};
       if (g == 0) {
-        p.part_m[row] = r.mt * kLn2;
+        p.part_m[row] = r.mt * kStreamUnit<Src>;
         p.part_l[row] = r.l;
       }
     }
@@ -1118,7 +1122,7 @@ __global__ void __launch_bounds__(64 * kWaves) attn_shared_merge_kernel(AttnShar
 #pragma unroll
       for (unsigned i = 0; i < kSplits; ++i) {
         const std::size_t at = at0 + static_cast<std::size_t>(min(s0 + i, n - 1)) * kGroup;
-        sm[i] = p.own_m[at] * decode_detail::kLog2e;
+        sm[i] = p.own_m[at];
         sl[i] = p.own_l[at];
         so[i] = *reinterpret_cast<const float4*>(p.own_o + at * attn::kDim + kDims * d + dim);
       }

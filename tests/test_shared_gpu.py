@@ -300,6 +300,65 @@ def test_extreme_scores(torch_mod, attn):
             assert ((got.double() - ref).norm(dim=-1) <= 1e-4 * ref.norm(dim=-1)).float().mean() > 0.98
 
 
+@pytest.mark.parametrize("b", [70, 12])  # own keys a wave's each, or by four waves
+@pytest.mark.parametrize("top", [500, 2000, 16000])
+def test_equal_scores_of_a_prefix_key_and_an_own_key_weigh_evenly(torch_mod, attn, top, b):
+    """One key of the prefix and one of the entry's own with the same large score, the others at 0: half the
+    weight each. Queries have one element, and that times log2(e) has 21 significant bits, so that both sides
+    hold the score exactly; what is left are the sums' and the gate's roundings, far below the 1e-5. (To natural
+    units and back a reference in [2^k, 2^(k+1)) moves by up to 2^(k-24).)"""
+    torch = torch_mod
+    rng = np.random.default_rng(top)
+    log2e = np.float32(1.4426950408889634)
+
+    def query():
+        while True:
+            t = top / 2 * (1 + rng.random())  # score 2 t in log2 units
+            t = np.round(t * 2.0 ** (20 - int(np.floor(np.log2(t))))) * 2.0 ** -(
+                20 - int(np.floor(np.log2(t))))
+            q = np.float32(t / np.float64(log2e))
+            if np.float32(q * log2e) == t:
+                return q
+
+    own = 40
+    c = Paged(torch, 16, 4, [64 + own - e % 5 for e in range(b)], 3)
+    finite = torch.isfinite(c.k)
+    c.k.mul_(torch.where(finite, 0, 1).half())  # 0, and NaN and infinity where nobody sees
+    c.q.zero_()
+    c.q[:, :, 0] = torch.from_numpy(np.array([[query() for _ in range(H)] for _ in range(b)])).cuda()
+    for e in range(b):
+        for key in (rng.integers(0, 64), rng.integers(64, c.lens[e])):
+            page = c.prefix[key // 16] if key < 64 else c.table[e, key // 16]
+            if key >= 64 or e == 0:  # one key of the prefix
+                c.k[int(page), :, int(key) % 16, 0] = 32
+    check(torch, c.run(attn), c.ref())
+    # The same behind a contiguous prefix.
+    r = ragged(torch, b, 64, own, top)
+    r["held"][:] = own
+    r["first"] = np.arange(b) * KV * own * D
+    rand = lambda *n: torch.randn(*n, device="cuda", dtype=torch.float16)  # noqa: E731
+    r["k"], r["v"] = torch.zeros(b * KV * own * D, device="cuda").half(), rand(b * KV * own * D)
+    r["k"].view(b, KV, own, D)[:, :, 17, 0] = 32
+    r["kp"][:, :64] = 0
+    r["kp"][:, 29, 0] = 32
+    r["q"] = c.q
+    core, ref = run_ragged(torch, attn, r)
+    check(torch, core, ref)
+
+
+@pytest.mark.parametrize("q_scale", [0.01, 1.0, 4.0])
+@pytest.mark.parametrize("batch", [3, 7, 19, 70])
+def test_precision_of_ordinary_scores(torch_mod, attn, batch, q_scale):
+    """1e-5 while no key's sum of |q_i k_i| / 16 exceeds 64 (about 54 here at most)."""
+    c = Paged(torch_mod, 16, 130, lengths(np.random.default_rng(batch), batch, 2080, 400), batch,
+              q_scale=q_scale)
+    for e in range(min(batch, 8)):
+        size = torch_mod.matmul(c.q[e].abs().view(KV, GROUP, D),
+                                c.keys(c.k, e).float().abs().transpose(1, 2).contiguous()) / 16
+        assert size.numel() == 0 or size.max() <= 64
+    check(torch_mod, c.run(attn), c.ref())
+
+
 def test_rows_are_independent(torch_mod, attn):
     """NaN and infinities in the queries of an entry stay in its rows; queries of zero weigh evenly."""
     torch = torch_mod
