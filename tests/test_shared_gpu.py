@@ -444,6 +444,24 @@ def test_ragged(torch_mod, attn, batch, prefix, own):
     check(torch_mod, core, ref)
 
 
+def test_ragged_without_a_prefix_takes_none(torch_mod, attn):
+    """prefix_len 0: the prefix's caches are not looked at, whether None or anything else."""
+    c = ragged(torch_mod, 5, 0, 70, 2)
+    core, ref = run_ragged(torch_mod, attn, c)
+    check(torch_mod, core, ref)
+    first = core.clone()
+    sc = attn.SharedScratch(5, 70, 0)
+    args = (c["q"], c["gate"], c["k"], c["v"], dev(torch_mod, c["first"], torch_mod.int64),
+            dev(torch_mod, c["held"]))
+    for none in (None, torch_mod.zeros(3)):
+        core.fill_(777.25)
+        attn.attn_decode_ragged_shared(*args, none, none, 0, 0, core, sc)
+        assert torch_mod.equal(core, first)
+    with pytest.raises(ValueError, match="k_prefix"):
+        attn.attn_decode_ragged_shared(*args, torch_mod.zeros(3), torch_mod.zeros(3), 1, 1, core,
+                                       attn.SharedScratch(5, 70, 1))
+
+
 def test_ragged_prefix_beyond_4_gib(torch_mod, attn):
     """A cache of 4.3 million rows a head: the second head's rows lie past 32-bit byte and half offsets."""
     torch = torch_mod
