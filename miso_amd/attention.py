@@ -745,11 +745,14 @@ def attn_prep_paged(qg, k, v, q_norm, k_norm, inv_freq, k_pages, v_pages, page_s
     at slots[t] of the page pool (int32, on the device); one without a slot in the pool is left out. qg /
     k / v are views into a token-major projection buffer, rows proj_stride floats apart. With `gate`
     ([n][16][256]) the gates are stored dense, as the batched decodes take them. The first rope_dims
-    dimensions are rotated by position * inv_freq (float32, rope_dims / 2; rope_frequencies makes them),
-    in pairs (i, i + rope_dims / 2) or neighbours (interleaved), cos and sin times rot_scale."""
+    dimensions are rotated by position * inv_freq (float32, rope_dims / 2; rope_frequencies makes them;
+    rope_dims 0: none, it may be None), in pairs (i, i + rope_dims / 2) or neighbours (interleaved), cos and
+    sin times rot_scale."""
     f32, int32, cache = torch.float32, torch.int32, _cache_dtype(k_pages)
     rows = (_count(n, "n") - 1) * _count(proj_stride, "proj_stride") if n else -QG_STRIDE
     heads = n * Q_HEADS * DIM
+    if not rope_dims:  # not looked at
+        inv_freq = q_norm
     _need_all(("qg", qg, f32, rows + QG_STRIDE), ("k", k, f32, rows + KV_HEADS * DIM),
               ("v", v, f32, rows + KV_HEADS * DIM), ("q_norm", q_norm, f32, DIM),
               ("k_norm", k_norm, f32, DIM),

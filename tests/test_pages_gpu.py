@@ -336,6 +336,19 @@ def test_prep_paged(torch_mod, attn, n, page, rope, interleaved, scale):
     check_prep(torch, c, before, page, prep_ref(torch, c, rope, interleaved, scale))
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_prep_paged_without_a_rotation_takes_no_frequencies(torch_mod, attn, interleaved):
+    torch = torch_mod
+    c = prep_case(torch, 9, 16, 4, 0, 5)
+    c["freq"] = None
+    before = {x: c[x].clone() for x in ("q", "gate", "k", "v")}
+    run_prep(attn, c, 16, 0, interleaved, 1.0)
+    check_prep(torch, c, before, 16, prep_ref(torch, c, 0, interleaved, 1.0))
+    c["freq"] = torch.zeros(31, device="cuda")
+    with pytest.raises(ValueError, match="inv_freq"):
+        run_prep(attn, c, 16, 64, interleaved, 1.0)
+
+
 def test_prep_paged_leaves_tokens_without_a_slot(torch_mod, attn):
     torch = torch_mod
     c = prep_case(torch, 40, 16, 4, 64, 3)
