@@ -822,22 +822,23 @@ def attn_decode_ragged_shared(q, gate, k_cache, v_cache, kv_offsets, lens, k_pre
                               stream=None) -> None:
     """attn_decode_ragged of lens.numel() sequences behind a shared prefix, keys [0, prefix_len) of the
     cache k_prefix / v_prefix ([2][prefix_ctx][256]; prefix_len 0: none, they may be None); lens and
-    kv_offsets: their own keys, 0 or more."""
+    kv_offsets: their own keys, 0 or more (caches of no elements: 0 of every sequence)."""
     rows = KV_HEADS * _count(prefix_ctx, "prefix_ctx") * DIM
     batch = _shared_batch(lens, scratch, _count(prefix_len, "prefix_len"))
+    if not prefix_len:  # not looked at
+        k_prefix, v_prefix, rows = k_cache, v_cache, 0
+    max_own = scratch.max_own if k_cache.numel() and v_cache.numel() else 0
     f32, cache, heads = torch.float32, _cache_dtype(k_cache), batch * Q_HEADS * DIM
     _need_all(("q", q, f32, heads), ("gate", gate, f32, heads), ("core", core, f32, heads),
               ("k_cache", k_cache, cache, 0), ("v_cache", v_cache, cache, 0),
+              ("k_prefix", k_prefix, cache, rows), ("v_prefix", v_prefix, cache, rows),
               ("kv_offsets", kv_offsets, torch.int64, batch), ("lens", lens, torch.int32, batch),
               ("scratch", scratch.ws, torch.uint8, 0))
-    if prefix_len:
-        _need_all(("k_prefix", k_prefix, cache, rows), ("v_prefix", v_prefix, cache, rows))
     _lib.check(_lib.load().miso_attn_decode_ragged_shared(
         q.data_ptr(), gate.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        kv_offsets.data_ptr(), lens.data_ptr(), batch, scratch.max_own,
-        k_prefix.data_ptr() if prefix_len else None, v_prefix.data_ptr() if prefix_len else None,
-        prefix_len, prefix_ctx, core.data_ptr(), scratch.ws.data_ptr(), scratch.nbytes,
-        _stream(stream)))
+        kv_offsets.data_ptr(), lens.data_ptr(), batch, max_own, k_prefix.data_ptr(),
+        v_prefix.data_ptr(), prefix_len, prefix_ctx, core.data_ptr(), scratch.ws.data_ptr(),
+        scratch.nbytes, _stream(stream)))
 
 
 # ------------------------------------------------------------------------------------------------

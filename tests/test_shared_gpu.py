@@ -462,6 +462,15 @@ def test_ragged_without_a_prefix_takes_none(torch_mod, attn):
                                        attn.SharedScratch(5, 70, 1))
 
 
+@pytest.mark.parametrize("prefix", [0, 100])
+def test_ragged_of_empty_caches(torch_mod, attn, prefix):
+    """No sequence has own keys, the caches are empty, the scratch is made for more: the prefix alone."""
+    c = ragged(torch_mod, 5, prefix, 0, 2)
+    c["k"], c["v"] = c["k"][:0], c["v"][:0]
+    core, ref = run_ragged(torch_mod, attn, c, attn.SharedScratch(6, 300, 128))
+    check(torch_mod, core, ref)
+
+
 def test_ragged_prefix_beyond_4_gib(torch_mod, attn):
     """A cache of 4.3 million rows a head: the second head's rows lie past 32-bit byte and half offsets."""
     torch = torch_mod
