@@ -631,8 +631,9 @@ uint64_t miso_attn_decode_shared_workspace_bytes(uint32_t max_batch, uint32_t ma
  * Precision as miso_attn_decode's: per-head relative L2 error <= 1e-5 over the same keys, where no key's
  * sum of |q_i k_i| / 16 over the 256 dimensions exceeds 64. Beyond, a score is held to about 2^-23 of
  * that sum, a key's weight is off by as large a factor, and the error grows with it (measured: 1e-5 at
- * 200, 7e-5 at 1800; miso_attn_decode_paged alike). Equal calls give equal bits. Queries are finite and, as miso_attn_decode's, below 2^19; the prefix's rows are
- * finite, also those that an entry does not see.
+ * 200, 7e-5 at 1800; miso_attn_decode_paged alike). Equal calls give equal bits. Queries are finite and,
+ * as miso_attn_decode's, below 2^19; so are the prefix's rows that some entry sees. Those that none sees
+ * may hold anything, but their pages are read (prefix_table's entries are all valid).
  * Table entries and rows are not validated. Rejects batch == 0 or > 65536, page_size as above,
  * prefix_pages > max_pages, max_pages * page_size >= 2^31 or < prefix_pages * page_size + max_own and a
  * workspace that is too small. */

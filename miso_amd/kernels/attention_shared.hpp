@@ -490,6 +490,19 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
   const unsigned sees = prefix_keys(p, seq);
   const bool full = __builtin_amdgcn_ballot_w64(seq < p.batch && sees < t1 * kKeys) == 0;
 
+  // And those that some row of the workgroup sees, with the first tile of the span that has others (~0: none
+  // has; only in the paged form an entry may see less than the prefix).
+  unsigned seen = 0, unseen_from = ~0u;
+  if constexpr (kPaged) {
+    const unsigned mine = prefix_keys(p, kSeqs * kRowBlocks * group + lane % (kSeqs * kRowBlocks));
+    if (__builtin_amdgcn_ballot_w64(mine >= min(t1 * kKeys, p.prefix.len)) == 0) {  // rare
+#pragma unroll
+      for (unsigned i = 0; i < kSeqs * kRowBlocks; ++i)
+        seen = max(seen, decode_detail::lane_value(mine, i));
+      unseen_from = seen / kKeys;
+    }
+  }
+
   // ---- Operand addresses of a stage (attention_prefill.hpp: the same tiles and swizzles).
   const unsigned kb = col * 512 + 16 * (hi ^ (col & 15u));
   unsigned vb[4];
@@ -522,9 +535,11 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
     after = after == lds + (kStages - 1) * kStageBytes ? lds : after + kStageBytes;
     spare = spare == lds + (kStages - 1) * kStageBytes ? lds : spare + kStageBytes;
   };
-  // Tile ti has landed: this wave's copies by the count (two tiles more are under way), every wave's by
-  // the barrier, which also says that every wave has read tile ti - 2, whose stage the next copy takes.
-  auto turn = [&](unsigned ti) __attribute__((always_inline)) {
+  // Tile ti has landed in stage `base`: this wave's copies by the count (two tiles more are under way), every
+  // wave's by the barrier, which also says that every wave has read tile ti - 2, whose stage the next copy
+  // takes. Rows of V that none of the workgroup's rows sees are cleared before: their numerators are 0, but
+  // they may hold NaN or infinity.
+  auto turn = [&](unsigned ti, unsigned base) __attribute__((always_inline)) {
     const unsigned behind = t1 - 1 - ti;
     if (behind >= 2)
       cdna4::wait_vmcnt<16>();
@@ -532,6 +547,13 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
       cdna4::wait_vmcnt<8>();
     else
       cdna4::wait_vmcnt<0>();
+    if (kPaged && __builtin_expect(ti >= unseen_from, 0)) {
+#pragma unroll 1
+      for (unsigned r = 8 * wave + (lane >> 5); r < 8 * wave + 8; r += 2)
+        if (ti * kKeys + r >= seen)
+          *reinterpret_cast<__attribute__((address_space(3))) cdna4::float4_t*>(
+              base + kTileBytes + 512 * r + 16 * (lane & 31u)) = cdna4::float4_t{};
+    }
     decode_detail::tile_barrier();
   };
   auto first_operands = [&](unsigned base) __attribute__((always_inline)) {
@@ -640,13 +662,13 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  turn(t0);
+  turn(t0, here);
   if (t0 + 3 < t1)
     issue(t0 + 3, 2 * kStageBytes);
   if (!active) {
     for (unsigned ti = t0 + 1; ti < t1; ++ti) {
       rotate();
-      turn(ti);
+      turn(ti, here);
       if (ti + 3 < t1)
         issue(ti + 3, spare - lds);
     }
@@ -674,7 +696,7 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
   // MFMAs; between those of P V the other half's pairs, the moves of cur to x, and behind the last V
   // operand the barrier and the next tile's first operands.
   if (t0 + 1 < t1) {
-    turn(t0 + 1);
+    turn(t0 + 1, after);
     first_operands(after);
     for (unsigned ti = t0 + 1;;) {
       rotate();
@@ -725,7 +747,7 @@ __device__ __attribute__((always_inline)) inline void prefix_span(const AttnShar
             asm volatile("" : "+v"(x[j]));
           }
         if (i == kValues - 3 && next_tile) {  // the V operands are here
-          turn(ti + 1);
+          turn(ti + 1, after);
           first_operands(after);
         }
       });

@@ -375,6 +375,45 @@ def test_rows_are_independent(torch_mod, attn):
     assert torch.equal(got[keep], good[keep])
 
 
+@pytest.mark.parametrize("batch,prefix_pages,most", [
+    (1, 4, 1), (1, 40, 613), (3, 300, 4799), (4, 64, 31), (7, 300, 4000), (8, 20, 0), (16, 40, 300),
+    (20, 300, 1025), (40, 300, 4769), (70, 9, 143), (520, 5, 33), (520, 5, 79)])
+def test_rows_of_the_prefix_that_nobody_sees_may_hold_anything(torch_mod, attn, batch, prefix_pages, most):
+    """Entries that all end inside the prefix, as the paged decode serves them: behind the longest's keys lie NaN
+    and infinities, in K and in V; an entry of length 0 sees none."""
+    torch, page = torch_mod, 16
+    rng = np.random.default_rng(batch + most)
+    lens = rng.integers(0, most + 1, batch)
+    lens[rng.integers(0, batch)] = most
+    c = Paged(torch, page, prefix_pages, lens, batch + most)
+    clean = c.run(attn).clone()
+    check(torch, clean, c.ref())
+    ids = torch.from_numpy(c.prefix).cuda()
+    for x, bad in ((c.k, float("nan")), (c.v, float("inf")), (c.v, float("nan")), (c.k, float("-inf"))):
+        rows = x[ids].transpose(0, 1).reshape(KV, -1, D)
+        rows[:, most:] = bad
+        x[ids] = rows.view(KV, prefix_pages, page, D).transpose(0, 1).contiguous()
+        c.core.fill_(777.25)
+        assert torch.equal(c.run(attn), clean)
+    assert torch.isfinite(clean).all()
+
+
+def test_unseen_rows_beside_entries_behind_the_prefix(torch_mod, attn):
+    """Row groups of their own: entries 0 .. 31 end inside the prefix at 700 or before, the last one sees up to
+    1100 of 1600 rows; the rows behind hold NaN."""
+    torch = torch_mod
+    rng = np.random.default_rng(5)
+    lens = np.concatenate([rng.integers(0, 701, 32), [1100]])
+    c = Paged(torch, 16, 100, lens, 9)
+    clean = c.run(attn).clone()
+    check(torch, clean, c.ref())
+    for x in (c.k, c.v):
+        x[torch.from_numpy(c.prefix[70:]).cuda()] = float("nan")
+        x[int(c.prefix[68]), :, 12:] = float("nan")
+        x[int(c.prefix[69])] = float("inf")
+    assert torch.equal(c.run(attn), clean)
+
+
 def test_padding_entries_read_nothing(torch_mod, attn):
     """Entries of length 0 with NaN queries, rows outside the table's use: zeros, the others whole."""
     torch = torch_mod
