@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 from conftest import REF_REL_L2
+from test_shared_rule import rule
 
 pytestmark = pytest.mark.gpu
 
@@ -646,3 +647,205 @@ def test_a_batch_served(torch_mod, attn):
                 mine = torch.stack([projs[s][i, 8704:].view(KV, D) for s, i in given[rows[t]]], 1)
                 assert torch.equal(v[:, pp * page:], mine.half())
     assert held.max() > 0
+
+
+def last_span(r, tiles):
+    """Tiles of the last span of a rule."""
+    return tiles - (r["spans"] - 1) * r["span_tiles"]
+
+
+@pytest.mark.parametrize("batch,row_blocks", [(3, 1), (7, 2), (12, 2), (515, 4)])
+@pytest.mark.parametrize("tiles", [1, 2, 3, 4, 5, 6, 7])
+def test_spans_of_every_few_tiles(torch_mod, attn, O, batch, row_blocks, tiles):
+    """One span of 1 .. 7 tiles, whole and ending inside a tile, by one, two and four row blocks a workgroup:
+    the ring's first copies, none and some left to issue in the loop. (Spans that the cut makes several of have
+    4 tiles and more, but the last one; see below.)"""
+    for page, cut in ((8, 0), (8, 24), (32, 0)):
+        keys = 32 * tiles - cut
+        r = rule(O, batch, keys, 0)
+        assert (r["row_blocks"], r["spans"], r["span_tiles"]) == (row_blocks, 1, tiles)
+        lens = np.array([max(keys - 5 * (e % 4), 0) for e in range(batch)])
+        c = Paged(torch_mod, page, keys // page, lens, batch + tiles)
+        check(torch_mod, c.run(attn, c.scratch(attn, max_own=0)), c.ref(), (page, cut))
+
+
+@pytest.mark.parametrize("batch,row_blocks", [(4, 1), (8, 2), (300, 4)])
+@pytest.mark.parametrize("last", [1, 2, 3, 4, 5])
+def test_last_spans_of_every_few_tiles(torch_mod, attn, O, batch, row_blocks, last):
+    """A last span of 1 .. 5 tiles behind longer ones, its last tile of one row, of 31 and whole."""
+    def fits(tiles, off):
+        r = rule(O, batch, 32 * tiles - off, 0)
+        return r["row_blocks"] == row_blocks and r["spans"] > 1 and last_span(r, tiles) == last
+
+    for off in (0, 1, 31):
+        tiles = next(t for t in range(5, 4000) if fits(t, off))
+        c = ragged(torch_mod, batch, 32 * tiles - off, 0, tiles)
+        core, ref = run_ragged(torch_mod, attn, c, attn.SharedScratch(batch, 0, c["prefix"]))
+        check(torch_mod, core, ref, (tiles, off))
+
+
+@pytest.mark.parametrize("q_scale,own", [(30.0, 90), (300.0, 90), (2.0 ** 13, 90), (2.0 ** 16, 90),
+                                         (2.0 ** 20, 0)])
+@pytest.mark.parametrize("batch", [3, 19, 70])
+def test_every_head_of_large_scores(torch_mod, attn, batch, q_scale, own):
+    """A score is off by at most d = 2^-17.8 of the sum of its |q_i k_i| / 16: queries as pairs 2^-21, log2(e)
+    and its product 2^-24 and 2^-25, 32 sums in f32 of 2^-23 at most (rounded or cut), 2^-18 of them. With the
+    largest such d over a head's keys, D, a weight is off by a factor of up to e^(2 D): the output by
+    (e^(2 D) - 1) sum w |v|. Where a key leads by more than 2 D + 20, the others weigh less than n e^-20, 2e-7
+    here, and the output is that key's value to the decodes' 1e-5. What is left are heads between: those lie
+    within the values."""
+    torch = torch_mod
+    c = Paged(torch, 16, 16, lengths(np.random.default_rng(batch), batch, 256, own), batch + 1,
+              q_scale=q_scale)
+    got = c.run(attn).double()
+    assert torch.isfinite(got).all()
+    held = heads = 0
+    for e in np.flatnonzero(c.lens):
+        k, v = c.keys(c.k, e).double(), c.keys(c.v, e).double()
+        q = c.q[e].double().view(KV, GROUP, D)
+        kt = k.transpose(1, 2).contiguous()
+        d = 2.0 ** -17.8 * (torch.matmul(q.abs(), kt.abs()) / 16).amax(-1)
+        s = torch.matmul(q, kt) / 16
+        w = torch.softmax(s, -1)
+        gate = torch.sigmoid(c.gate[e].double()).view(KV, GROUP, D)
+        ref, out = torch.matmul(w, v) * gate, got[e].view(KV, GROUP, D)
+        err, norm = (out - ref).norm(dim=-1), ref.norm(dim=-1)
+        spread = torch.matmul(w, v.norm(dim=-1, keepdim=True))[..., 0]
+        near = torch.expm1((2 * d).clamp(max=50.0)) * spread + REF_REL_L2 * norm
+        if s.shape[-1] > 1:
+            top = s.topk(2, dim=-1).values
+            leads = top[..., 0] - top[..., 1] > 2 * d + 20
+        else:
+            leads = torch.ones_like(norm, dtype=torch.bool)
+        bound = torch.where(leads, REF_REL_L2 * norm, near)
+        assert (err <= bound).all(), (int(e), float((err / bound).max()))
+        assert (out.abs() <= v.abs().amax(1)[:, None] * gate * (1 + 1e-5) + 1e-30).all()
+        held += int((bound <= 0.2 * norm).sum())
+        heads += norm.numel()
+    assert held >= 0.98 * heads, (held, heads)  # the bound says something of nearly all
+
+
+@pytest.mark.parametrize("capacity,live,prefix_pages,own", [(512, 64, 64, 300), (300, 1, 40, 30),
+                                                            (2000, 33, 16, 50), (64, 5, 400, 1)])
+def test_empty_entries_behind_the_live_ones(torch_mod, attn, capacity, live, prefix_pages, own):
+    """A step's capacity of which most is empty at the end, NaN queries there: zeros, the live ones whole."""
+    torch = torch_mod
+    lens = np.zeros(capacity, np.int64)
+    lens[:live] = lengths(np.random.default_rng(live), live, 16 * prefix_pages, own, zeros=False)
+    c = Paged(torch, 16, prefix_pages, lens, capacity)
+    ref = c.ref()
+    c.q[live:] = float("nan")
+    for _ in range(2):
+        c.core.fill_(777.25)
+        got = c.run(attn)
+        check(torch, got, ref)
+        assert (got[live:] == 0).all()
+
+
+def test_a_plan_of_large_capacity(torch_mod, attn):
+    """attn_page_plan's rows and visible for 512 tokens of which 40 are given, as one call's entries."""
+    torch = torch_mod
+    rng = np.random.default_rng(1)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(7)
+    b, page, pp, room, pool, most = 30, 16, 50, 60, 400, 512
+    ids = rng.permutation(pool)
+    rand = lambda *n, **kw: torch.randn(*n, generator=g, device="cuda", **kw)  # noqa: E731
+    k, v = (rand(pool, KV, page, D, dtype=torch.float16) for _ in range(2))
+    prefix, table = dev(torch, ids[:pp]), dev(torch, np.full((b, room), -1))
+    lens, stack = dev(torch, np.zeros(b)), dev(torch, np.concatenate([ids[pp:], np.full(pp, -1)]))
+    n_free, plan = dev(torch, [pool - pp]), attn.PagePlan(b, most)
+    new = np.ones(b, np.int64)
+    new[3] = 11  # a chunk among single tokens
+    attn.attn_page_plan(lens, dev(torch, new), table, page, stack, n_free, plan,
+                        prefix_table=prefix, prefix_pages=pp)
+    q, gate = 2 * rand(most, H, D), rand(most, H, D)
+    core = torch.full((most, H, D), 5.0, device="cuda")
+    sc = attn.SharedScratch(most, (room - pp) * page, pp * page)
+    sc.ws.fill_(255)
+    attn.attn_decode_paged_shared(q, gate, k, v, table, page, plan.visible, prefix, pp, core, sc,
+                                  rows=plan.rows)
+    torch.cuda.synchronize()
+    rows, sees, t_of = (x.cpu().numpy() for x in (plan.rows, plan.visible, table))
+    assert (sees[:40] > pp * page).all() and (sees[40:] == 0).all() and new.sum() == 40
+    assert (core[40:] == 0).all()
+    for t in range(40):
+        pages = torch.from_numpy(t_of[rows[t]][:-(-sees[t] // page)]).cuda().long()
+        keys, values = (x[pages].transpose(0, 1).reshape(KV, -1, D)[:, :sees[t]] for x in (k, v))
+        check(torch, core[t][None], attention(torch, q[t], gate[t], keys, values)[None], t)
+
+
+FAR = 4_300_003  # keys: more than 2^31 bytes of a head's rows
+
+
+def far_tolerance():
+    """The decodes' 1e-5 and what sums of FAR keys add to it: at most 4 f32 sums of 2^-23 for a tile of 32 keys
+    along a span, of which 128 at least share the keys."""
+    return REF_REL_L2 + 4 * (FAR / 32 / 128 + 1) * 2.0 ** -23
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_a_request_of_more_than_2_gib_in_pages(torch_mod, attn, own):
+    """Behind a prefix of FAR keys, or of FAR own keys: positions past 2^31 bytes of a head's rows, in a table
+    whose entries name the same 64 pages over and over, so that a key's weight counts as often as it comes."""
+    torch, page, n_pages = torch_mod, 16, 64
+    rng = np.random.default_rng(3)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    pp = FAR // page if not own else 3
+    room = -(-FAR // page) + 1 if own else pp + 2
+    table = rng.integers(0, n_pages, (1, room))
+    lens = np.array([FAR if own else pp * page + 9, pp * page + 2, pp * page - 3])
+    rand = lambda *n, **kw: torch.randn(*n, generator=g, device="cuda", **kw)  # noqa: E731
+    k, v = (rand(n_pages, KV, page, D, dtype=torch.float16) for _ in range(2))
+    q, gate, core = 2 * rand(3, H, D), rand(3, H, D), torch.full((3, H, D), 5.0, device="cuda")
+    sc = attn.SharedScratch(3, int(lens.max()) - pp * page, pp * page)
+    attn.attn_decode_paged_shared(q, gate, k, v, dev(torch, table), page, dev(torch, lens),
+                                  dev(torch, table[0, :pp]), pp, core, sc,
+                                  rows=dev(torch, np.zeros(3)))
+    for e in range(3):
+        n = int(lens[e])
+        times = np.repeat(np.bincount(table[0, :n // page], minlength=n_pages)[:, None], page, 1)
+        times[table[0, n // page], :n % page] += 1
+        times = torch.from_numpy(times.reshape(-1)).cuda().double()
+        keys, values = (x.double().transpose(0, 1).reshape(KV, -1, D) for x in (k, v))
+        s = torch.matmul(q[e].double().view(KV, GROUP, D), keys.transpose(1, 2).contiguous()) / 16
+        w = torch.exp(s - s.amax(-1, keepdim=True)) * times
+        ref = (torch.matmul(w / w.sum(-1, keepdim=True), values).view(H, D) *
+               torch.sigmoid(gate[e].double()))
+        err = ((core[e].double() - ref).norm(dim=-1) / ref.norm(dim=-1)).max()
+        assert err <= far_tolerance(), (e, float(err))
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_a_request_of_more_than_2_gib_of_rows(torch_mod, attn, own):
+    """The same of contiguous caches [2][FAR][256], as the prefix or as one sequence's own keys."""
+    torch = torch_mod
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    rand = lambda *n, **kw: torch.randn(*n, generator=g, device="cuda", **kw)  # noqa: E731
+    k, v, ks, vs = (rand(KV, n, D, dtype=torch.float16) for n in (FAR, FAR, 33, 33))
+    q, gate, core = 2 * rand(2, H, D), rand(2, H, D), torch.full((2, H, D), 5.0, device="cuda")
+    far, near = (k, v), (ks, vs)
+    prefix, mine = (near, far) if own else (far, near)
+    n_prefix, n_mine = prefix[0].shape[1], mine[0].shape[1]
+    sc = attn.SharedScratch(2, n_mine, n_prefix)
+    attn.attn_decode_ragged_shared(q, gate, mine[0].view(-1), mine[1].view(-1),
+                                   dev(torch, [0, 0], torch.int64), dev(torch, [n_mine, 0]),
+                                   *prefix, n_prefix, n_prefix, core, sc)
+    for e, parts in enumerate(((prefix, mine), (prefix,))):
+        x = q[e].double().view(KV, GROUP, D)
+        blocks = ((kk[:, i:i + 200_000].double(), vv[:, i:i + 200_000].double())
+                  for kk, vv in parts for i in range(0, kk.shape[1], 200_000))
+        top = torch.full((KV, GROUP, 1), -float("inf"), dtype=torch.float64, device="cuda")
+        all_w, out = torch.zeros_like(top), torch.zeros(KV, GROUP, D, dtype=torch.float64, device="cuda")
+        for kk, vv in blocks:
+            s = torch.matmul(x, kk.transpose(1, 2).contiguous()) / 16
+            new = torch.maximum(top, s.amax(-1, keepdim=True))
+            w = torch.exp(s - new)
+            all_w = all_w * torch.exp(top - new) + w.sum(-1, keepdim=True)
+            out = out * torch.exp(top - new) + torch.matmul(w, vv)
+            top = new
+        ref = (out / all_w).view(H, D) * torch.sigmoid(gate[e].double())
+        err = ((core[e].double() - ref).norm(dim=-1) / ref.norm(dim=-1)).max()
+        assert err <= far_tolerance(), (e, float(err))
