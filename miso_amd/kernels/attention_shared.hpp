@@ -1165,12 +1165,13 @@ __global__ void __launch_bounds__(64 * kWaves) attn_shared_merge_kernel(AttnShar
       }
     }
   }
+  // Without keys 0, also where the gate is NaN.
   const float inv = all != 0.0f ? 1.0f / all : 0.0f;
   const float gv[4] = {g.x, g.y, g.z, g.w};
   float r[4];
 #pragma unroll
   for (unsigned j = 0; j < 4; ++j)
-    r[j] = v[j] * inv / (1.0f + __expf(-gv[j]));
+    r[j] = all != 0.0f ? v[j] * inv / (1.0f + __expf(-gv[j])) : 0.0f;
   *reinterpret_cast<float4*>(p.core + out) = float4{r[0], r[1], r[2], r[3]};
 }
 

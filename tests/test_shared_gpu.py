@@ -742,6 +742,26 @@ def test_empty_entries_behind_the_live_ones(torch_mod, attn, capacity, live, pre
         assert (got[live:] == 0).all()
 
 
+@pytest.mark.parametrize("prefix_pages", [0, 10])
+def test_empty_entries_give_zeros_whatever_their_gates_hold(torch_mod, attn, prefix_pages):
+    """attn_prep_paged leaves the gates of tokens without a slot as they are: NaN, where nobody wrote them."""
+    torch = torch_mod
+    lens = np.array([0, 16 * prefix_pages + 40, 0, 16 * prefix_pages + 1, 0, 0])
+    c = Paged(torch, 16, prefix_pages, lens, 5)
+    ref = c.ref()
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        c.gate[torch.from_numpy(lens == 0).cuda()] = bad
+        c.core.fill_(777.25)
+        check(torch, c.run(attn), ref)
+    r = ragged(torch, 4, 0, 30, 6)
+    r["held"][1:3] = 0
+    core, ref = run_ragged(torch, attn, r)
+    check(torch, core, ref)
+    r["gate"][1:3] = float("nan")
+    run_ragged(torch, attn, r)
+    check(torch, r["core"], ref)
+
+
 def test_a_plan_of_large_capacity(torch_mod, attn):
     """attn_page_plan's rows and visible for 512 tokens of which 40 are given, as one call's entries."""
     torch = torch_mod
