@@ -719,7 +719,9 @@ def rope_frequencies(rope_dims: int, base: float, factor: float = 1.0, scaling: 
     rounded to float32, for contexts `factor` times as long as the model was trained on. "linear":
     every frequency divided by factor. "yarn" (Peng et al., 2023): a frequency that turns more than
     `fast` times over the original_ctx positions of training stays, one that turns less than `slow` times
-    is divided, those between by a linear ramp; rot_scale = 1 + 0.1 ln(factor) (1 for linear)."""
+    is divided, those between by a ramp linear in the number of turns, as in the paper's formula (a ramp over
+    the index i, as some checkpoints were made with, gives other frequencies there: pass those as inv_freq
+    instead); rot_scale = 1 + 0.1 ln(factor) (1 for linear)."""
     if rope_dims % 8 != 0 or not 0 <= rope_dims <= DIM:
         raise ValueError("rope_dims must be a multiple of 8, at most 256")
     if not (base > 0 and factor >= 1):

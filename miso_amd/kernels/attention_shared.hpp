@@ -3,7 +3,8 @@
 // Batched decode behind a prefix that all sequences share, for MI355X (gfx950 / CDNA4); no reference
 // counterpart (the reference is batch-1). The ragged and paged decodes (attention_decode.hpp) read the
 // prefix once per sequence: 64 sequences behind 32768 keys stream 4.3 GB. Here the queries of all
-// sequences meet the prefix's keys together, so that K and V are read once per 16 sequences:
+// sequences meet the prefix's keys together, so that K and V are read once per 16 sequences (8
+// behind short prefixes):
 //   attn_shared_split_kernel: partials of 8 query rows per sequence and KV head over spans of the prefix,
 //                             and the streaming split over each sequence's own keys behind it
 //   attn_shared_merge_kernel: both partials joined, the gate applied
@@ -84,7 +85,7 @@ struct AttnSharedCut {
 // What the tiles of a launch cost on `cus` CUs, a workgroup each, in us without the fixed part: the
 // slower side, or the span and its share of the `own` tiles of own keys (both heads') one after the
 // other. A tile of a span behind 64 sequences takes 1.5 us (32768 keys of 40 tiles a span: 70 us), behind
-// 8 1.0 (9 tiles: 23 us, 12: 26), behind 3 0.9; of the own keys 1.4 (48 workgroups: 72 us, 32: 97), four
+// 8 1.0 (9 tiles: 23 us, 12: 26), behind 3 0.9; of the own keys 1.5 (48 workgroups: 72 us, 32: 97), four
 // at a time, a wave each: a sequence of 5 keys counts as four tiles (106 of them on 32 CUs: 45 us); the own
 // keys' start behind a span 14 (256 behind 8192 keys, 256 each: 92 us of 32 tiles and 12, 80 of 43 beside 48).
 template <unsigned kRowBlocks>
@@ -159,7 +160,10 @@ __host__ __device__ constexpr AttnSharedCut attn_shared_cut(unsigned tiles, unsi
 // Sequences of up to kAttnSharedWaveKeys own keys, kAttnSharedWaveBatch or more of them, may be a wave's each
 // (wave_items): longer ones would leave one wave to work when the others are done, fewer leave waves idle. Of up
 // to 250 own keys behind 4096: 48 sequences 19.9 us with four waves an item, 20.3 with one; 64 26.3 and 22.3;
-// 200 51.8 and 48.8.
+// 200 51.8 and 48.8. Of more keys, the call with four waves an item and with one: behind 4096 keys 130 of up to
+// 500 48.6 and 50.4, 200 of up to 260 58.6 and 60.4, of up to 500 58.3 and 53.8, 400 of up to 400 124.8 and
+// 88.1: beyond the limit one wave costs a little for some batches and saves much for the largest. One sequence
+// above it sends the whole batch to four waves.
 constexpr unsigned kAttnSharedWaveKeys = 256, kAttnSharedWaveBatch = 64;
 
 namespace shared_detail {
@@ -325,7 +329,8 @@ __device__ __attribute__((always_inline)) inline unsigned own_keys(const AttnSha
 //
 // 64 sequences behind 131072 keys: 1.77 us a tile and CU, 1210 TFLOP/s of f16 products (an 8192^3 library
 // product: 1076), 2860 cycles for 2048 of MFMAs at 1.62 GHz. There the power sets the pace: 2980 cycles, with
-// the copies elsewhere, ran at 1.68 GHz. 8 behind 32768 keys: 22.5 us, 3.1 TB/s, 11 of them in the loop at 5.2
+// the copies elsewhere, ran at 1.68 GHz. Behind 32768, beside own keys on 56 CUs, it holds 1.97 GHz: 1.48 us a
+// tile. 8 behind 32768 keys: 23.3 us, 3.1 TB/s, 11 of them in the loop at 5.2
 // TB/s, 5 before it (queries from memory and cut, three tiles on their way).
 namespace shared_detail {
 template <unsigned kRowBlocks, bool kPaged>
